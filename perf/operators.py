@@ -454,7 +454,7 @@ def lora_own(s):
     mk, lib, ctx = library()
     if "call" not in s:
         c = s["case"]
-        work = workspace(s, lib.mk_lora_workspace(c["n"], s["rank"], c["cols"], c["rows"]))
+        work = workspace(s, lib.mk_lora_workspace(c["n"], s["rank"], c["cols"]))
         kind = {"f32": mk.F32, "f16": mk.F16, "bf16": mk.BF16}[c["type"]]
         s["call"] = (ctx, kind, ptr(s["table"]), c["adapters"], s["rank"], ptr(s["ids"]), ptr(s["x"]), c["cols"], c["n"],
                      c["rows"], c["cols"], ptr(s["base"]), c["rows"], ptr(s["y"]), c["rows"], *work)
@@ -474,7 +474,7 @@ def verify_own(s):
             s["call"] = (ctx, ptr(s["z"]), ptr(s["z_id"]), k, rows, ptr(s["w"]), ptr(s["w_id"]) if q else None, k, n,
                          *tail)
         else:
-            work = workspace(s, lib.mk_verify_workspace(rows, n, lanes, s["vocab"]))
+            work = workspace(s, lib.mk_verify_workspace(lanes, s["most"], s["vocab"]))
             s["call"] = (ctx, ptr(s["z"]), s["vocab"], rows, ptr(s["w"]), s["vocab"], n, s["vocab"], *tail, *work)
     mk.check((lib.mk_verify_topk if "z_id" in s else lib.mk_verify)(*s["call"]))
     return {"accepted": s["accepted"], "tokens": s["tokens"], "probs": s["probs"]}
