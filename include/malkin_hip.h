@@ -147,6 +147,26 @@ int mk_matmul_rows(mk_ctx* ctx, int type, const void* w, size_t row_bytes, int64
 int mk_matmul_gguf(mk_ctx* ctx, int type, const void* w, size_t row_bytes, int64_t rows, int64_t cols, const void* xq,
                    int n, float* y, int64_t y_stride, int accumulate);
 
+/* ---- low-rank adapters beside a shared projection (no reference counterpart: it serves one set of weights) ---- */
+/* One adapter, in a device array. a: [rank][cols], b: [rows][rank] (a GGUF adapter's lora_a / lora_b), device pointers
+   to values of the call's type; scale: alpha / rank. */
+typedef struct {
+  const void* a;
+  const void* b;
+  float scale;
+  int32_t rank;
+} mk_lora_adapter;
+/* y[t * y_stride + r] = base[t * base_stride + r] + scale * sum_i b[r][i] (a[i] . x[t]) with adapter ids[t], for t < n,
+   r < rows: the adapters of many requests, one per token, after the matmul they share (base: its output; y itself to
+   add in place, NULL for 0). ids[t] outside 0..n_adapters-1 (-1: none), or an entry whose rank is not in 1..max_rank:
+   y[t] = base[t]. type: MK_F32, MK_F16 or MK_BF16 for all adapters of a call; x and y are fp32, as are the sums.
+   max_rank 1..512. workspace: at least mk_lora_workspace bytes, 16-byte aligned; two calls that may run at the same
+   time need one each. x and y must not overlap, nor base and y unless they are the same rows. */
+size_t mk_lora_workspace(int n, int max_rank, int64_t cols);
+int mk_lora(mk_ctx* ctx, int type, const mk_lora_adapter* adapters, int n_adapters, int max_rank, const int32_t* ids,
+            const float* x, int64_t x_stride, int n, int64_t rows, int64_t cols, const float* base, int64_t base_stride,
+            float* y, int64_t y_stride, void* workspace, size_t workspace_bytes);
+
 /* ---- elementwise (model.cpp:46-49, kernels.h:39) ---- */
 /* y = rmsnorm(x) * w per row of n floats (model.cpp:46-49). */
 int mk_rmsnorm(mk_ctx* ctx, const float* x, const float* w, int rows, int n, float eps, float* y);
@@ -221,6 +241,23 @@ int mk_attention_decode_q8(mk_ctx* ctx, const float* qkv, int64_t stride, int n,
                            const float* k_norm, float eps, const float* cos_t, const float* sin_t,
                            const int32_t* rpos, const int32_t* seq, const int32_t* kv_row, const int32_t* n_keys,
                            const mk_kv_cache* kv, int layer, float* out, int64_t out_stride, int max_keys, void* xq);
+/* Attention of a batch whose sequences share a prefix (a system prompt, a document): its keys and values are read once
+   for all tokens instead of once per sequence. Token t attends to keys 0..n_keys[t]-1: key j < n_prefix is row j of
+   sequence prefix_seq of `prefix` (which may be kv itself, or a cache of its own with any n_seq and n_ctx, of the same
+   n_head_kv and head_dim; unused and may be NULL where n_prefix is 0), key j >= n_prefix row row0 + j - n_prefix of
+   sequence seq[t] of `kv`. With row0 = n_prefix and the prefix's rows also in every sequence it is mk_attention for
+   plain tokens (no ancestors), but its sums run in another order: its results agree with mk_attention's to fp32
+   rounding, not in every bit. A token with n_keys[t] <= 0 or seq[t] outside the cache (a row of a padded batch) gets
+   zeros. max_keys bounds n_keys[t]; keys past it are not read. xq: the BlockQ8 rows of out, as mk_attention_q8 (NULL:
+   not written). workspace: at least mk_attention_prefix_workspace bytes for the same sizes, 16-byte aligned; two calls
+   that may run at the same time need one each. out and q must not overlap; the caches' rows 16-byte aligned.
+   MK_ERR_UNSUPPORTED (nothing launched) for a head_dim other than 64 / 128 or more than 32 query heads per KV head.
+   No reference counterpart (its engine keeps every slot's own copy, engine.cpp:242-301). */
+size_t mk_attention_prefix_workspace(int n, int n_head, int n_head_kv, int head_dim, int n_prefix, int max_keys);
+int mk_attention_prefix(mk_ctx* ctx, const float* q, int64_t q_stride, float* out, int64_t out_stride, int n, int n_head,
+                        const mk_kv_cache* prefix, int prefix_seq, int n_prefix, const mk_kv_cache* kv, int row0,
+                        int layer, const int32_t* seq, const int32_t* n_keys, int max_keys, void* xq, void* workspace,
+                        size_t workspace_bytes);
 /* Model::move_kv (model.cpp:432-440): row `from` -> row `to` of sequence seq, K and V of every layer. */
 int mk_move_kv(mk_ctx* ctx, const mk_kv_cache* kv, int seq, int from, int to);
 
@@ -337,6 +374,41 @@ typedef struct {
    forward. */
 int mk_sample_draw(mk_ctx* ctx, const float* values, const int32_t* ids, int stride, int n_rows,
                    const mk_draw_params* params, uint64_t* states, int n_states, int32_t* out, int n_out);
+
+/* ---- verification of drafted tokens (Sampler::verify, sampler.cpp:124-141, over whole lanes; Leviathan et al. 2023) */
+/* A lane of a speculative step, in a device array: its drafts are drafts[first .. first + n_draft), its target rows
+   row .. row + n_draft (row j predicts draft j, the last one what follows them all), its draft rows those of its
+   drafts. temperature <= 0: greedy. min_p, top_p: mk_verify_topk's cut, as mk_draw_params (mk_verify keeps the whole
+   vocabulary and does not read them). */
+#define MK_VERIFY_MAX_DRAFT 256
+typedef struct {
+  int32_t row, first, n_draft;
+  float temperature, min_p, top_p;
+} mk_verify_lane;
+/* With P_j = softmax(target row j / T) and Q_j = softmax(draft row j / T) (T <= 0: all on the first maximum; q NULL: all
+   on the draft itself, a proposer without a model): draft j is accepted iff Q_j(d) > 0 and u[first + j] Q_j(d) < P_j(d),
+   up to the first refusal. The lane's next token comes from max(P_j - Q_j, 0) at the refused draft (from P_j where that
+   is zero everywhere), or from the last row's P where none was refused: the first id, in order, at which the running sum
+   reaches u_next[lane] times the total. Probabilities and sums are 64-bit. accepted [n_lanes]: drafts accepted; tokens
+   [n_lanes][max_draft + 1]: those, the next token, then -1; probs (NULL: not written) the target's probability P of each
+   token, 0 past them. u, u_next: uniform in [0, 1), one per draft / lane.
+   Logits: NaN counts as -inf (probability 0), +inf as the largest float; a row of nothing but those has no token (-1). A
+   draft outside the vocabulary is refused. A lane that does not fit (n_draft outside 0..max_draft, rows outside n_rows,
+   drafts outside n_drafts) is left out: accepted -1, tokens -1. All arrays are device arrays; rows p_stride / q_stride
+   floats apart. max_draft 0..MK_VERIFY_MAX_DRAFT. workspace: at least mk_verify_workspace bytes, 16-byte aligned; two
+   calls that may run at the same time need one each. */
+size_t mk_verify_workspace(int n_lanes, int max_draft, int n_vocab);
+int mk_verify(mk_ctx* ctx, const float* p, int64_t p_stride, int n_rows, const float* q, int64_t q_stride, int n_drafts,
+              int n_vocab, const mk_verify_lane* lanes, int n_lanes, int max_draft, const int32_t* drafts,
+              const double* u, const double* u_next, int32_t* accepted, int32_t* tokens, float* probs, void* workspace,
+              size_t workspace_bytes);
+/* The same over rows cut to their candidates, highest first (mk_topk's values / ids; p_k, q_k 1..1024 per row): P and Q
+   are the distributions mk_sample_draw draws from (float weights, min_p floor, top_p nucleus, float probabilities),
+   matched by id, and the next token is drawn in the candidates' order. q_values and q_ids both NULL: certain drafts. */
+int mk_verify_topk(mk_ctx* ctx, const float* p_values, const int32_t* p_ids, int p_k, int n_rows, const float* q_values,
+                   const int32_t* q_ids, int q_k, int n_drafts, const mk_verify_lane* lanes, int n_lanes, int max_draft,
+                   const int32_t* drafts, const double* u, const double* u_next, int32_t* accepted, int32_t* tokens,
+                   float* probs);
 
 /* dst[dst_index[i]] = src[src_index[i]] for i < n, in stream order (a NULL index array is the identity; a negative
    index skips i). Moves token ids between device arrays without a host round trip: draft picks into a proposal tree,

@@ -16,6 +16,9 @@ F32, F16, Q8_0, Q4_K, Q5_K, Q6_K, BF16 = 0, 1, 8, 12, 13, 14, 30
 MODEL_NO_WIDE, MODEL_NO_PACK, MODEL_PERSISTENT, MODEL_FUSED_ATTN = 1, 2, 4, 8
 
 BLOCK_Q8 = np.dtype([("d", "<f4"), ("s", "<i2", (2,)), ("qs", "i1", (32,))])
+LORA_ADAPTER = np.dtype([("a", "<u8"), ("b", "<u8"), ("scale", "<f4"), ("rank", "<i4")])
+VERIFY_LANE = np.dtype([("row", "<i4"), ("first", "<i4"), ("n_draft", "<i4"), ("temperature", "<f4"),
+                        ("min_p", "<f4"), ("top_p", "<f4")])
 BATCH_TOKEN = np.dtype([("id", "<i4"), ("seq", "<i4"), ("pos", "<i4"), ("logits", "<i4"), ("kv", "<i4"),
                         ("parent", "<i4")])
 
@@ -67,6 +70,13 @@ SIGNATURES = {
     "mk_attention_q8": (_I, [_P, _P, _I64, _P, _I64, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P]),
     "mk_attention_decode_q8": (_I, [_P, _P, _I64, _I, _I, _P, _P, _F, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I64, _I,
                                     _P]),
+    "mk_attention_prefix_workspace": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "mk_attention_prefix": (_I, [_P, _P, _I64, _P, _I64, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _P, _P, _SZ]),
+    "mk_lora_workspace": (_SZ, [_I, _I, _I64]),
+    "mk_lora": (_I, [_P, _I, _P, _I, _I, _P, _P, _I64, _I, _I64, _I64, _P, _I64, _P, _I64, _P, _SZ]),
+    "mk_verify_workspace": (_SZ, [_I, _I, _I]),
+    "mk_verify": (_I, [_P, _P, _I64, _I, _P, _I64, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ]),
+    "mk_verify_topk": (_I, [_P, _P, _P, _I, _I, _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P]),
     "mk_move_kv": (_I, [_P, _P, _I, _I, _I]),
     "mk_decode_plan_create": (_I, [_P, _P, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.POINTER(_P)]),
     "mk_decode_plan_destroy": (_I, [_P]),

@@ -26,10 +26,13 @@ HIP_SOURCES = [
     "csrc/kernels/quant.hip",
     "csrc/kernels/attn.hip",
     "csrc/kernels/attn_mma.hip",
+    "csrc/kernels/attn_prefix.hip",
     "csrc/kernels/decode.hip",
     "csrc/kernels/cut.hip",
+    "csrc/kernels/lora.hip",
     "csrc/kernels/rowpath.hip",
     "csrc/kernels/sample.hip",
+    "csrc/kernels/verify.hip",
     "csrc/kernels/capi.cpp",
     "csrc/host/gguf.cpp",
     "csrc/host/model.cpp",

@@ -50,6 +50,26 @@ int hip_fail(hipError_t e, const char* what) {
 
 }  // namespace mk
 
+namespace {
+// The context's device is the current one while this lives.
+class DeviceOf {
+ public:
+  explicit DeviceOf(const mk_ctx* c) {
+    mk::check(hipGetDevice(&was_), "hipGetDevice");
+    if (was_ == c->device) was_ = -1;
+    else mk::check(hipSetDevice(c->device), "hipSetDevice");
+  }
+  ~DeviceOf() {
+    if (was_ >= 0) (void)hipSetDevice(was_);
+  }
+  DeviceOf(const DeviceOf&) = delete;
+  DeviceOf& operator=(const DeviceOf&) = delete;
+
+ private:
+  int was_ = -1;
+};
+}  // namespace
+
 using mk::check;
 using mk::guard;
 using mk::require;
@@ -476,6 +496,82 @@ int mk_attention_decode(mk_ctx* c, const float* qkv, int64_t stride, int n, int 
   });
 }
 
+size_t mk_attention_prefix_workspace(int n, int n_head, int n_head_kv, int head_dim, int n_prefix, int max_keys) {
+  if (n <= 0 || n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv || head_dim <= 0 || n_prefix < 0 || max_keys < 0)
+    return 0;
+  return mk::attention_prefix_workspace(n, n_head, n_head_kv, head_dim, n_prefix, max_keys);
+}
+
+int mk_attention_prefix(mk_ctx* c, const float* q, int64_t q_stride, float* out, int64_t out_stride, int n, int n_head,
+                        const mk_kv_cache* prefix, int prefix_seq, int n_prefix, const mk_kv_cache* kv, int row0,
+                        int layer, const int32_t* seq, const int32_t* n_keys, int max_keys, void* xq, void* workspace,
+                        size_t workspace_bytes) {
+  return guard([&] {
+    require(n >= 0 && n_head > 0 && n_prefix >= 0 && row0 >= 0 && max_keys >= 0, "mk_attention_prefix: bad sizes");
+    if (n == 0) return;
+    const mk::KvLayer L = kv_layer(kv, layer);
+    const int KV = kv->n_head_kv, D = kv->head_dim;
+    require(KV > 0 && n_head % KV == 0, "mk_attention_prefix: bad head layout");
+    if ((D != 64 && D != 128) || n_head / KV > 32)
+      throw mk::Error(MK_ERR_UNSUPPORTED, "mk_attention_prefix: no kernel for this head layout");
+    require(q && out && seq && n_keys, "mk_attention_prefix: null array");
+    require(q_stride >= (int64_t)n_head * D && out_stride >= (int64_t)n_head * D,
+            "mk_attention_prefix: stride shorter than a row");
+    require((int64_t)n * n_head < (1 << 30), "mk_attention_prefix: too many rows");
+    require((int64_t)row0 + std::max(0, max_keys - n_prefix) <= kv->n_ctx,
+            "mk_attention_prefix: max_keys past the sequence's rows");
+    auto rows_ok = [](const mk_kv_cache* x) {
+      return x->k && x->v && x->k_scale && x->v_scale && (((uintptr_t)x->k | (uintptr_t)x->v) & 15) == 0;
+    };
+    require(rows_ok(kv), "mk_attention_prefix: cache rows null or not 16-byte aligned");
+    mk::PrefixAttn A{L, L, 0, kv->n_ctx, n, n_head, KV, kv->n_seq, n_prefix, row0, max_keys,
+                     1.0f / std::sqrt(static_cast<float>(D)), seq, n_keys};
+    if (n_prefix > 0) {
+      A.pre = kv_layer(prefix, layer);
+      require(prefix->n_head_kv == KV && prefix->head_dim == D, "mk_attention_prefix: the prefix has other heads");
+      require(prefix_seq >= 0 && prefix_seq < prefix->n_seq && n_prefix <= prefix->n_ctx,
+              "mk_attention_prefix: prefix outside its cache");
+      const size_t rows = (size_t)prefix_seq * KV * prefix->n_ctx;
+      require(rows_ok(prefix), "mk_attention_prefix: cache rows null or not 16-byte aligned");
+      A.pre = mk::KvLayer{A.pre.k + rows * D, A.pre.v + rows * D, A.pre.ks + rows, A.pre.vs + rows};
+      A.pre_ctx = prefix->n_ctx;
+    }
+    const size_t need = mk::attention_prefix_workspace(n, n_head, KV, D, n_prefix, max_keys);
+    require(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+            "mk_attention_prefix: workspace smaller than mk_attention_prefix_workspace, or not aligned");
+    require(c != nullptr, "mk_attention_prefix: null context");
+    const DeviceOf on(c);
+    mk::attention_prefix(c->stream, A, D, q, q_stride, out, out_stride, static_cast<mk::BlockQ8*>(xq), workspace);
+  });
+}
+
+size_t mk_lora_workspace(int n, int max_rank, int64_t cols) {
+  return n > 0 && max_rank > 0 && cols > 0 ? mk::lora_workspace(n, max_rank, cols) : 0;
+}
+
+int mk_lora(mk_ctx* c, int type, const mk_lora_adapter* adapters, int n_adapters, int max_rank, const int32_t* ids,
+            const float* x, int64_t x_stride, int n, int64_t rows, int64_t cols, const float* base, int64_t base_stride,
+            float* y, int64_t y_stride, void* workspace, size_t workspace_bytes) {
+  return guard([&] {
+    if (type != MK_F32 && type != MK_F16 && type != MK_BF16)
+      throw mk::Error(MK_ERR_UNSUPPORTED, "mk_lora: adapters are F32, F16 or BF16");
+    require(n >= 0 && n_adapters >= 0 && rows > 0 && cols > 0, "mk_lora: bad sizes");
+    require(max_rank >= 1 && max_rank <= 512, "mk_lora: max_rank outside 1..512");
+    require(rows <= (1 << 24) && cols <= (1 << 24), "mk_lora: matrix too large");
+    if (n == 0) return;
+    require(x && y && ids && (adapters || n_adapters == 0), "mk_lora: null array");
+    require(x_stride >= cols && y_stride >= rows && (!base || base_stride >= rows),
+            "mk_lora: stride shorter than a row");
+    require(base != y || base_stride == y_stride, "mk_lora: base and y share memory with other strides");
+    require(workspace && workspace_bytes >= mk::lora_workspace(n, max_rank, cols) && ((uintptr_t)workspace & 15) == 0,
+            "mk_lora: workspace smaller than mk_lora_workspace, or not aligned");
+    require(c != nullptr, "mk_lora: null context");
+    const DeviceOf on(c);
+    mk::lora(c->stream, type, adapters, n_adapters, max_rank, ids, x, x_stride, n, rows, cols, base, base_stride, y,
+             y_stride, workspace);
+  });
+}
+
 int mk_move_kv(mk_ctx* c, const mk_kv_cache* kv, int seq, int from, int to) {
   return guard([&] {
     require(kv && seq >= 0 && seq < kv->n_seq && from >= 0 && from < kv->n_ctx && to >= 0 && to < kv->n_ctx,
@@ -552,6 +648,57 @@ int mk_sample_draw(mk_ctx* c, const float* values, const int32_t* ids, int strid
     if (n_rows == 0) return;
     require(values && ids && params && states && out, "sample_draw: null array");
     mk::sample_draw(c->stream, values, ids, stride, n_rows, params, states, n_states, out, n_out);
+  });
+}
+
+size_t mk_verify_workspace(int n_lanes, int max_draft, int n_vocab) {
+  return n_lanes > 0 && max_draft >= 0 && n_vocab > 0 ? mk::verify_workspace(n_lanes, max_draft, n_vocab) : 0;
+}
+
+static void verify_args(int n_rows, int n_drafts, const void* lanes, int n_lanes, int max_draft, const void* drafts,
+                        const void* u, const void* u_next, const void* accepted, const void* tokens) {
+  require(n_rows >= 0 && n_drafts >= 0 && n_lanes >= 0, "mk_verify: bad sizes");
+  require(max_draft >= 0 && max_draft <= MK_VERIFY_MAX_DRAFT, "mk_verify: max_draft outside 0..256");
+  require((int64_t)n_lanes * (2 * max_draft + 1) < (1 << 30), "mk_verify: too many lanes");
+  require(n_lanes == 0 || (lanes && u_next && accepted && tokens && (n_drafts == 0 || (drafts && u))),
+          "mk_verify: null array");
+}
+
+int mk_verify(mk_ctx* c, const float* p, int64_t p_stride, int n_rows, const float* q, int64_t q_stride, int n_drafts,
+              int n_vocab, const mk_verify_lane* lanes, int n_lanes, int max_draft, const int32_t* drafts,
+              const double* u, const double* u_next, int32_t* accepted, int32_t* tokens, float* probs, void* workspace,
+              size_t workspace_bytes) {
+  return guard([&] {
+    verify_args(n_rows, n_drafts, lanes, n_lanes, max_draft, drafts, u, u_next, accepted, tokens);
+    require(n_vocab > 0 && n_vocab <= (1 << 27), "mk_verify: bad vocabulary");
+    require(p_stride >= n_vocab && (!q || q_stride >= n_vocab), "mk_verify: stride shorter than a row");
+    if (n_lanes == 0) return;
+    require(p || n_rows == 0, "mk_verify: null array");
+    require(workspace && workspace_bytes >= mk::verify_workspace(n_lanes, max_draft, n_vocab) &&
+                ((uintptr_t)workspace & 15) == 0,
+            "mk_verify: workspace smaller than mk_verify_workspace, or not aligned");
+    require(c != nullptr, "mk_verify: null context");
+    const DeviceOf on(c);
+    mk::verify(c->stream, p, p_stride, n_rows, q, q_stride, n_drafts, n_vocab, lanes, n_lanes, max_draft, drafts, u,
+               u_next, accepted, tokens, probs, workspace);
+  });
+}
+
+int mk_verify_topk(mk_ctx* c, const float* p_values, const int32_t* p_ids, int p_k, int n_rows, const float* q_values,
+                   const int32_t* q_ids, int q_k, int n_drafts, const mk_verify_lane* lanes, int n_lanes, int max_draft,
+                   const int32_t* drafts, const double* u, const double* u_next, int32_t* accepted, int32_t* tokens,
+                   float* probs) {
+  return guard([&] {
+    verify_args(n_rows, n_drafts, lanes, n_lanes, max_draft, drafts, u, u_next, accepted, tokens);
+    require(p_k >= 1 && p_k <= 1024 && (!q_values || (q_k >= 1 && q_k <= 1024)),
+            "mk_verify_topk: candidates outside 1..1024 (mk_topk's limit)");
+    require((q_values == nullptr) == (q_ids == nullptr), "mk_verify_topk: draft values without ids");
+    if (n_lanes == 0) return;
+    require((p_values && p_ids) || n_rows == 0, "mk_verify_topk: null array");
+    require(c != nullptr, "mk_verify_topk: null context");
+    const DeviceOf on(c);
+    mk::verify_topk(c->stream, p_values, p_ids, p_k, n_rows, q_values, q_ids, q_k, n_drafts, lanes, n_lanes, max_draft,
+                    drafts, u, u_next, accepted, tokens, probs);
   });
 }
 

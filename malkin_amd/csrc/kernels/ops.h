@@ -144,6 +144,21 @@ bool attention_mma_whole(int max_keys);  // a row's scores fit LDS (else they ar
 void attention_mma(hipStream_t s, const float* q, int64_t q_stride, float* out, int64_t out_stride, int n, int G, int KV,
                    float scale, const AttnAddr& a, const int32_t* seq, const int32_t* n_keys, int max_keys, BlockQ8* xq,
                    int64_t xq_stride, const int32_t* route);
+// Attention over a prefix shared by the batch and each sequence's own rows (attn_prefix.hip). Key j of token t, for
+// j < n_keys[t] (at most max_keys): row j of every head of `pre` (one sequence, heads pre_ctx rows apart) while
+// j < n_prefix, then row row0 + j - n_prefix of sequence seq[t] of `kv`. No keys, or a sequence outside the cache: zeros.
+struct PrefixAttn {
+  KvLayer pre, kv;
+  int64_t pre_ctx, n_ctx;
+  int n, H, KV, n_seq, n_prefix, row0, max_keys;
+  float scale;
+  const int32_t* seq;
+  const int32_t* n_keys;
+};
+size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int max_keys);
+void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q, int64_t q_stride, float* out,
+                      int64_t out_stride, BlockQ8* xq, void* workspace);
+
 // Scratch the attention of `pairs` (token, head) pairs over max_keys keys uses (0: none).
 size_t attention_scratch_bytes(int D, int max_keys, int pairs);
 
@@ -244,6 +259,22 @@ void sample_cut_tail(hipStream_t s, void* workspace, int n_rows, int n_vocab, in
 // One draw per top-k row from its std::mt19937_64 state (MK_MT64_WORDS words each, advanced in place).
 void sample_draw(hipStream_t s, const float* values, const int32_t* ids, int stride, int n_rows,
                  const mk_draw_params* params, uint64_t* states, int n_states, int32_t* out, int n_out);
+
+// Verification of drafted tokens (verify.hip): over whole rows of logits, and over rows cut to their top k.
+size_t verify_workspace(int n_lanes, int max_draft, int n_vocab);
+void verify(hipStream_t s, const float* p, int64_t p_stride, int n_rows, const float* q, int64_t q_stride, int n_drafts,
+            int n_vocab, const mk_verify_lane* lanes, int n_lanes, int max_draft, const int32_t* drafts, const double* u,
+            const double* u_next, int32_t* accepted, int32_t* tokens, float* probs, void* workspace);
+void verify_topk(hipStream_t s, const float* p_values, const int32_t* p_ids, int p_k, int n_rows, const float* q_values,
+                 const int32_t* q_ids, int q_k, int n_drafts, const mk_verify_lane* lanes, int n_lanes, int max_draft,
+                 const int32_t* drafts, const double* u, const double* u_next, int32_t* accepted, int32_t* tokens,
+                 float* probs);
+
+// y[t] = base[t] + scale B (A x[t]) with the adapter ids[t] (lora.hip).
+size_t lora_workspace(int n, int max_rank, int64_t cols);
+void lora(hipStream_t s, int type, const mk_lora_adapter* adapters, int n_adapters, int max_rank, const int32_t* ids,
+          const float* x, int64_t x_stride, int n, int64_t rows, int64_t cols, const float* base, int64_t base_stride,
+          float* y, int64_t y_stride, void* workspace);
 
 // dst[dst_idx[i]] = src[src_idx[i]], i < n; null index arrays are the identity, negative indices skip.
 void move_ids(hipStream_t s, int32_t* dst, const int32_t* dst_idx, const int32_t* src, const int32_t* src_idx,

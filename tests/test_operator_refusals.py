@@ -1,0 +1,149 @@
+"""Arguments that the shared-prefix attention, adapter and verification calls refuse, before anything touches a device
+(the context is the last thing they look at, so no GPU is needed), and the sizes that their workspaces report."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import malkin_amd as mk_
+
+X = 1 << 20  # a 16-byte aligned address that nothing reads
+
+
+def refused(rc, code, text):
+    assert rc == code, rc
+    assert text in mk_.load().mk_last_error().decode(), mk_.load().mk_last_error()
+
+
+def cache(**over):
+    f = dict(k=X, v=X, k_scale=X, v_scale=X, n_layer=2, n_seq=3, n_head_kv=2, head_dim=128, n_ctx=64)
+    f.update(over)
+    return mk_.MkKvCache(*(f[n] for n, _ in mk_.MkKvCache._fields_))
+
+
+def prefix_call(**over):
+    L = mk_.load()
+    a = dict(q=X, qs=512, out=X, os=512, n=5, H=4, pre=cache(), pseq=1, P=40, kv=cache(), row0=0, layer=1, seq=X,
+             keys=X, most=100, xq=None, ws=X, wsb=1 << 30)
+    a.update(over)
+    ref = [ctypes.byref(a[x]) if a[x] is not None else None for x in ("pre", "kv")]
+    return L.mk_attention_prefix(None, a["q"], a["qs"], a["out"], a["os"], a["n"], a["H"], ref[0], a["pseq"], a["P"],
+                                 ref[1], a["row0"], a["layer"], a["seq"], a["keys"], a["most"], a["xq"], a["ws"],
+                                 a["wsb"])
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(n=-1), "bad sizes"), (dict(H=0), "bad sizes"), (dict(P=-1), "bad sizes"), (dict(row0=-1), "bad sizes"),
+    (dict(most=-1), "bad sizes"), (dict(kv=None), "bad KV cache"), (dict(layer=2), "bad KV cache"),
+    (dict(layer=-1), "bad KV cache"), (dict(H=3), "bad head layout"), (dict(q=None), "null array"),
+    (dict(out=None), "null array"), (dict(seq=None), "null array"), (dict(keys=None), "null array"),
+    (dict(qs=511), "stride"), (dict(os=100), "stride"), (dict(most=105), "past the sequence's rows"),
+    (dict(row0=5), "past the sequence's rows"), (dict(n=1 << 29), "too many rows"),
+    (dict(kv=cache(k=X + 8)), "16-byte aligned"), (dict(kv=cache(v=0)), "16-byte aligned"),
+    (dict(kv=cache(v_scale=0)), "16-byte aligned"), (dict(pre=None), "bad KV cache"),
+    (dict(pre=cache(n_layer=1)), "bad KV cache"), (dict(pre=cache(n_head_kv=1)), "other heads"),
+    (dict(pre=cache(head_dim=64)), "other heads"), (dict(pseq=3), "outside its cache"),
+    (dict(pseq=-1), "outside its cache"), (dict(pre=cache(n_ctx=39)), "outside its cache"),
+    (dict(pre=cache(v=X + 4)), "16-byte aligned"), (dict(), "null context"),
+])
+def test_prefix_refusals(over, text):
+    refused(prefix_call(**over), mk_.MK_ERR_INVALID, text)
+
+
+def test_prefix_unsupported():
+    for kv in (cache(head_dim=96), cache(head_dim=32)):
+        refused(prefix_call(kv=kv, pre=kv), mk_.MK_ERR_UNSUPPORTED, "no kernel")
+    one = cache(n_head_kv=1)
+    refused(prefix_call(kv=one, pre=one, H=33, qs=33 * 128, os=33 * 128), mk_.MK_ERR_UNSUPPORTED, "no kernel")
+
+
+def test_prefix_workspace():
+    L = mk_.load()
+    need = L.mk_attention_prefix_workspace(5, 4, 2, 128, 40, 100)
+    if need:
+        refused(prefix_call(wsb=need - 1), mk_.MK_ERR_INVALID, "workspace")
+        refused(prefix_call(ws=X + 4), mk_.MK_ERR_INVALID, "workspace")
+        refused(prefix_call(ws=None), mk_.MK_ERR_INVALID, "workspace")
+    refused(prefix_call(wsb=need), mk_.MK_ERR_INVALID, "null context")
+    assert L.mk_attention_prefix_workspace(0, 4, 2, 128, 40, 100) == 0
+    assert L.mk_attention_prefix_workspace(5, 3, 2, 128, 40, 100) == 0
+    # No tokens: nothing to do, whatever the rest says.
+    assert prefix_call(n=0, kv=None) == mk_.MK_OK
+
+
+def lora_call(**over):
+    a = dict(type=mk_.F16, table=X, na=3, rank=16, ids=X, x=X, xs=256, n=4, rows=512, cols=256, base=X, bs=512, y=X + 64,
+             ys=512, ws=X, wsb=1 << 30)
+    a.update(over)
+    return mk_.load().mk_lora(None, *a.values())
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(n=-1), "bad sizes"), (dict(na=-1), "bad sizes"), (dict(rows=0), "bad sizes"), (dict(cols=0), "bad sizes"),
+    (dict(rank=0), "max_rank"), (dict(rank=513), "max_rank"), (dict(rows=1 << 25, ys=1 << 25, bs=1 << 25), "too large"),
+    (dict(x=None), "null array"), (dict(y=None), "null array"), (dict(ids=None), "null array"),
+    (dict(table=None), "null array"), (dict(xs=255), "stride"), (dict(ys=511), "stride"), (dict(bs=511), "stride"),
+    (dict(base=X, y=X, bs=520), "other strides"), (dict(ws=None), "workspace"), (dict(wsb=8), "workspace"),
+    (dict(ws=X + 8), "workspace"), (dict(), "null context"), (dict(base=None), "null context"),
+    (dict(table=None, na=0), "null context"),
+])
+def test_lora_refusals(over, text):
+    refused(lora_call(**over), mk_.MK_ERR_INVALID, text)
+
+
+def test_lora_types():
+    for t in (mk_.Q8_0, mk_.Q4_K, 5):
+        refused(lora_call(type=t), mk_.MK_ERR_UNSUPPORTED, "F32, F16 or BF16")
+    need = mk_.load().mk_lora_workspace(4, 16, 256)
+    refused(lora_call(wsb=need - 1), mk_.MK_ERR_INVALID, "workspace")
+    refused(lora_call(wsb=need), mk_.MK_ERR_INVALID, "null context")
+    assert lora_call(n=0, x=None) == mk_.MK_OK
+
+
+def verify_call(**over):
+    a = dict(p=X, ps=1000, rows=9, q=X, qs=1000, drafts=6, V=1000, lanes=X, nl=3, most=4, d=X, u=X, un=X, acc=X, tok=X,
+             pr=None, ws=X, wsb=1 << 30)
+    a.update(over)
+    return mk_.load().mk_verify(None, *a.values())
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(rows=-1), "bad sizes"), (dict(drafts=-1), "bad sizes"), (dict(nl=-1), "bad sizes"),
+    (dict(most=-1), "max_draft"), (dict(most=257), "max_draft"), (dict(nl=1 << 29, most=2), "too many lanes"),
+    (dict(lanes=None), "null array"), (dict(un=None), "null array"), (dict(acc=None), "null array"),
+    (dict(tok=None), "null array"), (dict(d=None), "null array"), (dict(u=None), "null array"),
+    (dict(p=None), "null array"), (dict(V=0), "bad vocabulary"), (dict(ps=999), "stride"), (dict(qs=999), "stride"),
+    (dict(ws=None), "workspace"), (dict(wsb=100), "workspace"), (dict(ws=X + 4), "workspace"),
+    (dict(), "null context"), (dict(q=None, qs=0), "null context"), (dict(drafts=0, d=None, u=None), "null context"),
+])
+def test_verify_refusals(over, text):
+    refused(verify_call(**over), mk_.MK_ERR_INVALID, text)
+
+
+def topk_call(**over):
+    a = dict(pv=X, pi=X, pk=40, rows=9, qv=X, qi=X, qk=40, drafts=6, lanes=X, nl=3, most=4, d=X, u=X, un=X, acc=X, tok=X,
+             pr=None)
+    a.update(over)
+    return mk_.load().mk_verify_topk(None, *a.values())
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(pk=0), "1..1024"), (dict(pk=1025), "1..1024"), (dict(qk=0), "1..1024"), (dict(qk=1025), "1..1024"),
+    (dict(qi=None), "without ids"), (dict(qv=None), "without ids"), (dict(pv=None), "null array"),
+    (dict(pi=None), "null array"), (dict(tok=None), "null array"), (dict(most=257), "max_draft"),
+    (dict(nl=-1), "bad sizes"), (dict(), "null context"), (dict(qv=None, qi=None, qk=0), "null context"),
+])
+def test_verify_topk_refusals(over, text):
+    refused(topk_call(**over), mk_.MK_ERR_INVALID, text)
+
+
+def test_empty_calls_and_tables():
+    L = mk_.load()
+    assert verify_call(nl=0, lanes=None, un=None, acc=None, tok=None) == mk_.MK_OK
+    assert topk_call(nl=0, lanes=None, un=None, acc=None, tok=None) == mk_.MK_OK
+    assert L.mk_verify_workspace(0, 4, 1000) == 0 and L.mk_verify_workspace(3, -1, 1000) == 0
+    assert L.mk_verify_workspace(3, 4, 1000) > 0
+    assert L.mk_lora_workspace(0, 16, 256) == 0
+    # The tables' Python layouts are the header's.
+    assert mk_.LORA_ADAPTER.itemsize == 24 and mk_.VERIFY_LANE.itemsize == 24
+    assert np.zeros(1, mk_.LORA_ADAPTER).dtype.fields["rank"][1] == 20
