@@ -1,67 +1,491 @@
 // Attention of a batch whose sequences share a prefix: key j < n_prefix of every token is row j of one sequence of the
-// prefix's cache, the others rows of the token's own sequence. Softmax statistics and sums are fp32.
+// prefix's cache, the others rows of the token's own sequence. out = sum_j p_j vs_j v_j, p = softmax(scale ks_j q.k_j).
+//
+// Rows and keys. A query row is a (token, query head); the rows of one KV head read the same prefix, so a workgroup takes
+// 32 of them (all tokens' heads in turn) over one chunk of the prefix's keys. A sequence's own keys are read by its own
+// tokens only: there a workgroup takes the rows of up to 32 / G neighbouring tokens of one sequence over one chunk of its
+// own rows. Both kinds are one launch (k_prefix_parts); each leaves a partial output with its softmax statistics, which
+// k_prefix_join adds.
+//
+// Arithmetic. An int8 key or value is exact in fp16, so the products run on v_mfma_f32_32x32x16_f16 with the fp32 side
+// split into two fp16 parts, hi = fp16(x) and lo = fp16(x - hi): the products keep 2^-23 of x at a quarter of the fp32
+// matrix instructions' time. A row of q is first brought to a largest value of 2^13 .. 2^14 by a power of two. The
+// softmax weights are shifted so that the largest p vs is about 2^6: a weight's lo part then lies within fp16 down to
+// 2^-17 of the largest, and what fp16 cannot hold of smaller ones is below 2^-30 of it. Scores, statistics and outputs
+// are fp32.
+//
+// S = K Q^T has the keys in its rows and the query rows in its columns: a lane's 16 scores belong to one query row, the
+// statistics are one register, and the weights are, as they lie, the second operand of O^T = V^T P^T. V^T comes from the
+// transposing LDS read. Each of a workgroup's four waves takes every fourth 32-key tile through a ring of its own, filled
+// by direct copies one tile ahead: no barrier until the waves' results are added.
 #include "ctx.h"
 #include "ops.h"
 
 namespace mk {
 namespace {
 
-// One wave per (token, query head), one key at a time.
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v2i lds_v2i;
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kRows = 32;        // query rows per workgroup
+constexpr int kKeys = 32;        // keys per tile
+constexpr float kNone = -3e38f;      // shift of a row that has seen no key
+constexpr float kLeast = 0x1p-100f;  // value scales below this count as this for the shift, so that sums of 2^-m stay finite
+constexpr float kLog2e = 1.44269504088896341f;
+
+// Chunks of the prefix's and of the own keys; a part's index is its prefix chunk, or np + its own chunk.
+struct Split {
+  int np, cp, no, co;
+  int tiles;      // row tiles of a KV head over the prefix
+  int64_t parts;  // rows of partial outputs
+};
+
+// Statistics of a row's part: its weights are 2^(score - base - m), l their sum. base is 0 but for rows of very large
+// scores; no key: kNone, kNone, 0.
+struct __align__(16) Sum {
+  float base, m, l, pad;
+  // The shift relative to another base, the largest of the parts'.
+  __device__ __forceinline__ float above(float b) const { return (base - b) + m; }
+};
+
 template <int D>
-__global__ __launch_bounds__(64) void k_prefix_attention(PrefixAttn A, const float* __restrict__ q, int64_t q_stride,
-                                                         float* __restrict__ out, int64_t out_stride,
-                                                         BlockQ8* __restrict__ xq) {
+struct Geo {
+  static constexpr int kSteps = D / 16;        // MFMAs' k steps over a row
+  static constexpr int kDt = D / 32;           // 32-value tiles of a row
+  static constexpr int kPieces = D / 16;       // 16-byte pieces of a row
+  static constexpr int kTileBytes = kKeys * D;
+  static constexpr int kCopies = kTileBytes / 1024;
+  static constexpr int kPer = 2 * kCopies + 1;             // copies per tile: K, V, both scales
+  static constexpr int kStage = 2 * kTileBytes + 8 * kKeys;
+  static constexpr int kShift = D == 128 ? 1 : 2;          // rows per 64 LDS banks, as a shift
+  static constexpr int kOutStride = D + 4;
+  static constexpr int kLds = kWaves * (2 * kStage > kRows * kOutStride * 4 ? 2 * kStage : kRows * kOutStride * 4);
+};
+
+// The piece of row `key` that lies in slot s, and the slot that holds piece s: rows whose LDS banks coincide hold their
+// pieces in different slots.
+template <int D>
+__device__ __forceinline__ int swizzle(int key, int s) {
+  return s ^ ((key >> Geo<D>::kShift) & (Geo<D>::kPieces - 1));
+}
+
+// Eight int8 as fp16, exactly: the byte x + 128 under the exponent of 1024 reads 1024 + 128 + x.
+__device__ __forceinline__ v8h cvt8(uint32_t a, uint32_t b) {
+  const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
+  a ^= 0x80808080u, b ^= 0x80808080u;
+  v2h r[4];
+  r[0] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) - off;
+  r[1] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) - off;
+  r[2] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - off;
+  r[3] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - off;
+  return v8h{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
+}
+
+// x as hi + lo.
+__device__ __forceinline__ void split8(const float (&x)[8], v8h& hi, v8h& lo) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const v2f f = {x[i], x[i + 1]};
+    const v2h h = __builtin_convertvector(f, v2h);
+    const v2f g = {x[i] - (float)h[0], x[i + 1] - (float)h[1]};
+    const v2h l = __builtin_convertvector(g, v2h);
+    hi[i] = h[0], hi[i + 1] = h[1], lo[i] = l[0], lo[i + 1] = l[1];
+  }
+}
+
+__device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Split S, const float* __restrict__ q,
+                                                              int64_t q_stride, bool q_vec, float* __restrict__ po,
+                                                              Sum* __restrict__ pml) {
+  using G_ = Geo<D>;
+  const int G = A.H / A.KV, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int li = lane & 31, h = lane >> 5;
+  const int n_pre = S.tiles * A.KV * S.np;
+  // Which rows, keys and cache: row r (0 .. rows - 1) is token t0 + r / G + .., see `token` and `head` below.
+  int part, g, first, rows, seq = 0, k0, k1;  // first: the first row among the KV head's rows t * G + i
+  const int8_t *kb, *vb;
+  const float *ksb, *vsb;
+  if ((int)blockIdx.x < n_pre) {
+    // Each XCD a contiguous run: the row tiles of one (KV head, chunk) read its keys into one L2.
+    const int it = xcd_run((int)blockIdx.x, n_pre), pair = it / S.tiles;
+    part = pair % S.np, g = pair / S.np;
+    first = it % S.tiles * kRows, rows = min(kRows, A.n * G - first);
+    k0 = part * S.cp, k1 = min(A.n_prefix, k0 + S.cp);
+    const int64_t row = (int64_t)g * A.pre_ctx;
+    kb = A.pre.k + row * D, vb = A.pre.v + row * D, ksb = A.pre.ks + row, vsb = A.pre.vs + row;
+  } else {
+    const int it = (int)blockIdx.x - n_pre, c = it % S.no, tg = it / S.no, t = tg / A.KV;
+    g = tg % A.KV, part = S.np + c;
+    // Token t leads the run of its sequence's tokens up to the next multiple of 32 / G; other tokens' workgroups leave.
+    const int tq = kRows / G;
+    seq = A.seq[t];
+    if (seq < 0 || seq >= A.n_seq || (t % tq && A.seq[t - 1] == seq)) return;
+    int m = 1;
+    while ((t + m) % tq && t + m < A.n && A.seq[t + m] == seq) ++m;
+    first = t * G, rows = m * G;
+    k0 = c * S.co, k1 = min(max(A.max_keys - A.n_prefix, 0), k0 + S.co);
+    const int64_t row = ((int64_t)seq * A.KV + g) * A.n_ctx + A.row0;
+    kb = A.kv.k + row * D, vb = A.kv.v + row * D, ksb = A.kv.ks + row, vsb = A.kv.vs + row;
+  }
+  const bool own = part >= S.np;
+  // This lane's query row: its token, head and keys (of this kind). Columns without a row, and rows without any key,
+  // whose results nobody reads, see every key.
+  const int r = first + min(li, rows - 1), t = r / G, head = g * G + r % G;
+  int lim = INT32_MAX, most = 0;
+  {
+    const int s = A.seq[t];
+    const int keys = s >= 0 && s < A.n_seq ? min(A.n_keys[t], A.max_keys) : 0;
+    const bool live = li < rows && keys > 0;
+    if (live) lim = own ? keys - A.n_prefix : keys;
+    most = live ? max(lim, 0) : 0;
+  }
+  int least = lim;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    most = max(most, __shfl_xor(most, o));
+    least = min(least, __shfl_xor(least, o));
+  }
+  k1 = min(k1, __builtin_amdgcn_readfirstlane(most));
+  least = min(__builtin_amdgcn_readfirstlane(least), k1);  // tiles up to here are whole for every row
+  if (k0 >= k1) return;
+  const int tiles = (k1 - k0 + kKeys - 1) / kKeys;
+
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t* ring = smem + w * (2 * G_::kStage);
+  auto issue = [&](int kt, int st) __attribute__((always_inline)) {
+    uint8_t* to = ring + st * G_::kStage;
+    const int base = k0 + kt * kKeys;
+#pragma unroll
+    for (int c = 0; c < G_::kCopies; ++c) {
+      const int at = c * 64 + lane, key = at / G_::kPieces;
+      const int64_t off = (int64_t)min(base + key, k1 - 1) * D + 16 * swizzle<D>(key, at % G_::kPieces);
+      lds_copy16(kb + off, to + 1024 * c);
+      lds_copy16(vb + off, to + G_::kTileBytes + 1024 * c);
+    }
+    lds_copy4((h ? vsb : ksb) + min(base + li, k1 - 1), to + 2 * G_::kTileBytes);
+  };
+  if (w < tiles) issue(w, 0);
+
+  // q of the lane's row in the order of its half of a K row's bytes: byte b of a row is element
+  // 16 (b % (D / 16)) + b / (D / 16); step j, value e of half h is byte D / 2 h + 8 j + e.
+  v8h qh[G_::kSteps], ql[G_::kSteps];
+  float rf;  // score, in bits, of one unit of a product
+  {
+    const float* qr = q + t * q_stride + head * D;
+    float x[G_::kSteps][8];
+    if constexpr (D == 128) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const float* at = qr + 16 * e + 8 * h + j;
+          const v4f v = q_vec ? *reinterpret_cast<const v4f*>(at) : v4f{at[0], at[1], at[2], at[3]};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j + i][e] = v[i];
+        }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const float* at = qr + 16 * e + 8 * h + j;
+          const v4f v = q_vec ? *reinterpret_cast<const v4f*>(at) : v4f{at[0], at[1], at[2], at[3]};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[(j + i) / 2][e + 4 * (i & 1)] = v[i];
+        }
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < G_::kSteps; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[j][e]));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    int ex = 0;
+    if (top > 0.0f && top < INFINITY) ex = min(14 - __builtin_amdgcn_frexp_expf(top), 100);
+    rf = __builtin_ldexpf(A.scale * kLog2e, -ex);
+#pragma unroll
+    for (int j = 0; j < G_::kSteps; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[j][e] = __builtin_ldexpf(x[j][e], ex);
+      split8(x[j], qh[j], ql[j]);
+    }
+  }
+
+  v16f o[G_::kDt];
+#pragma unroll
+  for (int i = 0; i < G_::kDt; ++i) o[i] = v16f{};
+  float m = kNone, l = 0.0f;  // shift and sum of this half's weights 2^(score - m)
+  bool fresh = true;
+  // Scores past 2^16 bits (`wide`): a shift's own rounding would count beside the 6 bits and the value scale in it. They
+  // are rounded to fp32 first (rg) and taken relative to `ms`, the row's largest when it left the range.
+  bool wide = false;
+  float rg = 1.0f, ms = 0.0f;
+
+  auto tile = [&](int kt, const uint8_t* at) __attribute__((always_inline)) {
+    const int base = k0 + kt * kKeys;
+    v16f s = {};
+#pragma unroll
+    for (int i = 0; i < G_::kSteps / 2; ++i) {
+      const v4u k = *reinterpret_cast<const v4u*>(at + li * D + 16 * swizzle<D>(li, h * (G_::kPieces / 2) + i));
+      const v8h a = cvt8(k[0], k[1]), b = cvt8(k[2], k[3]);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[2 * i], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[2 * i], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, qh[2 * i + 1], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ql[2 * i + 1], s, 0, 0, 0);
+    }
+    // Register i of a half is key 8 (i / 4) + 4 h + i % 4 of the tile.
+    const float* sc = reinterpret_cast<const float*>(at + 2 * G_::kTileBytes);
+    float vs[16], p[16], x[16];
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const v4f a = *reinterpret_cast<const v4f*>(sc + 2 * i + 4 * h);
+      const v4f b = *reinterpret_cast<const v4f*>(sc + kKeys + 2 * i + 4 * h);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[i + k] *= a[k], vs[i + k] = b[k];
+    }
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = s[i] * rg - ms;
+    }
+    if (base + kKeys > least) {  // some row ends in this tile: what it must not see has no weight and no value
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool in = base + 8 * (i / 4) + 4 * h + i % 4 < min(lim, k1);
+        s[i] = in ? s[i] : -INFINITY;
+        vs[i] = in ? vs[i] : 0.0f;
+      }
+    }
+    float sum, top;
+    auto weights = [&] __attribute__((always_inline)) {
+      sum = top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fma_(s[i], rf, -m));
+        x[i] = p[i] * vs[i];
+        sum += p[i];
+        top = fmaxf(top, x[i]);
+      }
+    };
+    if (!fresh) weights();
+    // The first tile, and one whose weights leave fp16 or whose sum nears fp32's end: a new shift.
+    if (fresh || __ballot(top > 32768.0f || !(sum < 0x1p114f))) {
+      auto shift = [&] __attribute__((always_inline)) {
+        float z = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z = fmaxf(z, fma_(s[i], rf, __builtin_amdgcn_logf(fmaxf(vs[i], kLeast))));
+        return fmaxf(m, fmaxf(z, __shfl_xor(z, 32)) - 6.0f);
+      };
+      float m1 = shift();
+      if (__ballot(fabsf(m1) > 65536.0f && m1 > kNone)) {
+        if (!wide) {
+          wide = true, rg = rf, rf = 1.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] *= rg;
+        }
+        float z = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z = fmaxf(z, s[i]);
+        z = fmaxf(z, __shfl_xor(z, 32));
+        if (z > 65536.0f || (m == kNone && z < -65536.0f && z > -INFINITY)) {
+          ms += z, m = m == kNone ? m : m - z;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] -= z;
+        }
+        m1 = shift();
+      }
+      const float f = __builtin_amdgcn_exp2f(m - m1);
+      m = m1, l *= f;
+      if (!fresh) {
+#pragma unroll
+        for (int i = 0; i < G_::kDt; ++i) o[i] *= f;
+      }
+      fresh = false;
+      weights();
+    }
+    l += sum;
+    v8h ph[2], pl[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = x[8 * u + e];
+      split8(y, ph[u], pl[u]);
+    }
+    // ds_read_b64_tr_b8: lane i of 16 reads 8 bytes, (row i / 2, half i % 2) of an 8 x 16 byte tile, and gets the
+    // tile's column i. Row e of step u is the key of weight 8 u + e.
+    const uint8_t* v = at + G_::kTileBytes;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int e = (lane & 15) >> 1, key = 16 * u + 8 * (e >> 2) + 4 * h + (e & 3);
+#pragma unroll
+      for (int i = 0; i < G_::kDt; ++i) {
+        const v2i b = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_v2i*)(v + key * D + 16 * swizzle<D>(key, 2 * i + ((lane >> 4) & 1)) + 8 * (lane & 1)));
+        const v8h a = cvt8((uint32_t)b[0], (uint32_t)b[1]);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[u], o[i], 0, 0, 0);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[u], o[i], 0, 0, 0);
+      }
+    }
+  };
+  int st = 0;
+  for (int kt = w; kt < tiles; kt += kWaves) {
+    fence();
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): reads of the stage refilled next are done
+    fence();
+    if (kt + kWaves < tiles) {
+      issue(kt + kWaves, st ^ 1);
+      wait_vm<G_::kPer>();
+    } else {
+      wait_vm<0>();
+    }
+    fence();
+    tile(kt, ring + st * G_::kStage);
+    st ^= 1;
+  }
+  l += __shfl_xor(l, 32);
+
+  // The waves' parts of each row, brought to their largest shift and added.
+  __shared__ Sum ml[kWaves][kRows];
+  __syncthreads();
+  float* ob = reinterpret_cast<float*>(smem);
+  if (h == 0) ml[w][li] = Sum{m == kNone ? kNone : ms, m, l, 0.0f};
+#pragma unroll
+  for (int i = 0; i < G_::kDt; ++i)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      *reinterpret_cast<v4f*>(ob + (w * kRows + li) * G_::kOutStride + 32 * i + 8 * a + 4 * h) =
+          v4f{o[i][4 * a], o[i][4 * a + 1], o[i][4 * a + 2], o[i][4 * a + 3]};
+  __syncthreads();
+  const int row = tid >> 3, x8 = tid & 7;
+  if (row >= rows) return;
+  float base = kNone, top = -INFINITY, f[kWaves], sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) base = fmaxf(base, ml[i][row].base);
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) top = fmaxf(top, f[i] = ml[i][row].above(base));
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    f[i] = __builtin_amdgcn_exp2f(f[i] - top);
+    sum = fma_(f[i], ml[i][row].l, sum);
+  }
+  const int rr = first + row;
+  const int64_t at = ((int64_t)part * A.n + rr / G) * A.H + g * G + rr % G;
+  if (x8 == 0) pml[at] = Sum{base, top, sum, 0.0f};
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const int d = 4 * (x8 + 8 * i);
+    v4f a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k)
+      a += f[k] * *reinterpret_cast<const v4f*>(ob + (k * kRows + row) * G_::kOutStride + d);
+    *reinterpret_cast<v4f*>(po + at * D + d) = a;
+  }
+}
+
+// One wave per query row: the parts that its keys reach, added.
+template <int D>
+__global__ __launch_bounds__(kThreads) void k_prefix_join(PrefixAttn A, Split S, const float* __restrict__ po,
+                                                          const Sum* __restrict__ pml, float* __restrict__ out,
+                                                          int64_t out_stride, BlockQ8* __restrict__ xq) {
   constexpr int E = D / 64;
-  const int t = blockIdx.x / A.H, h = blockIdx.x % A.H, g = h / (A.H / A.KV), lane = threadIdx.x;
-  const int seq = A.seq[t];
-  const int keys = seq >= 0 && seq < A.n_seq ? min(A.n_keys[t], A.max_keys) : 0;
-  // Byte b of a K row is element 16 (b % (D / 16)) + b / (D / 16).
-  float qv[E], o[E];
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= A.n * A.H) return;
+  const int t = row / A.H, head = row % A.H, seq = A.seq[t];
+  const int keys = seq >= 0 && seq < A.n_seq ? max(0, min(A.n_keys[t], A.max_keys)) : 0;
+  const int np = (min(keys, A.n_prefix) + S.cp - 1) / S.cp, no = (max(keys - A.n_prefix, 0) + S.co - 1) / S.co;
+  float v[E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int b = E * lane + i;
-    qv[i] = q[t * q_stride + h * D + 16 * (b % (D / 16)) + b / (D / 16)] * A.scale;
-    o[i] = 0.0f;
+  for (int i = 0; i < E; ++i) v[i] = 0.0f;
+  if (keys > 0) {
+    const int64_t step = (int64_t)A.n * A.H;
+    auto at = [&](int i) { return (i < np ? i : S.np + i - np) * step + row; };
+    Sum mine = {kNone, kNone, 0.0f, 0.0f};
+    if (lane < np + no) mine = pml[at(lane)];
+    float base = mine.base;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) base = fmaxf(base, __shfl_xor(base, o));
+    const float mm = mine.above(base);
+    float top = mm;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float f = __builtin_amdgcn_exp2f(mm - top);
+    float sum = f * mine.l;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+#pragma unroll 4
+    for (int i = 0; i < np + no; ++i) {
+      const float fi = __shfl(f, i);
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] = fma_(fi, po[at(i) * D + E * lane + k], v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) v[k] = v[k] / sum;
   }
-  float m = -INFINITY, l = 0.0f;
-  for (int j = 0; j < keys; ++j) {
-    const bool pre = j < A.n_prefix;
-    const int64_t row = pre ? (int64_t)g * A.pre_ctx + j
-                            : ((int64_t)seq * A.KV + g) * A.n_ctx + A.row0 + (j - A.n_prefix);
-    const KvLayer& L = pre ? A.pre : A.kv;
-    float s = 0.0f;
+  float* to = out + t * out_stride + head * D + E * lane;
 #pragma unroll
-    for (int i = 0; i < E; ++i) s = fma_(qv[i], (float)L.k[row * D + E * lane + i], s);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
-    s *= L.ks[row];
-    const float m1 = fmaxf(m, s), r = expf(m - m1), p = expf(s - m1), pv = p * L.vs[row];
-    l = fma_(l, r, p);
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = fma_(o[i], r, pv * (float)L.v[row * D + E * lane + i]);
-    m = m1;
-  }
-  float* row = out + t * out_stride + h * D;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    o[i] = keys > 0 ? o[i] / l : 0.0f;
-    row[E * lane + i] = o[i];
-  }
-  if (xq) quantize_block_lanes_n<E>(o, lane % (32 / E), xq + ((int64_t)t * A.H * D + h * D + E * lane) / 32);
+  for (int k = 0; k < E; ++k) to[k] = v[k];
+  if (xq) quantize_block_lanes_n<E>(v, lane % (32 / E), xq + ((int64_t)row * D + E * lane) / 32);
+}
+
+constexpr int kMaxPre = 48, kMaxOwn = 16;  // a row's parts fit one wave's lanes
+constexpr int kWanted = 512;               // workgroups: two per CU
+
+int chunk(int keys, int chunks) {  // keys per chunk, whole tiles for the four waves
+  const int c = (keys + chunks - 1) / chunks;
+  return std::max(1, (c + kWaves * kKeys - 1) / (kWaves * kKeys)) * kWaves * kKeys;
+}
+
+Split split_of(int n, int H, int KV, int n_prefix, int max_keys) {
+  Split s{};
+  const int G = H / KV;
+  s.tiles = (int)(((int64_t)n * G + kRows - 1) / kRows);
+  const int pre = std::min(n_prefix, max_keys), own = std::max(0, max_keys - n_prefix);
+  const int64_t pre_wgs = (int64_t)s.tiles * KV, own_wgs = (int64_t)n * KV;
+  s.cp = chunk(pre, (int)std::min<int64_t>(kMaxPre, std::max<int64_t>(1, kWanted / pre_wgs)));
+  s.np = (pre + s.cp - 1) / s.cp;
+  s.co = chunk(own, (int)std::min<int64_t>(kMaxOwn, std::max<int64_t>(1, kWanted / own_wgs)));
+  s.no = (own + s.co - 1) / s.co;
+  s.parts = (int64_t)(s.np + s.no) * n * H;
+  return s;
 }
 
 }  // namespace
 
-size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int max_keys) { return 0; }
+size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int max_keys) {
+  const Split s = split_of(n, H, KV, n_prefix, max_keys);
+  return (size_t)s.parts * (D * sizeof(float) + sizeof(Sum));
+}
 
 void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q, int64_t q_stride, float* out,
                       int64_t out_stride, BlockQ8* xq, void* workspace) {
-  const dim3 grid((unsigned)(A.n * A.H));
-  if (D == 128)
-    hipLaunchKernelGGL(k_prefix_attention<128>, grid, dim3(64), 0, s, A, q, q_stride, out, out_stride, xq);
-  else
-    hipLaunchKernelGGL(k_prefix_attention<64>, grid, dim3(64), 0, s, A, q, q_stride, out, out_stride, xq);
-  check_launch("attention_prefix");
+  const Split S = split_of(A.n, A.H, A.KV, A.n_prefix, A.max_keys);
+  float* po = static_cast<float*>(workspace);
+  Sum* pml = reinterpret_cast<Sum*>(po + S.parts * D);
+  const bool q_vec = ((uintptr_t)q & 15) == 0 && (q_stride & 3) == 0;
+  const int64_t wgs = (int64_t)S.tiles * A.KV * S.np + (int64_t)A.n * A.KV * S.no;
+  require(wgs < (1ll << 31), "mk_attention_prefix: too many rows");
+  auto go = [&]<int D_>() {
+    if (wgs > 0) {
+      allow_lds<k_prefix_parts<D_>>(Geo<D_>::kLds);
+      hipLaunchKernelGGL(k_prefix_parts<D_>, dim3((unsigned)wgs), dim3(kThreads), Geo<D_>::kLds, s, A, S, q, q_stride,
+                         q_vec, po, pml);
+      check_launch("attention_prefix parts");
+    }
+    hipLaunchKernelGGL(k_prefix_join<D_>, dim3((unsigned)(((int64_t)A.n * A.H + 3) / 4)), dim3(kThreads), 0, s, A, S, po,
+                       pml, out, out_stride, xq);
+    check_launch("attention_prefix join");
+  };
+  if (D == 128) go.template operator()<128>();
+  else go.template operator()<64>();
 }
 
 }  // namespace mk

@@ -24,7 +24,13 @@ def make_cache(rng, n_layer, n_seq, kv, n_ctx, d):
 def attention64(q, n_head, pre, pseq, n_prefix, kv, row0, layer, seq, keys):
     """Outputs [n][n_head * d] and their bounds. Every score is a sum of d products (and the scale's two), so it is off by
     at most (d + 8) EPS times the sum of their sizes A; exp turns that, and the rounding of s - m, into a relative error
-    of p; the sum over keys adds one rounding per key and side, the running maximum's rescaling another."""
+    of p; the sum over keys adds one rounding per key and side, the running maximum's rescaling another.
+
+    fp16 parts: x = hi + lo to half a step of lo, 2^-12 of 2^-11 of x, or 2^-25 where lo is subnormal. A row of q is
+    scaled to a largest value of at least 2^13, so the second adds at most 2^-38 of it to each of its values (to A as
+    2^-38 / EPS). The weights p vs are scaled so that the largest of a part was at least 2^6 when the shift was set (its
+    rounding aside: 2^5.9), scales below 2^-100 counting as that: a weight is off by at most 2^-30.9 of the largest,
+    times a value of at most 127."""
     k, v, ks, vs = kv
     n_seq, KV, d = k.shape[1], k.shape[2], k.shape[4]
     G, byte = n_head // KV, permuted(d)
@@ -36,21 +42,23 @@ def attention64(q, n_head, pre, pseq, n_prefix, kv, row0, layer, seq, keys):
             continue
         a, b = min(m, n_prefix), max(0, m - n_prefix)
         for g in range(KV):
-            K, V = [], []
+            K, V, S = [], [], []
             for (ck, cv, cks, cvs), i, lo, c in ((pre or kv, pseq, 0, a), (kv, seq[t], row0, b)):
                 if c:
                     at = (layer, i, g, slice(lo, lo + c))
                     K.append(ck[at][:, byte].astype(np.float64) * cks[at].astype(np.float64)[:, None])
                     V.append(cv[at].astype(np.float64) * cvs[at].astype(np.float64)[:, None])
-            K, V = np.concatenate(K), np.concatenate(V)
+                    S.append(cvs[at].astype(np.float64))
+            S, K, V = np.concatenate(S), np.concatenate(K), np.concatenate(V)
             for h in range(g * G, (g + 1) * G):
                 x = q[t, h * d:(h + 1) * d].astype(np.float64)
-                s, A = K @ x / np.sqrt(d), np.abs(K) @ np.abs(x) / np.sqrt(d)
+                s, A = K @ x / np.sqrt(d), np.abs(K) @ (np.abs(x) + 2.0 ** -14 * np.abs(x).max()) / np.sqrt(d)
                 p = np.exp(s - s.max())
                 p /= p.sum()
                 out[t, h] = p @ V
                 rel = 2 * ((d + 8) * A.max() + 2 * (s.max() - s.min()) + 16) + 4 * m
-                tol[t, h] = EPS * rel * (p @ np.abs(V))
+                W = (p * np.maximum(S, 2.0 ** -100)).max()
+                tol[t, h] = EPS * rel * (p @ np.abs(V)) + m * 127 * 2.0 ** -30.9 * W
     return out.reshape(len(seq), -1), tol.reshape(len(seq), -1)
 
 
