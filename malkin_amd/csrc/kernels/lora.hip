@@ -4,9 +4,11 @@
 //
 // Two launches: k_shrink makes h = A x for every token, the columns split over workgroups (partial sums in the
 // workspace, added in a fixed order by the next launch), k_expand adds scale B h to base. Both take the tokens of an
-// aligned 16-token tile that share an adapter together, as the 16 columns of v_mfma_f32_16x16x4_f32 (weights as its 16
-// rows): the workgroup of a token runs if the token is the first of its tile with its adapter and leaves at once
-// otherwise, so a tile costs one pass over each adapter that occurs in it.
+// aligned 64-token window that share an adapter together, as the 16 columns of up to four v_mfma_f32_16x16x4_f32
+// (weights as its 16 rows, so that a lane ends with four consecutive ranks or rows of one token): an adapter's weights
+// are read once per window that it occurs in.
+#include <type_traits>
+
 #include "ctx.h"
 #include "ops.h"
 
@@ -14,11 +16,13 @@ namespace mk {
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 16;      // tokens of a tile
-constexpr int kThreads = 256;  // 4 waves
-constexpr int kRowBlock = 256; // rows of y per k_expand workgroup, 64 per wave
+constexpr int kWindow = 64;     // tokens that are grouped by adapter
+constexpr int kShrinkWaves = 8;
+constexpr int kThreads = 256;   // of k_expand: 4 waves
+constexpr int kRowBlock = 256;  // rows of y per k_expand workgroup, 64 per wave
+constexpr int kStep = 32;       // columns per wave and step of k_shrink: 8 per lane
+constexpr int kFewSlots = 16;
 
 struct F16 { uint16_t v; };
 struct BF16 { uint16_t v; };
@@ -26,176 +30,306 @@ __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(F16 v) { return (float)__builtin_bit_cast(_Float16, v.v); }
 __device__ __forceinline__ float to_f(BF16 v) { return __builtin_bit_cast(float, (uint32_t)v.v << 16); }
 
-// Four consecutive values, from an address aligned to their size.
-__device__ __forceinline__ void load4(const float* p, float (&r)[4]) {
-  const float4 v = *reinterpret_cast<const float4*>(p);
-  r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
-}
-__device__ __forceinline__ void load4(const F16* p, float (&r)[4]) {
-  const v4h v = *reinterpret_cast<const v4h*>(p);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = (float)v[i];
-}
-__device__ __forceinline__ void load4(const BF16* p, float (&r)[4]) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-  r[0] = __builtin_bit_cast(float, v.x << 16), r[1] = __builtin_bit_cast(float, v.x & 0xFFFF0000u);
-  r[2] = __builtin_bit_cast(float, v.y << 16), r[3] = __builtin_bit_cast(float, v.y & 0xFFFF0000u);
+// The table's pointers are to global memory, which the compiler cannot know.
+template <typename T>
+using global = const __attribute__((address_space(1))) T;
+template <typename T>
+__device__ __forceinline__ global<T>* to_global(const void* p) {
+  return (global<T>*)(uintptr_t)p;
 }
 
-// What a workgroup does with token t's tile: the adapter (-1: none), its entry, and the tile's tokens that take it
-// (0: another token's workgroup covers t).
+// N values (4 or 8) from p on, the first `valid` of them (the others 0): vec: p is aligned to 16 bytes or to N values, and
+// valid is 0 or N. p[0] can always be read.
+template <int N>
+__device__ __forceinline__ void get(global<float>* p, int valid, bool vec, float (&r)[N]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const v4f v = *reinterpret_cast<global<v4f>*>(p + (valid ? i : 0));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[i + k] = v[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = p[i < valid ? i : 0];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = i < valid ? r[i] : 0.0f;
+}
+template <int N, typename T>
+__device__ __forceinline__ void get(global<T>* p, int valid, bool vec, float (&r)[N]) {
+  typedef uint32_t words __attribute__((ext_vector_type(N / 2)));
+  global<uint16_t>* q = reinterpret_cast<global<uint16_t>*>(p);
+  words v;
+  if (vec) {
+    v = *reinterpret_cast<global<words>*>(q);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      v[i] = (uint32_t)q[2 * i < valid ? 2 * i : 0] | (uint32_t)q[2 * i + 1 < valid ? 2 * i + 1 : 0] << 16;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = i < valid ? to_f(T{(uint16_t)(v[i / 2] >> (16 * (i & 1)))}) : 0.0f;
+}
+__device__ __forceinline__ int within(int64_t left, int n) { return left <= 0 ? 0 : left < n ? (int)left : n; }
+
+// What a workgroup does: tokens[0 .. count - 1] (in LDS) of a window, their adapter (rank 0: none). Count 0: nothing.
 struct Group {
-  int id, t0;
-  uint32_t tokens;
+  int count;
   mk_lora_adapter a;
 };
-__device__ __forceinline__ Group group_of(int t, int n, const int32_t* ids, const mk_lora_adapter* adapters,
-                                          int n_adapters, int max_rank) {
+
+// Slot j of a window is its j-th distinct adapter, in the order of their first tokens, where there are few slots (few
+// adapters in the table); with kWindow slots it is the group that token j is the first of. Slots are the grid's slow
+// dimension: workgroups are dealt to the XCDs and their shader engines in turn, and slots that a window does not have,
+// recurring at a fixed distance, would leave whole engines without work (3 adapters, 512 tokens: 87 us instead of 30).
+__device__ __forceinline__ Group group_of(int window, int j, int slots, int n, const int32_t* ids,
+                                          const mk_lora_adapter* adapters, int n_adapters, int max_rank, int* tokens) {
+  const int lane = threadIdx.x & 63, t0 = window * kWindow, u = t0 + lane;
+  const int got = u < n ? ids[u] : -1;
+  const int v = got >= 0 && got < n_adapters ? got : -1;
+  uint64_t left = __ballot(u < n), mask = 0;
   Group g;
-  g.t0 = t & ~(kTile - 1);
   g.a = mk_lora_adapter{nullptr, nullptr, 0.0f, 0};
-  const int u = g.t0 + (threadIdx.x & 15);
-  const int mine = u < n ? ids[u] : -1;
-  const int v = mine >= 0 && mine < n_adapters ? mine : -1;
-  const int own = __shfl(v, t - g.t0, 16);
-  g.tokens = (uint32_t)__ballot(u < n && v == own) & 0xFFFFu;
-  if (g.tokens & ((1u << (t - g.t0)) - 1)) g.tokens = 0;
-  g.id = __builtin_amdgcn_readfirstlane(own);
-  if (g.id >= 0) {
-    g.a = adapters[g.id];
+  g.count = 0;
+  int own = -1;
+  if (slots == kWindow) {
+    if (!((left >> j) & 1)) return g;
+    own = __builtin_amdgcn_readlane(v, j);
+    mask = __ballot(v == own) & left;
+    if (mask & ((1ull << j) - 1)) return g;
+  } else {
+    for (int i = 0; i <= j; ++i) {
+      if (!left) return g;
+      own = __builtin_amdgcn_readlane(v, __builtin_ctzll(left));
+      mask = __ballot(v == own) & left;
+      left &= ~mask;
+    }
+  }
+  if (own >= 0) {
+    g.a = adapters[own];
     if (g.a.rank < 1 || g.a.rank > max_rank || !g.a.a || !g.a.b) g.a.rank = 0;
   }
+  g.count = __popcll(mask);
+  if ((mask >> lane) & 1) tokens[__popcll(mask & ((1ull << lane) - 1))] = u;  // every wave the same
+  __syncthreads();
   return g;
 }
 
-// Partial sums h[split][t][r] of columns split * per .. over ranks 16 blockIdx.z ..: MFMA rows are ranks, columns
-// tokens; a lane holds eight consecutive columns of its rank row and of its token, one per MFMA.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_shrink(const mk_lora_adapter* __restrict__ adapters, int n_adapters,
-                                                     int max_rank, const int32_t* __restrict__ ids,
-                                                     const float* __restrict__ x, int64_t x_stride, int n, int64_t cols,
-                                                     int per, bool x_vec, float* __restrict__ h, int r_pad) {
-  const int t = blockIdx.x;
-  const Group g = group_of(t, n, ids, adapters, n_adapters, max_rank);
-  const int r0 = 16 * blockIdx.z;
-  if (!g.tokens || r0 >= g.a.rank) return;
+// Partial sums h[split][t][r] over columns split * per .. of ranks r0 .. r0 + 31. A lane holds eight consecutive columns
+// of two rank rows and of a token in each of NT tiles, one per MFMA.
+template <typename T, int NT>
+__device__ void shrink(const Group& g, const int* tokens, const float* __restrict__ x, int64_t x_stride, int64_t cols,
+                       int r0, int64_t k0, int64_t k1, bool x_vec, float* __restrict__ h, int r_pad,
+                       v4f (*part)[8][64]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, li = lane & 15, lq = lane >> 4;
-  const T* a = static_cast<const T*>(g.a.a) + (int64_t)min(r0 + li, g.a.rank - 1) * cols;
-  const float* xr = x + (int64_t)min(g.t0 + li, n - 1) * x_stride;
-  const bool row_on = r0 + li < g.a.rank, tok_on = (g.tokens >> li) & 1;
-  const bool vec = x_vec && (cols & 7) == 0 && ((uintptr_t)g.a.a & 15) == 0;
-  const int64_t k0 = (int64_t)blockIdx.y * per, k1 = min(cols, k0 + per);
-  v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t k = k0 + 32 * w; k < k1; k += 32 * 4) {
-    const int64_t at = k + 8 * lq;
-    float av[8], xv[8];
-    if (vec) {
-      const bool in = at < k1;  // per and cols are multiples of 8
-      float q[4];
+  const bool vec = x_vec && (cols & 7) == 0 && ((uintptr_t)g.a.a & 15) == 0;  // columns come in eights
+  const int tiles = (g.count + 15) / 16;
+  global<float>* xr[NT];
+  int on[NT];  // all ones: the column is a token
 #pragma unroll
-      for (int u = 0; u < 8; u += 4) {
-        load4(a + (in ? at + u : 0), q);
+  for (int i = 0; i < NT; ++i) {
+    on[i] = 16 * i + li < g.count ? -1 : 0;
+    xr[i] = to_global<float>(x + tokens[min(16 * i + li, g.count - 1)] * x_stride);
+  }
+  const bool two = r0 + 16 < g.a.rank;
+  global<T>* a[2];
+  int row_on[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) av[u + i] = row_on && in ? q[i] : 0.0f;
-        load4(xr + (in ? at + u : 0), q);
+  for (int i = 0; i < 2; ++i) {
+    row_on[i] = r0 + 16 * i + li < g.a.rank ? -1 : 0;
+    a[i] = to_global<T>(g.a.a) + (int64_t)min(r0 + 16 * i + li, g.a.rank - 1) * cols;
+  }
+  v4f acc[2][NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xv[u + i] = tok_on && in ? q[i] : 0.0f;
-      }
-    } else {
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = at + i < k1;
-        av[i] = row_on && in ? to_f(a[at + i]) : 0.0f;
-        xv[i] = tok_on && in ? xr[at + i] : 0.0f;
+    for (int k = 0; k < NT; ++k) acc[i][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  auto walk = [&](auto vec_) __attribute__((always_inline)) {
+    constexpr bool V = decltype(vec_)::value;
+#pragma unroll(V ? 2 : 1)
+    for (int64_t k = k0 + kStep * w; k < k1; k += kStep * kShrinkWaves) {
+      const int valid = within(k1 - k - 8 * lq, 8);
+      const int64_t at = valid ? k + 8 * lq : k0;
+      float av[2][8], xv[NT][8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) get<8>(a[i] + at, valid & row_on[i], V, av[i]);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) get<8>(xr[i] + at, valid & on[i], V, xv[i]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j && !two) break;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          if (i >= tiles) break;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[j][e], xv[i][e], acc[j][i], 0, 0, 0);
+        }
       }
     }
+  };
+  if (vec) walk(std::true_type{});
+  else walk(std::false_type{});
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(av[i], xv[i], acc, 0, 0, 0);
-  }
-  __shared__ v4f part[4][64];
-  part[w][lane] = acc;
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int k = 0; k < NT; ++k) part[w][i * NT + k][lane] = acc[i][k];
   __syncthreads();
-  if (w == 0 && tok_on) {
-    const v4f s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
-    *reinterpret_cast<v4f*>(h + ((int64_t)blockIdx.y * n + g.t0 + li) * r_pad + r0 + 4 * lq) = s;
+  // The waves' sums, a wave per (rank tile, token tile) in turn.
+#pragma unroll 1
+  for (int j = w; j < 2 * NT; j += kShrinkWaves) {
+    const int i = j / NT, k = j % NT, c = 16 * k + li;
+    if (c < g.count && (i == 0 || two))
+      *reinterpret_cast<v4f*>(h + (int64_t)tokens[c] * r_pad + r0 + 16 * i + 4 * lq) =
+          ((part[0][j][lane] + part[1][j][lane]) + (part[2][j][lane] + part[3][j][lane])) +
+          ((part[4][j][lane] + part[5][j][lane]) + (part[6][j][lane] + part[7][j][lane]));
   }
 }
 
-// y = base + scale B h for 256 rows: MFMA rows are rows of B, columns tokens, so a lane ends with four consecutive
-// rows of one token.
+template <typename T>
+__global__ __launch_bounds__(64 * kShrinkWaves) void k_shrink(const mk_lora_adapter* __restrict__ adapters, int n_adapters,
+                                                     int max_rank, const int32_t* __restrict__ ids, int windows,
+                                                     int slots,
+                                                     const float* __restrict__ x, int64_t x_stride, int n, int64_t cols,
+                                                     int64_t per, bool x_vec, float* __restrict__ h, int r_pad) {
+  __shared__ int tokens[kWindow];
+  __shared__ v4f part[kShrinkWaves][8][64];
+  const Group g = group_of(blockIdx.x % windows, blockIdx.y, slots, n, ids, adapters, n_adapters, max_rank, tokens);
+  const int r0 = 32 * blockIdx.z, split = blockIdx.x / windows;
+  if (!g.count || r0 >= g.a.rank) return;
+  const int64_t k0 = split * per, k1 = min(cols, k0 + per);
+  h += (int64_t)split * n * r_pad;
+  if (g.count <= 16) shrink<T, 1>(g, tokens, x, x_stride, cols, r0, k0, k1, x_vec, h, r_pad, part);
+  else shrink<T, 4>(g, tokens, x, x_stride, cols, r0, k0, k1, x_vec, h, r_pad, part);
+}
+
+// y = base + scale B h. A wave takes 64 rows of B in four MFMA tiles, and the group's tokens 16 at a time; the products go
+// through LDS, so that base is read and y written 256 bytes of a token at a time. The code is kept short (rolled loops):
+// a workgroup runs most of it once, and instruction fetches that miss would cost more than the arithmetic.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __restrict__ adapters, int n_adapters,
-                                                     int max_rank, const int32_t* __restrict__ ids, int n, int64_t rows,
-                                                     const float* __restrict__ h, int r_pad, int splits,
+                                                     int max_rank, const int32_t* __restrict__ ids, int windows,
+                                                     int slots, int n,
+                                                     int64_t rows, const float* __restrict__ h, int r_pad, int splits,
                                                      const float* base, int64_t base_stride, float* y, int64_t y_stride,
                                                      bool y_vec) {
-  const int t = blockIdx.x;
-  const Group g = group_of(t, n, ids, adapters, n_adapters, max_rank);
-  if (!g.tokens) return;
+  constexpr int kOut = 64 + 4;  // a token's stride in `out`
+  __shared__ int tokens[kWindow];
+  __shared__ __align__(16) float out_s[4][16 * kOut];
+  extern __shared__ __align__(16) float hs[];  // [16 or 64][r_pad + 4]: the group's h, scaled
+  const Group g = group_of(blockIdx.x % windows, blockIdx.y, slots, n, ids, adapters, n_adapters, max_rank, tokens);
   const int rank = g.a.rank;
-  if (rank == 0 && base == y) return;
-  extern __shared__ __align__(16) float hs[];  // [16][r_pad + 4]: the tile's h, scaled
-  const int hst = r_pad + 4;
-  const int rank16 = (rank + 15) & ~15;
-  for (int i = threadIdx.x; i < kTile * rank16; i += kThreads) {
-    const int tok = i / rank16, r = i % rank16;
-    float s = 0.0f;
-    if (((g.tokens >> tok) & 1) && r < rank)
-      for (int p = 0; p < splits; ++p) s += h[((int64_t)p * n + g.t0 + tok) * r_pad + r];
-    hs[tok * hst + r] = s * g.a.scale;
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, li = lane & 15, lq = lane >> 4;
+  if (!g.count || (!rank && base == y)) return;
+  const int hst = r_pad + 4, w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
+  const int64_t row0 = (int64_t)(blockIdx.x / windows) * kRowBlock + 64 * w, row = row0 + 4 * li;
+  const int valid = within(rows - row, 4), tiles = (g.count + 15) / 16;
   const bool b_vec = (rank & 3) == 0 && ((uintptr_t)g.a.b & (4 * sizeof(T) - 1)) == 0;
-  const bool tok_on = (g.tokens >> li) & 1;
-  for (int tile = 0; tile < 4; ++tile) {
-    const int64_t row0 = (int64_t)blockIdx.y * kRowBlock + 64 * w + 16 * tile;
-    if (row0 >= rows) break;
-    const T* b = static_cast<const T*>(g.a.b) + min(row0 + li, rows - 1) * rank;
-    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int r = 0; r < rank; r += 16) {
-      const int at = r + 4 * lq;
-      float bv[4];
-      if (b_vec) {
-        load4(b + min(at, rank - 4), bv);
-        if (at >= rank) bv[0] = bv[1] = bv[2] = bv[3] = 0.0f;
+  // What does not wait for h is asked for first: the base (lane: token 4 k + lq of a tile, four rows from 4 li) ..
+  v4f v[4][4];
+  int tok[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= tiles) break;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = 16 * j + 4 * k + lq;
+      tok[j][k] = c < g.count ? tokens[c] : -1;
+      float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (base && valid && tok[j][k] >= 0)
+        get<4>(to_global<float>(base + tok[j][k] * base_stride + row), valid, y_vec, q);
+      v[j][k] = v4f{q[0], q[1], q[2], q[3]};
+    }
+  }
+  // .. and the first 16 ranks of B.
+  global<T>* b[4];
+  float bv[4][4];
+  auto load_b = [&](int r) __attribute__((always_inline)) {
+    const int at = r + 4 * lq, in = within(rank - at, 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) get<4>(b[i] + (in ? at : 0), in, b_vec, bv[i]);
+  };
+  if (rank) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      b[i] = to_global<T>(g.a.b) + min(row0 + 16 * i + li, rows - 1) * rank;
+    load_b(0);
+    // h: its partial sums in order, four ranks a thread; where a group has few, 2^f threads take every 2^f-th split and
+    // are added across lanes.
+    const int quads = (rank + 15) / 16 * 4, used = g.count * quads, items = tiles * 16 * quads;
+    int f = 0;
+    while (f < 4 && (used << (f + 1)) <= kThreads) ++f;
+    const int part = threadIdx.x & ((1 << f) - 1);
+#pragma unroll 1
+    for (int i0 = 0; i0 < items; i0 += kThreads >> f) {
+      const int i = i0 + (threadIdx.x >> f), c = i / quads, r = 4 * (i - c * quads);
+      v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (i < used) {
+        const float* at = h + (int64_t)tokens[c] * r_pad + r;
+        const int64_t step = (int64_t)n * r_pad;
+#pragma unroll 8
+        for (int p = part; p < splits; p += 1 << f) s += *reinterpret_cast<const v4f*>(at + p * step);
+      }
+#pragma unroll 1
+      for (int m = 1; m < 1 << f; m <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] += __shfl_xor(s[k], m);
+      if (i < items && part == 0) *reinterpret_cast<v4f*>(hs + c * hst + r) = s * g.a.scale;
+    }
+    __syncthreads();
+  }
+  if (row0 >= rows) return;
+  float* out = out_s[w];
+  v4f acc[4][4];  // [token tile][row tile]
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int r = 0; r < rank; r += 16) {
+    if (r) load_b(r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= tiles) break;
+      const v4f hv = *reinterpret_cast<const v4f*>(hs + (16 * j + li) * hst + r + 4 * lq);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[i][k], hv[k], acc[j][i], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= tiles) break;
+    if (rank) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<v4f*>(out + li * kOut + 16 * i + 4 * lq) = acc[j][i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wave's LDS accesses happen in order
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[j][k] += *reinterpret_cast<const v4f*>(out + (4 * k + lq) * kOut + 4 * li);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (tok[j][k] < 0) continue;
+      float* to = y + tok[j][k] * y_stride + row;
+      if (y_vec) {
+        if (valid) *reinterpret_cast<v4f*>(to) = v[j][k];
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bv[i] = at + i < rank ? to_f(b[at + i]) : 0.0f;
+        for (int e = 0; e < 4; ++e)
+          if (e < valid) to[e] = v[j][k][e];
       }
-      const float4 hv = *reinterpret_cast<const float4*>(hs + li * hst + at);
-      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[0], hv.x, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[1], hv.y, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[2], hv.z, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[3], hv.w, acc, 0, 0, 0);
-    }
-    if (!tok_on) continue;
-    const int64_t row = row0 + 4 * lq;
-    const float* bp = base ? base + (g.t0 + li) * base_stride + row : nullptr;
-    float* yp = y + (g.t0 + li) * y_stride + row;
-    if (y_vec) {
-      if (row >= rows) continue;
-      v4f v = bp ? *reinterpret_cast<const v4f*>(bp) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
-      if (rank) v += acc;
-      *reinterpret_cast<v4f*>(yp) = v;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (row + i < rows) {
-          float v = bp ? bp[i] : 0.0f;
-          if (rank) v += acc[i];
-          yp[i] = v;
-        }
     }
   }
 }
 
 int rank_pad(int max_rank) { return (max_rank + 15) & ~15; }
 
-// Column splits of the first product: enough workgroups for the CUs twice over, of at least 256 columns each.
+// Column splits of the first product, of at least two steps of every wave each.
 int splits_of(int n, int64_t cols) {
-  const int tiles = (n + kTile - 1) / kTile;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({16, (512 + tiles - 1) / tiles, cols / 256}));
+  const int windows = (n + kWindow - 1) / kWindow;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({16, (256 + windows - 1) / windows, cols / (2 * kStep * kShrinkWaves)}));
 }
 
 bool aligned16(const void* p, int64_t stride) { return ((uintptr_t)p & 15) == 0 && (stride & 3) == 0; }
@@ -210,18 +344,26 @@ void lora(hipStream_t s, int type, const mk_lora_adapter* adapters, int n_adapte
           const float* x, int64_t x_stride, int n, int64_t rows, int64_t cols, const float* base, int64_t base_stride,
           float* y, int64_t y_stride, void* workspace) {
   const int splits = splits_of(n, cols), r_pad = rank_pad(max_rank);
-  const int per = (int)(((cols + splits - 1) / splits + 31) / 32 * 32);
+  const int64_t step = kStep * kShrinkWaves, per = ((cols + splits - 1) / splits + step - 1) / step * step;
   const bool x_vec = aligned16(x, x_stride);
   const bool y_vec = (rows & 3) == 0 && aligned16(y, y_stride) && (!base || aligned16(base, base_stride));
   float* h = static_cast<float*>(workspace);
-  const dim3 g1(n, splits, r_pad / 16), g2(n, (unsigned)((rows + kRowBlock - 1) / kRowBlock));
-  const size_t lds = (size_t)kTile * (r_pad + 4) * sizeof(float);
+  const int slots = n_adapters + 1 < kFewSlots ? n_adapters + 1 : kWindow;
+  const int windows = (n + kWindow - 1) / kWindow;
+  const int64_t blocks = (rows + kRowBlock - 1) / kRowBlock;
+  require(windows * std::max<int64_t>(blocks, splits) < (1ll << 31), "mk_lora: too many tokens");
+  const unsigned used = std::min(slots, n);
+  const dim3 g1((unsigned)(windows * splits), used, (r_pad + 31) / 32), g2((unsigned)(windows * blocks), used);
+  const size_t lds = (size_t)(n <= 16 ? 16 : kWindow) * (r_pad + 4) * sizeof(float);
   auto go = [&]<typename T>() {
-    hipLaunchKernelGGL(k_shrink<T>, g1, dim3(kThreads), 0, s, adapters, n_adapters, max_rank, ids, x, x_stride, n,
-                       cols, per, x_vec, h, r_pad);
-    check_launch("lora shrink");
-    hipLaunchKernelGGL(k_expand<T>, g2, dim3(kThreads), lds, s, adapters, n_adapters, max_rank, ids, n, rows, h, r_pad,
-                       splits, base, base_stride, y, y_stride, y_vec);
+    if (n_adapters > 0) {
+      hipLaunchKernelGGL(k_shrink<T>, g1, dim3(64 * kShrinkWaves), 0, s, adapters, n_adapters, max_rank, ids, windows, slots, x, x_stride,
+                         n, cols, per, x_vec, h, r_pad);
+      check_launch("lora shrink");
+    }
+    allow_lds<k_expand<T>>(kWindow * (512 + 4) * sizeof(float));
+    hipLaunchKernelGGL(k_expand<T>, g2, dim3(kThreads), lds, s, adapters, n_adapters, max_rank, ids, windows, slots, n, rows, h,
+                       r_pad, splits, base, base_stride, y, y_stride, y_vec);
     check_launch("lora expand");
   };
   if (type == MK_F32) go.template operator()<float>();
