@@ -71,6 +71,49 @@ __device__ __forceinline__ void get(global<T>* p, int valid, bool vec, float (&r
 #pragma unroll
   for (int i = 0; i < N; ++i) r[i] = i < valid ? to_f(T{(uint16_t)(v[i / 2] >> (16 * (i & 1)))}) : 0.0f;
 }
+// Values at .. at + 3 of a row of `rank`, as they lie in memory; 0 past its end.
+template <typename T>
+struct Raw {
+  typedef uint2 type;
+};
+template <>
+struct Raw<float> {
+  typedef v4f type;
+};
+__device__ __forceinline__ v4f get_raw(global<float>* row, int at, int rank, bool vec) {
+  float r[4];
+  get<4>(row + (at < rank ? at : 0), max(min(rank - at, 4), 0), vec, r);
+  return v4f{r[0], r[1], r[2], r[3]};
+}
+template <typename T>
+__device__ __forceinline__ uint2 get_raw(global<T>* row, int at, int rank, bool vec) {
+  typedef uint32_t two __attribute__((ext_vector_type(2)));
+  global<uint16_t>* q = reinterpret_cast<global<uint16_t>*>(row);
+  two v;
+  if (vec) {
+    v = *reinterpret_cast<global<two>*>(q + (at < rank ? at : 0));
+    if (at >= rank) v = two{0, 0};
+  } else {
+    uint32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      e[i] = q[at + i < rank ? at + i : 0];
+      e[i] = at + i < rank ? e[i] : 0;
+    }
+    v = two{e[0] | e[1] << 16, e[2] | e[3] << 16};
+  }
+  return make_uint2(v[0], v[1]);
+}
+template <typename T>
+__device__ __forceinline__ void from_raw(const v4f& v, float (&r)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = v[i];
+}
+template <typename T>
+__device__ __forceinline__ void from_raw(const uint2& v, float (&r)[4]) {
+  r[0] = to_f(T{(uint16_t)v.x}), r[1] = to_f(T{(uint16_t)(v.x >> 16)});
+  r[2] = to_f(T{(uint16_t)v.y}), r[3] = to_f(T{(uint16_t)(v.y >> 16)});
+}
 __device__ __forceinline__ int within(int64_t left, int n) { return left <= 0 ? 0 : left < n ? (int)left : n; }
 
 // What a workgroup does: tokens[0 .. count - 1] (in LDS) of a window, their adapter (rank 0: none). Count 0: nothing.
@@ -223,40 +266,43 @@ __global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __re
   if (!g.count || (!rank && base == y)) return;
   const int hst = r_pad + 4, w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
   const int64_t row0 = (int64_t)(blockIdx.x / windows) * kRowBlock + 64 * w, row = row0 + 4 * li;
-  const int valid = within(rows - row, 4), tiles = (g.count + 15) / 16;
+  const int valid = within(rows - row, 4);
   const bool b_vec = (rank & 3) == 0 && ((uintptr_t)g.a.b & (4 * sizeof(T) - 1)) == 0;
-  // What does not wait for h is asked for first: the base (lane: token 4 k + lq of a tile, four rows from 4 li) ..
-  v4f v[4][4];
-  int tok[4][4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j >= tiles) break;
+  // A tile of tokens: its base (lane: token 4 k + lq, four rows from 4 li).
+  auto load_base = [&](int c0, v4f(&v)[4], int(&tok)[4]) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int c = 16 * j + 4 * k + lq;
-      tok[j][k] = c < g.count ? tokens[c] : -1;
+      const int c = c0 + 4 * k + lq;
+      tok[k] = c < g.count ? tokens[c] : -1;
       float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (base && valid && tok[j][k] >= 0)
-        get<4>(to_global<float>(base + tok[j][k] * base_stride + row), valid, y_vec, q);
-      v[j][k] = v4f{q[0], q[1], q[2], q[3]};
+      if (base && valid && tok[k] >= 0) get<4>(to_global<float>(base + tok[k] * base_stride + row), valid, y_vec, q);
+      v[k] = v4f{q[0], q[1], q[2], q[3]};
     }
-  }
-  // .. and the first 16 ranks of B.
-  global<T>* b[4];
-  float bv[4][4];
-  auto load_b = [&](int r) __attribute__((always_inline)) {
-    const int at = r + 4 * lq, in = within(rank - at, 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) get<4>(b[i] + (in ? at : 0), in, b_vec, bv[i]);
   };
+  // 64 ranks of the wave's rows of B, four of a row per lane and step, as they lie in memory.
+  typedef typename Raw<T>::type raw;
+  raw bw[4][4];
+  global<T>* b[4];
+  auto load_b = [&](int r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (r + 16 * s >= rank) break;
+      const int at = r + 16 * s + 4 * lq;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bw[s][i] = get_raw(b[i], at, rank, b_vec);
+    }
+  };
+  // What does not wait for h is asked for first.
+  v4f now[4], later[4];
+  int tok[4], tok1[4];
+  load_base(0, now, tok);
   if (rank) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      b[i] = to_global<T>(g.a.b) + min(row0 + 16 * i + li, rows - 1) * rank;
+    for (int i = 0; i < 4; ++i) b[i] = to_global<T>(g.a.b) + min(row0 + 16 * i + li, rows - 1) * rank;
     load_b(0);
     // h: its partial sums in order, four ranks a thread; where a group has few, 2^f threads take every 2^f-th split and
     // are added across lanes.
-    const int quads = (rank + 15) / 16 * 4, used = g.count * quads, items = tiles * 16 * quads;
+    const int quads = (rank + 15) / 16 * 4, used = g.count * quads, items = (g.count + 15) / 16 * 16 * quads;
     int f = 0;
     while (f < 4 && (used << (f + 1)) <= kThreads) ++f;
     const int part = threadIdx.x & ((1 << f) - 1);
@@ -280,47 +326,50 @@ __global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __re
   }
   if (row0 >= rows) return;
   float* out = out_s[w];
-  v4f acc[4][4];  // [token tile][row tile]
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-  for (int r = 0; r < rank; r += 16) {
-    if (r) load_b(r);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j >= tiles) break;
-      const v4f hv = *reinterpret_cast<const v4f*>(hs + (16 * j + li) * hst + r + 4 * lq);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[i][k], hv[k], acc[j][i], 0, 0, 0);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j >= tiles) break;
+  for (int c0 = 0; c0 < g.count; c0 += 16) {
+    if (c0 + 16 < g.count) load_base(c0 + 16, later, tok1);
     if (rank) {
+      v4f acc[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<v4f*>(out + li * kOut + 16 * i + 4 * lq) = acc[j][i];
+      for (int i = 0; i < 4; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+      for (int r = 0; r < rank; r += 64) {
+        if (r || (c0 && rank > 64)) load_b(r);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if (r + 16 * s >= rank) break;
+          const v4f hv = *reinterpret_cast<const v4f*>(hs + (c0 + li) * hst + r + 16 * s + 4 * lq);
+          float bv[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) from_raw<T>(bw[s][i], bv[i]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[i][k], hv[k], acc[i], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<v4f*>(out + li * kOut + 16 * i + 4 * lq) = acc[i];
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wave's LDS accesses happen in order
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[j][k] += *reinterpret_cast<const v4f*>(out + (4 * k + lq) * kOut + 4 * li);
+      for (int k = 0; k < 4; ++k) now[k] += *reinterpret_cast<const v4f*>(out + (4 * k + lq) * kOut + 4 * li);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (tok[j][k] < 0) continue;
-      float* to = y + tok[j][k] * y_stride + row;
+      if (tok[k] < 0) continue;
+      float* to = y + tok[k] * y_stride + row;
       if (y_vec) {
-        if (valid) *reinterpret_cast<v4f*>(to) = v[j][k];
+        if (valid) *reinterpret_cast<v4f*>(to) = now[k];
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (e < valid) to[e] = v[j][k][e];
+          if (e < valid) to[e] = now[k][e];
       }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) now[k] = later[k], tok[k] = tok1[k];
   }
 }
 
