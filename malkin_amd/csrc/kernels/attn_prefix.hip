@@ -123,10 +123,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Spli
     const int64_t row = (int64_t)g * A.pre_ctx;
     kb = A.pre.k + row * D, vb = A.pre.v + row * D, ksb = A.pre.ks + row, vsb = A.pre.vs + row;
   } else {
-    const int it = (int)blockIdx.x - n_pre, c = it % S.no, tg = it / S.no, t = tg / A.KV;
-    g = tg % A.KV, part = S.np + c;
-    // Token t leads the run of its sequence's tokens up to the next multiple of 32 / G; other tokens' workgroups leave.
-    const int tq = kRows / G;
+    // Token t leads the run of its sequence's tokens up to the next multiple of 32 / G; other tokens' workgroups leave, as
+    // do those of chunks past a sequence's end. Both are the slow dimensions (first the tokens at those multiples, then
+    // the ones after them): workgroups are dealt to XCDs and their shader engines in turn, and idle ones at a fixed
+    // distance would leave whole engines without work.
+    const int tq = kRows / G, blocks = (A.n + tq - 1) / tq, per = blocks * A.KV;
+    const int it = (int)blockIdx.x - n_pre, c = it / per % S.no, t = it % per / A.KV * tq + it / per / S.no;
+    g = it % A.KV, part = S.np + c;
+    if (t >= A.n) return;
     seq = A.seq[t];
     if (seq < 0 || seq >= A.n_seq || (t % tq && A.seq[t - 1] == seq)) return;
     int m = 1;
@@ -471,7 +475,8 @@ void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q,
   float* po = static_cast<float*>(workspace);
   Sum* pml = reinterpret_cast<Sum*>(po + S.parts * D);
   const bool q_vec = ((uintptr_t)q & 15) == 0 && (q_stride & 3) == 0;
-  const int64_t wgs = (int64_t)S.tiles * A.KV * S.np + (int64_t)A.n * A.KV * S.no;
+  const int tq = kRows / (A.H / A.KV);
+  const int64_t wgs = (int64_t)S.tiles * A.KV * S.np + (int64_t)(A.n + tq - 1) / tq * tq * A.KV * S.no;
   require(wgs < (1ll << 31), "mk_attention_prefix: too many rows");
   auto go = [&]<int D_>() {
     if (wgs > 0) {
