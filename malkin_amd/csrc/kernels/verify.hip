@@ -7,8 +7,8 @@
 // 150 thousand tokens, whose steps are as small as the rounding of 32-bit sums: in 32 bits about one draw in a hundred
 // would land on a neighbouring token. Three launches: k_rows reads every row once, in segments of 4096 logits (their
 // maximum, its first place, and the sum of exp((z - max) / T)); k_excess makes each lane's decisions from those (every
-// workgroup of a lane for itself: a few hundred numbers) and sums the excess of its segment of the row that the next
-// token comes from; k_pick finds the segment and the token.
+// workgroup of a lane for itself: a few hundred numbers) and sums the excess over 1024 tokens at a time of the row that
+// the next token comes from; k_pick finds the block and the token.
 #include <cfloat>
 
 #include "ctx.h"
@@ -18,9 +18,12 @@ namespace mk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;               // logits per thread
-constexpr int kSeg = kThreads * kPer;  // logits per segment
+constexpr int kQuads = 4;                     // logits per thread, in fours
+constexpr int kBlock = 64 * 4 * kQuads;       // logits per wave, contiguous
+constexpr int kSeg = kThreads / 64 * kBlock;  // logits per segment
 constexpr int kMaxDraft = MK_VERIFY_MAX_DRAFT;
+
+typedef float v4f __attribute__((ext_vector_type(4)));
 
 struct Stat {  // a segment of a row, or a row
   double sum;  // of exp((z - max) / T); T <= 0: unused
@@ -36,29 +39,73 @@ struct Choice {  // of a lane
 };
 
 // NaN counts as -inf, +inf as the largest float.
-__device__ __forceinline__ float clean(float z) { return z != z ? -INFINITY : fminf(z, FLT_MAX); }
+__device__ __forceinline__ float clean(float z) { return fminf(fmaxf(z, -INFINITY), FLT_MAX); }
 
-__device__ __forceinline__ double weight(float z, float max, double inv_t) {
-  return z == -INFINITY ? 0.0 : exp(((double)z - (double)max) * inv_t);
+// 2^t for t <= about 1000: t = n + f, |f| <= 1/2, and the series of e^(f ln 2) to f^11, whose remainder is below
+// (ln 2 / 2)^12 / 12! = 7e-15 of it. Below 2^-1074 (-inf included) it is 0.
+__device__ __forceinline__ double pow2(double t) {
+  t = fmax(t, -1100.0);
+  const double n = __builtin_rint(t), f = t - n;
+  constexpr double c[12] = {1.0,
+                            6.931471805599453094e-1,
+                            2.402265069591007123e-1,
+                            5.550410866482157995e-2,
+                            9.618129107628477232e-3,
+                            1.333355814642844343e-3,
+                            1.540353039338160996e-4,
+                            1.525273380405984028e-5,
+                            1.321548679014430949e-6,
+                            1.017808600923969973e-7,
+                            7.054911620801123330e-9,
+                            4.445538271870811498e-10};
+  double p = c[11];
+#pragma unroll
+  for (int i = 10; i >= 0; --i) p = __builtin_fma(p, f, c[i]);
+  return __builtin_amdgcn_ldexp(p, (int)n);
 }
 
-// The larger maximum, at its first place; sums brought to it.
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, double inv_t) {
-  if (a.at < 0) return b;
-  if (b.at < 0) return a;
-  Stat r;
-  r.max = fmaxf(a.max, b.max);
-  r.at = a.max == b.max ? min(a.at, b.at) : a.max > b.max ? a.at : b.at;
-  r.sum = inv_t > 0.0 ? a.sum * weight(a.max, r.max, inv_t) + b.sum * weight(b.max, r.max, inv_t) : 0.0;
-  return r;
+// Logits to powers of two: log2(e) / T; 0 where T <= 0.
+__device__ __forceinline__ double per_unit(const mk_verify_lane& l) {
+  return l.temperature > 0.0f ? 1.4426950408889634074 / (double)l.temperature : 0.0;
 }
-__device__ __forceinline__ Stat shfl_xor(const Stat& s, int m) {
-  return Stat{__shfl_xor(s.sum, m), __shfl_xor(s.max, m), __shfl_xor(s.at, m)};
+__device__ __forceinline__ double weight(float z, float max, double c) {
+  return pow2(((double)z - (double)fmaxf(max, -FLT_MAX)) * c);
 }
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
   return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+// A value per lane (none: at -1), joined over the wave: the maximum, its first place, the sums brought to it.
+__device__ __forceinline__ Stat wave_join(Stat s, double c) {
+  Stat r;
+  r.max = wave_max(s.at < 0 ? -INFINITY : s.max);
+  int at = s.at >= 0 && s.max == r.max ? s.at : INT32_MAX;
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) at = min(at, __shfl_xor(at, m));
+  r.at = at == INT32_MAX ? -1 : at;
+  r.sum = c > 0.0 ? wave_sum(s.at < 0 ? 0.0 : s.sum * weight(s.max, r.max, c)) : 0.0;
+  return r;
+}
+// The same of a row's segments, by one wave.
+__device__ __forceinline__ Stat row_stat(const Stat* s, int segs, double c) {
+  const int lane = threadIdx.x & 63;
+  const Stat none{0.0, -INFINITY, -1};
+  Stat a = wave_join(lane < segs ? s[lane] : none, c);
+  for (int i = 64; i < segs; i += 64) {  // lane 63 carries the earlier ones
+    const Stat b = i + lane < segs && lane < 63 ? s[i + lane] : none;
+    a = wave_join(lane == 63 ? a : b, c);
+    if (i + 63 < segs) {
+      const Stat last = s[i + 63];
+      a = wave_join(lane == 0 ? a : lane == 1 ? last : none, c);
+    }
+  }
+  return a;
 }
 
 struct Rows {
@@ -68,6 +115,7 @@ struct Rows {
   const float* q;  // NULL: every draft is certain
   int64_t q_stride;
   int n_drafts, V;
+  bool vec;
 };
 
 // A lane whose parameters do not fit the call is left out: accepted -1, tokens -1.
@@ -76,12 +124,28 @@ __device__ __forceinline__ bool lane_ok(const mk_verify_lane& l, int max_draft, 
          l.first <= n_drafts - l.n_draft;
 }
 
-// Thread i's logits i, i + 256, .. of a segment (past the row: -inf).
-__device__ __forceinline__ void load_segment(const float* row, int seg, int V, float (&z)[kPer]) {
+// Logit of place i (quad, value) of this thread in a segment.
+__device__ __forceinline__ int place(int seg, int quad, int e) {
+  return seg * kSeg + (threadIdx.x >> 6) * kBlock + quad * 256 + (threadIdx.x & 63) * 4 + e;
+}
+// A segment's logits, a wave's 1024 contiguous (past the row: -inf). vec: rows are 16-byte aligned, V a multiple of 4.
+__device__ __forceinline__ void load_segment(const float* row, int seg, int V, bool vec, float (&z)[kQuads][4]) {
+  if (vec) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int at = seg * kSeg + i * kThreads + (int)threadIdx.x;
-    z[i] = at < V ? clean(row[at]) : -INFINITY;
+    for (int i = 0; i < kQuads; ++i) {
+      const int at = place(seg, i, 0);
+      const v4f v = *reinterpret_cast<const v4f*>(row + (at < V ? at : 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[i][e] = at < V ? clean(v[e]) : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = place(seg, i, e);
+        z[i][e] = at < V ? clean(row[at]) : -INFINITY;
+      }
   }
 }
 
@@ -95,50 +159,55 @@ __global__ __launch_bounds__(kThreads) void k_rows(Rows R, const mk_verify_lane*
   const int jj = draft ? j - max_draft - 1 : j;
   if (draft ? (jj >= L.n_draft || !R.q) : jj > L.n_draft) return;
   const float* row = draft ? R.q + (int64_t)(L.first + jj) * R.q_stride : R.p + (int64_t)(L.row + jj) * R.p_stride;
-  float z[kPer];
-  load_segment(row, seg, R.V, z);
-  float m = z[0];
+  float z[kQuads][4];
+  load_segment(row, seg, R.V, R.vec, z);
+  float m = -INFINITY;
 #pragma unroll
-  for (int i = 1; i < kPer; ++i) m = fmaxf(m, z[i]);
+  for (int i = 0; i < kQuads; ++i)
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  __shared__ float ms[4];
-  __shared__ double ss[4];
-  __shared__ int as[4];
-  const int w = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) ms[w] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-  const double inv_t = L.temperature > 0.0f ? 1.0 / (double)L.temperature : 0.0;
+    for (int e = 0; e < 4; ++e) m = fmaxf(m, z[i][e]);
+  m = wave_max(m);  // each wave against its own maximum: no barrier before the end
+  const double c = per_unit(L);
   double sum = 0.0;
-  int at = INT32_MAX;
+  int at = m == -INFINITY ? -1 : 0;
+  if (c > 0.0) {
+    if (at == 0) {
+      const double md = (double)m;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (z[i] == m) at = min(at, seg * kSeg + i * kThreads + (int)threadIdx.x);
-    if (inv_t > 0.0) sum += weight(z[i], m, inv_t);
+      for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += pow2(((double)z[i][e] - md) * c);
+    }
+    sum = wave_sum(sum);
+  } else if (at == 0) {
+    at = INT32_MAX;
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) at = z[i][e] == m ? min(at, place(seg, i, e)) : at;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
   }
-  sum = wave_sum(sum);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
-  if ((threadIdx.x & 63) == 0) ss[w] = sum, as[w] = at;
+  __shared__ Stat ws[kThreads / 64];
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) ws[threadIdx.x >> 6] = Stat{sum, m, at};
   __syncthreads();
-  if (threadIdx.x == 0)
-    stats[(int64_t)blockIdx.x * gridDim.y + seg] =
-        Stat{(ss[0] + ss[1]) + (ss[2] + ss[3]), m,
-             m == -INFINITY ? -1 : min(min(as[0], as[1]), min(as[2], as[3]))};
+  if (threadIdx.x >= 64) return;
+  const Stat s = wave_join(lane < kThreads / 64 ? ws[lane] : Stat{0.0, -INFINITY, -1}, c);
+  if (lane == 0) stats[(int64_t)blockIdx.x * gridDim.y + seg] = s;
 }
 
 // P(x) of a row from its statistics.
-__device__ __forceinline__ double prob(const Stat& s, float z, int x, double inv_t) {
+__device__ __forceinline__ double prob(const Stat& s, float z, int x, double c) {
   if (s.at < 0) return 0.0;
-  return inv_t > 0.0 ? weight(z, s.max, inv_t) / s.sum : x == s.at ? 1.0 : 0.0;
+  return c > 0.0 ? weight(z, s.max, c) / s.sum : x == s.at ? 1.0 : 0.0;
 }
 
 // What of token x the next token is drawn by.
-__device__ __forceinline__ double excess(const Choice& c, float zp, float zq, bool has_q, int x, double inv_t) {
-  const double p = prob(c.p, zp, x, inv_t);
+__device__ __forceinline__ double excess(const Choice& c, float zp, float zq, bool has_q, int x, double unit) {
+  const double p = prob(c.p, zp, x, unit);
   if (!c.refused) return p;
-  const double q = has_q ? prob(c.q, zq, x, inv_t) : x == c.draft ? 1.0 : 0.0;
+  const double q = has_q ? prob(c.q, zq, x, unit) : x == c.draft ? 1.0 : 0.0;
   return fmax(p - q, 0.0);
 }
 
@@ -162,19 +231,14 @@ __global__ __launch_bounds__(kThreads) void k_excess(Rows R, const mk_verify_lan
     }
     return;
   }
-  const double inv_t = L.temperature > 0.0f ? 1.0 / (double)L.temperature : 0.0;
+  const double unit = per_unit(L);
   __shared__ Stat row_s[2 * kMaxDraft + 1];
   __shared__ int stop_s;
   if (threadIdx.x == 0) stop_s = L.n_draft;
-  // Rows of the lane in turn over the waves: their segments joined.
   const int rows = L.n_draft + 1 + (R.q ? L.n_draft : 0);
-  for (int r = w; r < rows; r += 4) {
+  for (int r = w; r < rows; r += kThreads / 64) {
     const int j = r <= L.n_draft ? r : max_draft + r - L.n_draft;
-    const Stat* s = stats + ((int64_t)li * per + j) * segs;
-    Stat a{0.0, -INFINITY, -1};
-    for (int i = lane; i < segs; i += 64) a = join(a, s[i], inv_t);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = join(a, shfl_xor(a, o), inv_t);
+    const Stat a = row_stat(stats + ((int64_t)li * per + j) * segs, segs, unit);
     if (lane == 0) row_s[r] = a;
   }
   __syncthreads();
@@ -182,8 +246,8 @@ __global__ __launch_bounds__(kThreads) void k_excess(Rows R, const mk_verify_lan
     const int d = drafts[L.first + j];
     double p = 0.0, q = 1.0;
     if (d >= 0 && d < R.V) {
-      p = prob(row_s[j], clean(R.p[(int64_t)(L.row + j) * R.p_stride + d]), d, inv_t);
-      if (R.q) q = prob(row_s[L.n_draft + 1 + j], clean(R.q[(int64_t)(L.first + j) * R.q_stride + d]), d, inv_t);
+      p = prob(row_s[j], clean(R.p[(int64_t)(L.row + j) * R.p_stride + d]), d, unit);
+      if (R.q) q = prob(row_s[L.n_draft + 1 + j], clean(R.q[(int64_t)(L.first + j) * R.q_stride + d]), d, unit);
     }
     if (!(q > 0.0 && u[L.first + j] * q < p)) atomicMin(&stop_s, j);
     if (seg == 0 && pr) pr[j] = (float)p;  // past the refusal cleared below
@@ -206,114 +270,145 @@ __global__ __launch_bounds__(kThreads) void k_excess(Rows R, const mk_verify_lan
     }
   }
   const bool both = c.refused && R.q;
-  float zp[kPer], zq[kPer];
-  load_segment(R.p + (int64_t)(L.row + c.n_acc) * R.p_stride, seg, R.V, zp);
-  if (both) load_segment(R.q + (int64_t)(L.first + c.n_acc) * R.q_stride, seg, R.V, zq);
+  float zp[kQuads][4], zq[kQuads][4];
+  load_segment(R.p + (int64_t)(L.row + c.n_acc) * R.p_stride, seg, R.V, R.vec, zp);
+  if (both) load_segment(R.q + (int64_t)(L.first + c.n_acc) * R.q_stride, seg, R.V, R.vec, zq);
   double sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int x = seg * kSeg + i * kThreads + (int)threadIdx.x;
-    if (x < R.V) sum += excess(c, zp[i], both ? zq[i] : 0.0f, R.q != nullptr, x, inv_t);
-  }
+  for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int x = place(seg, i, e);
+      if (x < R.V) sum += excess(c, zp[i][e], both ? zq[i][e] : 0.0f, R.q != nullptr, x, unit);
+    }
   sum = wave_sum(sum);
-  __shared__ double ss[4];
-  if (lane == 0) ss[w] = sum;
+  if (lane == 0) sums[((int64_t)li * segs + seg) * (kThreads / 64) + w] = sum;
+}
+
+// The inclusive running sum over the workgroup's threads, and in `total` that of all.
+__device__ __forceinline__ double block_scan(double v, double* wave_s, double& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double t = __shfl_up(v, o);
+    if (lane >= o) v += t;
+  }
+  __syncthreads();  // the last scan's sums have been read
+  if (lane == 63) wave_s[w] = v;
   __syncthreads();
-  if (threadIdx.x == 0) sums[(int64_t)li * segs + seg] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+  total = 0.0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    if (i == w) v += total;
+    total += wave_s[i];
+  }
+  return v;
 }
 
 // The first token in order whose running sum reaches v times the total; one workgroup per lane.
 __global__ __launch_bounds__(kThreads) void k_pick(Rows R, const mk_verify_lane* __restrict__ lanes, int max_draft,
                                                    const double* __restrict__ u_next,
                                                    const Choice* __restrict__ choices, const double* __restrict__ sums,
-                                                   int segs, int32_t* __restrict__ tokens, float* __restrict__ probs) {
-  const int li = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+                                                   int blocks, int32_t* __restrict__ tokens,
+                                                   float* __restrict__ probs) {
+  const int li = blockIdx.x, tid = threadIdx.x;
   const mk_verify_lane L = lanes[li];
   if (!lane_ok(L, max_draft, R.n_rows, R.n_drafts)) return;
   Choice c = choices[li];
-  const double inv_t = L.temperature > 0.0f ? 1.0 / (double)L.temperature : 0.0;
-  const double v = u_next[li];
+  const double unit = per_unit(L);
   const float* prow = R.p + (int64_t)(L.row + c.n_acc) * R.p_stride;
   const float* qrow = c.refused && R.q ? R.q + (int64_t)(L.first + c.n_acc) * R.q_stride : nullptr;
-  __shared__ double ss[4];
-  __shared__ int pick_s, last_s;
-  const double* lane_sums = sums + (int64_t)li * segs;
+  __shared__ double wave_s[kThreads / 64];
+  __shared__ int found_s, last_s;
+  const double* lane_sums = sums + (int64_t)li * blocks;
   double total = 0.0;
-  for (int i = 0; i < segs; ++i) total += lane_sums[i];
-  bool walk = false;  // P itself, segment by segment: no segment sums of it are at hand
-  if (!(total > 0.0) && c.refused) {
-    c.refused = 0;
-    qrow = nullptr;
-    walk = true;
-    total = 1.0;
+  for (int b0 = 0; b0 < blocks; b0 += kThreads) {
+    double t;
+    block_scan(b0 + tid < blocks ? lane_sums[b0 + tid] : 0.0, wave_s, t);
+    total += t;
   }
-  const double goal = v * total;
+  // Nothing over Q: P itself, whose blocks have no sums at hand.
+  const bool walk = !(total > 0.0) && c.refused;
+  if (walk) c.refused = 0, qrow = nullptr, total = 1.0;
+  const double goal = u_next[li] * total;
+  // The block: the first whose running sum reaches the goal (rounding aside, the last with anything).
   double run = 0.0;
-  int pick = -1, last = -1;
-  for (int seg = 0; seg < segs && pick < 0; ++seg) {
-    // Past segments whose sum stays below the goal, unless none follows with anything in it.
-    if (!walk) {
-      const double s = lane_sums[seg];
-      if (!(s > 0.0)) continue;
-      bool more = false;
-      if (!(run + s >= goal))
-        for (int k = seg + 1; k < segs && !more; ++k) more = lane_sums[k] > 0.0;
-      if (more) {
-        run += s;
-        continue;
+  int first = 0, end = blocks;
+  if (!walk) {
+    int block = -1, last = -1;
+    double before = 0.0;
+    for (int b0 = 0; b0 < blocks && block < 0; b0 += kThreads) {
+      const double s = b0 + tid < blocks ? lane_sums[b0 + tid] : 0.0;
+      double t;
+      const double scan = block_scan(s, wave_s, t);
+      if (tid == 0) found_s = INT32_MAX, last_s = -1;
+      __syncthreads();
+      if (s > 0.0) {
+        atomicMax(&last_s, b0 + tid);
+        if (before + scan >= goal) atomicMin(&found_s, b0 + tid);
       }
+      __syncthreads();
+      if (last_s >= 0) last = last_s;
+      if (found_s != INT32_MAX) block = found_s;
+      before += t;
     }
-    // Thread i holds 16 consecutive tokens; their running sums through the waves.
-    double r[kPer];
-    double mine = 0.0;
+    if (block < 0) block = last;
+    if (block >= 0) {
+      // What lies before it, summed in the same order by every thread.
+      for (int b0 = 0; b0 < block; b0 += kThreads) {
+        double t;
+        block_scan(b0 + tid < block ? lane_sums[b0 + tid] : 0.0, wave_s, t);
+        run += t;
+      }
+      first = block, end = block + 1;
+    } else {
+      end = 0;
+    }
+  }
+  int pick = -1, last = -1;
+  for (int b = first; b < end && pick < 0; ++b) {
+    // Four consecutive tokens per thread.
+    double r[4], mine = 0.0;
+    const int x0 = b * kBlock + 4 * tid;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int x = seg * kSeg + tid * kPer + i;
-      r[i] = x < R.V ? excess(c, clean(prow[x]), qrow ? clean(qrow[x]) : 0.0f, R.q != nullptr, x, inv_t) : 0.0;
-      mine += r[i];
+    for (int e = 0; e < 4; ++e) {
+      const int x = x0 + e;
+      r[e] = x < R.V ? excess(c, clean(prow[x]), qrow ? clean(qrow[x]) : 0.0f, R.q != nullptr, x, unit) : 0.0;
+      mine += r[e];
     }
-    double scan = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double t = __shfl_up(scan, o);
-      if (lane >= o) scan += t;
-    }
-    if (tid == 0) pick_s = INT32_MAX, last_s = -1;
+    double t;
+    double upto = run + (block_scan(mine, wave_s, t) - mine);
+    if (tid == 0) found_s = INT32_MAX, last_s = -1;
     __syncthreads();
-    if (lane == 63) ss[w] = scan;
-    __syncthreads();
-    double before = run + (scan - mine);
-    for (int k = 0; k < w; ++k) before += ss[k];
     int hit = INT32_MAX, tail = -1;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      before += r[i];
-      const int x = seg * kSeg + tid * kPer + i;
-      if (r[i] > 0.0) {
-        tail = x;
-        if (before >= goal && hit == INT32_MAX) hit = x;
+    for (int e = 0; e < 4; ++e) {
+      upto += r[e];
+      if (r[e] > 0.0) {
+        tail = x0 + e;
+        if (upto >= goal && hit == INT32_MAX) hit = x0 + e;
       }
     }
-    if (hit != INT32_MAX) atomicMin(&pick_s, hit);
+    if (hit != INT32_MAX) atomicMin(&found_s, hit);
     if (tail >= 0) atomicMax(&last_s, tail);
     __syncthreads();
-    if (pick_s != INT32_MAX) pick = pick_s;
+    if (found_s != INT32_MAX) pick = found_s;
     if (last_s >= 0) last = last_s;
-    run += ((ss[0] + ss[1]) + ss[2]) + ss[3];
-    __syncthreads();
+    run += t;
   }
   if (pick < 0) pick = last;  // rounding left the goal above the whole sum: the last token with any
   if (tid == 0) {
     tokens[(int64_t)li * (max_draft + 1) + c.n_acc] = pick;
     if (probs)
       probs[(int64_t)li * (max_draft + 1) + c.n_acc] =
-          pick < 0 ? 0.0f : (float)prob(c.p, clean(prow[pick]), pick, inv_t);
+          pick < 0 ? 0.0f : (float)prob(c.p, clean(prow[pick]), pick, unit);
   }
 }
+static_assert(kBlock == 4 * kThreads, "a block of tokens is four per thread");
 
 // ---- rows cut to their top k ----
 
-constexpr int kMaxK = 1024;
+constexpr int kMaxK = 1024, kTopkThreads = 512;
 
 struct Cands {
   const float* values;
@@ -379,83 +474,90 @@ __device__ __forceinline__ float prob_in(const float* v, const int32_t* ids, con
   return 0.0f;
 }
 
-// One workgroup per lane: wave w decides drafts w, w + 4, ..; wave 0 draws the next token.
-__global__ __launch_bounds__(kThreads) void k_verify_topk(Cands P, Cands Q, const mk_verify_lane* __restrict__ lanes,
-                                                          int max_draft, int n_drafts,
-                                                          const int32_t* __restrict__ drafts,
-                                                          const double* __restrict__ u,
-                                                          const double* __restrict__ u_next,
-                                                          int32_t* __restrict__ accepted, int32_t* __restrict__ tokens,
-                                                          float* __restrict__ probs) {
+// One workgroup per lane: the rows' heads in turn over the waves, each with the probability of the draft it judges;
+// then wave 0 draws the next token.
+__global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, const mk_verify_lane* __restrict__ lanes,
+                                                              int max_draft, int n_drafts,
+                                                              const int32_t* __restrict__ drafts,
+                                                              const double* __restrict__ u,
+                                                              const double* __restrict__ u_next,
+                                                              int32_t* __restrict__ accepted,
+                                                              int32_t* __restrict__ tokens, float* __restrict__ probs) {
   const int li = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const mk_verify_lane L = lanes[li];
   int32_t* tok = tokens + (int64_t)li * (max_draft + 1);
   float* pr = probs ? probs + (int64_t)li * (max_draft + 1) : nullptr;
   const bool ok = lane_ok(L, max_draft, P.n, n_drafts);
   __shared__ int stop_s;
-  __shared__ float pd_s[kMaxDraft];
+  __shared__ Head head_s[2 * kMaxDraft + 1];  // target rows, then draft rows
+  __shared__ float prob_s[2 * kMaxDraft + 1];
   __shared__ int32_t q_id[kMaxK];
   __shared__ float q_pr[kMaxK];
   if (tid == 0) stop_s = ok ? L.n_draft : -1;
-  __syncthreads();
   const float t = L.temperature;
+  const int rows = ok ? L.n_draft + 1 + (Q.values ? L.n_draft : 0) : 0;
+  for (int r = w; r < rows; r += kTopkThreads / 64) {
+    const bool draft = r > L.n_draft;
+    const int j = draft ? r - L.n_draft - 1 : r, k = draft ? Q.k : P.k;
+    const int64_t at = draft ? (int64_t)(L.first + j) * Q.k : (int64_t)(L.row + j) * P.k;
+    const float* v = (draft ? Q.values : P.values) + at;
+    const Head h = head_of(v, k, L);
+    const float p = j < L.n_draft ? prob_in(v, (draft ? Q.ids : P.ids) + at, h, drafts[L.first + j], t) : 0.0f;
+    if (lane == 0) head_s[r] = h, prob_s[r] = p;
+  }
+  __syncthreads();
   if (ok)
-    for (int j = w; j < L.n_draft; j += 4) {
-      const int d = drafts[L.first + j];
-      const float* pv = P.values + (int64_t)(L.row + j) * P.k;
-      const float p = prob_in(pv, P.ids + (int64_t)(L.row + j) * P.k, head_of(pv, P.k, L), d, t);
-      float q = 1.0f;
-      if (Q.values) {
-        const float* qv = Q.values + (int64_t)(L.first + j) * Q.k;
-        q = prob_in(qv, Q.ids + (int64_t)(L.first + j) * Q.k, head_of(qv, Q.k, L), d, t);
-      }
-      if (lane == 0) {
-        pd_s[j] = p;
-        if (!(q > 0.0f && u[L.first + j] * (double)q < (double)p)) atomicMin(&stop_s, j);
-      }
+    for (int j = tid; j < L.n_draft; j += kTopkThreads) {
+      const float p = prob_s[j], q = Q.values ? prob_s[L.n_draft + 1 + j] : 1.0f;
+      if (!(q > 0.0f && u[L.first + j] * (double)q < (double)p)) atomicMin(&stop_s, j);
     }
   __syncthreads();
   const int n_acc = stop_s;
-  for (int j = tid; j <= max_draft; j += kThreads) {
+  for (int j = tid; j <= max_draft; j += kTopkThreads) {
     if (j == n_acc) continue;
     tok[j] = j < n_acc ? drafts[L.first + j] : -1;
-    if (pr) pr[j] = j < n_acc ? pd_s[j] : 0.0f;
+    if (pr) pr[j] = j < n_acc ? prob_s[j] : 0.0f;
   }
   if (tid == 0) accepted[li] = n_acc;
   if (!ok) return;
   const bool refused = n_acc < L.n_draft;
-  const float* pv = P.values + (int64_t)(L.row + n_acc) * P.k;
-  const int32_t* pi = P.ids + (int64_t)(L.row + n_acc) * P.k;
   // The draft's probabilities at the refusal, by candidate.
   int q_n = 0;
   if (refused && Q.values) {
-    const float* qv = Q.values + (int64_t)(L.first + n_acc) * Q.k;
-    const Head qh = head_of(qv, Q.k, L);
+    const int64_t at = (int64_t)(L.first + n_acc) * Q.k;
+    const Head qh = head_s[L.n_draft + 1 + n_acc];
     q_n = qh.keep;
-    for (int i = tid; i < q_n; i += kThreads) {
-      q_id[i] = Q.ids[(int64_t)(L.first + n_acc) * Q.k + i];
-      q_pr[i] = cand_prob(qh, qv[i], qv[0], i, t);
+    for (int i = tid; i < q_n; i += kTopkThreads) {
+      q_id[i] = Q.ids[at + i];
+      q_pr[i] = cand_prob(qh, Q.values[at + i], Q.values[at], i, t);
     }
   } else if (refused) {
     q_n = 1;
     if (tid == 0) q_id[0] = drafts[L.first + n_acc], q_pr[0] = 1.0f;
   }
+  // What each target candidate is drawn by (at most kMaxK: kept in LDS).
+  __shared__ float left_s[kMaxK];
+  const float* pv = P.values + (int64_t)(L.row + n_acc) * P.k;
+  const int32_t* pi = P.ids + (int64_t)(L.row + n_acc) * P.k;
+  const Head ph = head_s[n_acc];
+  __syncthreads();
+  for (int i = tid; i < ph.keep; i += kTopkThreads) {
+    const int id = pi[i];
+    float q = 0.0f;
+    for (int k = 0; k < q_n; ++k)
+      if (q_id[k] == id) q = q_pr[k];
+    left_s[i] = fmaxf(cand_prob(ph, pv[i], pv[0], i, t) - q, 0.0f);
+  }
   __syncthreads();
   if (w != 0) return;
-  const Head ph = head_of(pv, P.k, L);
-  auto left = [&](int i, bool over) {
-    const float p = cand_prob(ph, pv[i], pv[0], i, t);
-    float q = 0.0f;
-    if (over)
-      for (int k = 0; k < q_n; ++k)
-        if (q_id[k] == pi[i]) q = q_pr[k];
-    return fmaxf(p - q, 0.0f);
-  };
   double total = 0.0;
-  bool over = refused;
+  bool over = true;
+  auto left = [&](int i) {
+    return i >= ph.keep ? 0.0 : over ? (double)left_s[i] : (double)cand_prob(ph, pv[i], pv[0], i, t);
+  };
   for (;;) {
     total = 0.0;
-    for (int c = 0; c < ph.keep; c += 64) total += wave_sum(c + lane < ph.keep ? (double)left(c + lane, over) : 0.0);
+    for (int c = 0; c < ph.keep; c += 64) total += wave_sum(left(c + lane));
     if (total > 0.0 || !over) break;
     over = false;  // nothing is left over the draft's probabilities: the row itself
   }
@@ -463,7 +565,7 @@ __global__ __launch_bounds__(kThreads) void k_verify_topk(Cands P, Cands Q, cons
   double run = 0.0;
   int pick = -1, last = -1;
   for (int c = 0; c < ph.keep && pick < 0; c += 64) {
-    const double r = c + lane < ph.keep ? (double)left(c + lane, over) : 0.0;
+    const double r = left(c + lane);
     double scan = r;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -491,7 +593,7 @@ size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 size_t verify_workspace(int n_lanes, int max_draft, int n_vocab) {
   const size_t segs = segments(n_vocab), lanes = n_lanes;
   return lanes * (2 * (size_t)max_draft + 1) * segs * sizeof(Stat) + up16(lanes * sizeof(Choice)) +
-         lanes * segs * sizeof(double);
+         lanes * segs * (kThreads / 64) * sizeof(double);
 }
 
 void verify(hipStream_t s, const float* p, int64_t p_stride, int n_rows, const float* q, int64_t q_stride, int n_drafts,
@@ -501,14 +603,16 @@ void verify(hipStream_t s, const float* p, int64_t p_stride, int n_rows, const f
   Stat* stats = static_cast<Stat*>(workspace);
   Choice* choices = reinterpret_cast<Choice*>(stats + (size_t)n_lanes * per * segs);
   double* sums = reinterpret_cast<double*>(reinterpret_cast<uint8_t*>(choices) + up16(n_lanes * sizeof(Choice)));
-  const Rows R{p, p_stride, n_rows, q, q_stride, n_drafts, n_vocab};
+  auto aligned = [](const float* x, int64_t stride) { return !x || (((uintptr_t)x & 15) == 0 && (stride & 3) == 0); };
+  const Rows R{p, p_stride, n_rows, q, q_stride, n_drafts, n_vocab,
+               (n_vocab & 3) == 0 && aligned(p, p_stride) && aligned(q, q_stride)};
   hipLaunchKernelGGL(k_rows, dim3(n_lanes * per, segs), dim3(kThreads), 0, s, R, lanes, max_draft, stats);
   check_launch("verify rows");
   hipLaunchKernelGGL(k_excess, dim3(n_lanes, segs), dim3(kThreads), 0, s, R, lanes, max_draft, drafts, u, stats, choices,
                      sums, accepted, tokens, probs);
   check_launch("verify excess");
-  hipLaunchKernelGGL(k_pick, dim3(n_lanes), dim3(kThreads), 0, s, R, lanes, max_draft, u_next, choices, sums, segs,
-                     tokens, probs);
+  hipLaunchKernelGGL(k_pick, dim3(n_lanes), dim3(kThreads), 0, s, R, lanes, max_draft, u_next, choices, sums,
+                     segs * (kThreads / 64), tokens, probs);
   check_launch("verify pick");
 }
 
@@ -516,7 +620,7 @@ void verify_topk(hipStream_t s, const float* p_values, const int32_t* p_ids, int
                  const int32_t* q_ids, int q_k, int n_drafts, const mk_verify_lane* lanes, int n_lanes, int max_draft,
                  const int32_t* drafts, const double* u, const double* u_next, int32_t* accepted, int32_t* tokens,
                  float* probs) {
-  hipLaunchKernelGGL(k_verify_topk, dim3(n_lanes), dim3(kThreads), 0, s, Cands{p_values, p_ids, p_k, n_rows},
+  hipLaunchKernelGGL(k_verify_topk, dim3(n_lanes), dim3(kTopkThreads), 0, s, Cands{p_values, p_ids, p_k, n_rows},
                      Cands{q_values, q_ids, q_k, n_drafts}, lanes, max_draft, n_drafts, drafts, u, u_next, accepted,
                      tokens, probs);
   check_launch("verify_topk");
