@@ -5,10 +5,10 @@
 //
 // Whole vocabulary: every probability, sum and running sum is held in 64 bits. The draw walks a running sum over
 // 150 thousand tokens, whose steps are as small as the rounding of 32-bit sums: in 32 bits about one draw in a hundred
-// would land on a neighbouring token. Three launches: k_rows reads every row once, in segments of 4096 logits (their
+// would land on a neighbouring token. Two launches: k_rows reads every row once, in segments of 4096 logits (their
 // maximum, its first place, and the sum of exp((z - max) / T)); k_excess makes each lane's decisions from those (every
-// workgroup of a lane for itself: a few hundred numbers) and sums the excess over 1024 tokens at a time of the row that
-// the next token comes from; k_pick finds the block and the token.
+// workgroup of a lane for itself: a few hundred numbers) and sums the excess over 256 tokens at a time of the row that
+// the next token comes from; a lane's last workgroup to finish finds the block and the token.
 #include <cfloat>
 
 #include "ctx.h"
@@ -18,94 +18,160 @@ namespace mk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kQuads = 4;                     // logits per thread, in fours
-constexpr int kBlock = 64 * 4 * kQuads;       // logits per wave, contiguous
-constexpr int kSeg = kThreads / 64 * kBlock;  // logits per segment
+constexpr int kQuads = 4;                         // logits per thread, in fours
+constexpr int kBlock = 64 * 4;                    // logits of a wave's fours
+constexpr int kSeg = kThreads / 64 * kQuads * kBlock;  // logits per segment, a wave's contiguous
 constexpr int kMaxDraft = MK_VERIFY_MAX_DRAFT;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
-struct Stat {  // a segment of a row, or a row
+struct Stat {  // part of a row, or a row
   double sum;  // of exp((z - max) / T); T <= 0: unused
-  float max;
-  int32_t at;  // first place of max; -1: nothing but -inf
+  float max;   // T > 0: near the maximum, what the sum is against; else the maximum
+  int32_t at;  // T <= 0: first place of max; -1: nothing but -inf
 };
 struct Choice {  // of a lane
-  int32_t n_acc;
-  int32_t refused;  // a draft was: the excess over Q counts
-  int32_t draft;    // that draft
-  int32_t pad;
-  Stat p, q;
+  int n_acc;
+  bool refused;  // a draft was: the excess over Q counts
+  int draft;     // that draft
+  Stat p, q;     // sum: its inverse
 };
 
 // NaN counts as -inf, +inf as the largest float.
 __device__ __forceinline__ float clean(float z) { return fminf(fmaxf(z, -INFINITY), FLT_MAX); }
 
-// 2^t for t <= about 1000: t = n + f, |f| <= 1/2, and the series of e^(f ln 2) to f^11, whose remainder is below
-// (ln 2 / 2)^12 / 12! = 7e-15 of it. Below 2^-1074 (-inf included) it is 0.
-__device__ __forceinline__ double pow2(double t) {
-  t = fmax(t, -1100.0);
-  const double n = __builtin_rint(t), f = t - n;
-  constexpr double c[12] = {1.0,
-                            6.931471805599453094e-1,
-                            2.402265069591007123e-1,
-                            5.550410866482157995e-2,
-                            9.618129107628477232e-3,
-                            1.333355814642844343e-3,
-                            1.540353039338160996e-4,
-                            1.525273380405984028e-5,
-                            1.321548679014430949e-6,
-                            1.017808600923969973e-7,
-                            7.054911620801123330e-9,
-                            4.445538271870811498e-10};
-  double p = c[11];
-#pragma unroll
-  for (int i = 10; i >= 0; --i) p = __builtin_fma(p, f, c[i]);
-  return __builtin_amdgcn_ldexp(p, (int)n);
-}
-
-// Logits to powers of two: log2(e) / T; 0 where T <= 0.
-__device__ __forceinline__ double per_unit(const mk_verify_lane& l) {
-  return l.temperature > 0.0f ? 1.4426950408889634074 / (double)l.temperature : 0.0;
-}
-__device__ __forceinline__ double weight(float z, float max, double c) {
-  return pow2(((double)z - (double)fmaxf(max, -FLT_MAX)) * c);
-}
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
-  return v;
-}
-// A value per lane (none: at -1), joined over the wave: the maximum, its first place, the sums brought to it.
-__device__ __forceinline__ Stat wave_join(Stat s, double c) {
-  Stat r;
-  r.max = wave_max(s.at < 0 ? -INFINITY : s.max);
-  int at = s.at >= 0 && s.max == r.max ? s.at : INT32_MAX;
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) at = min(at, __shfl_xor(at, m));
-  r.at = at == INT32_MAX ? -1 : at;
-  r.sum = c > 0.0 ? wave_sum(s.at < 0 ? 0.0 : s.sum * weight(s.max, r.max, c)) : 0.0;
+// p f + c with c in scalar registers (left to itself the compiler copies the constant into the result first, and a power
+// takes twice the instructions).
+__device__ __forceinline__ double fma_s(double p, double f, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(p), "v"(f), "s"(c));
   return r;
 }
-// The same of a row's segments, by one wave.
-__device__ __forceinline__ Stat row_stat(const Stat* s, int segs, double c) {
-  const int lane = threadIdx.x & 63;
-  const Stat none{0.0, -INFINITY, -1};
-  Stat a = wave_join(lane < segs ? s[lane] : none, c);
-  for (int i = 64; i < segs; i += 64) {  // lane 63 carries the earlier ones
-    const Stat b = i + lane < segs && lane < 63 ? s[i + lane] : none;
-    a = wave_join(lane == 63 ? a : b, c);
-    if (i + 63 < segs) {
-      const Stat last = s[i + 63];
-      a = wave_join(lane == 0 ? a : lane == 1 ? last : none, c);
-    }
+
+// 2^(d / 64) in two factors: d = 64 n + j + g, |g| <= 1/2; the table has 2^(j / 64), and 2^(g / 64) is the series of
+// e^x to x^4 (x = g ln 2 / 64 at most 0.0054: what follows is below 4e-14 of it). d is rounded by adding 1.5 * 2^52,
+// whose low word then holds 64 n + j; a table entry's high word is kept less j << 14, so that adding that word << 14 puts
+// n into the exponent. |d| < 64000.
+constexpr int kTable = 64;
+// 2^(j / 64), rounded, less j << 46 (j << 14 of the high word).
+__device__ const uint64_t kPowers[kTable] = {
+    0x3ff0000000000000, 0x3fefec9a3e778061, 0x3fefd9b0d3158574, 0x3fefc74518759bc8,
+    0x3fefb5586cf9890f, 0x3fefa3ec32d3d1a2, 0x3fef9301d0125b51, 0x3fef829aaea92de0,
+    0x3fef72b83c7d517b, 0x3fef635beb6fcb75, 0x3fef54873168b9aa, 0x3fef463b88628cd6,
+    0x3fef387a6e756238, 0x3fef2b4565e27cdd, 0x3fef1e9df51fdee1, 0x3fef1285a6e4030b,
+    0x3fef06fe0a31b715, 0x3feefc08b26416ff, 0x3feef1a7373aa9cb, 0x3feee7db34e59ff7,
+    0x3feedea64c123422, 0x3feed60a21f72e2a, 0x3feece086061892d, 0x3feec6a2b5c13cd0,
+    0x3feebfdad5362a27, 0x3feeb9b2769d2ca7, 0x3feeb42b569d4f82, 0x3feeaf4736b527da,
+    0x3feeab07dd485429, 0x3feea76f15ad2148, 0x3feea47eb03a5585, 0x3feea23882552225,
+    0x3feea09e667f3bcd, 0x3fee9fb23c651a2f, 0x3fee9f75e8ec5f74, 0x3fee9feb564267c9,
+    0x3feea11473eb0187, 0x3feea2f336cf4e62, 0x3feea589994cce13, 0x3feea8d99b4492ed,
+    0x3feeace5422aa0db, 0x3feeb1ae99157736, 0x3feeb737b0cdc5e5, 0x3feebd829fde4e50,
+    0x3feec49182a3f090, 0x3feecc667b5de565, 0x3feed503b23e255d, 0x3feede6b5579fdbf,
+    0x3feee89f995ad3ad, 0x3feef3a2b84f15fb, 0x3feeff76f2fb5e47, 0x3fef0c1e904bc1d2,
+    0x3fef199bdd85529c, 0x3fef27f12e57d14b, 0x3fef3720dcef9069, 0x3fef472d4a07897c,
+    0x3fef5818dcfba487, 0x3fef69e603db3285, 0x3fef7c97337b9b5f, 0x3fef902ee78b3ff6,
+    0x3fefa4afa2a490da, 0x3fefba1bee615a27, 0x3fefd0765b6e4540, 0x3fefe7c1819e90d8,
+};
+struct Power {
+  double factor, rest;  // their product is the power
+};
+__device__ __forceinline__ Power pow2(double d, const double* table) {
+  constexpr double kRound = 0x1.8p52, k1 = 6.931471805599453094e-1 / 64;
+  const double r = d + kRound, g = d - (r - kRound);
+  const uint32_t word = (uint32_t)__builtin_bit_cast(uint64_t, r);
+  v2u t = __builtin_bit_cast(v2u, table[word & (kTable - 1)]);
+  t[1] += word << 14;
+  double p = fma_s(g, k1 * k1 * k1 * k1 / 24, k1 * k1 * k1 / 6);
+  p = fma_s(p, g, k1 * k1 / 2);
+  p = fma_s(p, g, k1);
+  return Power{__builtin_bit_cast(double, t), __builtin_fma(p, g, 1.0)};
+}
+// The table to LDS, where lanes read entries of their own; a barrier follows before its first use.
+__device__ __forceinline__ void load_table(double* table) {
+  if (threadIdx.x < kTable) table[threadIdx.x] = __builtin_bit_cast(double, kPowers[threadIdx.x]);
+}
+
+// Logits to 64ths of a power of two: 64 log2(e) / T; 0 where T <= 0.
+__device__ __forceinline__ double per_unit(const mk_verify_lane& l) {
+  return l.temperature > 0.0f ? 64 * 1.4426950408889634074 / (double)l.temperature : 0.0;
+}
+constexpr double kLeast = -63000.0;  // in such 64ths: below 2^-984 there is nothing
+// exp((z - max) / T), c its per_unit; 0 for z of -inf.
+__device__ __forceinline__ double weight(float z, float max, double c, const double* table) {
+  const double d = ((double)z - (double)max) * c;
+  const bool in = d > kLeast;
+  const Power v = pow2(in ? d : 0.0, table);
+  return in ? v.factor * v.rest : 0.0;
+}
+// Moves between lanes in registers (DPP): lanes that have no source, or are masked, get `none`.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float v, float none) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                                               CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double v, double none) {
+  const v2u a = __builtin_bit_cast(v2u, v), b = __builtin_bit_cast(v2u, none);
+  v2u r;
+  r[0] = __builtin_amdgcn_update_dpp((int)b[0], (int)a[0], CTRL, ROWS, 0xF, false);
+  r[1] = __builtin_amdgcn_update_dpp((int)b[1], (int)a[1], CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, r);
+}
+// The inclusive running sum over the wave's lanes: within rows of 16 (row_shr 1, 2, 4, 8), then row 0's and 2's ends on
+// rows 1 and 3 (row_bcast:15), then lane 31's on rows 2 and 3 (row_bcast:31).
+__device__ __forceinline__ double wave_scan(double v) {
+  v += dpp<0x111, 0xF>(v, 0.0);
+  v += dpp<0x112, 0xF>(v, 0.0);
+  v += dpp<0x114, 0xF>(v, 0.0);
+  v += dpp<0x118, 0xF>(v, 0.0);
+  v += dpp<0x142, 0xA>(v, 0.0);
+  return v + dpp<0x143, 0xC>(v, 0.0);
+}
+__device__ __forceinline__ double last_lane(double v) {
+  v2u a = __builtin_bit_cast(v2u, v);
+  a[0] = __builtin_amdgcn_readlane(a[0], 63), a[1] = __builtin_amdgcn_readlane(a[1], 63);
+  return __builtin_bit_cast(double, a);
+}
+__device__ __forceinline__ double wave_sum(double v) { return last_lane(wave_scan(v)); }
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp<0x111, 0xF>(v, -INFINITY));
+  v = fmaxf(v, dpp<0x112, 0xF>(v, -INFINITY));
+  v = fmaxf(v, dpp<0x114, 0xF>(v, -INFINITY));
+  v = fmaxf(v, dpp<0x118, 0xF>(v, -INFINITY));
+  v = fmaxf(v, dpp<0x142, 0xA>(v, -INFINITY));
+  v = fmaxf(v, dpp<0x143, 0xC>(v, -INFINITY));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+// The statistics of s[0 .. n - 1] together (at -1: nothing), by a row of 16 lanes: the maximum, its first place, the
+// sums brought to it (added in another order in every lane: lane 0's is used).
+__device__ __forceinline__ Stat join16(const Stat* s, int n, double c, const double* table) {
+  const int lane = threadIdx.x & 15;
+  Stat r{0.0, -INFINITY, -1};
+  for (int i = lane; i < n; i += 16)
+    if (s[i].at >= 0) r.max = fmaxf(r.max, s[i].max);
+  r.max = fmaxf(r.max, dpp<0x128, 0xF>(r.max, -INFINITY));  // row_ror 8, 4, 2, 1
+  r.max = fmaxf(r.max, dpp<0x124, 0xF>(r.max, -INFINITY));
+  r.max = fmaxf(r.max, dpp<0x122, 0xF>(r.max, -INFINITY));
+  r.max = fmaxf(r.max, dpp<0x121, 0xF>(r.max, -INFINITY));
+  if (r.max == -INFINITY) return r;
+  if (c > 0.0) {
+    r.at = 0;
+    for (int i = lane; i < n; i += 16)
+      if (s[i].at >= 0) r.sum += s[i].sum * weight(s[i].max, r.max, c, table);
+    r.sum += dpp<0x128, 0xF>(r.sum, 0.0);
+    r.sum += dpp<0x124, 0xF>(r.sum, 0.0);
+    r.sum += dpp<0x122, 0xF>(r.sum, 0.0);
+    r.sum += dpp<0x121, 0xF>(r.sum, 0.0);
+  } else {
+    int at = INT32_MAX;
+    for (int i = lane; i < n; i += 16)
+      if (s[i].at >= 0 && s[i].max == r.max) at = min(at, s[i].at);
+#pragma unroll
+    for (int m = 8; m > 0; m >>= 1) at = min(at, __shfl_xor(at, m, 16));
+    r.at = at;
   }
-  return a;
+  return r;
 }
 
 struct Rows {
@@ -115,7 +181,6 @@ struct Rows {
   const float* q;  // NULL: every draft is certain
   int64_t q_stride;
   int n_drafts, V;
-  bool vec;
 };
 
 // A lane whose parameters do not fit the call is left out: accepted -1, tokens -1.
@@ -124,175 +189,125 @@ __device__ __forceinline__ bool lane_ok(const mk_verify_lane& l, int max_draft, 
          l.first <= n_drafts - l.n_draft;
 }
 
-// Logit of place i (quad, value) of this thread in a segment.
-__device__ __forceinline__ int place(int seg, int quad, int e) {
-  return seg * kSeg + (threadIdx.x >> 6) * kBlock + quad * 256 + (threadIdx.x & 63) * 4 + e;
+// Place of this thread's four logits `quad` of a segment.
+__device__ __forceinline__ int place(int seg, int quad) {
+  return seg * kSeg + ((threadIdx.x >> 6) * kQuads + quad) * kBlock + (threadIdx.x & 63) * 4;
 }
-// A segment's logits, a wave's 1024 contiguous (past the row: -inf). vec: rows are 16-byte aligned, V a multiple of 4.
-__device__ __forceinline__ void load_segment(const float* row, int seg, int V, bool vec, float (&z)[kQuads][4]) {
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) {
-      const int at = place(seg, i, 0);
-      const v4f v = *reinterpret_cast<const v4f*>(row + (at < V ? at : 0));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) z[i][e] = at < V ? clean(v[e]) : -INFINITY;
-    }
+// Four logits (past the row: -inf). VEC: rows are 16-byte aligned, V a multiple of 4.
+template <bool VEC>
+__device__ __forceinline__ v4f load4(const float* row, int at, int V) {
+  v4f v;
+  if constexpr (VEC) {
+    v = *reinterpret_cast<const v4f*>(row + (at < V ? at : 0));
   } else {
 #pragma unroll
-    for (int i = 0; i < kQuads; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int at = place(seg, i, e);
-        z[i][e] = at < V ? clean(row[at]) : -INFINITY;
-      }
+    for (int e = 0; e < 4; ++e) v[e] = row[at + e < V ? at + e : 0];
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = clean(v[e]);
+  if (__builtin_expect((at & ~(kBlock - 1)) + kBlock > V, 0)) {  // a wave's last logits
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = at + e < V ? v[e] : -INFINITY;
+  }
+  return v;
 }
 
-// Grid (lanes x (2 max_draft + 1), segments): rows j <= max_draft of a lane are the target's, the others the draft's.
+// Grid (lanes x (2 max_draft + 1), spans of `span` segments): rows j <= max_draft of a lane are the target's, the others
+// the draft's. Each thread sums against the first maximum that it meets (64 bits reach 2^900 past it), asks for a
+// segment's logits while the one before is summed, and the threads' sums meet once per span.
+template <bool VEC>
 __global__ __launch_bounds__(kThreads) void k_rows(Rows R, const mk_verify_lane* __restrict__ lanes, int max_draft,
-                                                   Stat* __restrict__ stats) {
-  const int per = 2 * max_draft + 1, li = blockIdx.x / per, j = blockIdx.x % per, seg = blockIdx.y;
+                                                   int span, Stat* __restrict__ stats,
+                                                   uint32_t* __restrict__ arrived) {
+  const int per = 2 * max_draft + 1, li = blockIdx.x / per, j = blockIdx.x % per;
   const mk_verify_lane L = lanes[li];
   if (!lane_ok(L, max_draft, R.n_rows, R.n_drafts)) return;
+  if (j == 0 && blockIdx.y == 0 && threadIdx.x == 0) arrived[li] = 0;  // for k_excess
   const bool draft = j > max_draft;
   const int jj = draft ? j - max_draft - 1 : j;
   if (draft ? (jj >= L.n_draft || !R.q) : jj > L.n_draft) return;
   const float* row = draft ? R.q + (int64_t)(L.first + jj) * R.q_stride : R.p + (int64_t)(L.row + jj) * R.p_stride;
-  float z[kQuads][4];
-  load_segment(row, seg, R.V, R.vec, z);
-  float m = -INFINITY;
+  const int seg0 = blockIdx.y * span, seg1 = min(seg0 + span, (R.V + kSeg - 1) / kSeg);
+  v4f z[kQuads], next[kQuads];
 #pragma unroll
-  for (int i = 0; i < kQuads; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = fmaxf(m, z[i][e]);
-  m = wave_max(m);  // each wave against its own maximum: no barrier before the end
+  for (int i = 0; i < kQuads; ++i) z[i] = load4<VEC>(row, place(seg0, i), R.V);
+  __shared__ double table[kTable];
+  load_table(table);
   const double c = per_unit(L);
+  const float reach = c > 0.0 ? (float)(32000.0 / c) : 0.0f;  // a maximum further than 2^500 up is a new one to sum against
+  float m = -INFINITY;
   double sum = 0.0;
-  int at = m == -INFINITY ? -1 : 0;
-  if (c > 0.0) {
-    if (at == 0) {
+  int at = -1;
+  __syncthreads();
+#pragma unroll 1
+  for (int seg = seg0; seg < seg1; ++seg) {
+    if (seg + 1 < seg1)
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) next[i] = load4<VEC>(row, place(seg + 1, i), R.V);
+    float top = z[0][0];
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, z[i][e]);
+    if (top > m && (m == -INFINITY || c == 0.0 || top - m > reach)) {
+      sum = m == -INFINITY ? 0.0 : sum * weight(m, top, c, table);
+      m = top, at = INT32_MAX;
+#pragma unroll
+      for (int i = kQuads - 1; i >= 0; --i)
+#pragma unroll
+        for (int e = 3; e >= 0; --e) at = z[i][e] == m ? place(seg, i) + e : at;
+    }
+    if (c > 0.0 && m > -INFINITY) {
       const double md = (double)m;
 #pragma unroll
       for (int i = 0; i < kQuads; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += pow2(((double)z[i][e] - md) * c);
+        for (int e = 0; e < 4; ++e) {
+          const Power v = pow2(fmax(((double)z[i][e] - md) * c, kLeast), table);
+          sum = __builtin_fma(v.factor, v.rest, sum);
+        }
     }
-    sum = wave_sum(sum);
-  } else if (at == 0) {
-    at = INT32_MAX;
 #pragma unroll
-    for (int i = 0; i < kQuads; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) at = z[i][e] == m ? min(at, place(seg, i, e)) : at;
+    for (int i = 0; i < kQuads; ++i) z[i] = next[i];
+  }
+  // A wave's threads, then the waves.
+  const int lane = threadIdx.x & 63;
+  const float wm = wave_max(m);
+  if (c > 0.0) {
+    sum = wave_sum(m == -INFINITY ? 0.0 : sum * weight(m, wm, c, table));
+    at = wm == -INFINITY ? INT32_MAX : 0;
+  } else {
+    at = m == wm && at >= 0 ? at : INT32_MAX;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
   }
   __shared__ Stat ws[kThreads / 64];
-  const int lane = threadIdx.x & 63;
-  if (lane == 0) ws[threadIdx.x >> 6] = Stat{sum, m, at};
+  if (lane == 0) ws[threadIdx.x >> 6] = Stat{sum, wm, at == INT32_MAX ? -1 : at};
   __syncthreads();
-  if (threadIdx.x >= 64) return;
-  const Stat s = wave_join(lane < kThreads / 64 ? ws[lane] : Stat{0.0, -INFINITY, -1}, c);
-  if (lane == 0) stats[(int64_t)blockIdx.x * gridDim.y + seg] = s;
+  if (threadIdx.x >= 16) return;
+  const Stat s = join16(ws, kThreads / 64, c, table);
+  if (threadIdx.x == 0) stats[(int64_t)blockIdx.x * gridDim.y + blockIdx.y] = s;
 }
 
-// P(x) of a row from its statistics.
-__device__ __forceinline__ double prob(const Stat& s, float z, int x, double c) {
+// P(x) of a row from its statistics (sum: its inverse).
+__device__ __forceinline__ double prob(const Stat& s, float z, int x, double c, const double* table) {
   if (s.at < 0) return 0.0;
-  return c > 0.0 ? weight(z, s.max, c) / s.sum : x == s.at ? 1.0 : 0.0;
+  return c > 0.0 ? weight(z, s.max, c, table) * s.sum : x == s.at ? 1.0 : 0.0;
 }
 
 // What of token x the next token is drawn by.
-__device__ __forceinline__ double excess(const Choice& c, float zp, float zq, bool has_q, int x, double unit) {
-  const double p = prob(c.p, zp, x, unit);
+__device__ __forceinline__ double excess(const Choice& c, float zp, float zq, bool has_q, int x, double unit,
+                                         const double* table) {
+  const double p = prob(c.p, zp, x, unit, table);
   if (!c.refused) return p;
-  const double q = has_q ? prob(c.q, zq, x, unit) : x == c.draft ? 1.0 : 0.0;
+  const double q = has_q ? prob(c.q, zq, x, unit, table) : x == c.draft ? 1.0 : 0.0;
   return fmax(p - q, 0.0);
-}
-
-__global__ __launch_bounds__(kThreads) void k_excess(Rows R, const mk_verify_lane* __restrict__ lanes, int max_draft,
-                                                     const int32_t* __restrict__ drafts, const double* __restrict__ u,
-                                                     const Stat* __restrict__ stats, Choice* __restrict__ choices,
-                                                     double* __restrict__ sums, int32_t* __restrict__ accepted,
-                                                     int32_t* __restrict__ tokens, float* __restrict__ probs) {
-  const int li = blockIdx.x, segs = gridDim.y, seg = blockIdx.y, per = 2 * max_draft + 1;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const mk_verify_lane L = lanes[li];
-  int32_t* tok = tokens + (int64_t)li * (max_draft + 1);
-  float* pr = probs ? probs + (int64_t)li * (max_draft + 1) : nullptr;
-  if (!lane_ok(L, max_draft, R.n_rows, R.n_drafts)) {
-    if (seg == 0) {
-      for (int j = threadIdx.x; j <= max_draft; j += kThreads) {
-        tok[j] = -1;
-        if (pr) pr[j] = 0.0f;
-      }
-      if (threadIdx.x == 0) accepted[li] = -1;
-    }
-    return;
-  }
-  const double unit = per_unit(L);
-  __shared__ Stat row_s[2 * kMaxDraft + 1];
-  __shared__ int stop_s;
-  if (threadIdx.x == 0) stop_s = L.n_draft;
-  const int rows = L.n_draft + 1 + (R.q ? L.n_draft : 0);
-  for (int r = w; r < rows; r += kThreads / 64) {
-    const int j = r <= L.n_draft ? r : max_draft + r - L.n_draft;
-    const Stat a = row_stat(stats + ((int64_t)li * per + j) * segs, segs, unit);
-    if (lane == 0) row_s[r] = a;
-  }
-  __syncthreads();
-  for (int j = threadIdx.x; j < L.n_draft; j += kThreads) {
-    const int d = drafts[L.first + j];
-    double p = 0.0, q = 1.0;
-    if (d >= 0 && d < R.V) {
-      p = prob(row_s[j], clean(R.p[(int64_t)(L.row + j) * R.p_stride + d]), d, unit);
-      if (R.q) q = prob(row_s[L.n_draft + 1 + j], clean(R.q[(int64_t)(L.first + j) * R.q_stride + d]), d, unit);
-    }
-    if (!(q > 0.0 && u[L.first + j] * q < p)) atomicMin(&stop_s, j);
-    if (seg == 0 && pr) pr[j] = (float)p;  // past the refusal cleared below
-  }
-  __syncthreads();
-  Choice c;
-  c.n_acc = stop_s;
-  c.refused = c.n_acc < L.n_draft;
-  c.draft = c.refused ? drafts[L.first + c.n_acc] : -1;
-  c.p = row_s[c.n_acc];
-  c.q = c.refused && R.q ? row_s[L.n_draft + 1 + c.n_acc] : Stat{0.0, -INFINITY, -1};
-  if (seg == 0) {
-    for (int j = threadIdx.x; j <= max_draft; j += kThreads) {
-      tok[j] = j < c.n_acc ? drafts[L.first + j] : -1;
-      if (pr && j >= c.n_acc) pr[j] = 0.0f;
-    }
-    if (threadIdx.x == 0) {
-      accepted[li] = c.n_acc;
-      choices[li] = c;
-    }
-  }
-  const bool both = c.refused && R.q;
-  float zp[kQuads][4], zq[kQuads][4];
-  load_segment(R.p + (int64_t)(L.row + c.n_acc) * R.p_stride, seg, R.V, R.vec, zp);
-  if (both) load_segment(R.q + (int64_t)(L.first + c.n_acc) * R.q_stride, seg, R.V, R.vec, zq);
-  double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < kQuads; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int x = place(seg, i, e);
-      if (x < R.V) sum += excess(c, zp[i][e], both ? zq[i][e] : 0.0f, R.q != nullptr, x, unit);
-    }
-  sum = wave_sum(sum);
-  if (lane == 0) sums[((int64_t)li * segs + seg) * (kThreads / 64) + w] = sum;
 }
 
 // The inclusive running sum over the workgroup's threads, and in `total` that of all.
 __device__ __forceinline__ double block_scan(double v, double* wave_s, double& total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double t = __shfl_up(v, o);
-    if (lane >= o) v += t;
-  }
+  v = wave_scan(v);
   __syncthreads();  // the last scan's sums have been read
   if (lane == 63) wave_s[w] = v;
   __syncthreads();
@@ -305,106 +320,202 @@ __device__ __forceinline__ double block_scan(double v, double* wave_s, double& t
   return v;
 }
 
-// The first token in order whose running sum reaches v times the total; one workgroup per lane.
-__global__ __launch_bounds__(kThreads) void k_pick(Rows R, const mk_verify_lane* __restrict__ lanes, int max_draft,
-                                                   const double* __restrict__ u_next,
-                                                   const Choice* __restrict__ choices, const double* __restrict__ sums,
-                                                   int blocks, int32_t* __restrict__ tokens,
-                                                   float* __restrict__ probs) {
-  const int li = blockIdx.x, tid = threadIdx.x;
-  const mk_verify_lane L = lanes[li];
-  if (!lane_ok(L, max_draft, R.n_rows, R.n_drafts)) return;
-  Choice c = choices[li];
-  const double unit = per_unit(L);
-  const float* prow = R.p + (int64_t)(L.row + c.n_acc) * R.p_stride;
-  const float* qrow = c.refused && R.q ? R.q + (int64_t)(L.first + c.n_acc) * R.q_stride : nullptr;
-  __shared__ double wave_s[kThreads / 64];
+// Sums of the excess, which other workgroups of the lane read: stored and read past the caches that XCDs do not share.
+__device__ __forceinline__ void put(double* p, double v) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double get(const double* p) {
+  return __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                      __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// The first token in order whose running sum reaches v times the total, by one workgroup. sums: of blocks of 256 tokens.
+__device__ __forceinline__ int pick_token(const Rows& R, const float* prow, const float* qrow, Choice& c, double unit,
+                                          double v, const double* sums, int blocks, const double* table) {
+  const int tid = threadIdx.x;
+  __shared__ double wave_s[kThreads / 64], run_s[2];
   __shared__ int found_s, last_s;
-  const double* lane_sums = sums + (int64_t)li * blocks;
-  double total = 0.0;
-  for (int b0 = 0; b0 < blocks; b0 += kThreads) {
-    double t;
-    block_scan(b0 + tid < blocks ? lane_sums[b0 + tid] : 0.0, wave_s, t);
-    total += t;
-  }
+  // Thread i has the sums of `each` neighbouring blocks; their running sum and total.
+  const int each = (blocks + kThreads - 1) / kThreads, b0 = min(tid * each, blocks), b1 = min(b0 + each, blocks);
+  constexpr int kKept = 4;  // in registers, of vocabularies up to 262144
+  double kept[kKept], mine = 0.0, total;
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) kept[i] = b0 + i < b1 ? get(sums + b0 + i) : 0.0;
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) mine += kept[i];
+  for (int b = b0 + kKept; b < b1; ++b) mine += get(sums + b);
+  double before = block_scan(mine, wave_s, total) - mine;
   // Nothing over Q: P itself, whose blocks have no sums at hand.
   const bool walk = !(total > 0.0) && c.refused;
-  if (walk) c.refused = 0, qrow = nullptr, total = 1.0;
-  const double goal = u_next[li] * total;
-  // The block: the first whose running sum reaches the goal (rounding aside, the last with anything).
+  if (walk) c.refused = 0, total = 1.0;
+  const double goal = v * total;
+  // The block: the first whose running sum reaches the goal (rounding aside, the last with anything), and what lies
+  // before it.
   double run = 0.0;
   int first = 0, end = blocks;
   if (!walk) {
-    int block = -1, last = -1;
-    double before = 0.0;
-    for (int b0 = 0; b0 < blocks && block < 0; b0 += kThreads) {
-      const double s = b0 + tid < blocks ? lane_sums[b0 + tid] : 0.0;
-      double t;
-      const double scan = block_scan(s, wave_s, t);
-      if (tid == 0) found_s = INT32_MAX, last_s = -1;
-      __syncthreads();
+    int block = INT32_MAX, last = -1;
+    double block_run = 0.0, last_run = 0.0;
+    auto look = [&](int b, double s) {
       if (s > 0.0) {
-        atomicMax(&last_s, b0 + tid);
-        if (before + scan >= goal) atomicMin(&found_s, b0 + tid);
+        last = b, last_run = before;
+        if (block == INT32_MAX && before + s >= goal) block = b, block_run = before;
       }
-      __syncthreads();
-      if (last_s >= 0) last = last_s;
-      if (found_s != INT32_MAX) block = found_s;
-      before += t;
-    }
-    if (block < 0) block = last;
-    if (block >= 0) {
-      // What lies before it, summed in the same order by every thread.
-      for (int b0 = 0; b0 < block; b0 += kThreads) {
-        double t;
-        block_scan(b0 + tid < block ? lane_sums[b0 + tid] : 0.0, wave_s, t);
-        run += t;
-      }
-      first = block, end = block + 1;
-    } else {
-      end = 0;
-    }
-  }
-  int pick = -1, last = -1;
-  for (int b = first; b < end && pick < 0; ++b) {
-    // Four consecutive tokens per thread.
-    double r[4], mine = 0.0;
-    const int x0 = b * kBlock + 4 * tid;
+      before += s;
+    };
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int x = x0 + e;
-      r[e] = x < R.V ? excess(c, clean(prow[x]), qrow ? clean(qrow[x]) : 0.0f, R.q != nullptr, x, unit) : 0.0;
-      mine += r[e];
-    }
-    double t;
-    double upto = run + (block_scan(mine, wave_s, t) - mine);
+    for (int i = 0; i < kKept; ++i) look(b0 + i, kept[i]);
+    for (int b = b0 + kKept; b < b1; ++b) look(b, get(sums + b));
     if (tid == 0) found_s = INT32_MAX, last_s = -1;
     __syncthreads();
-    int hit = INT32_MAX, tail = -1;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      upto += r[e];
-      if (r[e] > 0.0) {
-        tail = x0 + e;
-        if (upto >= goal && hit == INT32_MAX) hit = x0 + e;
-      }
+    if (block != INT32_MAX) atomicMin(&found_s, block);
+    if (last >= 0) atomicMax(&last_s, last);
+    __syncthreads();
+    if (block != INT32_MAX && block == found_s) run_s[0] = block_run;
+    if (last >= 0 && last == last_s) run_s[1] = last_run;
+    __syncthreads();
+    const bool hit = found_s != INT32_MAX;
+    run = hit ? run_s[0] : run_s[1];
+    first = hit ? found_s : max(last_s, 0), end = (hit ? found_s : last_s) + 1;
+    __syncthreads();
+  }
+  int pick = -1, last = -1;
+#pragma unroll 1
+  for (int b = first; b < end && pick < 0; ++b) {
+    const int x = b * kBlock + tid;  // a token per thread
+    const double r = x < R.V ? excess(c, clean(prow[x]), clean(qrow[x]), R.q != nullptr, x, unit, table) : 0.0;
+    double t;
+    const double upto = run + block_scan(r, wave_s, t);
+    if (tid == 0) found_s = INT32_MAX, last_s = -1;
+    __syncthreads();
+    if (r > 0.0) {
+      atomicMax(&last_s, x);
+      if (upto >= goal) atomicMin(&found_s, x);
     }
-    if (hit != INT32_MAX) atomicMin(&found_s, hit);
-    if (tail >= 0) atomicMax(&last_s, tail);
     __syncthreads();
     if (found_s != INT32_MAX) pick = found_s;
     if (last_s >= 0) last = last_s;
     run += t;
   }
-  if (pick < 0) pick = last;  // rounding left the goal above the whole sum: the last token with any
+  return pick < 0 ? last : pick;  // rounding may leave the goal above the whole sum: the last token with any
+}
+
+// Grid (lanes, segments). The lane's last workgroup to have its sums in memory draws the token.
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void k_excess(Rows R, const mk_verify_lane* __restrict__ lanes, int max_draft,
+                                                     const int32_t* __restrict__ drafts, const double* __restrict__ u,
+                                                     const double* __restrict__ u_next, const Stat* __restrict__ stats,
+                                                     int spans, double* __restrict__ sums,
+                                                     uint32_t* __restrict__ arrived, int32_t* __restrict__ accepted,
+                                                     int32_t* __restrict__ tokens, float* __restrict__ probs) {
+  const int li = blockIdx.x, segs = gridDim.y, seg = blockIdx.y, per = 2 * max_draft + 1, tid = threadIdx.x;
+  const int lane = tid & 63, w = tid >> 6;
+  const mk_verify_lane L = lanes[li];
+  int32_t* tok = tokens + (int64_t)li * (max_draft + 1);
+  float* pr = probs ? probs + (int64_t)li * (max_draft + 1) : nullptr;
+  if (!lane_ok(L, max_draft, R.n_rows, R.n_drafts)) {
+    if (seg == 0) {
+      for (int j = tid; j <= max_draft; j += kThreads) {
+        tok[j] = -1;
+        if (pr) pr[j] = 0.0f;
+      }
+      if (tid == 0) accepted[li] = -1;
+    }
+    return;
+  }
+  __shared__ double table[kTable];
+  load_table(table);
+  const double unit = per_unit(L), v = u_next[li];
+  // Thread j's draft (at most 256: one each), asked for before the rows' statistics.
+  static_assert(kMaxDraft <= kThreads, "a draft per thread");
+  int d = -1;
+  float zp_d = -INFINITY, zq_d = -INFINITY;
+  double u_d = 0.0;
+  if (tid < L.n_draft) {
+    d = drafts[L.first + tid], u_d = u[L.first + tid];
+    if (d >= 0 && d < R.V) {
+      zp_d = R.p[(int64_t)(L.row + tid) * R.p_stride + d];
+      if (R.q) zq_d = R.q[(int64_t)(L.first + tid) * R.q_stride + d];
+    }
+  }
+  __shared__ Stat row_s[2 * kMaxDraft + 1];
+  __shared__ int stop_s, d_s[kMaxDraft + 1], last_s;
+  if (tid == 0) stop_s = L.n_draft;
+  __syncthreads();
+  // Sixteen lanes a row.
+  const int rows = L.n_draft + 1 + (R.q ? L.n_draft : 0);
+  for (int r = tid >> 4; r < rows; r += kThreads / 16) {
+    const int j = r <= L.n_draft ? r : max_draft + r - L.n_draft;
+    Stat a = join16(stats + ((int64_t)li * per + j) * spans, spans, unit, table);
+    if (a.at >= 0 && unit > 0.0) a.sum = 1.0 / a.sum;
+    if ((tid & 15) == 0) row_s[r] = a;
+  }
+  __syncthreads();
+  float p_d = 0.0f;
+  if (tid < L.n_draft) {
+    double p = 0.0, q = 1.0;
+    if (d >= 0 && d < R.V) {
+      p = prob(row_s[tid], clean(zp_d), d, unit, table);
+      if (R.q) q = prob(row_s[L.n_draft + 1 + tid], clean(zq_d), d, unit, table);
+    }
+    if (!(q > 0.0 && u_d * q < p)) atomicMin(&stop_s, tid);
+    p_d = (float)p;
+    d_s[tid] = d;
+  }
+  __syncthreads();
+  Choice c;
+  c.n_acc = stop_s;
+  c.refused = c.n_acc < L.n_draft;
+  c.draft = c.refused ? d_s[c.n_acc] : -1;
+  c.p = row_s[c.n_acc];
+  c.q = c.refused && R.q ? row_s[L.n_draft + 1 + c.n_acc] : Stat{0.0, -INFINITY, -1};
+  const bool both = c.refused && R.q;
+  const float* prow = R.p + (int64_t)(L.row + c.n_acc) * R.p_stride;
+  const float* qrow = both ? R.q + (int64_t)(L.first + c.n_acc) * R.q_stride : prow;
+  v4f zp[kQuads], zq[kQuads];
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i) {
+    zp[i] = load4<VEC>(prow, place(seg, i), R.V);
+    zq[i] = load4<VEC>(qrow, place(seg, i), R.V);
+  }
+  if (seg == 0) {
+    for (int j = tid; j <= max_draft; j += kThreads) {
+      if (j == c.n_acc) continue;
+      tok[j] = j < c.n_acc ? d : -1;
+      if (pr) pr[j] = j < c.n_acc ? p_d : 0.0f;
+    }
+    if (tid == 0) accepted[li] = c.n_acc;
+  }
+  const int blocks = segs * (kSeg / kBlock);
+  double* lane_sums = sums + (int64_t)li * blocks;
+  double sum[kQuads];
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i) {
+    sum[i] = 0.0;
+    const int x = place(seg, i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[i] += excess(c, zp[i][e], zq[i][e], R.q != nullptr, x + e, unit, table);
+  }
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i) sum[i] = wave_sum(sum[i]);
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) put(lane_sums + seg * (kSeg / kBlock) + w * kQuads + i, sum[i]);
+  // Every wave's sums have reached memory before the lane's counter says so.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0)
+    last_s = __hip_atomic_fetch_add(arrived + li, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)segs - 1;
+  __syncthreads();
+  if (!last_s) return;
+  const int pick = pick_token(R, prow, qrow, c, unit, v, lane_sums, blocks, table);
   if (tid == 0) {
-    tokens[(int64_t)li * (max_draft + 1) + c.n_acc] = pick;
-    if (probs)
-      probs[(int64_t)li * (max_draft + 1) + c.n_acc] =
-          pick < 0 ? 0.0f : (float)prob(c.p, clean(prow[pick]), pick, unit);
+    tok[c.n_acc] = pick;
+    if (pr) pr[c.n_acc] = pick < 0 ? 0.0f : (float)prob(c.p, clean(prow[pick]), pick, unit, table);
   }
 }
-static_assert(kBlock == 4 * kThreads, "a block of tokens is four per thread");
+static_assert(kBlock == kThreads, "a token of a block per thread");
 
 // ---- rows cut to their top k ----
 
@@ -437,13 +548,7 @@ __device__ __forceinline__ Head head_of(const float* v, int k, const mk_verify_l
   for (int c = 0; c < k; c += 64) {
     const int i = c + lane;
     const double w = i < k ? cand_weight(v[i], top, L.temperature) : 0.0;
-    double scan = w;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double t = __shfl_up(scan, o);
-      if (lane >= o) scan += t;
-    }
-    scan += run;
+    const double scan = wave_scan(w) + run;
     const uint64_t below = __ballot(i < k && i > 0 && w < floor_w), reach = __ballot(i < k && scan >= nucleus);
     const int b = below ? __builtin_ctzll(below) : 64, e = reach ? __builtin_ctzll(reach) : 64;
     if (b < 64 || e < 64) {
@@ -566,13 +671,7 @@ __global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, 
   int pick = -1, last = -1;
   for (int c = 0; c < ph.keep && pick < 0; c += 64) {
     const double r = left(c + lane);
-    double scan = r;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double s = __shfl_up(scan, o);
-      if (lane >= o) scan += s;
-    }
-    scan += run;
+    const double scan = wave_scan(r) + run;
     const uint64_t some = __ballot(r > 0.0), hit = __ballot(r > 0.0 && scan >= goal);
     if (some) last = c + 63 - __builtin_clzll(some);
     if (hit) pick = c + __builtin_ctzll(hit);
@@ -586,14 +685,15 @@ __global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, 
 }
 
 int segments(int V) { return (V + kSeg - 1) / kSeg; }
-size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+// Segments a workgroup of k_rows takes: one where rows are few, more once they fill the CUs eight times over.
+int span_of(int64_t rows, int segs) { return (int)std::min<int64_t>(8, std::max<int64_t>(1, rows * segs / 4096)); }
 
 }  // namespace
 
 size_t verify_workspace(int n_lanes, int max_draft, int n_vocab) {
   const size_t segs = segments(n_vocab), lanes = n_lanes;
-  return lanes * (2 * (size_t)max_draft + 1) * segs * sizeof(Stat) + up16(lanes * sizeof(Choice)) +
-         lanes * segs * (kThreads / 64) * sizeof(double);
+  return lanes * (2 * (size_t)max_draft + 1) * segs * sizeof(Stat) + lanes * segs * (kSeg / kBlock) * sizeof(double) +
+         lanes * sizeof(uint32_t);
 }
 
 void verify(hipStream_t s, const float* p, int64_t p_stride, int n_rows, const float* q, int64_t q_stride, int n_drafts,
@@ -601,19 +701,22 @@ void verify(hipStream_t s, const float* p, int64_t p_stride, int n_rows, const f
             const double* u_next, int32_t* accepted, int32_t* tokens, float* probs, void* workspace) {
   const int segs = segments(n_vocab), per = 2 * max_draft + 1;
   Stat* stats = static_cast<Stat*>(workspace);
-  Choice* choices = reinterpret_cast<Choice*>(stats + (size_t)n_lanes * per * segs);
-  double* sums = reinterpret_cast<double*>(reinterpret_cast<uint8_t*>(choices) + up16(n_lanes * sizeof(Choice)));
+  double* sums = reinterpret_cast<double*>(stats + (size_t)n_lanes * per * segs);
+  uint32_t* arrived = reinterpret_cast<uint32_t*>(sums + (size_t)n_lanes * segs * (kSeg / kBlock));
   auto aligned = [](const float* x, int64_t stride) { return !x || (((uintptr_t)x & 15) == 0 && (stride & 3) == 0); };
-  const Rows R{p, p_stride, n_rows, q, q_stride, n_drafts, n_vocab,
-               (n_vocab & 3) == 0 && aligned(p, p_stride) && aligned(q, q_stride)};
-  hipLaunchKernelGGL(k_rows, dim3(n_lanes * per, segs), dim3(kThreads), 0, s, R, lanes, max_draft, stats);
-  check_launch("verify rows");
-  hipLaunchKernelGGL(k_excess, dim3(n_lanes, segs), dim3(kThreads), 0, s, R, lanes, max_draft, drafts, u, stats, choices,
-                     sums, accepted, tokens, probs);
-  check_launch("verify excess");
-  hipLaunchKernelGGL(k_pick, dim3(n_lanes), dim3(kThreads), 0, s, R, lanes, max_draft, u_next, choices, sums,
-                     segs * (kThreads / 64), tokens, probs);
-  check_launch("verify pick");
+  const Rows R{p, p_stride, n_rows, q, q_stride, n_drafts, n_vocab};
+  const int64_t rows = std::min<int64_t>((int64_t)n_lanes * per, (int64_t)n_rows + (q ? n_drafts : 0));
+  const int span = span_of(rows, segs), spans = (segs + span - 1) / span;
+  auto go = [&]<bool VEC>() {
+    hipLaunchKernelGGL(k_rows<VEC>, dim3(n_lanes * per, spans), dim3(kThreads), 0, s, R, lanes, max_draft, span, stats,
+                       arrived);
+    check_launch("verify rows");
+    hipLaunchKernelGGL(k_excess<VEC>, dim3(n_lanes, segs), dim3(kThreads), 0, s, R, lanes, max_draft, drafts, u, u_next,
+                       stats, spans, sums, arrived, accepted, tokens, probs);
+    check_launch("verify excess");
+  };
+  if ((n_vocab & 3) == 0 && aligned(p, p_stride) && aligned(q, q_stride)) go.template operator()<true>();
+  else go.template operator()<false>();
 }
 
 void verify_topk(hipStream_t s, const float* p_values, const int32_t* p_ids, int p_k, int n_rows, const float* q_values,
