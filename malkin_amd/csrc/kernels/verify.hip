@@ -234,7 +234,7 @@ __global__ __launch_bounds__(kThreads) void k_rows(Rows R, const mk_verify_lane*
   __shared__ double table[kTable];
   load_table(table);
   const double c = per_unit(L);
-  const float reach = c > 0.0 ? (float)(32000.0 / c) : 0.0f;  // a maximum further than 2^500 up is a new one to sum against
+  const float reach = 346.0f * L.temperature;  // a maximum further than 2^499 up is a new one to sum against
   float m = -INFINITY;
   double sum = 0.0;
   int at = -1;
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, 
 
 int segments(int V) { return (V + kSeg - 1) / kSeg; }
 // Segments a workgroup of k_rows takes: one where rows are few, more once they fill the CUs eight times over.
-int span_of(int64_t rows, int segs) { return (int)std::min<int64_t>(8, std::max<int64_t>(1, rows * segs / 4096)); }
+int span_of(int64_t rows, int segs) { return (int)std::min<int64_t>(8, std::max<int64_t>(1, rows * segs / 2048)); }
 
 }  // namespace
 
