@@ -29,6 +29,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef v4f v4f_any __attribute__((aligned(4)));  // a row of q may start anywhere
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v2i lds_v2i;
@@ -104,8 +105,7 @@ __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
 
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Split S, const float* __restrict__ q,
-                                                              int64_t q_stride, bool q_vec, float* __restrict__ po,
-                                                              Sum* __restrict__ pml) {
+                                                              int64_t q_stride, float* __restrict__ po, Sum* __restrict__ pml) {
   using G_ = Geo<D>;
   const int G = A.H / A.KV, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 31, h = lane >> 5;
@@ -141,9 +141,42 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Spli
     kb = A.kv.k + row * D, vb = A.kv.v + row * D, ksb = A.kv.ks + row, vsb = A.kv.vs + row;
   }
   const bool own = part >= S.np;
-  // This lane's query row: its token, head and keys (of this kind). Columns without a row, and rows without any key,
-  // whose results nobody reads, see every key.
+  // This lane's query row: its token, head and values, in the order of its half of a K row's bytes: byte b of a row is
+  // element 16 (b % (D / 16)) + b / (D / 16); step j, value e of half h is byte D / 2 h + 8 j + e. Asked for before
+  // anything is waited for.
   const int r = first + min(li, rows - 1), t = r / G, head = g * G + r % G;
+  float x[G_::kSteps][8];
+  {
+    const float* qr = q + t * q_stride + head * D + 8 * h;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const v4f v = *reinterpret_cast<const v4f_any*>(qr + 16 * e + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if constexpr (D == 128) x[j + i][e] = v[i];
+          else x[(j + i) / 2][e + 4 * (i & 1)] = v[i];
+      }
+  }
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t* ring = smem + w * (2 * G_::kStage);
+  auto issue = [&](int kt, int st) __attribute__((always_inline)) {
+    uint8_t* to = ring + st * G_::kStage;
+    const int base = k0 + kt * kKeys;
+#pragma unroll
+    for (int c = 0; c < G_::kCopies; ++c) {
+      const int at = c * 64 + lane, key = at / G_::kPieces;
+      const int64_t off = (int64_t)min(base + key, k1 - 1) * D + 16 * swizzle<D>(key, at % G_::kPieces);
+      lds_copy16(kb + off, to + 1024 * c);
+      lds_copy16(vb + off, to + G_::kTileBytes + 1024 * c);
+    }
+    lds_copy4((h ? vsb : ksb) + min(base + li, k1 - 1), to + 2 * G_::kTileBytes);
+  };
+  // The prefix's first tile does not wait for the tokens' keys either.
+  const bool early = !own && k0 + w * kKeys < k1;
+  if (early) issue(w, 0);
+  // Its keys (of this kind). Columns without a row, and rows without any key, whose results nobody reads, see every key.
   int lim = INT32_MAX, most = 0;
   {
     const int s = A.seq[t];
@@ -160,53 +193,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Spli
   }
   k1 = min(k1, __builtin_amdgcn_readfirstlane(most));
   least = min(__builtin_amdgcn_readfirstlane(least), k1);  // tiles up to here are whole for every row
-  if (k0 >= k1) return;
+  if (k0 >= k1) {
+    wait_vm<0>();  // LDS is not left with a copy under way
+    return;
+  }
   const int tiles = (k1 - k0 + kKeys - 1) / kKeys;
+  if (!early && w < tiles) issue(w, 0);
 
-  extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* ring = smem + w * (2 * G_::kStage);
-  auto issue = [&](int kt, int st) __attribute__((always_inline)) {
-    uint8_t* to = ring + st * G_::kStage;
-    const int base = k0 + kt * kKeys;
-#pragma unroll
-    for (int c = 0; c < G_::kCopies; ++c) {
-      const int at = c * 64 + lane, key = at / G_::kPieces;
-      const int64_t off = (int64_t)min(base + key, k1 - 1) * D + 16 * swizzle<D>(key, at % G_::kPieces);
-      lds_copy16(kb + off, to + 1024 * c);
-      lds_copy16(vb + off, to + G_::kTileBytes + 1024 * c);
-    }
-    lds_copy4((h ? vsb : ksb) + min(base + li, k1 - 1), to + 2 * G_::kTileBytes);
-  };
-  if (w < tiles) issue(w, 0);
-
-  // q of the lane's row in the order of its half of a K row's bytes: byte b of a row is element
-  // 16 (b % (D / 16)) + b / (D / 16); step j, value e of half h is byte D / 2 h + 8 j + e.
   v8h qh[G_::kSteps], ql[G_::kSteps];
   float rf;  // score, in bits, of one unit of a product
   {
-    const float* qr = q + t * q_stride + head * D;
-    float x[G_::kSteps][8];
-    if constexpr (D == 128) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const float* at = qr + 16 * e + 8 * h + j;
-          const v4f v = q_vec ? *reinterpret_cast<const v4f*>(at) : v4f{at[0], at[1], at[2], at[3]};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[j + i][e] = v[i];
-        }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const float* at = qr + 16 * e + 8 * h + j;
-          const v4f v = q_vec ? *reinterpret_cast<const v4f*>(at) : v4f{at[0], at[1], at[2], at[3]};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[(j + i) / 2][e + 4 * (i & 1)] = v[i];
-        }
-    }
     float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < G_::kSteps; ++j)
@@ -400,20 +396,30 @@ template <int D>
 __global__ __launch_bounds__(kThreads) void k_prefix_join(PrefixAttn A, Split S, const float* __restrict__ po,
                                                           const Sum* __restrict__ pml, float* __restrict__ out,
                                                           int64_t out_stride, BlockQ8* __restrict__ xq) {
-  constexpr int E = D / 64;
+  constexpr int E = D / 64, kAhead = 8;
   const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= A.n * A.H) return;
-  const int t = row / A.H, head = row % A.H, seq = A.seq[t];
+  const int t = row / A.H, head = row % A.H, parts = S.np + S.no;
+  // Everything is asked for at once: parts that the row's keys do not reach hold nothing of use, and have no weight.
+  const int64_t step = (int64_t)A.n * A.H;
+  const float* mine_o = po + (int64_t)row * D + E * lane;
+  float ahead[kAhead][E];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (i < parts)
+#pragma unroll
+      for (int k = 0; k < E; ++k) ahead[i][k] = mine_o[i * step * D + k];
+  Sum mine = lane < parts ? pml[lane * step + row] : Sum{};
+  const int seq = A.seq[t];
   const int keys = seq >= 0 && seq < A.n_seq ? max(0, min(A.n_keys[t], A.max_keys)) : 0;
-  const int np = (min(keys, A.n_prefix) + S.cp - 1) / S.cp, no = (max(keys - A.n_prefix, 0) + S.co - 1) / S.co;
+  const bool live = lane < S.np ? lane * S.cp < min(keys, A.n_prefix)
+                                : lane < parts && (int64_t)A.n_prefix + (int64_t)(lane - S.np) * S.co < keys;
+  if (!live) mine = Sum{kNone, kNone, 0.0f, 0.0f};
+  const uint64_t all = __ballot(live);
   float v[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) v[i] = 0.0f;
-  if (keys > 0) {
-    const int64_t step = (int64_t)A.n * A.H;
-    auto at = [&](int i) { return (i < np ? i : S.np + i - np) * step + row; };
-    Sum mine = {kNone, kNone, 0.0f, 0.0f};
-    if (lane < np + no) mine = pml[at(lane)];
+  if (all) {
     float base = mine.base;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) base = fmaxf(base, __shfl_xor(base, o));
@@ -425,12 +431,20 @@ __global__ __launch_bounds__(kThreads) void k_prefix_join(PrefixAttn A, Split S,
     float sum = f * mine.l;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-#pragma unroll 4
-    for (int i = 0; i < np + no; ++i) {
-      const float fi = __shfl(f, i);
 #pragma unroll
-      for (int k = 0; k < E; ++k) v[k] = fma_(fi, po[at(i) * D + E * lane + k], v[k]);
-    }
+    for (int i = 0; i < kAhead; ++i)
+      if ((all >> i) & 1) {
+        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = fma_(fi, ahead[i][k], v[k]);
+      }
+#pragma unroll 4
+    for (int i = kAhead; i < parts; ++i)
+      if ((all >> i) & 1) {
+        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = fma_(fi, mine_o[i * step * D + k], v[k]);
+      }
 #pragma unroll
     for (int k = 0; k < E; ++k) v[k] = v[k] / sum;
   }
@@ -474,15 +488,14 @@ void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q,
   const Split S = split_of(A.n, A.H, A.KV, A.n_prefix, A.max_keys);
   float* po = static_cast<float*>(workspace);
   Sum* pml = reinterpret_cast<Sum*>(po + S.parts * D);
-  const bool q_vec = ((uintptr_t)q & 15) == 0 && (q_stride & 3) == 0;
   const int tq = kRows / (A.H / A.KV);
   const int64_t wgs = (int64_t)S.tiles * A.KV * S.np + (int64_t)(A.n + tq - 1) / tq * tq * A.KV * S.no;
   require(wgs < (1ll << 31), "mk_attention_prefix: too many rows");
   auto go = [&]<int D_>() {
     if (wgs > 0) {
       allow_lds<k_prefix_parts<D_>>(Geo<D_>::kLds);
-      hipLaunchKernelGGL(k_prefix_parts<D_>, dim3((unsigned)wgs), dim3(kThreads), Geo<D_>::kLds, s, A, S, q, q_stride,
-                         q_vec, po, pml);
+      hipLaunchKernelGGL(k_prefix_parts<D_>, dim3((unsigned)wgs), dim3(kThreads), Geo<D_>::kLds, s, A, S, q, q_stride, po,
+                         pml);
       check_launch("attention_prefix parts");
     }
     hipLaunchKernelGGL(k_prefix_join<D_>, dim3((unsigned)(((int64_t)A.n * A.H + 3) / 4)), dim3(kThreads), 0, s, A, S, po,

@@ -139,6 +139,11 @@ __device__ __forceinline__ uint32_t lds_addr(const void* l) {
 __device__ __forceinline__ void lds_copy16(const void* g, void* l) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_addr(l)) : "m0");
 }
+// The same from a wave-uniform address plus 32-bit offsets of the lanes' own.
+__device__ __forceinline__ void lds_copy16(const void* base, uint32_t off, void* l) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_addr(l))
+               : "m0");
+}
 __device__ __forceinline__ void lds_copy4(const void* g, void* l) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_addr(l)) : "m0");
 }
