@@ -29,7 +29,6 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef v4f v4f_any __attribute__((aligned(4)));  // a row of q may start anywhere
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v2i lds_v2i;
@@ -63,11 +62,14 @@ struct Geo {
   static constexpr int kPieces = D / 16;       // 16-byte pieces of a row
   static constexpr int kTileBytes = kKeys * D;
   static constexpr int kCopies = kTileBytes / 1024;
-  static constexpr int kPer = 2 * kCopies + 1;             // copies per tile: K, V, both scales
-  static constexpr int kStage = 2 * kTileBytes + 8 * kKeys;
   static constexpr int kShift = D == 128 ? 1 : 2;          // rows per 64 LDS banks, as a shift
-  static constexpr int kOutStride = D + 4;
-  static constexpr int kLds = kWaves * (2 * kStage > kRows * kOutStride * 4 ? 2 * kStage : kRows * kOutStride * 4);
+  static constexpr int kQSteps = kSteps / kWaves;          // steps of q that a wave prepares
+  static constexpr int kQBytes = kSteps * 2 * 1024;        // q: [step][hi, lo][lane] 16 bytes
+  static constexpr int kWaveBytes = 2 * kTileBytes + 2 * 8 * kKeys;  // K, V, two tiles' scales
+  static constexpr int kOutStride = 64 + 4;                // 64 values of a row at a time
+  static constexpr int kOutBytes = kWaves * kRows * kOutStride * 4;
+  static constexpr int kRing = kWaves * kWaveBytes > kOutBytes ? kWaves * kWaveBytes : kOutBytes;
+  static constexpr int kLds = kQBytes + kRing;
 };
 
 // The piece of row `key` that lies in slot s, and the slot that holds piece s: rows whose LDS banks coincide hold their
@@ -104,7 +106,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], v8h& hi, v8h& lo) {
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Split S, const float* __restrict__ q,
+__global__ __launch_bounds__(kThreads, 3) void k_prefix_parts(PrefixAttn A, Split S, const float* __restrict__ q,
                                                               int64_t q_stride, float* __restrict__ po, Sum* __restrict__ pml) {
   using G_ = Geo<D>;
   const int G = A.H / A.KV, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -142,40 +144,54 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Spli
   }
   const bool own = part >= S.np;
   // This lane's query row: its token, head and values, in the order of its half of a K row's bytes: byte b of a row is
-  // element 16 (b % (D / 16)) + b / (D / 16); step j, value e of half h is byte D / 2 h + 8 j + e. Asked for before
-  // anything is waited for.
+  // element 16 (b % (D / 16)) + b / (D / 16); step j, value e of half h is byte D / 2 h + 8 j + e. A wave prepares a
+  // quarter of the steps, which it asks for before anything is waited for.
   const int r = first + min(li, rows - 1), t = r / G, head = g * G + r % G;
-  float x[G_::kSteps][8];
+  float x[G_::kQSteps][8];
   {
-    const float* qr = q + t * q_stride + head * D + 8 * h;
+    const float* qr = q + t * q_stride + head * D;
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e)
+    for (int j = 0; j < G_::kQSteps; ++j)
 #pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const v4f v = *reinterpret_cast<const v4f_any*>(qr + 16 * e + j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if constexpr (D == 128) x[j + i][e] = v[i];
-          else x[(j + i) / 2][e + 4 * (i & 1)] = v[i];
+      for (int e = 0; e < 8; ++e) {
+        const int byte = D / 2 * h + 8 * (G_::kQSteps * w + j) + e;
+        x[j][e] = qr[16 * (byte % (D / 16)) + byte / (D / 16)];
       }
   }
   extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* ring = smem + w * (2 * G_::kStage);
-  auto issue = [&](int kt, int st) __attribute__((always_inline)) {
-    uint8_t* to = ring + st * G_::kStage;
-    const int base = k0 + kt * kKeys;
+  __shared__ Sum ml[kWaves][kRows];
+  uint8_t* kt_s = smem + G_::kQBytes + w * G_::kWaveBytes;
+  uint8_t* vt_s = kt_s + G_::kTileBytes;
+  auto scales_s = [&](int st) { return vt_s + G_::kTileBytes + st * (8 * kKeys); };
+  // This lane's part of a whole tile's copies.
+  uint32_t off[G_::kCopies];
+#pragma unroll
+  for (int c = 0; c < G_::kCopies; ++c) {
+    const int at = c * 64 + lane, key = at / G_::kPieces;
+    off[c] = key * D + 16 * swizzle<D>(key, at % G_::kPieces);
+  }
+  auto copy = [&](const int8_t* from, int kt, uint8_t* to) __attribute__((always_inline)) {
+    const int base = k0 + kt * kKeys, last = k1 - 1 - base;  // keys past the end: the last one again
 #pragma unroll
     for (int c = 0; c < G_::kCopies; ++c) {
-      const int at = c * 64 + lane, key = at / G_::kPieces;
-      const int64_t off = (int64_t)min(base + key, k1 - 1) * D + 16 * swizzle<D>(key, at % G_::kPieces);
-      lds_copy16(kb + off, to + 1024 * c);
-      lds_copy16(vb + off, to + G_::kTileBytes + 1024 * c);
+      uint32_t o = off[c];
+      if (last < kKeys - 1) {
+        const int at = c * 64 + lane, key = at / G_::kPieces;
+        o = min(key, last) * D + 16 * swizzle<D>(key, at % G_::kPieces);
+      }
+      lds_copy16(from + (int64_t)base * D, o, to + 1024 * c);
     }
-    lds_copy4((h ? vsb : ksb) + min(base + li, k1 - 1), to + 2 * G_::kTileBytes);
   };
+  constexpr int kKeyCopies = G_::kCopies + 1;
+  auto issue_k = [&](int kt, int st) __attribute__((always_inline)) {
+    copy(kb, kt, kt_s);
+    const int base = k0 + kt * kKeys;
+    lds_copy4((h ? vsb : ksb) + base + min(li, k1 - 1 - base), scales_s(st));
+  };
+  auto issue_v = [&](int kt) __attribute__((always_inline)) { copy(vb, kt, vt_s); };
   // The prefix's first tile does not wait for the tokens' keys either.
   const bool early = !own && k0 + w * kKeys < k1;
-  if (early) issue(w, 0);
+  if (early) issue_k(w, 0), issue_v(w);
   // Its keys (of this kind). Columns without a row, and rows without any key, whose results nobody reads, see every key.
   int lim = INT32_MAX, most = 0;
   {
@@ -198,27 +214,36 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Spli
     return;
   }
   const int tiles = (k1 - k0 + kKeys - 1) / kKeys;
-  if (!early && w < tiles) issue(w, 0);
+  if (!early && w < tiles) issue_k(w, 0), issue_v(w);
 
-  v8h qh[G_::kSteps], ql[G_::kSteps];
   float rf;  // score, in bits, of one unit of a product
   {
     float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < G_::kSteps; ++j)
+    for (int j = 0; j < G_::kQSteps; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[j][e]));
     top = fmaxf(top, __shfl_xor(top, 32));
+    float* top_s = reinterpret_cast<float*>(ml);
+    if (h == 0) top_s[w * kRows + li] = top;
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, top_s[i * kRows + li]);
     int ex = 0;
     if (top > 0.0f && top < INFINITY) ex = min(14 - __builtin_amdgcn_frexp_expf(top), 100);
     rf = __builtin_ldexpf(A.scale * kLog2e, -ex);
 #pragma unroll
-    for (int j = 0; j < G_::kSteps; ++j) {
+    for (int j = 0; j < G_::kQSteps; ++j) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[j][e] = __builtin_ldexpf(x[j][e], ex);
-      split8(x[j], qh[j], ql[j]);
+      v8h hi, lo;
+      split8(x[j], hi, lo);
+      v8h* to = reinterpret_cast<v8h*>(smem + (G_::kQSteps * w + j) * 2048) + lane;
+      to[0] = hi, to[64] = lo;
     }
+    lds_barrier();
   }
+  const v8h* qs = reinterpret_cast<const v8h*>(smem) + lane;
 
   v16f o[G_::kDt];
 #pragma unroll
@@ -230,20 +255,31 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Spli
   bool wide = false;
   float rg = 1.0f, ms = 0.0f;
 
-  auto tile = [&](int kt, const uint8_t* at) __attribute__((always_inline)) {
+  int st = 0;
+  auto tile = [&](int kt) __attribute__((always_inline)) {
     const int base = k0 + kt * kKeys;
+    const bool more = kt + kWaves < tiles;
+    wait_vm<G_::kCopies>();  // this tile's K and scales; its V may be under way
+    fence();
+    v4u k[G_::kSteps / 2];
+#pragma unroll
+    for (int i = 0; i < G_::kSteps / 2; ++i)
+      k[i] = *reinterpret_cast<const v4u*>(kt_s + li * D + 16 * swizzle<D>(li, h * (G_::kPieces / 2) + i));
+    fence();
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): K is in registers, and its place free for the next tile's
+    fence();
+    if (more) issue_k(kt + kWaves, st ^ 1);
     v16f s = {};
 #pragma unroll
     for (int i = 0; i < G_::kSteps / 2; ++i) {
-      const v4u k = *reinterpret_cast<const v4u*>(at + li * D + 16 * swizzle<D>(li, h * (G_::kPieces / 2) + i));
-      const v8h a = cvt8(k[0], k[1]), b = cvt8(k[2], k[3]);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[2 * i], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[2 * i], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, qh[2 * i + 1], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ql[2 * i + 1], s, 0, 0, 0);
+      const v8h a = cvt8(k[i][0], k[i][1]), b = cvt8(k[i][2], k[i][3]);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qs[256 * i], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qs[256 * i + 64], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, qs[256 * i + 128], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, qs[256 * i + 192], s, 0, 0, 0);
     }
     // Register i of a half is key 8 (i / 4) + 4 h + i % 4 of the tile.
-    const float* sc = reinterpret_cast<const float*>(at + 2 * G_::kTileBytes);
+    const float* sc = reinterpret_cast<const float*>(scales_s(st));
     float vs[16], p[16], x[16];
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
@@ -320,74 +356,78 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefix_parts(PrefixAttn A, Spli
       for (int e = 0; e < 8; ++e) y[e] = x[8 * u + e];
       split8(y, ph[u], pl[u]);
     }
+    if (more) wait_vm<kKeyCopies>();  // this tile's V; the next tile's K may be under way
+    else wait_vm<0>();
+    fence();
     // ds_read_b64_tr_b8: lane i of 16 reads 8 bytes, (row i / 2, half i % 2) of an 8 x 16 byte tile, and gets the
     // tile's column i. Row e of step u is the key of weight 8 u + e.
-    const uint8_t* v = at + G_::kTileBytes;
+    v2i vv[2][G_::kDt];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int e = (lane & 15) >> 1, key = 16 * u + 8 * (e >> 2) + 4 * h + (e & 3);
 #pragma unroll
+      for (int i = 0; i < G_::kDt; ++i)
+        vv[u][i] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_v2i*)(vt_s + key * D + 16 * swizzle<D>(key, 2 * i + ((lane >> 4) & 1)) + 8 * (lane & 1)));
+    }
+    fence();
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // as K
+    fence();
+    if (more) issue_v(kt + kWaves);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
       for (int i = 0; i < G_::kDt; ++i) {
-        const v2i b = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (lds_v2i*)(v + key * D + 16 * swizzle<D>(key, 2 * i + ((lane >> 4) & 1)) + 8 * (lane & 1)));
-        const v8h a = cvt8((uint32_t)b[0], (uint32_t)b[1]);
+        const v8h a = cvt8((uint32_t)vv[u][i][0], (uint32_t)vv[u][i][1]);
         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[u], o[i], 0, 0, 0);
         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[u], o[i], 0, 0, 0);
       }
-    }
-  };
-  int st = 0;
-  for (int kt = w; kt < tiles; kt += kWaves) {
-    fence();
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): reads of the stage refilled next are done
-    fence();
-    if (kt + kWaves < tiles) {
-      issue(kt + kWaves, st ^ 1);
-      wait_vm<G_::kPer>();
-    } else {
-      wait_vm<0>();
-    }
-    fence();
-    tile(kt, ring + st * G_::kStage);
     st ^= 1;
-  }
+  };
+  for (int kt = w; kt < tiles; kt += kWaves) tile(kt);
   l += __shfl_xor(l, 32);
 
   // The waves' parts of each row, brought to their largest shift and added.
-  __shared__ Sum ml[kWaves][kRows];
+  wait_vm<0>();  // a copy issued before the rows' keys were known may still be under way
   __syncthreads();
-  float* ob = reinterpret_cast<float*>(smem);
+  float* ob = reinterpret_cast<float*>(smem + G_::kQBytes);
   if (h == 0) ml[w][li] = Sum{m == kNone ? kNone : ms, m, l, 0.0f};
-#pragma unroll
-  for (int i = 0; i < G_::kDt; ++i)
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-      *reinterpret_cast<v4f*>(ob + (w * kRows + li) * G_::kOutStride + 32 * i + 8 * a + 4 * h) =
-          v4f{o[i][4 * a], o[i][4 * a + 1], o[i][4 * a + 2], o[i][4 * a + 3]};
-  __syncthreads();
-  const int row = tid >> 3, x8 = tid & 7;
-  if (row >= rows) return;
-  float base = kNone, top = -INFINITY, f[kWaves], sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) base = fmaxf(base, ml[i][row].base);
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) top = fmaxf(top, f[i] = ml[i][row].above(base));
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    f[i] = __builtin_amdgcn_exp2f(f[i] - top);
-    sum = fma_(f[i], ml[i][row].l, sum);
-  }
-  const int rr = first + row;
+  const int row = tid >> 3, x8 = tid & 7, rr = first + min(row, rows - 1);
   const int64_t at = ((int64_t)part * A.n + rr / G) * A.H + g * G + rr % G;
-  if (x8 == 0) pml[at] = Sum{base, top, sum, 0.0f};
+  float f[kWaves];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const int d = 4 * (x8 + 8 * i);
-    v4f a = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int d0 = 0; d0 < G_::kDt; d0 += 2) {  // 64 values at a time
+    if (d0) lds_barrier();
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k)
-      a += f[k] * *reinterpret_cast<const v4f*>(ob + (k * kRows + row) * G_::kOutStride + d);
-    *reinterpret_cast<v4f*>(po + at * D + d) = a;
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        *reinterpret_cast<v4f*>(ob + (w * kRows + li) * G_::kOutStride + 32 * i + 8 * a + 4 * h) =
+            v4f{o[d0 + i][4 * a], o[d0 + i][4 * a + 1], o[d0 + i][4 * a + 2], o[d0 + i][4 * a + 3]};
+    lds_barrier();
+    if (row >= rows) continue;
+    if (d0 == 0) {
+      float base = kNone, top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) base = fmaxf(base, ml[i][row].base);
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, f[i] = ml[i][row].above(base));
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        f[i] = __builtin_amdgcn_exp2f(f[i] - top);
+        sum = fma_(f[i], ml[i][row].l, sum);
+      }
+      if (x8 == 0) pml[at] = Sum{base, top, sum, 0.0f};
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = 4 * (x8 + 8 * i);
+      v4f a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k)
+        a += f[k] * *reinterpret_cast<const v4f*>(ob + (k * kRows + row) * G_::kOutStride + d);
+      *reinterpret_cast<v4f*>(po + at * D + 32 * d0 + d) = a;
+    }
   }
 }
 
