@@ -495,7 +495,11 @@ __global__ __launch_bounds__(kThreads) void k_prefix_join(PrefixAttn A, Split S,
 }
 
 constexpr int kMaxPre = 48, kMaxOwn = 16;  // a row's parts fit one wave's lanes
-constexpr int kWanted = 512;               // workgroups: two per CU
+// Workgroups wanted of each kind. The prefix's are long and set up once (q, the join of their waves): one per CU is best
+// (62 users over 8192 + 1024 keys: 43.9 us, with 192 wanted 42.9, with 384 44.6, with 512 46.9; 16 users over 4000 + 300:
+// 16.8, 15.6, 17.0, 21.1). The own rows' are as many as there are (token run, KV head) pairs, and split only where those
+// do not fill the CUs twice (8 users over 1500 + 600 keys: 14.1 us, with 256 wanted 15.2, with 128 14.7).
+constexpr int kWantedPre = 256, kWantedOwn = 512;
 
 int chunk(int keys, int chunks) {  // keys per chunk, whole tiles for the four waves
   const int c = (keys + chunks - 1) / chunks;
@@ -508,9 +512,9 @@ Split split_of(int n, int H, int KV, int n_prefix, int max_keys) {
   s.tiles = (int)(((int64_t)n * G + kRows - 1) / kRows);
   const int pre = std::min(n_prefix, max_keys), own = std::max(0, max_keys - n_prefix);
   const int64_t pre_wgs = (int64_t)s.tiles * KV, own_wgs = (int64_t)n * KV;
-  s.cp = chunk(pre, (int)std::min<int64_t>(kMaxPre, std::max<int64_t>(1, kWanted / pre_wgs)));
+  s.cp = chunk(pre, (int)std::min<int64_t>(kMaxPre, std::max<int64_t>(1, kWantedPre / pre_wgs)));
   s.np = (pre + s.cp - 1) / s.cp;
-  s.co = chunk(own, (int)std::min<int64_t>(kMaxOwn, std::max<int64_t>(1, kWanted / own_wgs)));
+  s.co = chunk(own, (int)std::min<int64_t>(kMaxOwn, std::max<int64_t>(1, kWantedOwn / own_wgs)));
   s.no = (own + s.co - 1) / s.co;
   s.parts = (int64_t)(s.np + s.no) * n * H;
   return s;
