@@ -97,7 +97,7 @@ def sample_drafts(rng, q, lanes):
 
 CASES = [  # drafts per lane, vocabulary
     ([0], 1), ([1], 2), ([3], 17), ([2, 0, 5], 1000), ([4, 4, 1], 4096), ([1, 6], 4097), ([3, 8, 2, 1, 0, 7], 8191),
-    ([2, 2], 151936), ([33], 5000), ([1] * 50, 300),
+    ([2, 2], 151936), ([33], 5000), ([1] * 50, 300), ([1, 0, 2, 3] * 8, 35001), ([2, 1] * 16, 32768),
 ]
 
 
@@ -156,6 +156,20 @@ def test_dense_ends_and_masks(mk):
     assert got[0][7] == 0 and got[0][8] <= 1 and got[0][9] == 0 and got[0][10] >= 1 and got[0][11] == 0
     got = Dense(mk, p, None, lanes, drafts, u, un, 2).run().read()
     check(got, want_dense(p, None, lanes, drafts, u, un, 2))
+
+
+def test_extreme_temperatures(mk):
+    """From the smallest positive number, which is greedy but for ties, to infinity, which is uniform."""
+    V, rng = 9000, np.random.default_rng(4)
+    temps = [1e-45, 1e-30, 1e-3, 1e4, 3.4e38, np.inf]
+    counts = [2] * len(temps)
+    lanes = lanes_of(counts, temps)
+    p, q, u, un = inputs(rng, counts, V)
+    p[lanes["row"][0], [7, 70]] = p.max() + 1  # ties share
+    drafts = sample_drafts(rng, q, lanes)
+    print("verify, extreme temperatures", flush=True)
+    for qq in (q, None):
+        check(Dense(mk, p, qq, lanes, drafts, u, un, 2).run().read(), want_dense(p, qq, lanes, drafts, u, un, 2))
 
 
 def test_lanes_that_do_not_fit(mk):
