@@ -1,13 +1,17 @@
 """A speculative step of several users behind one shared prefix, each with an adapter of its own: q|k|v projection, adapters,
 QK-norm + RoPE + KV write, attention over the prefix and the users' rows, LM head, verification of the drafts, whole
 vocabulary and top-k. Every operator is checked against a 64-bit form on the values that it was given, and the whole chain
-captured in one graph gives the eager run's bits."""
+captured in one graph gives the eager run's bits. Two contexts at work at the same time, each call with a workspace of its
+own, do not change each other's results."""
 import ctypes
 
 import numpy as np
 import pytest
 
 import malkin_amd as mk_
+import test_gpu_attn_prefix as prefix
+import test_gpu_lora as adapters
+import test_gpu_verify as drafted
 from operator_cases import EPS, attention64, cut64, lora64, make_cache, softmax64, verify64
 
 pytestmark = pytest.mark.gpu
@@ -129,7 +133,7 @@ def test_step(mk, synth_lib):
     cache = [b.download(t).reshape(a.shape) for b, a, t in zip(kv_b, kv, (np.int8, np.int8, np.float32, np.float32))]
     want, tol = attention64(r["qkv"][:, :H * D], H, pre, 1, P, cache, 0, 0, seq, keys)
     assert (np.abs(r["att"] - want) <= tol).all()
-    # Verification, on the logits.
+    # Verification, on the logits; the cut's weights, their quotient and the result are each rounded to floats.
     order = np.arange(V)
     tv, ti = get("tv", n, 40), get("ti", n, 40, dtype=np.int32)
     u, un = d["u"].download(np.float64), d["un"].download(np.float64)
@@ -164,3 +168,39 @@ def test_step(mk, synth_lib):
             for y, z in zip(a[k], b[k]):
                 assert np.array_equal(np.asarray(y).view(np.uint8), np.asarray(z).view(np.uint8)), k
     assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
+def test_two_contexts_at_once(mk):
+    other, lib, jobs = mk_.Context(0), mk_.load(), []
+    for i, m in enumerate((mk, other)):
+        rng = np.random.default_rng(i)
+        q, pre, kv, seq, keys = prefix.build(rng, 32, 8, 128, [1] * 8, 900, [60 + 9 * j for j in range(8)], 0)
+        att = prefix.Call(m, q, 32, pre, 1, 900, kv, 0, 1, seq, keys, max(keys))
+        ids, ranks = [0, 1, -1, 2] * 5, [16, 8, 32]
+        x = rng.standard_normal((20, 512)).astype(np.float32)
+        table = adapters.Set(m, rng, "f16", ranks, 1024, 512)
+        _, lora, keep = adapters.call(m, "f16", table, 3, 32, ids, x, 1024, rng.standard_normal((20, 1024)).astype(np.float32))
+        counts = [3, 1, 0, 2]
+        lanes = drafted.lanes_of(counts, [0.7, 0.0, 1.0, 1.3])
+        p, w, u, un = drafted.inputs(rng, counts, 20000)
+        ver = drafted.Dense(m, p, w, lanes, drafted.sample_drafts(rng, w, lanes), u, un, 3)
+
+        def run(att=att, lora=lora, ver=ver):
+            att.run()
+            mk_.check(lib.mk_lora(*lora))
+            ver.run()
+
+        def read(att=att, keep=keep, ver=ver, table=table):
+            return [att.result(), keep[3].download(np.float32), *ver.read()]
+
+        run()
+        jobs.append((run, read, read()))
+    print("two contexts", flush=True)
+    for _ in range(50):
+        for run, _, _ in jobs:
+            run()
+    for _, read, alone in jobs:
+        for a, b in zip(alone, read()):
+            assert np.array_equal(a, b)
+    del jobs, att, keep, ver, table, run, read
+    other.close()
