@@ -11,8 +11,9 @@
 // the next token comes from; a lane's last workgroup to finish finds the block and the token.
 //
 // Measured (k_rows + k_excess, 151936 tokens): one lane of 4 drafts with a draft model 5 + 12 us, which is latency (a chain
-// of about eight loads from memory); 24 lanes of up to 8 drafts 40 + 19 us: 30 million 64-bit powers of about 16
-// instructions, over 120 MB, 3 TB/s; 16 lanes of up to 5 drafts without a model 15 + 17.5 us.
+// of about eight loads from memory); 24 lanes of up to 8 drafts 40 + 19 us: 37 million logits, 150 MB, at 3.7 TB/s with
+// the vector units busy for 58 % of the cycles (about 20 instructions a logit, 12 of them 64-bit); 16 lanes of up to 5
+// drafts without a model 15 + 17.5 us.
 #include <cfloat>
 
 #include "ctx.h"
