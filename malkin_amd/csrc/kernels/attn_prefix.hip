@@ -441,24 +441,25 @@ __global__ __launch_bounds__(kThreads, 3) void k_prefix_parts(PrefixAttn A, Spli
   }
 }
 
-// One wave per query row: the parts that its keys reach, added.
-template <int D>
+// W waves per query row: the parts that its keys reach, added. Wave w of a row takes every W-th part, at most kAhead of them,
+// and asks for all at once.
+template <int D, int W, int kAhead>
 __global__ __launch_bounds__(kThreads) void k_prefix_join(PrefixAttn A, Split S, const float* __restrict__ po,
                                                           const Sum* __restrict__ pml, float* __restrict__ out,
                                                           int64_t out_stride, BlockQ8* __restrict__ xq) {
-  constexpr int E = D / 64, kAhead = 8;
-  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % W, row = blockIdx.x * (4 / W) + wave / W;
   if (row >= A.n * A.H) return;
   const int t = row / A.H, head = row % A.H, parts = S.np + S.no;
-  // Everything is asked for at once: parts that the row's keys do not reach hold nothing of use, and have no weight.
+  // Parts that the row's keys do not reach hold nothing of use, and have no weight.
   const int64_t step = (int64_t)A.n * A.H;
   const float* mine_o = po + (int64_t)row * D + E * lane;
   float ahead[kAhead][E];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
-    if (i < parts)
+    if (W * i + w < parts)
 #pragma unroll
-      for (int k = 0; k < E; ++k) ahead[i][k] = mine_o[i * step * D + k];
+      for (int k = 0; k < E; ++k) ahead[i][k] = mine_o[(W * i + w) * step * D + k];
   Sum mine = lane < parts ? pml[lane * step + row] : Sum{};
   const int seq = A.seq[t];
   const int keys = seq >= 0 && seq < A.n_seq ? max(0, min(A.n_keys[t], A.max_keys)) : 0;
@@ -466,7 +467,7 @@ __global__ __launch_bounds__(kThreads) void k_prefix_join(PrefixAttn A, Split S,
                                 : lane < parts && (int64_t)A.n_prefix + (int64_t)(lane - S.np) * S.co < keys;
   if (!live) mine = Sum{kNone, kNone, 0.0f, 0.0f};
   const uint64_t all = __ballot(live);
-  float v[E];
+  float v[E], sum = 1.0f;
 #pragma unroll
   for (int i = 0; i < E; ++i) v[i] = 0.0f;
   if (all) {
@@ -478,26 +479,32 @@ __global__ __launch_bounds__(kThreads) void k_prefix_join(PrefixAttn A, Split S,
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const float f = __builtin_amdgcn_exp2f(mm - top);
-    float sum = f * mine.l;
+    sum = f * mine.l;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-      if ((all >> i) & 1) {
-        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+      if ((all >> (W * i + w)) & 1) {
+        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), W * i + w));
 #pragma unroll
         for (int k = 0; k < E; ++k) v[k] = fma_(fi, ahead[i][k], v[k]);
       }
-#pragma unroll 4
-    for (int i = kAhead; i < parts; ++i)
-      if ((all >> i) & 1) {
-        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
-#pragma unroll
-        for (int k = 0; k < E; ++k) v[k] = fma_(fi, mine_o[i * step * D + k], v[k]);
-      }
-#pragma unroll
-    for (int k = 0; k < E; ++k) v[k] = v[k] / sum;
   }
+  if constexpr (W > 1) {
+    __shared__ float part[W - 1][D];
+    static_assert(W == 4, "one row per workgroup");
+    if (w)
+#pragma unroll
+      for (int k = 0; k < E; ++k) part[w - 1][E * lane + k] = v[k];
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i)
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] += part[i][E * lane + k];
+  }
+#pragma unroll
+  for (int k = 0; k < E; ++k) v[k] = v[k] / sum;
   float* to = out + t * out_stride + head * D + E * lane;
 #pragma unroll
   for (int k = 0; k < E; ++k) to[k] = v[k];
@@ -508,7 +515,10 @@ constexpr int kMaxPre = 48, kMaxOwn = 16;  // a row's parts fit one wave's lanes
 // Workgroups wanted of each kind. The prefix's are long and set up once (q, the join of their waves): one per CU is best
 // (62 users over 8192 + 1024 keys: 43.9 us, with 192 wanted 42.9, with 384 44.6, with 512 46.9; 16 users over 4000 + 300:
 // 16.8, 15.6, 17.0, 21.1). The own rows' are as many as there are (token run, KV head) pairs, and split only where those
-// do not fill the CUs twice (8 users over 1500 + 600 keys: 14.1 us, with 256 wanted 15.2, with 128 14.7).
+// do not fill the CUs twice (8 users over 1500 + 600 keys: 14.1 us, with 256 wanted 15.2, with 128 14.7). A run ends at a
+// multiple of 32 / G tokens or where the next sequence begins, so with n_seq sequences, each one's tokens together, there are
+// at most n G / 32 + n_seq of them (50 drafted tokens of 10 users over 1361 keys: 21.7 us, with n counted instead 26.8; 135 of
+// 45 users over 5851 + 1498: 17.0 and 22.4; other orders are only slower).
 constexpr int kWantedPre = 256, kWantedOwn = 512;
 
 int chunk(int keys, int chunks) {  // keys per chunk, whole tiles for the four waves
@@ -516,12 +526,12 @@ int chunk(int keys, int chunks) {  // keys per chunk, whole tiles for the four w
   return std::max(1, (c + kWaves * kKeys - 1) / (kWaves * kKeys)) * kWaves * kKeys;
 }
 
-Split split_of(int n, int H, int KV, int n_prefix, int max_keys) {
+Split split_of(int n, int H, int KV, int n_prefix, int max_keys, int n_seq) {
   Split s{};
-  const int G = H / KV;
+  const int G = H / KV, tq = std::max(1, kRows / G);
   s.tiles = (int)(((int64_t)n * G + kRows - 1) / kRows);
   const int pre = std::min(n_prefix, max_keys), own = std::max(0, max_keys - n_prefix);
-  const int64_t pre_wgs = (int64_t)s.tiles * KV, own_wgs = (int64_t)n * KV;
+  const int64_t pre_wgs = (int64_t)s.tiles * KV, own_wgs = std::min<int64_t>(n, (n + (int64_t)tq - 1) / tq + n_seq) * KV;
   s.cp = chunk(pre, (int)std::min<int64_t>(kMaxPre, std::max<int64_t>(1, kWantedPre / pre_wgs)));
   s.np = (pre + s.cp - 1) / s.cp;
   s.co = chunk(own, (int)std::min<int64_t>(kMaxOwn, std::max<int64_t>(1, kWantedOwn / own_wgs)));
@@ -533,13 +543,13 @@ Split split_of(int n, int H, int KV, int n_prefix, int max_keys) {
 }  // namespace
 
 size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int max_keys) {
-  const Split s = split_of(n, H, KV, n_prefix, max_keys);
+  const Split s = split_of(n, H, KV, n_prefix, max_keys, 0);
   return (size_t)s.parts * (D * sizeof(float) + sizeof(Sum));
 }
 
 void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q, int64_t q_stride, float* out,
                       int64_t out_stride, BlockQ8* xq, void* workspace) {
-  const Split S = split_of(A.n, A.H, A.KV, A.n_prefix, A.max_keys);
+  const Split S = split_of(A.n, A.H, A.KV, A.n_prefix, A.max_keys, A.n_seq);
   float* po = static_cast<float*>(workspace);
   Sum* pml = reinterpret_cast<Sum*>(po + S.parts * D);
   const int tq = kRows / (A.H / A.KV);
@@ -552,9 +562,19 @@ void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q,
                          pml);
       check_launch("attention_prefix parts");
     }
-    hipLaunchKernelGGL(k_prefix_join<D_>, dim3((unsigned)(((int64_t)A.n * A.H + 3) / 4)), dim3(kThreads), 0, s, A, S, po,
-                       pml, out, out_stride, xq);
-    check_launch("attention_prefix join");
+    const int64_t rows = (int64_t)A.n * A.H;
+    auto join = [&]<int W, int kAhead>() {
+      hipLaunchKernelGGL((k_prefix_join<D_, W, kAhead>), dim3((unsigned)((rows * W + 3) / 4)), dim3(kThreads), 0, s, A, S, po, pml,
+                         out, out_stride, xq);
+      check_launch("attention_prefix join");
+    };
+    // One round trip whatever the number of parts; with eight asked for at once and the others four at a time, one token
+    // behind 8682 keys (35 parts of 8 rows) took 18.4 us a pass instead of 12.6, 16 tokens behind 4000 + 300 (19 parts of
+    // 512 rows) 17.0 instead of 16.2. Four waves from nine parts on: 17.5 there, 24 parts ahead for one wave everywhere: the
+    // registers of the small ones.
+    if (S.np + S.no <= 8) join.template operator()<1, 8>();
+    else if (S.np + S.no <= 24) join.template operator()<1, 24>();
+    else join.template operator()<4, 16>();
   };
   if (D == 128) go.template operator()<128>();
   else go.template operator()<64>();
