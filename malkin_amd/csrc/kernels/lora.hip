@@ -196,7 +196,7 @@ __device__ void shrink(const Group& g, const int* tokens, const float* __restric
     for (int k = 0; k < NT; ++k) acc[i][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   auto walk = [&](auto vec_) __attribute__((always_inline)) {
     constexpr bool V = decltype(vec_)::value;
-#pragma unroll(V ? 2 : 1)
+#pragma unroll 2
     for (int64_t k = k0 + kStep * w; k < k1; k += kStep * kShrinkWaves) {
       const int valid = within(k1 - k - 8 * lq, 8);
       const int64_t at = valid ? k + 8 * lq : k0;
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __re
     while (f < 4 && (used << (f + 1)) <= kThreads) ++f;
     const int part = threadIdx.x & ((1 << f) - 1);
 #pragma unroll 1
-    for (int i0 = 0; i0 < items; i0 += kThreads >> f) {
+    for (int i0 = 0; i0 < used; i0 += kThreads >> f) {
       const int i = i0 + (threadIdx.x >> f), c = i / quads, r = 4 * (i - c * quads);
       v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
       if (i < used) {
@@ -325,8 +325,10 @@ __global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __re
       for (int m = 1; m < 1 << f; m <<= 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k) s[k] += __shfl_xor(s[k], m);
-      if (i < items && part == 0) *reinterpret_cast<v4f*>(hs + c * hst + r) = s * g.a.scale;
+      if (i < used && part == 0) *reinterpret_cast<v4f*>(hs + c * hst + r) = s * g.a.scale;
     }
+    for (int i = used + threadIdx.x; i < items; i += kThreads)
+      *reinterpret_cast<v4f*>(hs + i / quads * hst + 4 * (i % quads)) = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     __syncthreads();
   }
   if (row0 >= rows) return;
