@@ -77,7 +77,8 @@ __device__ __forceinline__ void get(global<T>* p, int valid, bool vec, float (&r
 #pragma unroll
   for (int i = 0; i < N; ++i) r[i] = i < valid ? to_f(T{(uint16_t)(v[i / 2] >> (16 * (i & 1)))}) : 0.0f;
 }
-// Values at .. at + 3 of a row of `rank`, as they lie in memory; 0 past its end.
+// Values at .. at + 3 of a row of `rank`, as they lie in memory; 0 past its end. VEC: rank is a multiple of four, the row
+// aligned to four values.
 template <typename T>
 struct Raw {
   typedef uint2 type;
@@ -86,17 +87,18 @@ template <>
 struct Raw<float> {
   typedef v4f type;
 };
-__device__ __forceinline__ v4f get_raw(global<float>* row, int at, int rank, bool vec) {
+template <bool VEC>
+__device__ __forceinline__ v4f get_raw(global<float>* row, int at, int rank) {
   float r[4];
-  get<4>(row + (at < rank ? at : 0), max(min(rank - at, 4), 0), vec, r);
+  get<4>(row + (at < rank ? at : 0), max(min(rank - at, 4), 0), VEC, r);
   return v4f{r[0], r[1], r[2], r[3]};
 }
-template <typename T>
-__device__ __forceinline__ uint2 get_raw(global<T>* row, int at, int rank, bool vec) {
+template <bool VEC, typename T>
+__device__ __forceinline__ uint2 get_raw(global<T>* row, int at, int rank) {
   typedef uint32_t two __attribute__((ext_vector_type(2)));
   global<uint16_t>* q = reinterpret_cast<global<uint16_t>*>(row);
   two v;
-  if (vec) {
+  if constexpr (VEC) {
     v = *reinterpret_cast<global<two>*>(q + (at < rank ? at : 0));
     if (at >= rank) v = two{0, 0};
   } else {
@@ -256,12 +258,14 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void k_shrink(const mk_lora_adap
 // through LDS, so that base is read and y written 256 bytes of a token at a time. (512 rows per workgroup: 10.2 / 22.7 /
 // 36.6 us for the three calls above instead of 10.8 / 19.9 / 38.4, and no room for rank 512.) The code is kept short
 // (rolled loops): a workgroup runs most of it once, and instruction fetches that miss would cost more than the arithmetic.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __restrict__ adapters, int n_adapters,
+// YV: rows of y and base are aligned to four floats, and of a multiple of four. The loop over the tokens has no branches of
+// a lane's own but its stores: with them every turn waited for the stores of the one before.
+template <typename T, bool YV>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) void k_expand(const mk_lora_adapter* __restrict__ adapters, int n_adapters,
                                                      int max_rank, const int32_t* __restrict__ ids, int windows, int slots,
                                                      int n, int64_t rows, const float* __restrict__ h, int r_pad, int splits,
-                                                     const float* base, int64_t base_stride, float* y, int64_t y_stride,
-                                                     bool y_vec) {
+                                                     const float* base, int64_t base_stride, float* y,
+                                                     int64_t y_stride) {
   constexpr int kOut = 64 + 4;  // a token's stride in `out`
   __shared__ int tokens[kWindow];
   __shared__ __align__(16) float out_s[4][16 * kOut];
@@ -273,15 +277,25 @@ __global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __re
   const int64_t row0 = (int64_t)(blockIdx.x / windows) * kRowBlock + 64 * w, row = row0 + 4 * li;
   const int valid = within(rows - row, 4);
   const bool b_vec = (rank & 3) == 0 && ((uintptr_t)g.a.b & (4 * sizeof(T) - 1)) == 0;
-  // A tile of tokens: its base (lane: token 4 k + lq, four rows from 4 li).
+  // A tile of tokens (those past the last: the last) and its base; lane: token 4 k + lq, four rows from 4 li.
   auto load_base = [&](int c0, v4f(&v)[4], int(&tok)[4]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int c = c0 + 4 * k + lq;
-      tok[k] = c < g.count ? tokens[c] : -1;
-      float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (base && valid && tok[k] >= 0) get<4>(to_global<float>(base + tok[k] * base_stride + row), valid, y_vec, q);
-      v[k] = v4f{q[0], q[1], q[2], q[3]};
+    for (int k = 0; k < 4; ++k) tok[k] = tokens[min(c0 + 4 * k + lq, g.count - 1)];
+    if (base) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        global<float>* p = to_global<float>(base + tok[k] * base_stride + (valid ? row : 0));
+        if constexpr (YV) {
+          v[k] = *reinterpret_cast<global<v4f>*>(p);
+        } else {
+          float q[4];
+          get<4>(p, valid, false, q);
+          v[k] = v4f{q[0], q[1], q[2], q[3]};
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
   };
   // 64 ranks of the wave's rows of B, four of a row per lane and step, as they lie in memory.
@@ -289,12 +303,20 @@ __global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __re
   raw bw[4][4];
   global<T>* b[4];
   auto load_b = [&](int r) __attribute__((always_inline)) {
+    if (b_vec) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (r + 16 * s >= rank) break;
-      const int at = r + 16 * s + 4 * lq;
+      for (int s = 0; s < 4; ++s) {
+        if (r + 16 * s >= rank) break;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bw[s][i] = get_raw(b[i], at, rank, b_vec);
+        for (int i = 0; i < 4; ++i) bw[s][i] = get_raw<true>(b[i], r + 16 * s + 4 * lq, rank);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if (r + 16 * s >= rank) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bw[s][i] = get_raw<false>(b[i], r + 16 * s + 4 * lq, rank);
+      }
     }
   };
   // What does not wait for h is asked for first.
@@ -365,14 +387,14 @@ __global__ __launch_bounds__(kThreads) void k_expand(const mk_lora_adapter* __re
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (tok[k] < 0) continue;
+      const bool on = c0 + 4 * k + lq < g.count;
       float* to = y + tok[k] * y_stride + row;
-      if (y_vec) {
-        if (valid) *reinterpret_cast<v4f*>(to) = now[k];
+      if constexpr (YV) {
+        if (on && valid) *reinterpret_cast<v4f*>(to) = now[k];
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (e < valid) to[e] = now[k][e];
+          if (on && e < valid) to[e] = now[k][e];
       }
     }
 #pragma unroll
@@ -420,9 +442,13 @@ void lora(hipStream_t s, int type, const mk_lora_adapter* adapters, int n_adapte
                          slots, x, x_stride, n, cols, per, x_vec, h, r_pad);
       check_launch("lora shrink");
     }
-    allow_lds<k_expand<T>>(kWindow * (512 + 4) * sizeof(float));
-    hipLaunchKernelGGL(k_expand<T>, g2, dim3(kThreads), lds, s, adapters, n_adapters, max_rank, ids, windows, slots, n,
-                       rows, h, r_pad, splits, base, base_stride, y, y_stride, y_vec);
+    auto expand = [&]<bool YV>() {
+      allow_lds<k_expand<T, YV>>(kWindow * (512 + 4) * sizeof(float));
+      hipLaunchKernelGGL((k_expand<T, YV>), g2, dim3(kThreads), lds, s, adapters, n_adapters, max_rank, ids, windows, slots,
+                         n, rows, h, r_pad, splits, base, base_stride, y, y_stride);
+    };
+    if (y_vec) expand.template operator()<true>();
+    else expand.template operator()<false>();
     check_launch("lora expand");
   };
   if (type == MK_F32) go.template operator()<float>();
