@@ -519,23 +519,34 @@ constexpr int kMaxPre = 48, kMaxOwn = 16;  // a row's parts fit one wave's lanes
 // multiple of 32 / G tokens or where the next sequence begins, so with n_seq sequences, each one's tokens together, there are
 // at most n G / 32 + n_seq of them (50 drafted tokens of 10 users over 1361 keys: 21.7 us, with n counted instead 26.8; 135 of
 // 45 users over 5851 + 1498: 17.0 and 22.4; other orders are only slower).
-constexpr int kWantedPre = 256, kWantedOwn = 512;
+//
+// Long chunks of the prefix go two to a CU, or nearly, where a third place is left for the own rows' (400 prompt tokens of
+// 16 heads behind 8000 keys: 85 us instead of 92 .. 95, 150 of 40 heads behind 9000 92 instead of 104; without room 399
+// tokens of 57 users behind 4743 + 1157 51 instead of 48, with short chunks 12 users behind 8000 20 instead of 16, with
+// few more 40 users behind 12000 35 instead of 32.4).
+constexpr int kWantedPre = 256, kWantedOwn = 512, kLongChunk = 1536;
 
 int chunk(int keys, int chunks) {  // keys per chunk, whole tiles for the four waves
   const int c = (keys + chunks - 1) / chunks;
   return std::max(1, (c + kWaves * kKeys - 1) / (kWaves * kKeys)) * kWaves * kKeys;
 }
 
+// n_seq < 0: the most parts, whatever it is.
 Split split_of(int n, int H, int KV, int n_prefix, int max_keys, int n_seq) {
   Split s{};
   const int G = H / KV, tq = std::max(1, kRows / G);
   s.tiles = (int)(((int64_t)n * G + kRows - 1) / kRows);
   const int pre = std::min(n_prefix, max_keys), own = std::max(0, max_keys - n_prefix);
-  const int64_t pre_wgs = (int64_t)s.tiles * KV, own_wgs = std::min<int64_t>(n, (n + (int64_t)tq - 1) / tq + n_seq) * KV;
-  s.cp = chunk(pre, (int)std::min<int64_t>(kMaxPre, std::max<int64_t>(1, kWantedPre / pre_wgs)));
-  s.np = (pre + s.cp - 1) / s.cp;
+  const int64_t pre_wgs = (int64_t)s.tiles * KV;
+  const int64_t own_wgs = std::min<int64_t>(n, (n + (int64_t)tq - 1) / tq + std::max(n_seq, 0)) * KV;
   s.co = chunk(own, (int)std::min<int64_t>(kMaxOwn, std::max<int64_t>(1, kWantedOwn / own_wgs)));
   s.no = (own + s.co - 1) / s.co;
+  int64_t chunks = std::max<int64_t>(1, kWantedPre / pre_wgs);
+  const int64_t more = std::min<int64_t>(2 * kWantedPre / pre_wgs, pre / kLongChunk);
+  if (2 * more * pre_wgs >= 3 * kWantedPre && (n_seq < 0 || more * pre_wgs + own_wgs <= 3 * kWantedPre))
+    chunks = std::max(chunks, more);
+  s.cp = chunk(pre, (int)std::min<int64_t>(kMaxPre, chunks));
+  s.np = (pre + s.cp - 1) / s.cp;
   s.parts = (int64_t)(s.np + s.no) * n * H;
   return s;
 }
@@ -543,7 +554,7 @@ Split split_of(int n, int H, int KV, int n_prefix, int max_keys, int n_seq) {
 }  // namespace
 
 size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int max_keys) {
-  const Split s = split_of(n, H, KV, n_prefix, max_keys, 0);
+  const Split s = split_of(n, H, KV, n_prefix, max_keys, -1);
   return (size_t)s.parts * (D * sizeof(float) + sizeof(Sum));
 }
 

@@ -70,6 +70,8 @@ CASES = [
     (16, 8, 128, [1, 1], 5000, [700, 1], 0),
     (6, 2, 128, [4, 4], 0, [40, 4], 0),               # no prefix
     (4, 4, 64, [1], 0, [1], 0),
+    (8, 8, 64, [770], 3333, [770], 0),                # long chunks, two workgroups a CU
+    (8, 2, 128, [5] * 10, 92, [300 + 13 * i for i in range(10)], 0),  # runs of drafts, their own rows split
 ]
 
 
