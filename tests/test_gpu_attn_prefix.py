@@ -144,6 +144,26 @@ def test_rows_without_keys_and_inside_the_prefix(mk, d):
         check(c.result(), want, tol)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_any_order_and_garbage_beside(mk, d):
+    """Tokens of a sequence that do not follow each other, the same token twice, keys in any order; q of padded rows is
+    NaN or infinite, and one live token's is: only its own row shows it."""
+    rng = np.random.default_rng(5)
+    H, KV, P = 8, 2, 150
+    q, pre, kv, _, _ = build(rng, H, KV, d, [1] * 20, P, [90] * 20, 0)
+    seq = [0, 1, 0, 1, 2, 2, 1, 0, 0, 5, 5, 4, 5, 4, 3, 3, 3, 3, 0, 1]
+    keys = [240, 160, 200, 239, 10, 240, 0, 151, 240, 170, 169, 168, 0, 240, 200, 199, 198, 200, 0, 150]
+    want, tol = attention64(q, H, pre, 1, P, kv, 0, 1, seq, keys)
+    for i, bad in ((6, np.nan), (12, np.inf), (18, -np.inf), (9, np.nan), (15, np.inf)):
+        q[i, 3::7] = bad
+    c = Call(mk, q, H, pre, 1, P, kv, 0, 1, seq, keys, 240)
+    print("prefix attention, any order", d, flush=True)
+    c.run()
+    got, ok = c.result(), [i for i in range(20) if i not in (9, 15)]
+    check(got[ok], want[ok], tol[ok])
+    assert (got[[6, 12, 18]] == 0).all() and np.isnan(got[[9, 15]]).any(axis=1).all()
+
+
 def test_prefix_in_the_same_cache_agrees_with_attention(mk):
     """Sequences that all hold the prefix's rows: mk_attention's results, by another order of the sums."""
     rng = np.random.default_rng(8)

@@ -128,6 +128,26 @@ def test_strides_and_alignment(mk, kind, off, pads):
         check(got, want, tol)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+def test_one_token_shows_nothing_of_another(mk, kind):
+    """A token of NaN or infinities, beside others of the same adapter and of others, changes its own row alone."""
+    rng = np.random.default_rng(11)
+    ranks, rows, cols = [16, 40], 300, 544
+    ids = [0, 1, 0, -1, 1, 0, 0] * 4
+    s = Set(mk, rng, kind, ranks, rows, cols)
+    x = rng.standard_normal((len(ids), cols)).astype(np.float32)
+    base = rng.standard_normal((len(ids), rows)).astype(np.float32)
+    want, tol = lora64(x, s.host, ids, base, rows)
+    x[2, 5:], x[11], x[10, ::3], base[13, ::2] = np.nan, np.inf, np.nan, np.nan
+    print("lora, one token of NaN", kind, flush=True)
+    ok = [i for i in range(len(ids)) if i not in (2, 11, 13)]  # token 10 has no adapter
+    for in_place in (False, True):
+        got, _, _ = call(mk, kind, s, 2, 40, ids, x, rows, base, in_place=in_place)
+        check(got[ok], want[ok], tol[ok])
+        assert not np.isfinite(got[[2, 11]]).any() and np.isnan(got[13, ::2]).all()
+        check(got[13, 1::2], want[13, 1::2], tol[13, 1::2])
+
+
 def test_entries_that_take_no_part(mk):
     """Ranks of 0, negative or past max_rank, ids outside the table: the base as it is, its -0 and NaN included."""
     rng = np.random.default_rng(4)
