@@ -349,7 +349,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) void k_expand(con
       for (int m = 1; m < 1 << f; m <<= 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k) s[k] += __shfl_xor(s[k], m);
-      if (i < used && part == 0) *reinterpret_cast<v4f*>(hs + c * hst + r) = s * g.a.scale;
+      // Ranks past the last are 0 times x in h, which is NaN where x is infinite, and meet B's padding of 0.
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] = r + k < rank ? s[k] * g.a.scale : 0.0f;
+      if (i < used && part == 0) *reinterpret_cast<v4f*>(hs + c * hst + r) = s;
     }
     for (int i = used + threadIdx.x; i < items; i += kThreads)
       *reinterpret_cast<v4f*>(hs + i / quads * hst + 4 * (i % quads)) = v4f{0.0f, 0.0f, 0.0f, 0.0f};

@@ -197,3 +197,27 @@ def test_captured_and_replayed(mk):
         mk_.check(mk_.load().mk_lora(*args))
         assert np.array_equal(got.view(np.uint32), keep[3].download(np.uint32).reshape(n, rows))
     assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("ranks", [[1], [8, 3], [16, 20]])
+def test_infinite_x(mk, ranks, kind):
+    """Infinities in a token give what the formula gives, infinities with their sign or NaN, at ranks that no tile of
+    sixteen fills too; the other tokens of the adapter are as without them."""
+    rng = np.random.default_rng(21)
+    rows, cols, n = 272, 160, 40
+    s = Set(mk, rng, kind, ranks, rows, cols)
+    ids = [t % len(ranks) for t in range(n)]
+    x = rng.standard_normal((n, cols)).astype(np.float32)
+    base = rng.standard_normal((n, rows)).astype(np.float32)
+    want, tol = lora64(x, s.host, ids, base, rows)
+    for t, c in ((0, 0), (5, 7), (18, cols - 1), (39, 64)):
+        x[t, c] = np.inf if t % 2 else -np.inf
+        with np.errstate(invalid="ignore"):
+            want[t], _ = lora64(x[t:t + 1], s.host, ids[t:t + 1], base[t:t + 1], rows)
+    print("lora, infinite x", ranks, kind, flush=True)
+    got, _, _ = call(mk, kind, s, len(ranks), max(ranks), ids, x, rows, base)
+    odd = ~np.isfinite(want)
+    assert odd[[0, 5, 18, 39]].all() and odd.sum() == 4 * rows and (ranks != [1] or np.isinf(want[odd]).all())
+    assert np.array_equal(got[odd].astype(np.float64), want[odd], equal_nan=True)
+    check(got[~odd], want[~odd], tol[~odd])
