@@ -405,7 +405,10 @@ int mk_verify(mk_ctx* ctx, const float* p, int64_t p_stride, int n_rows, const f
               size_t workspace_bytes);
 /* The same over rows cut to their candidates, highest first (mk_topk's values / ids; p_k, q_k 1..1024 per row): P and Q
    are the distributions mk_sample_draw draws from (float weights, min_p floor, top_p nucleus, float probabilities),
-   matched by id, and the next token is drawn in the candidates' order. q_values and q_ids both NULL: certain drafts. */
+   matched by id, and the next token is drawn in the candidates' order. q_values and q_ids both NULL: certain drafts. The
+   weights' 64-bit totals are added in another order than mk_sample_draw's, so the nucleus can end at another candidate
+   where a running sum is within 2^-50 of top_p. Logits as above: the highest candidate is the first that is not NaN
+   (mk_topk puts NaN ahead of the others) or -inf, and those have no part in the cut. */
 int mk_verify_topk(mk_ctx* ctx, const float* p_values, const int32_t* p_ids, int p_k, int n_rows, const float* q_values,
                    const int32_t* q_ids, int q_k, int n_drafts, const mk_verify_lane* lanes, int n_lanes, int max_draft,
                    const int32_t* drafts, const double* u, const double* u_next, int32_t* accepted, int32_t* tokens,

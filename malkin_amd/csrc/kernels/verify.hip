@@ -523,44 +523,61 @@ struct Cands {
   const int32_t* ids;
   int k, n;  // candidates per row, rows
 };
-struct Head {  // what of a row of candidates is kept: the first `keep`, of total weight `sum`
+struct Head {  // what of a row of candidates is kept: the first `keep`, of total weight `sum`; 0: nothing but -inf
   double sum;
   int32_t keep;
+  int32_t first;  // the highest candidate, behind those of NaN, which mk_topk puts ahead of the others
+  float top;      // its logit
 };
 
+// A candidate of v against the highest one, both clean: one of -inf has no weight (top is finite).
 __device__ __forceinline__ double cand_weight(float v, float top, float t) {
   return (double)(float)exp((double)((v - top) / t));
 }
 
-// One wave: the kept head (sampler.cpp:37-56), 64 candidates at a time, their running sums by a scan.
-__device__ __forceinline__ Head head_of(const float* v, int k, const mk_verify_lane& L) {
+// One wave: the kept head (sampler.cpp:37-56), 64 candidates at a time, their running sums by a scan. t: the lane's
+// temperature, at most FLT_MAX; 0: greedy.
+__device__ __forceinline__ Head head_of(const float* v, int k, const mk_verify_lane& L, float t) {
   const int lane = threadIdx.x & 63;
-  if (!(L.temperature > 0.0f)) return Head{1.0, 1};
-  const float top = v[0];
-  double all = 0.0;
-  for (int c = 0; c < k; c += 64)
-    all += wave_sum(c + lane < k ? cand_weight(v[c + lane], top, L.temperature) : 0.0);
-  const double floor_w = (double)L.min_p * cand_weight(top, top, L.temperature), nucleus = (double)L.top_p * all;
+  auto logit = [&](int i) { return i < k ? clean(v[i]) : -INFINITY; };
+  const float z0 = logit(lane);
+  int from = 0;
+  float z = z0;
+  uint64_t some = __ballot(z > -INFINITY);
+  while (!some) {
+    if ((from += 64) >= k) return Head{1.0, 0, 0, 0.0f};
+    z = logit(from + lane), some = __ballot(z > -INFINITY);
+  }
+  const int first = from + __builtin_ctzll(some);
+  const float top =
+      __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, z), __builtin_ctzll(some)));
+  if (!(t > 0.0f)) return Head{1.0, first + 1, first, top};
+  const double w0 = cand_weight(z0, top, t);
+  double all = wave_sum(w0);
+  for (int c = 64; c < k; c += 64) all += wave_sum(cand_weight(logit(c + lane), top, t));
+  const double floor_w = (double)L.min_p, nucleus = (double)L.top_p * all;  // the first weight is 1
   double run = 0.0;
   for (int c = 0; c < k; c += 64) {
     const int i = c + lane;
-    const double w = i < k ? cand_weight(v[i], top, L.temperature) : 0.0;
-    const double scan = wave_scan(w) + run;
-    const uint64_t below = __ballot(i < k && i > 0 && w < floor_w), reach = __ballot(i < k && scan >= nucleus);
+    z = c ? logit(i) : z0;
+    const double w = c ? cand_weight(z, top, t) : w0, scan = wave_scan(w) + run;
+    const uint64_t below = __ballot(i > first && z > -INFINITY && w < floor_w),
+                   reach = __ballot(i < k && i >= first && scan >= nucleus);
     const int b = below ? __builtin_ctzll(below) : 64, e = reach ? __builtin_ctzll(reach) : 64;
     if (b < 64 || e < 64) {
       // Candidate b is not kept, candidate e is the last; one that is both is below the floor.
       const int last = b <= e ? b - 1 : e;  // in this chunk; -1: the chunk before's last
-      return Head{last < 0 ? run : __shfl(scan, last), c + last + 1};
+      return Head{last < 0 ? run : __shfl(scan, last), c + last + 1, first, top};
     }
     run = __shfl(scan, min(63, k - 1 - c));
   }
-  return Head{run, k};
+  return Head{run, k, first, top};
 }
 
-__device__ __forceinline__ float cand_prob(const Head& h, float v, float top, int i, float t) {
+// Candidate i's probability in the row v.
+__device__ __forceinline__ float cand_prob(const Head& h, const float* v, int i, float t) {
   if (i >= h.keep) return 0.0f;
-  return t > 0.0f ? (float)(cand_weight(v, top, t) / h.sum) : 1.0f;
+  return t > 0.0f ? (float)(cand_weight(clean(v[i]), h.top, t) / h.sum) : i == h.first ? 1.0f : 0.0f;
 }
 
 // Probability of token d in a row (sampler.cpp prob_in), by one wave.
@@ -570,14 +587,14 @@ __device__ __forceinline__ float prob_in(const float* v, const int32_t* ids, con
     const uint64_t hit = __ballot(c + lane < h.keep && ids[c + lane] == d);
     if (hit) {
       const int i = c + __builtin_ctzll(hit);
-      return cand_prob(h, v[i], v[0], i, t);
+      return cand_prob(h, v, i, t);
     }
   }
   return 0.0f;
 }
 
 // One workgroup per lane: the rows' heads in turn over the waves, each with the probability of the draft it judges;
-// then wave 0 draws the next token. Latency: 32 lanes of up to 8 drafts and 40 candidates a row 8.2 us.
+// then wave 0 draws the next token. Latency: 32 lanes of up to 8 drafts and 40 candidates a row 7.9 us a pass.
 __global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, const mk_verify_lane* __restrict__ lanes,
                                                               int max_draft, int n_drafts,
                                                               const int32_t* __restrict__ drafts,
@@ -596,14 +613,14 @@ __global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, 
   __shared__ int32_t q_id[kMaxK];
   __shared__ float q_pr[kMaxK];
   if (tid == 0) stop_s = ok ? L.n_draft : -1;
-  const float t = L.temperature;
+  const float t = L.temperature > 0.0f ? fminf(L.temperature, FLT_MAX) : 0.0f;
   const int rows = ok ? L.n_draft + 1 + (Q.values ? L.n_draft : 0) : 0;
   for (int r = w; r < rows; r += kTopkThreads / 64) {
     const bool draft = r > L.n_draft;
     const int j = draft ? r - L.n_draft - 1 : r, k = draft ? Q.k : P.k;
     const int64_t at = draft ? (int64_t)(L.first + j) * Q.k : (int64_t)(L.row + j) * P.k;
     const float* v = (draft ? Q.values : P.values) + at;
-    const Head h = head_of(v, k, L);
+    const Head h = head_of(v, k, L, t);
     const float p = j < L.n_draft ? prob_in(v, (draft ? Q.ids : P.ids) + at, h, drafts[L.first + j], t) : 0.0f;
     if (lane == 0) head_s[r] = h, prob_s[r] = p;
   }
@@ -631,7 +648,7 @@ __global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, 
     q_n = qh.keep;
     for (int i = tid; i < q_n; i += kTopkThreads) {
       q_id[i] = Q.ids[at + i];
-      q_pr[i] = cand_prob(qh, Q.values[at + i], Q.values[at], i, t);
+      q_pr[i] = cand_prob(qh, Q.values + at, i, t);
     }
   } else if (refused) {
     q_n = 1;
@@ -648,14 +665,14 @@ __global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, 
     float q = 0.0f;
     for (int k = 0; k < q_n; ++k)
       if (q_id[k] == id) q = q_pr[k];
-    left_s[i] = fmaxf(cand_prob(ph, pv[i], pv[0], i, t) - q, 0.0f);
+    left_s[i] = fmaxf(cand_prob(ph, pv, i, t) - q, 0.0f);
   }
   __syncthreads();
   if (w != 0) return;
   double total = 0.0;
   bool over = true;
   auto left = [&](int i) {
-    return i >= ph.keep ? 0.0 : over ? (double)left_s[i] : (double)cand_prob(ph, pv[i], pv[0], i, t);
+    return i >= ph.keep ? 0.0 : over ? (double)left_s[i] : (double)cand_prob(ph, pv, i, t);
   };
   for (;;) {
     total = 0.0;
@@ -677,7 +694,7 @@ __global__ __launch_bounds__(kTopkThreads) void k_verify_topk(Cands P, Cands Q, 
   if (pick < 0) pick = last;
   if (lane == 0) {
     tok[n_acc] = pick < 0 ? -1 : pi[pick];
-    if (pr) pr[n_acc] = pick < 0 ? 0.0f : cand_prob(ph, pv[pick], pv[0], pick, t);
+    if (pr) pr[n_acc] = pick < 0 ? 0.0f : cand_prob(ph, pv, pick, t);
   }
 }
 

@@ -142,3 +142,16 @@ def verify64(lane, target, draft, drafts, u, u_next, n_out):
         out.append(int(p[0][i]))
         pr.append(float(p[1][i]))
     return acc, out + [-1] * (n_out - len(out)), pr + [0.0] * (n_out - len(pr))
+
+
+def cut_any64(values, ids, lane):
+    """cut64 of a row with any logits in it: NaN counts as -inf, +inf as the largest float, an infinite temperature as the
+    largest float; what is -inf then is no candidate."""
+    v = np.where(np.isnan(values), -np.inf, np.minimum(values, np.finfo(np.float32).max)).astype(np.float32)
+    on = v > -np.inf
+    if not on.any():
+        return ids[:0], np.zeros(0, np.float32)
+    lane = {k: float(lane[k]) for k in ("temperature", "min_p", "top_p")}
+    lane["temperature"] = min(lane["temperature"], float(np.finfo(np.float32).max))
+    with np.errstate(over="ignore"):
+        return cut64(v[on], ids[on], lane, 0)

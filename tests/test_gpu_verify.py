@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import malkin_amd as mk_
-from operator_cases import EPS, cut64, softmax64, verify64
+from operator_cases import EPS, cut64, cut_any64, softmax64, verify64
 
 pytestmark = pytest.mark.gpu
 
@@ -356,3 +356,72 @@ def test_captured_and_replayed(mk):
         again = c.run().read()
         assert all(np.array_equal(a, b) for a, b in zip(got, again))
     assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
+def highest_first(z, k):
+    """mk_topk's rows: values and ids by the order of their bits, NaN ahead of infinity, then by id."""
+    u = z.view(np.uint32)
+    key = np.where(u >> 31, ~u, u | np.uint32(1 << 31))
+    ids = np.argsort(~key, 1, kind="stable")[:, :k].astype(np.int32)
+    return np.take_along_axis(z, ids, 1), ids
+
+
+@pytest.mark.parametrize("k", [40, 200])
+def test_topk_infinities_and_nan(mk, k):
+    """Candidates' logits by mk_verify's rules: NaN counts as -inf, which is no candidate, +inf as the largest float, a row
+    of nothing but those has no token and refuses every draft, whatever the temperature and the cut."""
+    rng = np.random.default_rng(31)
+    temps = [1.0, 0.0, np.inf, 1e-45]
+    kinds, V = 12, 500
+    counts = [2] * (kinds * len(temps))
+    lanes = lanes_of(counts, np.repeat(np.float32(temps), kinds), 0.05, 0.95)
+    p, q, u, un = inputs(rng, counts, V)
+    for i, l in enumerate(lanes):
+        a, b, kind = l["row"], l["first"], i % kinds
+        u[b:b + 2] = [0.0, 0.3]
+        if kind == 0:                                      # one token has everything
+            p[a, 17] = np.inf
+        elif kind == 1:                                    # three share it
+            p[a:a + 3, [9, 30, 77]] = np.inf
+            q[b:b + 2, [30, 60]] = np.inf
+        elif kind == 2:                                    # NaN ahead of the candidates, more of them than a wave's lanes
+            p[a:a + 3, 40:40 + k // 2] = q[b, 11:20] = np.nan
+        elif kind == 3:                                    # few candidates left
+            p[a:a + 3, 5:] = q[b:b + 2, 7:] = -np.inf
+        elif kind == 4:
+            p[a] = -np.inf
+        elif kind == 5:
+            p[a] = np.nan
+        elif kind == 6:                                    # nothing in the draft's row
+            q[b] = -np.inf
+        elif kind == 7:
+            p[a, 3], q[b, 100:] = np.nan, np.nan
+            lanes["min_p"][i] = 1.0
+        elif kind == 8:
+            p[a, 3] = q[b, 8] = np.nan
+            lanes["top_p"][i] = 0.0
+        elif kind == 9:                                    # the whole of the candidates, infinities of all kinds
+            p[a:a + 3, ::3], p[a:a + 3, 1::3], p[a:a + 3, 4] = -np.inf, np.nan, np.inf
+            lanes["min_p"][i], lanes["top_p"][i] = 0.0, 1.0
+        elif kind == 10:                                   # negative NaN, the last of all
+            p[a:a + 3, ::2] = np.uint32(0xFFC00000).view(np.float32)
+        else:
+            p[a + 1:a + 3] = -np.inf
+    (pv, pi), (qv, qi) = highest_first(p, k), highest_first(q, k)
+    drafts = qi[:, 0].copy()
+    for i, l in enumerate(lanes):                          # drafts that the target likes, or its row's first entry
+        drafts[l["first"]] = pi[l["row"], 0] if i % kinds in (3, 4, 5, 11) else drafts[l["first"]]
+
+    def plain(cert):
+        out = [verify64(l, lambda j: cut_any64(pv[l["row"] + j], pi[l["row"] + j], l),
+                        None if cert else lambda j: cut_any64(qv[l["first"] + j], qi[l["first"] + j], l), drafts, u,
+                        un[i], 3) for i, l in enumerate(lanes)]
+        return [np.array([o[j] for o in out]) for j in range(3)]
+
+    for cert in (False, True):
+        print("verify topk, infinities and NaN", k, cert, flush=True)
+        got = Topk(mk, pv, pi, None if cert else qv, None if cert else qi, lanes, drafts, u, un, 2).run().read()
+        check(got, plain(cert), 4 * EPS)
+        for i in range(len(lanes)):
+            if i % kinds in (4, 5):
+                assert got[0][i] == 0 and (got[1][i] == -1).all() and (got[2][i] == 0).all()
