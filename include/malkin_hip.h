@@ -250,8 +250,8 @@ int mk_attention_decode_q8(mk_ctx* ctx, const float* qkv, int64_t stride, int n,
    rounding, not in every bit. A token with n_keys[t] <= 0 or seq[t] outside the cache (a row of a padded batch) gets
    zeros. max_keys bounds n_keys[t]; keys past it are not read. xq: the BlockQ8 rows of out, as mk_attention_q8 (NULL:
    not written). Tokens may come in any order; those of one sequence that follow each other read its rows together.
-   workspace: at least mk_attention_prefix_workspace bytes for the same sizes, 16-byte aligned; two calls that may run at
-   the same time need one each. out and q must not overlap; the caches' rows 16-byte aligned.
+   workspace: at least mk_attention_prefix_workspace bytes for the same sizes, or for more tokens or more max_keys, 16-byte
+   aligned; two calls that may run at the same time need one each. out and q must not overlap; the caches' rows 16-byte aligned.
    MK_ERR_UNSUPPORTED (nothing launched) for a head_dim other than 64 / 128 or more than 32 query heads per KV head.
    No reference counterpart (its engine keeps every slot's own copy, engine.cpp:242-301). */
 size_t mk_attention_prefix_workspace(int n, int n_head, int n_head_kv, int head_dim, int n_prefix, int max_keys);

@@ -531,7 +531,6 @@ int chunk(int keys, int chunks) {  // keys per chunk, whole tiles for the four w
   return std::max(1, (c + kWaves * kKeys - 1) / (kWaves * kKeys)) * kWaves * kKeys;
 }
 
-// n_seq < 0: the most parts, whatever it is.
 Split split_of(int n, int H, int KV, int n_prefix, int max_keys, int n_seq) {
   Split s{};
   const int G = H / KV, tq = std::max(1, kRows / G);
@@ -543,7 +542,7 @@ Split split_of(int n, int H, int KV, int n_prefix, int max_keys, int n_seq) {
   s.no = (own + s.co - 1) / s.co;
   int64_t chunks = std::max<int64_t>(1, kWantedPre / pre_wgs);
   const int64_t more = std::min<int64_t>(2 * kWantedPre / pre_wgs, pre / kLongChunk);
-  if (2 * more * pre_wgs >= 3 * kWantedPre && (n_seq < 0 || more * pre_wgs + own_wgs <= 3 * kWantedPre))
+  if (2 * more * pre_wgs >= 3 * kWantedPre && more * pre_wgs + own_wgs <= 3 * kWantedPre)
     chunks = std::max(chunks, more);
   s.cp = chunk(pre, (int)std::min<int64_t>(kMaxPre, chunks));
   s.np = (pre + s.cp - 1) / s.cp;
@@ -553,9 +552,24 @@ Split split_of(int n, int H, int KV, int n_prefix, int max_keys, int n_seq) {
 
 }  // namespace
 
+// The most that split_of gives up to n tokens and up to max_keys keys, whatever n_seq is: fewer tokens have more parts, in
+// all too (32 / 8 heads behind 2048 + 1024 keys: 64 tokens 24576 rows of parts, 65 14560). A row has c chunks of a kind
+// only where the wanted workgroups allow that many of so few tokens, and where the keys fill c of the least length.
 size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int max_keys) {
-  const Split s = split_of(n, H, KV, n_prefix, max_keys, -1);
-  return (size_t)s.parts * (D * sizeof(float) + sizeof(Sum));
+  const int64_t G = H / KV, tq = std::max<int64_t>(1, kRows / G), least = kWaves * kKeys;
+  const int64_t pre = std::min(n_prefix, max_keys), own = std::max(0, max_keys - n_prefix);
+  int64_t parts_pre = 0, parts_own = 0;  // times tokens
+  for (int64_t c = 1; c <= std::min<int64_t>(kMaxPre, (pre + least - 1) / least); ++c) {
+    const int64_t wgs = (c * kLongChunk <= pre ? 2 : 1) * kWantedPre / c;
+    parts_pre = std::max(parts_pre, c * (c == 1 ? n : std::min<int64_t>(n, wgs / KV * kRows / G)));
+  }
+  for (int64_t c = 1; c <= std::min<int64_t>(kMaxOwn, (own + least - 1) / least); ++c)
+    parts_own = std::max(parts_own, c * (c == 1 ? n : std::min<int64_t>(n, kWantedOwn / c / KV * tq)));
+  return (size_t)((parts_pre + parts_own) * H) * (D * sizeof(float) + sizeof(Sum));
+}
+
+size_t attention_prefix_need(const PrefixAttn& A, int D) {
+  return (size_t)split_of(A.n, A.H, A.KV, A.n_prefix, A.max_keys, A.n_seq).parts * (D * sizeof(float) + sizeof(Sum));
 }
 
 void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q, int64_t q_stride, float* out,

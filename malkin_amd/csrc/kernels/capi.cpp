@@ -536,7 +536,7 @@ int mk_attention_prefix(mk_ctx* c, const float* q, int64_t q_stride, float* out,
       A.pre = mk::KvLayer{A.pre.k + rows * D, A.pre.v + rows * D, A.pre.ks + rows, A.pre.vs + rows};
       A.pre_ctx = prefix->n_ctx;
     }
-    const size_t need = mk::attention_prefix_workspace(n, n_head, KV, D, n_prefix, max_keys);
+    const size_t need = mk::attention_prefix_need(A, D);
     require(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
             "mk_attention_prefix: workspace smaller than mk_attention_prefix_workspace, or not aligned");
     require(c != nullptr, "mk_attention_prefix: null context");

@@ -147,3 +147,26 @@ def test_empty_calls_and_tables():
     # The tables' Python layouts are the header's.
     assert mk_.LORA_ADAPTER.itemsize == 24 and mk_.VERIFY_LANE.itemsize == 24
     assert np.zeros(1, mk_.LORA_ADAPTER).dtype.fields["rank"][1] == 20
+
+
+@pytest.mark.parametrize("H,KV,D", [(32, 8, 128), (40, 8, 128), (4, 4, 64), (16, 1, 128)])
+def test_prefix_workspace_holds_smaller_calls(H, KV, D):
+    """A workspace for a number of tokens and a bound on the keys is enough for every smaller one, and no call asks for
+    more than its own sizes report."""
+    L = mk_.load()
+    kv, few = (cache(n_head_kv=KV, head_dim=D, n_ctx=20000, n_seq=m) for m in (300, 1))
+    for P in (0, 100, 2048, 9000):
+        had = 0
+        for n in list(range(1, 70)) + [100, 127, 128, 129, 255, 256, 257, 400, 512, 513, 1024, 1100, 4096]:
+            row, most_need = [], 0
+            for most in (P // 2, P, P + 1, P + 128, P + 129, P + 1024, P + 6200):
+                row.append(L.mk_attention_prefix_workspace(n, H, KV, D, P, most))
+                assert row[-1] >= most_need, (P, n, most)
+                most_need = row[-1]
+                for own in (kv, few):
+                    refused(prefix_call(n=n, H=H, qs=H * D, os=H * D, kv=own, pre=kv, P=P, most=most, wsb=row[-1]),
+                            mk_.MK_ERR_INVALID, "null context")
+            assert row[-1] >= had, (P, n)
+            had = row[-1]
+            # Not a multiple of what the call uses: at most 64 parts of a row.
+            assert row[-1] <= 64 * n * H * (4 * D + 16)
