@@ -160,8 +160,8 @@ typedef struct {
    r < rows: the adapters of many requests, one per token, after the matmul they share (base: its output; y itself to
    add in place, NULL for 0). ids[t] outside 0..n_adapters-1 (-1: none), or an entry whose rank is not in 1..max_rank:
    y[t] = base[t]. type: MK_F32, MK_F16 or MK_BF16 for all adapters of a call; x and y are fp32, as are the sums.
-   max_rank 1..512. workspace: at least mk_lora_workspace bytes, 16-byte aligned; two calls that may run at the same
-   time need one each. x and y must not overlap, nor base and y unless they are the same rows. */
+   max_rank 1..512. workspace: at least mk_lora_workspace bytes for the call's sizes or larger ones, 16-byte aligned; two
+   calls that may run at the same time need one each. x and y must not overlap, nor base and y unless they are the same rows. */
 size_t mk_lora_workspace(int n, int max_rank, int64_t cols);
 int mk_lora(mk_ctx* ctx, int type, const mk_lora_adapter* adapters, int n_adapters, int max_rank, const int32_t* ids,
             const float* x, int64_t x_stride, int n, int64_t rows, int64_t cols, const float* base, int64_t base_stride,

@@ -413,17 +413,28 @@ int rank_pad(int max_rank) { return (max_rank + 15) & ~15; }
 // long, fewer the chain of steps (8 / 64 / 512 tokens as above 9.7 / 16.8 / 38.3 us, with at most 4 splits 10.8 / 21.6 /
 // 42.8, with at least one step 10.4 / 22.8 / 40.7; 310 tokens of rank 64 over 8 adapters, 12288 columns: 35 us with 16
 // splits at most, with 8 34.5, with 12 39, but 64 tokens 18 with 8).
+constexpr int kMostSplits = 16, kWantedWindows = 256;  // splits times windows
+int most_splits(int64_t cols) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, cols / (2 * kStep * kShrinkWaves)));
+}
 int splits_of(int n, int64_t cols) {
   const int windows = (n + kWindow - 1) / kWindow;
-  const int64_t most = cols / (2 * kStep * kShrinkWaves);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({16, (256 + windows - 1) / windows, most}));
+  return std::min(most_splits(cols), (kWantedWindows + windows - 1) / windows);
 }
 
 bool aligned16(const void* p, int64_t stride) { return ((uintptr_t)p & 15) == 0 && (stride & 3) == 0; }
 
 }  // namespace
 
+// The most of any batch up to n: fewer tokens have more splits, and s of them up to (kWantedWindows - 1) / (s - 1) windows.
 size_t lora_workspace(int n, int max_rank, int64_t cols) {
+  int64_t sums = n;
+  for (int s = 2; s <= most_splits(cols); ++s)
+    sums = std::max(sums, s * std::min<int64_t>(n, (kWantedWindows - 1) / (s - 1) * kWindow));
+  return (size_t)sums * rank_pad(max_rank) * sizeof(float);
+}
+
+size_t lora_need(int n, int max_rank, int64_t cols) {
   return (size_t)splits_of(n, cols) * n * rank_pad(max_rank) * sizeof(float);
 }
 

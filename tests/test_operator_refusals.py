@@ -170,3 +170,17 @@ def test_prefix_workspace_holds_smaller_calls(H, KV, D):
             had = row[-1]
             # Not a multiple of what the call uses: at most 64 parts of a row.
             assert row[-1] <= 64 * n * H * (4 * D + 16)
+
+
+def test_lora_workspace_holds_smaller_calls():
+    L = mk_.load()
+    for cols in (32, 512, 1000, 4096, 20000):
+        had = 0
+        for n in range(1, 20000, 7):
+            need = L.mk_lora_workspace(n, 16, cols)
+            assert need >= had and need <= 16 * n * 16 * 4, (cols, n)
+            had = need
+            if n % 50 == 1:
+                refused(lora_call(n=n, cols=cols, xs=cols, wsb=need), mk_.MK_ERR_INVALID, "null context")
+        assert L.mk_lora_workspace(100, 16, cols) <= L.mk_lora_workspace(100, 64, cols) <= \
+            L.mk_lora_workspace(100, 64, 2 * cols)
