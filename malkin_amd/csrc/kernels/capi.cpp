@@ -655,13 +655,16 @@ size_t mk_verify_workspace(int n_lanes, int max_draft, int n_vocab) {
   return n_lanes > 0 && max_draft >= 0 && n_vocab > 0 ? mk::verify_workspace(n_lanes, max_draft, n_vocab) : 0;
 }
 
-static void verify_args(int n_rows, int n_drafts, const void* lanes, int n_lanes, int max_draft, const void* drafts,
-                        const void* u, const void* u_next, const void* accepted, const void* tokens) {
-  require(n_rows >= 0 && n_drafts >= 0 && n_lanes >= 0, "mk_verify: bad sizes");
-  require(max_draft >= 0 && max_draft <= MK_VERIFY_MAX_DRAFT, "mk_verify: max_draft outside 0..256");
-  require((int64_t)n_lanes * (2 * max_draft + 1) < (1 << 30), "mk_verify: too many lanes");
-  require(n_lanes == 0 || (lanes && u_next && accepted && tokens && (n_drafts == 0 || (drafts && u))),
-          "mk_verify: null array");
+static void verify_args(const char* call, int n_rows, int n_drafts, const void* lanes, int n_lanes, int max_draft,
+                        const void* drafts, const void* u, const void* u_next, const void* accepted,
+                        const void* tokens) {
+  auto need = [&](bool ok, const char* what) {
+    if (!ok) throw mk::Error(MK_ERR_INVALID, std::string(call) + ": " + what);
+  };
+  need(n_rows >= 0 && n_drafts >= 0 && n_lanes >= 0, "bad sizes");
+  need(max_draft >= 0 && max_draft <= MK_VERIFY_MAX_DRAFT, "max_draft outside 0..256");
+  need((int64_t)n_lanes * (2 * max_draft + 1) < (1 << 30), "too many lanes");
+  need(n_lanes == 0 || (lanes && u_next && accepted && tokens && (n_drafts == 0 || (drafts && u))), "null array");
 }
 
 int mk_verify(mk_ctx* c, const float* p, int64_t p_stride, int n_rows, const float* q, int64_t q_stride, int n_drafts,
@@ -669,7 +672,7 @@ int mk_verify(mk_ctx* c, const float* p, int64_t p_stride, int n_rows, const flo
               const double* u, const double* u_next, int32_t* accepted, int32_t* tokens, float* probs, void* workspace,
               size_t workspace_bytes) {
   return guard([&] {
-    verify_args(n_rows, n_drafts, lanes, n_lanes, max_draft, drafts, u, u_next, accepted, tokens);
+    verify_args("mk_verify", n_rows, n_drafts, lanes, n_lanes, max_draft, drafts, u, u_next, accepted, tokens);
     require(n_vocab > 0 && n_vocab <= (1 << 27), "mk_verify: bad vocabulary");
     require(p_stride >= n_vocab && (!q || q_stride >= n_vocab), "mk_verify: stride shorter than a row");
     if (n_lanes == 0) return;
@@ -689,7 +692,8 @@ int mk_verify_topk(mk_ctx* c, const float* p_values, const int32_t* p_ids, int p
                    const int32_t* drafts, const double* u, const double* u_next, int32_t* accepted, int32_t* tokens,
                    float* probs) {
   return guard([&] {
-    verify_args(n_rows, n_drafts, lanes, n_lanes, max_draft, drafts, u, u_next, accepted, tokens);
+    verify_args("mk_verify_topk", n_rows, n_drafts, lanes, n_lanes, max_draft, drafts, u, u_next,
+                accepted, tokens);
     require(p_k >= 1 && p_k <= 1024 && (!q_values || (q_k >= 1 && q_k <= 1024)),
             "mk_verify_topk: candidates outside 1..1024 (mk_topk's limit)");
     require((q_values == nullptr) == (q_ids == nullptr), "mk_verify_topk: draft values without ids");

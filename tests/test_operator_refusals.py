@@ -184,3 +184,10 @@ def test_lora_workspace_holds_smaller_calls():
                 refused(lora_call(n=n, cols=cols, xs=cols, wsb=need), mk_.MK_ERR_INVALID, "null context")
         assert L.mk_lora_workspace(100, 16, cols) <= L.mk_lora_workspace(100, 64, cols) <= \
             L.mk_lora_workspace(100, 64, 2 * cols)
+
+
+@pytest.mark.parametrize("over", [dict(rows=-1), dict(most=257), dict(nl=1 << 29), dict(lanes=None), dict(d=None)])
+def test_refusals_name_their_call(over):
+    for call, name in ((verify_call, "mk_verify: "), (topk_call, "mk_verify_topk: ")):
+        assert call(**over) == mk_.MK_ERR_INVALID
+        assert mk_.load().mk_last_error().decode().startswith(name)
