@@ -550,6 +550,14 @@ Split split_of(int n, int H, int KV, int n_prefix, int max_keys, int n_seq) {
   return s;
 }
 
+// Workgroups of k_prefix_parts, and of the join, whose rows have several waves where there are many parts.
+int64_t parts_wgs(const PrefixAttn& A, const Split& S) {
+  const int tq = kRows / (A.H / A.KV);
+  return (int64_t)S.tiles * A.KV * S.np + ((int64_t)A.n + tq - 1) / tq * tq * A.KV * S.no;
+}
+int join_waves(const Split& S) { return S.np + S.no <= 24 ? 1 : 4; }
+int64_t join_wgs(const PrefixAttn& A, const Split& S) { return ((int64_t)A.n * A.H * join_waves(S) + 3) / 4; }
+
 }  // namespace
 
 // The most that split_of gives up to n tokens and up to max_keys keys, whatever n_seq is: fewer tokens have more parts, in
@@ -569,7 +577,9 @@ size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int
 }
 
 size_t attention_prefix_need(const PrefixAttn& A, int D) {
-  return (size_t)split_of(A.n, A.H, A.KV, A.n_prefix, A.max_keys, A.n_seq).parts * (D * sizeof(float) + sizeof(Sum));
+  const Split S = split_of(A.n, A.H, A.KV, A.n_prefix, A.max_keys, A.n_seq);
+  require(std::max(parts_wgs(A, S), join_wgs(A, S)) * kThreads < (1ll << 32), "mk_attention_prefix: too many rows");
+  return (size_t)S.parts * (D * sizeof(float) + sizeof(Sum));
 }
 
 void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q, int64_t q_stride, float* out,
@@ -577,9 +587,7 @@ void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q,
   const Split S = split_of(A.n, A.H, A.KV, A.n_prefix, A.max_keys, A.n_seq);
   float* po = static_cast<float*>(workspace);
   Sum* pml = reinterpret_cast<Sum*>(po + S.parts * D);
-  const int tq = kRows / (A.H / A.KV);
-  const int64_t wgs = (int64_t)S.tiles * A.KV * S.np + (int64_t)(A.n + tq - 1) / tq * tq * A.KV * S.no;
-  require(wgs < (1ll << 31), "mk_attention_prefix: too many rows");
+  const int64_t wgs = parts_wgs(A, S);
   auto go = [&]<int D_>() {
     if (wgs > 0) {
       allow_lds<k_prefix_parts<D_>>(Geo<D_>::kLds);
@@ -587,9 +595,8 @@ void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q,
                          pml);
       check_launch("attention_prefix parts");
     }
-    const int64_t rows = (int64_t)A.n * A.H;
     auto join = [&]<int W, int kAhead>() {
-      hipLaunchKernelGGL((k_prefix_join<D_, W, kAhead>), dim3((unsigned)((rows * W + 3) / 4)), dim3(kThreads), 0, s, A, S, po, pml,
+      hipLaunchKernelGGL((k_prefix_join<D_, W, kAhead>), dim3((unsigned)join_wgs(A, S)), dim3(kThreads), 0, s, A, S, po, pml,
                          out, out_stride, xq);
       check_launch("attention_prefix join");
     };
@@ -598,7 +605,7 @@ void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q,
     // 512 rows) 17.0 instead of 16.2. Four waves from nine parts on: 17.5 there, 24 parts ahead for one wave everywhere: the
     // registers of the small ones.
     if (S.np + S.no <= 8) join.template operator()<1, 8>();
-    else if (S.np + S.no <= 24) join.template operator()<1, 24>();
+    else if (join_waves(S) == 1) join.template operator()<1, 24>();
     else join.template operator()<4, 16>();
   };
   if (D == 128) go.template operator()<128>();

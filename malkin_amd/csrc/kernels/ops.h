@@ -156,7 +156,8 @@ struct PrefixAttn {
   const int32_t* n_keys;
 };
 size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int max_keys);  // never less for a larger batch
-size_t attention_prefix_need(const PrefixAttn& A, int D);                                    // what this call uses of it
+// What this call uses of it; throws where its launches would have 2^32 threads.
+size_t attention_prefix_need(const PrefixAttn& A, int D);
 void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q, int64_t q_stride, float* out,
                       int64_t out_stride, BlockQ8* xq, void* workspace);
 

@@ -191,3 +191,15 @@ def test_refusals_name_their_call(over):
     for call, name in ((verify_call, "mk_verify: "), (topk_call, "mk_verify_topk: ")):
         assert call(**over) == mk_.MK_ERR_INVALID
         assert mk_.load().mk_last_error().decode().startswith(name)
+
+
+def test_prefix_launch_limits():
+    """A launch has fewer than 2^32 threads."""
+    one = cache(n_head_kv=1, head_dim=64, n_ctx=200)
+    a = dict(H=1, qs=64, os=64, kv=one, pre=None, P=0, most=100, wsb=1 << 50)
+    refused(prefix_call(n=1 << 24, **a), mk_.MK_ERR_INVALID, "too many rows")
+    refused(prefix_call(n=(1 << 24) - 64, **a), mk_.MK_ERR_INVALID, "null context")
+    wide = cache(n_head_kv=8)
+    a = dict(H=256, qs=1 << 15, os=1 << 15, kv=wide, pre=wide, P=40, most=40, wsb=1 << 50)
+    refused(prefix_call(n=1 << 18, **a), mk_.MK_ERR_INVALID, "too many rows")
+    refused(prefix_call(n=(1 << 18) - 1, **a), mk_.MK_ERR_INVALID, "null context")
