@@ -563,7 +563,8 @@ int mk_lora(mk_ctx* c, int type, const mk_lora_adapter* adapters, int n_adapters
     require(x_stride >= cols && y_stride >= rows && (!base || base_stride >= rows),
             "mk_lora: stride shorter than a row");
     require(base != y || base_stride == y_stride, "mk_lora: base and y share memory with other strides");
-    require(workspace && workspace_bytes >= mk::lora_need(n, max_rank, cols) && ((uintptr_t)workspace & 15) == 0,
+    const size_t need = mk::lora_need(n, max_rank, rows, cols);
+    require(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
             "mk_lora: workspace smaller than mk_lora_workspace, or not aligned");
     require(c != nullptr, "mk_lora: null context");
     const DeviceOf on(c);

@@ -417,10 +417,12 @@ constexpr int kMostSplits = 16, kWantedWindows = 256;  // splits times windows
 int most_splits(int64_t cols) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, cols / (2 * kStep * kShrinkWaves)));
 }
+int windows_of(int n) { return (n - 1) / kWindow + 1; }  // n > 0
 int splits_of(int n, int64_t cols) {
-  const int windows = (n + kWindow - 1) / kWindow;
+  const int windows = windows_of(n);
   return std::min(most_splits(cols), (kWantedWindows + windows - 1) / windows);
 }
+int64_t blocks_of(int64_t rows) { return (rows + kRowBlock - 1) / kRowBlock; }
 
 bool aligned16(const void* p, int64_t stride) { return ((uintptr_t)p & 15) == 0 && (stride & 3) == 0; }
 
@@ -434,7 +436,10 @@ size_t lora_workspace(int n, int max_rank, int64_t cols) {
   return (size_t)sums * rank_pad(max_rank) * sizeof(float);
 }
 
-size_t lora_need(int n, int max_rank, int64_t cols) {
+size_t lora_need(int n, int max_rank, int64_t rows, int64_t cols) {
+  const int64_t windows = windows_of(n);
+  require(std::max(windows * splits_of(n, cols) * 64 * kShrinkWaves, windows * blocks_of(rows) * kThreads) < (1ll << 32),
+          "mk_lora: too many tokens");
   return (size_t)splits_of(n, cols) * n * rank_pad(max_rank) * sizeof(float);
 }
 
@@ -447,11 +452,9 @@ void lora(hipStream_t s, int type, const mk_lora_adapter* adapters, int n_adapte
   const bool y_vec = (rows & 3) == 0 && aligned16(y, y_stride) && (!base || aligned16(base, base_stride));
   float* h = static_cast<float*>(workspace);
   const int slots = n_adapters + 1 < kFewSlots ? n_adapters + 1 : kWindow;
-  const int windows = (n + kWindow - 1) / kWindow;
-  const int64_t blocks = (rows + kRowBlock - 1) / kRowBlock;
-  require(windows * std::max<int64_t>(blocks, splits) < (1ll << 31), "mk_lora: too many tokens");
+  const int windows = windows_of(n);
   const unsigned used = std::min(slots, n);
-  const dim3 g1((unsigned)(windows * splits), used, (r_pad + 31) / 32), g2((unsigned)(windows * blocks), used);
+  const dim3 g1((unsigned)(windows * splits), used, (r_pad + 31) / 32), g2((unsigned)(windows * blocks_of(rows)), used);
   const size_t lds = (size_t)(n <= 16 ? 16 : kWindow) * (r_pad + 4) * sizeof(float);
   auto go = [&]<typename T>() {
     if (n_adapters > 0) {

@@ -274,7 +274,8 @@ void verify_topk(hipStream_t s, const float* p_values, const int32_t* p_ids, int
 
 // y[t] = base[t] + scale B (A x[t]) with the adapter ids[t] (lora.hip).
 size_t lora_workspace(int n, int max_rank, int64_t cols);  // never less for a larger batch, rank or number of columns
-size_t lora_need(int n, int max_rank, int64_t cols);       // what a call of these sizes uses of it
+// What a call of these sizes uses of it; throws where its launches would have 2^32 threads.
+size_t lora_need(int n, int max_rank, int64_t rows, int64_t cols);
 void lora(hipStream_t s, int type, const mk_lora_adapter* adapters, int n_adapters, int max_rank, const int32_t* ids,
           const float* x, int64_t x_stride, int n, int64_t rows, int64_t cols, const float* base, int64_t base_stride,
           float* y, int64_t y_stride, void* workspace);

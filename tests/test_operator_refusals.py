@@ -203,3 +203,15 @@ def test_prefix_launch_limits():
     a = dict(H=256, qs=1 << 15, os=1 << 15, kv=wide, pre=wide, P=40, most=40, wsb=1 << 50)
     refused(prefix_call(n=1 << 18, **a), mk_.MK_ERR_INVALID, "too many rows")
     refused(prefix_call(n=(1 << 18) - 1, **a), mk_.MK_ERR_INVALID, "null context")
+
+
+def test_lora_launch_limits():
+    """A launch has fewer than 2^32 threads, and no count wraps on the way there."""
+    a = dict(cols=1, xs=1, rank=1, rows=1, ys=1, bs=1, wsb=1 << 60)
+    for n in (1 << 29, (1 << 31) - 64, (1 << 31) - 1):
+        refused(lora_call(n=n, **a), mk_.MK_ERR_INVALID, "too many tokens")
+        assert mk_.load().mk_lora_workspace(n, 1, 1) == 64 * n
+    refused(lora_call(n=(1 << 29) - 64, **a), mk_.MK_ERR_INVALID, "null context")
+    a.update(rows=1 << 24, ys=1 << 24, bs=1 << 24)
+    refused(lora_call(n=1 << 14, **a), mk_.MK_ERR_INVALID, "too many tokens")
+    refused(lora_call(n=(1 << 14) - 64, **a), mk_.MK_ERR_INVALID, "null context")
