@@ -678,6 +678,7 @@ int mk_verify(mk_ctx* c, const float* p, int64_t p_stride, int n_rows, const flo
     require(p_stride >= n_vocab && (!q || q_stride >= n_vocab), "mk_verify: stride shorter than a row");
     if (n_lanes == 0) return;
     require(p || n_rows == 0, "mk_verify: null array");
+    require(mk::verify_fits(n_rows, q, n_drafts, n_vocab, n_lanes, max_draft), "mk_verify: too many lanes");
     require(workspace && workspace_bytes >= mk::verify_workspace(n_lanes, max_draft, n_vocab) &&
                 ((uintptr_t)workspace & 15) == 0,
             "mk_verify: workspace smaller than mk_verify_workspace, or not aligned");
@@ -700,6 +701,7 @@ int mk_verify_topk(mk_ctx* c, const float* p_values, const int32_t* p_ids, int p
     require((q_values == nullptr) == (q_ids == nullptr), "mk_verify_topk: draft values without ids");
     if (n_lanes == 0) return;
     require((p_values && p_ids) || n_rows == 0, "mk_verify_topk: null array");
+    require(mk::verify_topk_fits(n_lanes), "mk_verify_topk: too many lanes");
     require(c != nullptr, "mk_verify_topk: null context");
     const DeviceOf on(c);
     mk::verify_topk(c->stream, p_values, p_ids, p_k, n_rows, q_values, q_ids, q_k, n_drafts, lanes, n_lanes, max_draft,

@@ -264,6 +264,9 @@ void sample_draw(hipStream_t s, const float* values, const int32_t* ids, int str
 
 // Verification of drafted tokens (verify.hip): over whole rows of logits, and over rows cut to their top k.
 size_t verify_workspace(int n_lanes, int max_draft, int n_vocab);
+// Whether the launches have fewer than 2^32 threads.
+bool verify_fits(int n_rows, bool q, int n_drafts, int n_vocab, int n_lanes, int max_draft);
+bool verify_topk_fits(int n_lanes);
 void verify(hipStream_t s, const float* p, int64_t p_stride, int n_rows, const float* q, int64_t q_stride, int n_drafts,
             int n_vocab, const mk_verify_lane* lanes, int n_lanes, int max_draft, const int32_t* drafts, const double* u,
             const double* u_next, int32_t* accepted, int32_t* tokens, float* probs, void* workspace);

@@ -702,6 +702,18 @@ int segments(int V) { return (V + kSeg - 1) / kSeg; }
 // Segments a workgroup of k_rows takes: one where rows are few, more once they fill the CUs eight times over (24 lanes of
 // eight drafts, 151936 tokens: 2 segments 47 us, 4 40, 8 42).
 int span_of(int64_t rows, int segs) { return (int)std::min<int64_t>(8, std::max<int64_t>(1, rows * segs / 2048)); }
+// A lane's rows in k_rows' grid, and its workgroups per row.
+struct Spans {
+  int per, span, spans;
+};
+Spans spans_of(int n_rows, bool q, int n_drafts, int n_vocab, int n_lanes, int max_draft) {
+  Spans s;
+  const int segs = segments(n_vocab);
+  s.per = q ? 2 * max_draft + 1 : max_draft + 1;
+  s.span = span_of(std::min<int64_t>((int64_t)n_lanes * s.per, (int64_t)n_rows + (q ? n_drafts : 0)), segs);
+  s.spans = (segs + s.span - 1) / s.span;
+  return s;
+}
 
 }  // namespace
 
@@ -711,18 +723,22 @@ size_t verify_workspace(int n_lanes, int max_draft, int n_vocab) {
          lanes * sizeof(uint32_t);
 }
 
+bool verify_fits(int n_rows, bool q, int n_drafts, int n_vocab, int n_lanes, int max_draft) {
+  const Spans s = spans_of(n_rows, q, n_drafts, n_vocab, n_lanes, max_draft);
+  return std::max<int64_t>((int64_t)n_lanes * s.per * s.spans, n_lanes) * kThreads < (1ll << 32);
+}
+bool verify_topk_fits(int n_lanes) { return (int64_t)n_lanes * kTopkThreads < (1ll << 32); }
+
 void verify(hipStream_t s, const float* p, int64_t p_stride, int n_rows, const float* q, int64_t q_stride, int n_drafts,
             int n_vocab, const mk_verify_lane* lanes, int n_lanes, int max_draft, const int32_t* drafts, const double* u,
             const double* u_next, int32_t* accepted, int32_t* tokens, float* probs, void* workspace) {
-  const int segs = segments(n_vocab), per = q ? 2 * max_draft + 1 : max_draft + 1;
+  const int segs = segments(n_vocab);
+  const auto [per, span, spans] = spans_of(n_rows, q, n_drafts, n_vocab, n_lanes, max_draft);
   Stat* stats = static_cast<Stat*>(workspace);
   double* sums = reinterpret_cast<double*>(stats + (size_t)n_lanes * per * segs);
   uint32_t* arrived = reinterpret_cast<uint32_t*>(sums + (size_t)n_lanes * segs * (kSeg / kBlock));
   auto aligned = [](const float* x, int64_t stride) { return !x || (((uintptr_t)x & 15) == 0 && (stride & 3) == 0); };
   const Rows R{p, p_stride, n_rows, q, q_stride, n_drafts, n_vocab};
-  const int64_t rows = std::min<int64_t>((int64_t)n_lanes * per, (int64_t)n_rows + (q ? n_drafts : 0));
-  const int span = span_of(rows, segs), spans = (segs + span - 1) / span;
-  require((int64_t)n_lanes * per * spans < (1ll << 31), "mk_verify: too many lanes");
   auto go = [&]<bool VEC>() {
     hipLaunchKernelGGL(k_rows<VEC>, dim3((unsigned)(n_lanes * per * spans)), dim3(kThreads), 0, s, R, lanes, max_draft,
                        per, span, spans, stats, arrived);

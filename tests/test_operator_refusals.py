@@ -215,3 +215,17 @@ def test_lora_launch_limits():
     a.update(rows=1 << 24, ys=1 << 24, bs=1 << 24)
     refused(lora_call(n=1 << 14, **a), mk_.MK_ERR_INVALID, "too many tokens")
     refused(lora_call(n=(1 << 14) - 64, **a), mk_.MK_ERR_INVALID, "null context")
+
+
+def test_verify_launch_limits():
+    """A launch has fewer than 2^32 threads."""
+    a = dict(most=0, drafts=0, d=None, u=None, wsb=1 << 60)
+    refused(verify_call(nl=1 << 24, **a), mk_.MK_ERR_INVALID, "too many lanes")
+    refused(verify_call(nl=(1 << 24) - 1, **a), mk_.MK_ERR_INVALID, "null context")
+    # 257 + 256 rows a lane, of 2^27 logits each: 4096 workgroups a row.
+    a = dict(most=256, rows=1 << 20, drafts=1 << 20, V=1 << 27, ps=1 << 27, qs=1 << 27, wsb=1 << 60)
+    refused(verify_call(nl=8, **a), mk_.MK_ERR_INVALID, "too many lanes")
+    refused(verify_call(nl=7, **a), mk_.MK_ERR_INVALID, "null context")
+    a = dict(most=0, drafts=0, d=None, u=None)
+    refused(topk_call(nl=1 << 23, **a), mk_.MK_ERR_INVALID, "too many lanes")
+    refused(topk_call(nl=(1 << 23) - 1, **a), mk_.MK_ERR_INVALID, "null context")
