@@ -451,7 +451,7 @@ void lora(hipStream_t s, int type, const mk_lora_adapter* adapters, int n_adapte
   const bool x_vec = aligned16(x, x_stride);
   const bool y_vec = (rows & 3) == 0 && aligned16(y, y_stride) && (!base || aligned16(base, base_stride));
   float* h = static_cast<float*>(workspace);
-  const int slots = n_adapters + 1 < kFewSlots ? n_adapters + 1 : kWindow;
+  const int slots = n_adapters < kFewSlots - 1 ? n_adapters + 1 : kWindow;
   const int windows = windows_of(n);
   const unsigned used = std::min(slots, n);
   const dim3 g1((unsigned)(windows * splits), used, (r_pad + 31) / 32), g2((unsigned)(windows * blocks_of(rows)), used);

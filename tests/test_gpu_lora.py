@@ -221,3 +221,20 @@ def test_infinite_x(mk, ranks, kind):
     assert odd[[0, 5, 18, 39]].all() and odd.sum() == 4 * rows and (ranks != [1] or np.isinf(want[odd]).all())
     assert np.array_equal(got[odd].astype(np.float64), want[odd], equal_nan=True)
     check(got[~odd], want[~odd], tol[~odd])
+
+
+def test_any_bound_on_the_table(mk):
+    """The number of adapters only bounds the ids: the largest int, a bound that the caller does not know better."""
+    rng = np.random.default_rng(8)
+    ranks, rows, cols, ids = [16, 8, 5], 128, 64, [0, 2, 1, -1, 1, 2, 0, -5] * 10
+    s = Set(mk, rng, "f16", ranks, rows, cols)
+    x = rng.standard_normal((len(ids), cols)).astype(np.float32)
+    base = rng.standard_normal((len(ids), rows)).astype(np.float32)
+    want, tol = lora64(x, s.host, ids, base, rows)
+    bits = []
+    for bound in (3, 13, 14, 15, 16, 2**31 - 1):
+        print("lora, bound", bound, flush=True)
+        got, _, _ = call(mk, "f16", s, bound, 16, ids, x, rows, base)
+        check(got, want, tol)
+        bits.append(got.view(np.uint32))
+    assert all(np.array_equal(bits[0], b) for b in bits)
