@@ -155,3 +155,51 @@ def cut_any64(values, ids, lane):
     lane["temperature"] = min(lane["temperature"], float(np.finfo(np.float32).max))
     with np.errstate(over="ignore"):
         return cut64(v[on], ids[on], lane, 0)
+
+
+def attention_norms64(q, n_head, pre, pseq, n_prefix, kv, row0, layer, seq, keys):
+    """Outputs [n][n_head][d] and what fp32 sums leave the 2-norm of a row's error at. Roundings are independent of each
+    other: a sum of L terms walks to half a step times the root of L times the root of the terms' squares, B for a score's
+    products (two of them, hi and lo) and S for the output's, while the keys' weights have no more than a few half steps of
+    the score's range each, and their sum's error moves the whole row. A q or weights with the lo part missing, or a key
+    left out, are ten times and more beyond it."""
+    k, v, ks, vs = kv
+    KV, d, byte = k.shape[2], k.shape[4], permuted(k.shape[4])
+    G = n_head // KV
+    out, tol = np.zeros((len(seq), n_head, d)), np.zeros((len(seq), n_head))
+    for t in range(len(seq)):
+        a, b = min(int(keys[t]), n_prefix), max(0, int(keys[t]) - n_prefix)
+        for g in range(KV):
+            K, V = [], []
+            for (ck, cv, cks, cvs), i, lo, c in ((pre or kv, pseq, 0, a), (kv, seq[t], row0, b)):
+                at = (layer, i, g, slice(lo, lo + c))
+                if c:
+                    K.append(ck[at][:, byte].astype(np.float64) * cks[at].astype(np.float64)[:, None])
+                    V.append(cv[at].astype(np.float64) * cvs[at].astype(np.float64)[:, None])
+            K, V = np.concatenate(K), np.concatenate(V)
+            for h in range(g * G, (g + 1) * G):
+                x = q[t, h * d:(h + 1) * d].astype(np.float64)
+                s, B = K @ x / np.sqrt(d), np.sqrt((K ** 2 @ x ** 2).max() / d)
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                out[t, h] = p @ V
+                S, walk = np.sqrt((p ** 2 @ V ** 2).sum()), 2 * np.sqrt(len(K))
+                tol[t, h] = EPS * ((2 * np.sqrt(d) * B + 4 * (s.max() - s.min()) + 32 + walk) * S +
+                                   walk * np.sqrt((out[t, h] ** 2).sum()))
+    return out, tol
+
+
+def lora_norms64(x, adapters, ids, rows):
+    """The adapters' part alone and what fp32 sums leave the 2-norm of a token's error at: both products' sums walk as in
+    attention_norms64, relative to the root of the terms' squares. x in fp16 is twenty times and more beyond it, a column
+    left out a thousand."""
+    y, tol = np.zeros((len(x), rows)), np.zeros(len(x))
+    for t, i in enumerate(ids):
+        if not 0 <= i < len(adapters) or adapters[i] is None:
+            continue
+        a, b, xt = (z.astype(np.float64) for z in (adapters[i][0], adapters[i][1], x[t]))
+        scale = float(np.float32(adapters[i][2]))
+        y[t] = scale * (b @ (a @ xt))
+        size = abs(scale) * np.sqrt((b ** 2 @ (a ** 2 @ xt ** 2)).sum())
+        tol[t] = EPS * (np.sqrt(a.shape[1]) + np.sqrt(a.shape[0]) + 8) * size
+    return y, tol

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import malkin_amd as mk_
-from operator_cases import attention64, make_cache
+from operator_cases import attention64, attention_norms64, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -260,3 +260,17 @@ def test_captured_and_replayed(mk):
             c.run()  # eager, between the replays
             assert np.array_equal(got.view(np.uint32), c.result().view(np.uint32))
     assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x) for x in c[:3]) + f"-n{sum(c[3])}-p{c[4]}")
+def test_close_as_a_whole(mk, case):
+    """The error of every row of the output is as small as sums in fp32 leave it."""
+    H, KV, d, new, P, rows, row0 = case
+    rng = np.random.default_rng(sum(new) + P + 1)
+    q, pre, kv, seq, keys = build(rng, H, KV, d, new, P, rows, row0)
+    want, tol = attention_norms64(q, H, pre, 1, P, kv, row0, 1, seq, keys)
+    c = Call(mk, q, H, pre, 1, P, kv, row0, 1, seq, keys, max(keys))
+    print("prefix attention as a whole", case[:5], flush=True)
+    c.run()
+    off = np.sqrt(((c.result().reshape(want.shape) - want) ** 2).sum(-1))
+    assert (off <= tol).all(), (off / tol).max()

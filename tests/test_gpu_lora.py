@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import malkin_amd as mk_
-from operator_cases import lora64
+from operator_cases import lora64, lora_norms64
 
 pytestmark = pytest.mark.gpu
 
@@ -238,3 +238,35 @@ def test_any_bound_on_the_table(mk):
         check(got, want, tol)
         bits.append(got.view(np.uint32))
     assert all(np.array_equal(bits[0], b) for b in bits)
+
+
+# Large ranks over several 16-token tiles and 64-token windows, more adapters than a window's few slots.
+LARGE = [
+    ([65], 272, 256, [0] * 17),
+    ([200, 65], 260, 288, [0] * 30 + [1] * 34),
+    ([512, 128], 320, 256, [0] * 40 + [1] * 40 + [0] * 20),
+    ([128, 512], 200, 136, [t % 3 - 1 for t in range(100)]),
+    ([100], 70, 45, [0] * 33),
+    ([8 + 3 * i for i in range(20)], 264, 320, [(7 * t) % 21 - 1 for t in range(200)]),
+    ([96] * 15, 256, 2048, [t % 15 for t in range(130)]),
+]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("case", CASES + LARGE, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{c[1]}-{c[2]}-n{len(c[3])}")
+def test_close_as_a_whole(mk, case, kind):
+    """Every element within its bound, and the error of every token's row as small as sums in fp32 leave it."""
+    ranks, rows, cols, ids = case
+    rng = np.random.default_rng(rows + cols + 1)
+    s = Set(mk, rng, kind, ranks, rows, cols)
+    x = rng.standard_normal((len(ids), cols)).astype(np.float32)
+    base = rng.standard_normal((len(ids), rows)).astype(np.float32)
+    print("lora as a whole", case[1:3], len(ids), kind, flush=True)
+    want, tol = lora64(x, s.host, ids, base, rows)
+    for in_place in (False, True):
+        got, _, _ = call(mk, kind, s, len(ranks), max(ranks), ids, x, rows, base, in_place=in_place)
+        check(got, want, tol)
+    got, _, _ = call(mk, kind, s, len(ranks), max(ranks), ids, x, rows, None)
+    want, tol = lora_norms64(x, s.host, ids, rows)
+    off = np.sqrt(((got - want) ** 2).sum(-1))
+    assert (off <= tol).all(), (off / np.maximum(tol, 1e-30)).max()

@@ -425,3 +425,105 @@ def test_topk_infinities_and_nan(mk, k):
         for i in range(len(lanes)):
             if i % kinds in (4, 5):
                 assert got[0][i] == 0 and (got[1][i] == -1).all() and (got[2][i] == 0).all()
+
+
+# Rows of several segments per workgroup (a span, from 4096 segments in all): 3 of 38, 5 of 9 whose rows no vector
+# divides, the last span shorter; vocabularies whose blocks a wave's registers do not hold (past 163840).
+SPANS = [([8] * 12, 151936, (0, 0)), ([8] * 12, 151936, (3, 1)), ([1, 0, 2, 3] * 80, 35001, (0, 0)),
+         ([2, 1, 0, 3, 1, 2], 262144, (0, 0)), ([1, 2, 2], 200001, (0, 0)), ([3] * 12, 262144, (0, 0))]
+
+
+@pytest.mark.parametrize("certain", [False, True])
+@pytest.mark.parametrize("counts,V,pads", SPANS, ids=lambda v: f"{len(v)}x{max(v)}" if isinstance(v, list) else str(v))
+def test_dense_spans_of_segments(mk, counts, V, pads, certain):
+    rng = np.random.default_rng(V + len(counts) + 5)
+    lanes = lanes_of(counts, [[0.7, 0.0, 1.0, 1.3, 2.0][i % 5] for i in range(len(counts))])
+    p, q, u, un = inputs(rng, counts, V, 1.0, 0.3)
+    p[:, :16] -= 30.0  # no draw ends in the first tokens
+    drafts = rng.integers(0, V, len(q)).astype(np.int32)
+    drafts[::2] = q[::2].argmax(1)
+    print("verify, spans", len(counts), V, pads, certain, flush=True)
+    c = Dense(mk, p, None if certain else q, lanes, drafts, u, un, max(counts), pads)
+    got = c.run().read()
+    check(got, want_dense(p, None if certain else q, lanes, drafts, u, un, max(counts)))
+    again = c.run().read()
+    assert all(np.array_equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("V", [36864, 36866])
+def test_dense_maxima_across_segments(mk, V):
+    """Nine segments, in spans of several: maxima that each segment raises by more than its sums reach (346 T), or lowers,
+    ties of a greedy row in a later segment of a span and in several, one finite logit in a row's end."""
+    rng = np.random.default_rng(3)
+    counts = [1] * 360  # 1080 rows: spans of four, without draft rows three
+    temps = np.float32([1.0, 0.0, 0.3, 1.0, 0.0, 2.0])
+    lanes = lanes_of(counts, np.tile(temps, 60))
+    p, q, u, un = inputs(rng, counts, V, 1.0, 0.3)
+    seg = np.arange(V) // 4096
+    for i, l in enumerate(lanes):
+        for row in (p[l["row"]], p[l["row"] + 1], q[l["first"]]):
+            kind = i // 6 % 6
+            step = np.float32(400.0) * max(l["temperature"], np.float32(1.0))
+            if kind == 0:
+                row += step * seg
+            elif kind == 1:
+                row -= step * seg
+            elif kind == 2:                # up and down, the highest in the middle
+                row += step * np.array([0, 3, 1, 4, 6, 2, 5, 6, 0, 0])[seg]
+            elif kind == 3:                # ties, first in the third segment
+                row[[2 * 4096 + 1500, 2 * 4096 + 1501, 3 * 4096 + 2, 7 * 4096]] = 60.0
+            elif kind == 4:                # nothing but one token near the end
+                row[:] = -np.inf
+                row[V - 1 - i % 5] = -3.0
+            else:                          # a high start in one thread's logits, masked segments behind it
+                row[16:20] += step
+                row[4096:5 * 4096] = -np.inf
+    drafts = q.argmax(1).astype(np.int32)
+    drafts[::7] = 5 * 4096 + 77
+    for qq in (q, None):
+        print("verify, maxima across segments", V, qq is None, flush=True)
+        got, want = Dense(mk, p, qq, lanes, drafts, u, un, 1).run().read(), want_dense(p, qq, lanes, drafts, u, un, 1)
+        assert np.array_equal(got[0], want[0])
+        # Where the draft was refused although P and Q are equal up to rounding (a draft that neither gives, four ties
+        # that share both), the next token is drawn by rounding: a power is within 4e-14 < 2^-44 of its value and a
+        # probability, its quotient by a sum of them, within 2^-43, so P - Q is known to 2^-42 max(P, Q), and a positive
+        # part that sums to less than 2^-42 (sum P + sum Q) = 2^-41 not at all. (Numpy's roundings are others, not
+        # fewer.) Any token may come whose difference can be positive.
+        same = np.ones(len(lanes), bool)
+        for i in np.flatnonzero((got[1] != want[1]).any(1)):
+            l, n = lanes[i], got[0][i]
+            assert qq is not None and n < l["n_draft"] and np.array_equal(got[1][i, :n], want[1][i, :n])
+            P, Q = (softmax64(x, l["temperature"]) for x in (p[l["row"] + n], q[l["first"] + n]))
+            x = got[1][i, n]
+            assert np.maximum(P - Q, 0.0).sum() < 2.0 ** -41 and P[x] > Q[x] - 2.0 ** -42 * Q[x] and P[x] > 0
+            same[i] = False
+        check([g[same] for g in got], [w[same] for w in want])
+        assert same.sum() >= len(lanes) - 60
+
+
+@pytest.mark.parametrize("certain", [False, True])
+def test_as_many_drafts_as_there_may_be(mk, certain):
+    """256 drafts, all accepted, refused at the last, in the middle and at the first; whole rows and candidates."""
+    rng = np.random.default_rng(6)
+    counts, V, k = [256, 256, 255, 0, 256, 129, 256], 300, 40
+    lanes = lanes_of(counts, [1.0, 0.8, 1.0, 1.0, 1.0, 1.2, 0.0])
+    p, q, u, un = inputs(rng, counts, V, 1.0, 0.2)
+    (pv, pi), (qv, qi) = highest_first(p, k), highest_first(q, k)
+    drafts, first = np.zeros(len(q), np.int32), lanes["first"]
+    for l in lanes:
+        for j in range(l["n_draft"]):  # a token that both rows have among their first
+            drafts[l["first"] + j] = pi[l["row"] + j, 0]
+    u *= 1e-9
+    for i, j in ((1, 255), (2, 254), (4, 100), (5, 0)):
+        drafts[first[i] + j] = pi[lanes["row"][i] + j, -1]
+        u[first[i] + j] = 1.0 - 1e-9
+        q[first[i] + j, drafts[first[i] + j]] = 9.0
+    qv, qi = highest_first(q, k)
+    print("verify, 256 drafts", certain, flush=True)
+    got = Dense(mk, p, None if certain else q, lanes, drafts, u, un, 256).run().read()
+    check(got, want_dense(p, None if certain else q, lanes, drafts, u, un, 256))
+    assert list(got[0][[1, 2, 3, 4, 5]]) == [255, 254, 0, 100, 0] and (got[0][0] == 256 or not certain)
+    a = (None, None) if certain else (qv, qi)
+    got = Topk(mk, pv, pi, *a, lanes, drafts, u, un, 256).run().read()
+    check(got, want_topk(pv, pi, *a, lanes, drafts, u, un, 256), 4 * EPS)
+    assert list(got[0][[1, 2, 3, 4, 5]]) == [255, 254, 0, 100, 0]
