@@ -390,9 +390,9 @@ typedef struct {
    on the draft itself, a proposer without a model): draft j is accepted iff Q_j(d) > 0 and u[first + j] Q_j(d) < P_j(d),
    up to the first refusal. The lane's next token comes from max(P_j - Q_j, 0) at the refused draft (from P_j where that
    is zero everywhere), or from the last row's P where none was refused: the first id of any weight, in order, at which the
-   running sum reaches u_next[lane] times the total. Probabilities and sums are 64-bit. accepted [n_lanes]: drafts accepted; tokens
-   [n_lanes][max_draft + 1]: those, the next token, then -1; probs (NULL: not written) the target's probability P of each
-   token, 0 past them. u, u_next: uniform in [0, 1), one per draft / lane.
+   running sum reaches u_next[lane] times the total. Probabilities and sums are 64-bit, a probability within 2^-40 of its
+   value. accepted [n_lanes]: drafts accepted; tokens [n_lanes][max_draft + 1]: those, the next token, then -1; probs (NULL:
+   not written) the target's probability P of each token, 0 past them. u, u_next: uniform in [0, 1), one per draft / lane.
    Logits: NaN counts as -inf (probability 0), +inf as the largest float; a row of nothing but those has no token (-1). A
    draft outside the vocabulary is refused. A lane that does not fit (n_draft outside 0..max_draft, rows outside n_rows,
    drafts outside n_drafts) is left out: accepted -1, tokens -1. All arrays are device arrays; rows p_stride / q_stride

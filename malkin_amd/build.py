@@ -1,4 +1,4 @@
-"""Builds the native libraries in-tree (they travel to the GPU box with the source tree):
+"""Builds the native libraries in-tree, so that they go wherever the source tree goes:
 
   malkin_amd/libmalkin_hip.so    gfx950 kernels + C ABI (include/malkin_hip.h, include/malkin_model.h) + host model
   malkin_amd/libmalkin_synth.so  deterministic synthetic GGUF writer (host only)

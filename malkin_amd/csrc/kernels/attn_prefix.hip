@@ -19,15 +19,15 @@
 // transposing LDS read. Each of a workgroup's four waves takes every fourth 32-key tile through a K and a V buffer of its
 // own, which direct copies fill: a buffer's next tile is asked for as soon as this one is in registers, and no barrier
 // stands between the preparation of q and the addition of the waves' results. q's fp16 parts lie in LDS, read beside
-// each MFMA: that leaves registers for three waves per SIMD (62 users over 8192 + 1024 keys: 48 us a pass; with q in
-// registers, two waves and a second K and V buffer, 56).
+// each MFMA: that leaves registers for three waves per SIMD (when it was chosen, 62 users over 8192 + 1024 keys took 48 us a
+// pass, and with q in registers, two waves and a second K and V buffer 56).
 //
-// What bounds it. A 32 x 32 tile of head_dim 128 takes 32 MFMAs (33 cycles each) and about 330 vector instructions (160
-// of them make fp16 of int8, 48 split the weights, 90 are the softmax), which overlap with MFMAs of other waves but
-// for about ten issue cycles per MFMA. 62 users x 32 heads over 8192 + 1024 keys: 41.8 us, 2.4 TB/s and 430 TFLOP/s of
-// matrix instructions; 512 prompt tokens behind 2048: 56.5 us, 670 TFLOP/s; the join 4 .. 8 us. A few tokens behind a few
-// hundred keys take 7 us and 3.8 us to join, which is the latency of the launches and of the loads that wait for each
-// other.
+// What bounds it. A 32 x 32 tile of head_dim 128 takes 32 MFMAs (32 cycles each) and about 330 vector instructions (160
+// of them make fp16 of int8, 48 split the weights, 90 are the softmax), which overlap with MFMAs of other waves in part: 62
+// users x 32 heads over 8192 + 1024 keys 45 us, 2.2 TB/s and 600 TFLOP/s of matrix instructions, the vector units issuing in
+// 61 % of the cycles, the matrix units at work in 36 %, both in 21 %; 512 prompt tokens behind 2048 61 us, 620 TFLOP/s, 66,
+// 38 and 23 % (on another card 44 and 57 us); the join 4 .. 9 us. A few tokens behind a few hundred keys take 7 us and 3.6 us
+// to join, which is the latency of the launches and of the loads that wait for each other.
 #include "ctx.h"
 #include "ops.h"
 
@@ -512,18 +512,26 @@ __global__ __launch_bounds__(kThreads) void k_prefix_join(PrefixAttn A, Split S,
 }
 
 constexpr int kMaxPre = 48, kMaxOwn = 16;  // a row's parts fit one wave's lanes
-// Workgroups wanted of each kind. The prefix's are long and set up once (q, the join of their waves): one per CU is best
-// (62 users over 8192 + 1024 keys: 43.9 us, with 192 wanted 42.9, with 384 44.6, with 512 46.9; 16 users over 4000 + 300:
-// 16.8, 15.6, 17.0, 21.1). The own rows' are as many as there are (token run, KV head) pairs, and split only where those
-// do not fill the CUs twice (8 users over 1500 + 600 keys: 14.1 us, with 256 wanted 15.2, with 128 14.7). A run ends at a
-// multiple of 32 / G tokens or where the next sequence begins, so with n_seq sequences, each one's tokens together, there are
-// at most n G / 32 + n_seq of them (50 drafted tokens of 10 users over 1361 keys: 21.7 us, with n counted instead 26.8; 135 of
-// 45 users over 5851 + 1498: 17.0 and 22.4; other orders are only slower).
+// Workgroups wanted of each kind; times are us a pass, 32 / 8 heads of 128 where none are named.
 //
-// Long chunks of the prefix go two to a CU, or nearly, where a third place is left for the own rows' (400 prompt tokens of
-// 16 heads behind 8000 keys: 85 us instead of 92 .. 95, 150 of 40 heads behind 9000 92 instead of 104; without room 399
-// tokens of 57 users behind 4743 + 1157 51 instead of 48, with short chunks 12 users behind 8000 20 instead of 16, with
-// few more 40 users behind 12000 35 instead of 32.4).
+// The prefix's are long and set up once (q, the join of their waves): about one per CU. 256, or 192 / 384 / 512: 62 users
+// over 8192 + 1024 keys 50, 50 / 54 / 53; 16 users over 4000 + 300 16.9, 15.5 / 16.9 / 21.1; 16 x 5 drafts of 40 heads over
+// 1999 + 301 23.5, 32.2 / 25.0 / 26.6; 40 users over 12000 + 300 35.4, 41.9 / 38.3 / 35.4; 12 users over 8000 + 300 17.7,
+// 18.7 / 19.8 / 22.4. Fewer leave CUs without work where the row tiles do not divide them; more are set up more often, and
+// gain with the many drafts of many users (45 x 3 over 5851 + 1498 83, 83 / 71 / 68).
+//
+// The own rows' are as many as there are (token run, KV head) pairs, and split only where those do not fill the CUs twice.
+// 512, or 256 / 128: 8 users over 1500 + 600 keys 13.5, 14.5 / 13.9; 12 users over 8000 + 300 17.7, 17.2 / 18.4; 16 users over
+// 4000 + 300 16.9, 16.0 / 17.1; 10 x 5 drafts over 92 + 1361 22.1, 27.4 with 256. A run ends at a multiple of 32 / G tokens or
+// where the next sequence begins, so with n_seq sequences, each one's tokens together, there are at most n G / 32 + n_seq of
+// them; with n counted instead 45 x 3 drafts of 4 / 2 heads over 5851 + 1498 take 29 instead of 22.2, 57 x 7 over 4743 + 1157
+// 35.5 instead of 31.3 and 10 x 5 of 32 / 8 heads over 92 + 1361 27.4 instead of 22.1 (other orders are only slower).
+//
+// Long chunks of the prefix go two to a CU, or nearly, where a third place is left for the own rows': 400 prompt tokens of
+// 16 / 8 heads behind 8000 keys 86 instead of 94, 150 of 40 / 8 heads behind 9000 93 instead of 104. Each condition costs a
+// call where it is left out: the third place 57 x 7 drafts of 16 / 8 heads over 4743 + 1157 80 instead of 77 (but 45 x 3 of 32 /
+// 8 heads over 5851 + 1498 68 instead of 83), chunks from 512 keys on 57 x 7 of 8 / 2 heads 47 instead of 40, less than one
+// and a half per CU the same 44 instead of 40 and 40 users over 12000 + 300 37 instead of 35.4.
 constexpr int kWantedPre = 256, kWantedOwn = 512, kLongChunk = 1536;
 
 int chunk(int keys, int chunks) {  // keys per chunk, whole tiles for the four waves

@@ -9,9 +9,9 @@
 // are read once per window that it occurs in. The products run on fp32 matrix instructions, which need no roundings of x
 // or h; the rest is memory: x, base and y are read and written once.
 //
-// Measured (shrink + expand): 8 tokens with an adapter each, rank 16, 4096 -> 6144: 4.4 + 5.3 us, latency; 64 tokens over
-// 24 adapters of rank up to 64, 5120 -> 7168: 7.1 + 9.8 us; 512 tokens over 3 adapters, rank 32, 4096 -> 24576: 9.4 +
-// 22.9 us, of which base and y are 100 MB, 4.4 TB/s.
+// Measured (shrink + expand): 8 tokens with an adapter each, rank 16, 4096 -> 6144: 4.7 + 5.4 us, latency; 64 tokens over
+// 24 adapters of rank up to 64, 5120 -> 7168: 7.3 + 10.0 us, latency; 512 tokens over 3 adapters, rank 32, 4096 -> 24576:
+// 9.4 us, its workgroups on two fifths of the CUs, and 22.9 us, of which base and y are 100 MB, 4.4 TB/s.
 #include <type_traits>
 
 #include "ctx.h"
@@ -254,14 +254,15 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void k_shrink(const mk_lora_adap
 }
 
 // y = base + scale B h. A wave takes 64 rows of B in four MFMA tiles, and the group's tokens 16 at a time; the products go
-// through LDS, so that base is read and y written 256 bytes of a token at a time. (512 rows per workgroup: 64
-// tokens as above 22.7 us instead of 19.9, 512 tokens 36.6 instead of 38.4, and no room for rank 512.) The code is kept short
+// through LDS, so that base is read and y written 256 bytes of a token at a time. (512 rows per workgroup: 8 / 64 / 512
+// tokens as above 9.8 / 21.4 / 43 us a pass instead of 9.6 / 17.0 / 38.3, and no room for rank 512.) The code is kept short
 // (rolled loops): a workgroup runs most of it once, and instruction fetches that miss would cost more than the arithmetic.
 // YV: rows of y and base are aligned to four floats, and of a multiple of four. The loop over the tokens has no branches of
 // a lane's own but its stores: with them every turn waited for the stores of the one before (512 tokens as above 38 us
-// instead of 31.6, 310 tokens of rank 64 48 instead of 35). Three workgroups per CU for 16-bit adapters (two 36.8, four,
-// with spills, 52), two for fp32, whose weights take twice the registers (three, with spills: 34 us instead of 25 for 245
-// tokens of rank 62).
+// instead of 31.6, 310 tokens of rank 64 48 instead of 35, when they were taken out). Three workgroups per CU for 16-bit
+// adapters, at the cost of one spilled register with YV and eleven without (64 / 512 tokens 17.0 / 38.3 us; two, without
+// spills, 19.2 / 43, four 21.7 / 60), two for fp32, whose weights take twice the registers (245 tokens of rank 62, 4096 -> 4096,
+// 27 us; three, with spills, 36).
 template <typename T, bool YV>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) void k_expand(const mk_lora_adapter* __restrict__ adapters, int n_adapters,
                                                      int max_rank, const int32_t* __restrict__ ids, int windows, int slots,
@@ -410,9 +411,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) void k_expand(con
 int rank_pad(int max_rank) { return (max_rank + 15) & ~15; }
 
 // Column splits of the first product, of at least two steps of every wave each: more make the sum over them in k_expand
-// long, fewer the chain of steps (8 / 64 / 512 tokens as above 9.7 / 16.8 / 38.3 us, with at most 4 splits 10.8 / 21.6 /
-// 42.8, with at least one step 10.4 / 22.8 / 40.7; 310 tokens of rank 64 over 8 adapters, 12288 columns: 35 us with 16
-// splits at most, with 8 34.5, with 12 39, but 64 tokens 18 with 8).
+// long, fewer the chain of steps (8 / 64 / 512 tokens as above 9.6 / 17.0 / 38.3 us a pass, with at most 4 splits 10.5 /
+// 22.1 / 45.8, with at most 8 9.6 / 18.8 / 38.3, with at least one step 9.2 / 20.3 / 35.9; 245 fp32 tokens of rank 62, 4096 ->
+// 4096, 27.3, with one step 33.6; 310 tokens of rank 64 over 8 adapters, 12288 -> 4096, 35.0, with 8 splits 34.7, with 12
+// 40.2, and in fp32 45.0, 38.7 and 43.3).
 constexpr int kMostSplits = 16, kWantedWindows = 256;  // splits times windows
 int most_splits(int64_t cols) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, cols / (2 * kStep * kShrinkWaves)));

@@ -10,10 +10,10 @@
 // workgroup of a lane for itself: a few hundred numbers) and sums the excess over 256 tokens at a time of the row that
 // the next token comes from; a lane's last workgroup to finish finds the block and the token.
 //
-// Measured (k_rows + k_excess, 151936 tokens): one lane of 4 drafts with a draft model 5 + 12 us, which is latency (a chain
+// Measured (k_rows + k_excess, 151936 tokens): one lane of 4 drafts with a draft model 5 + 13 us, which is latency (a chain
 // of about eight loads from memory); 24 lanes of up to 8 drafts 40 + 19 us: 37 million logits, 150 MB, at 3.7 TB/s with
-// the vector units busy for 58 % of the cycles (about 20 instructions a logit, 12 of them 64-bit); 16 lanes of up to 5
-// drafts without a model 15 + 17.5 us.
+// the vector units issuing in 67 % of the cycles (about 20 instructions a logit, 12 of them 64-bit); 16 lanes of up to 5
+// drafts without a model 15 + 17.6 us.
 #include <cfloat>
 
 #include "ctx.h"
@@ -54,7 +54,8 @@ __device__ __forceinline__ double fma_s(double p, double f, double c) {
   return r;
 }
 
-// 2^(d / 64) in two factors: d = 64 n + j + g, |g| <= 1/2; the table has 2^(j / 64), and 2^(g / 64) is the series of
+// 2^(d / 64) in two factors, by a table and a short series (Tang, Table-driven implementation of the exponential function,
+// 1989): d = 64 n + j + g, |g| <= 1/2; the table has 2^(j / 64), and 2^(g / 64) is the series of
 // e^x to x^4 (x = g ln 2 / 64 at most 0.0054: what follows is below 4e-14 of it). d is rounded by adding 1.5 * 2^52,
 // whose low word then holds 64 n + j; a table entry's high word is kept less j << 14, so that adding that word << 14 puts
 // n into the exponent. |d| < 64000.
