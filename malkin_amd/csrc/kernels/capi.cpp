@@ -511,7 +511,7 @@ int mk_attention_prefix(mk_ctx* c, const float* q, int64_t q_stride, float* out,
     if (n == 0) return;
     const mk::KvLayer L = kv_layer(kv, layer);
     const int KV = kv->n_head_kv, D = kv->head_dim;
-    require(KV > 0 && n_head % KV == 0, "mk_attention_prefix: bad head layout");
+    require(KV > 0 && n_head % KV == 0 && (int64_t)n_head * D < (1ll << 31), "mk_attention_prefix: bad head layout");
     if ((D != 64 && D != 128) || n_head / KV > 32)
       throw mk::Error(MK_ERR_UNSUPPORTED, "mk_attention_prefix: no kernel for this head layout");
     require(q && out && seq && n_keys, "mk_attention_prefix: null array");

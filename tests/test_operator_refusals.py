@@ -229,3 +229,11 @@ def test_verify_launch_limits():
     a = dict(most=0, drafts=0, d=None, u=None)
     refused(topk_call(nl=1 << 23, **a), mk_.MK_ERR_INVALID, "too many lanes")
     refused(topk_call(nl=(1 << 23) - 1, **a), mk_.MK_ERR_INVALID, "null context")
+
+
+def test_prefix_row_past_32_bits():
+    """The kernels' offsets inside a token's row are 32-bit."""
+    kv = cache(n_head_kv=1 << 20, n_ctx=41)
+    a = dict(n=1, kv=kv, pre=kv, P=40, most=41, qs=1 << 40, os=1 << 40, wsb=1 << 50)
+    refused(prefix_call(H=1 << 24, **a), mk_.MK_ERR_INVALID, "bad head layout")
+    refused(prefix_call(H=(1 << 24) - (1 << 20), **a), mk_.MK_ERR_INVALID, "null context")
