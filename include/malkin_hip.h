@@ -262,6 +262,93 @@ int mk_attention_prefix(mk_ctx* ctx, const float* q, int64_t q_stride, float* ou
 /* Model::move_kv (model.cpp:432-440): row `from` -> row `to` of sequence seq, K and V of every layer. */
 int mk_move_kv(mk_ctx* ctx, const mk_kv_cache* kv, int seq, int from, int to);
 
+/* ---- KV cache in 4 bits and in pages (no reference counterpart: its cache is int8, a slot's rows in one piece) ----
+ * A row of head_dim elements is held in groups of 32, each with an fp16 scale s: element n of 0..15 stands for s (n - 8) in
+ * fp16. mk_rope_kv4 writes scales of at most 8 significant bits, of which that is exact. Byte b of a row has element 2 b in its low and 2 b + 1 in its high
+ * half. Rows lie in pages of `page` positions (a power of two, 16..1024) of all layers and KV heads, taken from one pool;
+ * position j of sequence q is row j % page of page table[q * max_pages + j / page]. head_dim 64 or 128
+ * (MK_ERR_UNSUPPORTED otherwise). Device arrays; k and v 16-byte aligned, k_scale 8, v_scale 16. Beams and chats that go
+ * on from one text share its pages: refs counts the entries of the table that name a page. table, len and refs are the
+ * caller's to fill at first (-1, 0 and 0: nothing held); mk_kv4_fork, mk_kv4_resize and mk_kv4_compact keep them. */
+typedef struct {
+  uint8_t* k;        /* [n_page][n_layer][n_head_kv][page][head_dim / 2] */
+  uint8_t* v;
+  uint16_t* k_scale; /* [n_page][n_layer][n_head_kv][page][head_dim / 32] */
+  uint16_t* v_scale; /* [n_page][n_layer][n_head_kv][head_dim / 32][page] */
+  int32_t* table;    /* [n_seq][max_pages]; -1 past a sequence's pages */
+  int32_t* len;      /* [n_seq] rows that a sequence holds; NULL where no call below that reads it is made */
+  int32_t* refs;     /* [n_page]; 0: the page is free; NULL as len */
+  int32_t n_layer, n_page, page, n_head_kv, head_dim, n_seq, max_pages;
+} mk_kv4_cache;
+
+/* How the frequencies of mk_rope_tables are made for contexts longer than the trained ones. */
+enum {
+  MK_ROPE_PLAIN = 0,
+  MK_ROPE_LINEAR = 1, /* positions divided by factor */
+  MK_ROPE_NTK = 2,    /* base * factor^(dim / (dim - 2)) */
+  MK_ROPE_YARN = 3    /* Peng et al. 2023: slow elements as LINEAR, fast ones as PLAIN, a ramp between */
+};
+typedef struct {
+  int32_t dim;     /* elements of a head that rotate; even, 2..256 */
+  int32_t scaling; /* MK_ROPE_* */
+  double base, factor;
+  int32_t n_orig;              /* YARN: the trained context */
+  double beta_fast, beta_slow; /* YARN: turns over n_orig where the ramp begins and ends (32, 1) */
+  double attn_factor;          /* YARN: cosines and sines are multiplied by it; 0: 0.1 ln(factor) + 1 */
+} mk_rope;
+/* cos_t / sin_t [n_pos][dim / 2] (as mk_qk_norm_rope_kv and mk_rope_kv4 take them) of positions first .. first + n_pos - 1,
+   angles in 64 bits. divide: dim / 2 divisors of the frequencies (a GGUF's rope_freqs.weight), on the device, or NULL. */
+int mk_rope_tables(mk_ctx* ctx, const mk_rope* rope, const float* divide, int64_t first, int n_pos, float* cos_t,
+                   float* sin_t);
+/* Which elements of a head rotate together: i and i + rope_dim / 2 (NeoX), or 2 i and 2 i + 1. */
+enum { MK_ROPE_HALVES = 0, MK_ROPE_PAIRS = 1 };
+/* mk_qk_norm_rope_kv for the 4-bit cache: per token t, rmsnorm with q_norm / k_norm (NULL, both: none) of the query and key
+   heads, rotation of each one's first rope_dim elements at position rpos[t] of the tables [n_pos][rope_dim / 2], the query
+   heads to q_out (q itself: in place, of the same stride), keys and values in 4 bits into row kv_row[t] of sequence seq[t] of
+   `layer`: s is the group's element furthest from 0 over -8 (the positive one of two), rounded to 8 significant bits, within
+   +-4096 and to fp16; n = rint(x / s) + 8 within 0..15. NaN counts as 0 there. q, k and v share the token stride. A token whose seq, rpos or kv_row lies outside, or whose row has no page, is left
+   out: its row of q_out and the cache stay as they were. Rows of one call are different ones, and no two sequences share a page
+   that is written (mk_kv4_resize sees to that). */
+int mk_rope_kv4(mk_ctx* ctx, const float* q, const float* k, const float* v, int64_t stride, int n, int n_head,
+                const float* q_norm, const float* k_norm, float eps, int layout, int rope_dim, const float* cos_t,
+                const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row,
+                const mk_kv4_cache* kv, int layer, float* q_out, int64_t q_out_stride);
+/* Rows row[i] of sequences seq[i] of `layer` as fp16, [n][n_head_kv][head_dim], exactly what they stand for (zeros for rows
+   without a page). k_out or v_out may be NULL. 16-byte aligned. */
+int mk_kv4_rows(mk_ctx* ctx, const mk_kv4_cache* kv, int layer, const int32_t* seq, const int32_t* row, int n, void* k_out,
+                void* v_out);
+/* mk_attention for plain tokens over the 4-bit cache: token t attends with its n_head query heads to positions
+   0..n_keys[t]-1 of sequence seq[t]; fp32 sums. max_keys bounds n_keys[t]: keys past it are not read. max_run is the number
+   of tokens of one sequence that follow each other at most (1: decoding), a hint that changes no result beyond rounding. A
+   token with n_keys[t] <= 0 or seq[t] outside the cache gets zeros, and keys whose page is not in the pool have no weight.
+   Tokens may come in any order; those of one sequence that follow each other read its rows together. xq: the BlockQ8 rows of
+   out, as mk_attention_q8 (NULL: not written). workspace: at least mk_attention_kv4_workspace bytes for the same sizes or
+   larger ones, 16-byte aligned; two calls that may run at the same time need one each. out and q must not overlap.
+   MK_ERR_UNSUPPORTED for more than 32 query heads per KV head. */
+size_t mk_attention_kv4_workspace(int n, int n_head, int n_head_kv, int head_dim, int max_keys, int max_run);
+int mk_attention_kv4(mk_ctx* ctx, const float* q, int64_t q_stride, float* out, int64_t out_stride, int n, int n_head,
+                     const mk_kv4_cache* kv, int layer, const int32_t* seq, const int32_t* n_keys, int max_keys,
+                     int max_run, void* xq, void* workspace, size_t workspace_bytes);
+/* Sequence dst[i] (dst NULL: i) holds what sequence src[i] held before the call, for all i at once: its pages are shared, no
+   row is copied; what dst[i] held is let go. src[i] outside the cache: dst[i] holds nothing then. An entry whose dst[i] lies
+   outside, or comes again further on, has no effect. Beam search: src from mk_beam_select. workspace: 16-byte aligned, one per
+   call at a time (mk_kv4_resize and mk_kv4_compact too). */
+size_t mk_kv4_fork_workspace(int n, int max_pages);
+int mk_kv4_fork(mk_ctx* ctx, const mk_kv4_cache* kv, const int32_t* dst, const int32_t* src, int n, void* workspace,
+                size_t workspace_bytes);
+/* Sequence seq[i] (seq NULL: i) is to hold new_len[i] rows: pages past a shorter end are let go; a longer one gets pages, and
+   where its last page is shared and not full, a copy of the rows it holds there (all layers), so that it can be written.
+   Shorter ends come first, then the longer ones in order, each taking the free pages of the lowest numbers; of those that
+   share a page and nobody else, the last keeps it. status[i]: 0, or 1 where new_len[i] needs a page and the pool has too few for it and
+   all entries before it, or -1 where seq[i] or new_len[i] (0..max_pages * page) lies outside or seq[i] comes again further
+   on; such entries change nothing. */
+size_t mk_kv4_resize_workspace(int n, int n_page);
+int mk_kv4_resize(mk_ctx* ctx, const mk_kv4_cache* kv, const int32_t* seq, const int32_t* new_len, int n, int32_t* status,
+                  void* workspace, size_t workspace_bytes);
+/* Moves the pages in use to numbers 0 .. *n_live - 1 of the pool: those beyond, in order, into the free ones below, in order. */
+size_t mk_kv4_compact_workspace(int n_page);
+int mk_kv4_compact(mk_ctx* ctx, const mk_kv4_cache* kv, int32_t* n_live, void* workspace, size_t workspace_bytes);
+
 /* ---- persistent decode step: the layer loop of Model::run for one token (model.cpp:355-417 at n = 1) ----
  * Per layer: rmsnorm + q|k|v, QK-norm + RoPE + KV write + attention, attn_output + residual, rmsnorm + gate|up,
  * silu * up, down + residual; all layers of a step in one launch, one workgroup per CU handing off between the steps
@@ -413,6 +500,19 @@ int mk_verify_topk(mk_ctx* ctx, const float* p_values, const int32_t* p_ids, int
                    const int32_t* q_ids, int q_k, int n_drafts, const mk_verify_lane* lanes, int n_lanes, int max_draft,
                    const int32_t* drafts, const double* u, const double* u_next, int32_t* accepted, int32_t* tokens,
                    float* probs);
+
+/* ---- beam search (no reference counterpart: its engine samples) ----
+ * Per group of `beams` rows of logits (row g * beams + b: beam b of group g, `stride` floats apart), the k best ways to go on,
+ * best first: beam b with token v has the score scores[row] + logits[row][v] - log(sum_u exp(logits[row][u])), in 64 bits; a
+ * beam with done[row] != 0 (done NULL: none) has only itself, token eos, its score as it is. Equal scores: the lower beam, then
+ * the lower token. Logits: NaN counts as -inf (no candidate), +inf as the largest float; a beam whose score is not finite has
+ * no part. out_scores (rounded), out_seq (the row it goes on from: mk_kv4_fork's src) and out_tokens are [n_group][k]; places
+ * without a candidate: -inf, -1, -1. beams 1..64, k 1..128. workspace: at least mk_beam_workspace bytes, 16-byte aligned; two
+ * calls that may run at the same time need one each. */
+size_t mk_beam_workspace(int n_group, int beams, int n_vocab, int k);
+int mk_beam_select(mk_ctx* ctx, const float* logits, int64_t stride, int n_group, int beams, int n_vocab,
+                   const float* scores, const int32_t* done, int eos, int k, float* out_scores, int32_t* out_seq,
+                   int32_t* out_tokens, void* workspace, size_t workspace_bytes);
 
 /* dst[dst_index[i]] = src[src_index[i]] for i < n, in stream order (a NULL index array is the identity; a negative
    index skips i). Moves token ids between device arrays without a host round trip: draft picks into a proposal tree,

@@ -13,6 +13,8 @@ LIB_PATH = os.path.join(HERE, "libmalkin_hip.so")
 
 MK_OK, MK_ERR_INVALID, MK_ERR_HIP, MK_ERR_UNSUPPORTED, MK_ERR_NO_DEVICE = 0, 1, 2, 3, 4
 F32, F16, Q8_0, Q4_K, Q5_K, Q6_K, BF16 = 0, 1, 8, 12, 13, 14, 30
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3  # how frequencies are scaled
+ROPE_HALVES, ROPE_PAIRS = 0, 1  # which elements rotate together
 MODEL_NO_WIDE, MODEL_NO_PACK, MODEL_PERSISTENT, MODEL_FUSED_ATTN = 1, 2, 4, 8
 
 BLOCK_Q8 = np.dtype([("d", "<f4"), ("s", "<i2", (2,)), ("qs", "i1", (32,))])
@@ -78,6 +80,19 @@ SIGNATURES = {
     "mk_verify": (_I, [_P, _P, _I64, _I, _P, _I64, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ]),
     "mk_verify_topk": (_I, [_P, _P, _P, _I, _I, _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P]),
     "mk_move_kv": (_I, [_P, _P, _I, _I, _I]),
+    "mk_rope_tables": (_I, [_P, _P, _P, _I64, _I, _P, _P]),
+    "mk_rope_kv4": (_I, [_P, _P, _P, _P, _I64, _I, _I, _P, _P, _F, _I, _I, _P, _P, _I, _P, _P, _P, _P, _I, _P, _I64]),
+    "mk_kv4_rows": (_I, [_P, _P, _I, _P, _P, _I, _P, _P]),
+    "mk_attention_kv4_workspace": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "mk_attention_kv4": (_I, [_P, _P, _I64, _P, _I64, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _SZ]),
+    "mk_kv4_fork_workspace": (_SZ, [_I, _I]),
+    "mk_kv4_fork": (_I, [_P, _P, _P, _P, _I, _P, _SZ]),
+    "mk_kv4_resize_workspace": (_SZ, [_I, _I]),
+    "mk_kv4_resize": (_I, [_P, _P, _P, _P, _I, _P, _P, _SZ]),
+    "mk_kv4_compact_workspace": (_SZ, [_I]),
+    "mk_kv4_compact": (_I, [_P, _P, _P, _P, _SZ]),
+    "mk_beam_workspace": (_SZ, [_I, _I, _I, _I]),
+    "mk_beam_select": (_I, [_P, _P, _I64, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _P, _SZ]),
     "mk_decode_plan_create": (_I, [_P, _P, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.POINTER(_P)]),
     "mk_decode_plan_destroy": (_I, [_P]),
     "mk_decode_supported": (_I, [_P, _I]),
@@ -265,6 +280,17 @@ class MkKvCache(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
                 ("v_scale", ctypes.c_void_p), ("n_layer", ctypes.c_int32), ("n_seq", ctypes.c_int32),
                 ("n_head_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("n_ctx", ctypes.c_int32)]
+
+
+class MkKv4Cache(ctypes.Structure):
+    _fields_ = [(x, ctypes.c_void_p) for x in ("k", "v", "k_scale", "v_scale", "table", "len", "refs")] + \
+               [(x, ctypes.c_int32) for x in ("n_layer", "n_page", "page", "n_head_kv", "head_dim", "n_seq", "max_pages")]
+
+
+class MkRope(ctypes.Structure):
+    _fields_ = [("dim", ctypes.c_int32), ("scaling", ctypes.c_int32), ("base", ctypes.c_double),
+                ("factor", ctypes.c_double), ("n_orig", ctypes.c_int32), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double), ("attn_factor", ctypes.c_double)]
 
 
 class MkModelConfig(ctypes.Structure):

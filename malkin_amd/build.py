@@ -27,9 +27,13 @@ HIP_SOURCES = [
     "csrc/kernels/attn.hip",
     "csrc/kernels/attn_mma.hip",
     "csrc/kernels/attn_prefix.hip",
+    "csrc/kernels/attn_kv4.hip",
+    "csrc/kernels/beam.hip",
     "csrc/kernels/decode.hip",
     "csrc/kernels/cut.hip",
+    "csrc/kernels/kv4.hip",
     "csrc/kernels/lora.hip",
+    "csrc/kernels/pages.hip",
     "csrc/kernels/rowpath.hip",
     "csrc/kernels/sample.hip",
     "csrc/kernels/verify.hip",

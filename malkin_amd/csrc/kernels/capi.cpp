@@ -545,6 +545,226 @@ int mk_attention_prefix(mk_ctx* c, const float* q, int64_t q_stride, float* out,
   });
 }
 
+namespace {
+
+// The cache's own sizes; 2^31 bounds what the kernels count in 32 bits: the rows of one page of all layers and heads, a
+// sequence's positions, the table's entries.
+void kv4_sizes(const mk_kv4_cache* kv, const char* call) {
+  auto need = [&](bool ok, const char* what) {
+    if (!ok) throw mk::Error(MK_ERR_INVALID, std::string(call) + what);
+  };
+  need(kv != nullptr, ": null cache");
+  need(kv->n_layer > 0 && kv->n_page > 0 && kv->n_head_kv > 0 && kv->n_seq > 0 && kv->max_pages > 0, ": bad cache sizes");
+  need(kv->page >= 16 && kv->page <= 1024 && (kv->page & (kv->page - 1)) == 0, ": page is not a power of two in 16..1024");
+  if (kv->head_dim != 64 && kv->head_dim != 128)
+    throw mk::Error(MK_ERR_UNSUPPORTED, std::string(call) + ": no kernel for this head_dim");
+  const int64_t most = 1ll << 31;
+  need((int64_t)kv->n_layer * kv->n_head_kv < (1 << 20) && (int64_t)kv->n_seq * kv->max_pages < most &&
+           (int64_t)kv->max_pages * kv->page < most,
+       ": cache too large");
+  need(kv->k && kv->v && kv->k_scale && kv->v_scale && kv->table, ": null cache array");
+  need((((uintptr_t)kv->k | (uintptr_t)kv->v | (uintptr_t)kv->v_scale) & 15) == 0 && ((uintptr_t)kv->k_scale & 7) == 0,
+       ": cache rows not aligned");
+}
+
+mk::Kv4 kv4_layer(const mk_kv4_cache* kv, int layer, const char* call) {
+  kv4_sizes(kv, call);
+  if (layer < 0 || layer >= kv->n_layer) throw mk::Error(MK_ERR_INVALID, std::string(call) + ": bad layer");
+  return mk::Kv4{kv->k, kv->v, kv->k_scale, kv->v_scale, kv->table, kv->n_layer, layer, kv->n_page, kv->n_head_kv, kv->n_seq,
+                 kv->max_pages, __builtin_ctz(kv->page)};
+}
+
+mk::Kv4Pool kv4_pool(const mk_kv4_cache* kv, const char* call) {
+  kv4_sizes(kv, call);
+  if (!kv->len || !kv->refs) throw mk::Error(MK_ERR_INVALID, std::string(call) + ": null cache array");
+  return mk::Kv4Pool{kv->k, kv->v, kv->k_scale, kv->v_scale, kv->table, kv->len, kv->refs, kv->n_page, kv->n_seq,
+                     kv->max_pages, __builtin_ctz(kv->page), kv->n_layer * kv->n_head_kv};
+}
+
+bool holds(const void* workspace, size_t bytes, size_t need) {
+  return need == 0 || (workspace && bytes >= need && ((uintptr_t)workspace & 15) == 0);
+}
+
+}  // namespace
+
+int mk_rope_tables(mk_ctx* c, const mk_rope* rope, const float* divide, int64_t first, int n_pos, float* cos_t,
+                   float* sin_t) {
+  return guard([&] {
+    require(rope != nullptr, "mk_rope_tables: null parameters");
+    require(rope->dim >= 2 && rope->dim <= 256 && rope->dim % 2 == 0, "mk_rope_tables: dim is not even in 2..256");
+    require(rope->scaling >= MK_ROPE_PLAIN && rope->scaling <= MK_ROPE_YARN, "mk_rope_tables: unknown scaling");
+    require(rope->base > 0.0 && std::isfinite(rope->base), "mk_rope_tables: bad base");
+    require(rope->scaling == MK_ROPE_PLAIN || (rope->factor > 0.0 && std::isfinite(rope->factor)),
+            "mk_rope_tables: bad factor");
+    require(rope->scaling != MK_ROPE_NTK || rope->dim > 2, "mk_rope_tables: NTK scaling needs more than one pair");
+    if (rope->scaling == MK_ROPE_YARN)
+      require(rope->n_orig > 0 && rope->base != 1.0 && rope->beta_fast > 0.0 && rope->beta_slow > 0.0 &&
+                  std::isfinite(rope->beta_fast) && std::isfinite(rope->beta_slow) && std::isfinite(rope->attn_factor),
+              "mk_rope_tables: bad YaRN parameters");
+    require(n_pos >= 0 && first >= 0 && first + n_pos <= (1ll << 31), "mk_rope_tables: bad positions");
+    if (n_pos == 0) return;
+    require(cos_t && sin_t, "mk_rope_tables: null array");
+    require(c != nullptr, "mk_rope_tables: null context");
+    const DeviceOf on(c);
+    mk::rope_tables(c->stream, *rope, divide, first, n_pos, cos_t, sin_t);
+  });
+}
+
+int mk_rope_kv4(mk_ctx* c, const float* q, const float* k, const float* v, int64_t stride, int n, int n_head,
+                const float* q_norm, const float* k_norm, float eps, int layout, int rope_dim, const float* cos_t,
+                const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row,
+                const mk_kv4_cache* kv, int layer, float* q_out, int64_t q_out_stride) {
+  return guard([&] {
+    require(n >= 0 && n_head > 0 && n_pos >= 0, "mk_rope_kv4: bad sizes");
+    if (n == 0) return;
+    const mk::Kv4 K = kv4_layer(kv, layer, "mk_rope_kv4");
+    const int D = kv->head_dim;
+    require(layout == MK_ROPE_HALVES || layout == MK_ROPE_PAIRS, "mk_rope_kv4: unknown layout");
+    require(rope_dim >= 0 && rope_dim <= D && rope_dim % 2 == 0, "mk_rope_kv4: rope_dim is not even in 0..head_dim");
+    require(q && k && v && q_out && rpos && seq && kv_row && (rope_dim == 0 || (cos_t && sin_t)), "mk_rope_kv4: null array");
+    require((q_norm == nullptr) == (k_norm == nullptr), "mk_rope_kv4: one norm without the other");
+    require((int64_t)n_head * D < (1ll << 31), "mk_rope_kv4: bad head layout");
+    require(stride >= (int64_t)std::max(n_head, K.KV) * D && q_out_stride >= (int64_t)n_head * D,
+            "mk_rope_kv4: stride shorter than a row");
+    require(q != q_out || stride == q_out_stride, "mk_rope_kv4: q and q_out share memory with other strides");
+    require((int64_t)n * (n_head + 2ll * K.KV) * (D / 8) < (1ll << 32) - 1024, "mk_rope_kv4: too many rows");
+    require(c != nullptr, "mk_rope_kv4: null context");
+    const DeviceOf on(c);
+    mk::rope_kv4(c->stream, K, D, q, k, v, stride, n, n_head, q_norm, k_norm, eps, layout == MK_ROPE_PAIRS, rope_dim, cos_t,
+                 sin_t, n_pos, rpos, seq, kv_row, q_out, q_out_stride);
+  });
+}
+
+int mk_kv4_rows(mk_ctx* c, const mk_kv4_cache* kv, int layer, const int32_t* seq, const int32_t* row, int n, void* k_out,
+                void* v_out) {
+  return guard([&] {
+    require(n >= 0, "mk_kv4_rows: bad sizes");
+    if (n == 0) return;
+    const mk::Kv4 K = kv4_layer(kv, layer, "mk_kv4_rows");
+    require(seq && row, "mk_kv4_rows: null array");
+    require((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "mk_kv4_rows: output not 16-byte aligned");
+    require(2ll * n * K.KV * (kv->head_dim / 8) < (1ll << 32) - 1024, "mk_kv4_rows: too many rows");
+    require(c != nullptr, "mk_kv4_rows: null context");
+    if (!k_out && !v_out) return;
+    const DeviceOf on(c);
+    mk::kv4_rows(c->stream, K, kv->head_dim, seq, row, n, k_out, v_out);
+  });
+}
+
+size_t mk_attention_kv4_workspace(int n, int n_head, int n_head_kv, int head_dim, int max_keys, int max_run) {
+  if (n <= 0 || n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv || n_head / n_head_kv > 32 ||
+      (head_dim != 64 && head_dim != 128) || max_keys <= 0)
+    return 0;
+  return mk::attention_kv4_workspace(n, n_head, n_head_kv, head_dim, max_keys, max_run);
+}
+
+int mk_attention_kv4(mk_ctx* c, const float* q, int64_t q_stride, float* out, int64_t out_stride, int n, int n_head,
+                     const mk_kv4_cache* kv, int layer, const int32_t* seq, const int32_t* n_keys, int max_keys,
+                     int max_run, void* xq, void* workspace, size_t workspace_bytes) {
+  return guard([&] {
+    require(n >= 0 && n_head > 0 && max_keys >= 0 && max_run >= 0, "mk_attention_kv4: bad sizes");
+    if (n == 0) return;
+    const mk::Kv4 K = kv4_layer(kv, layer, "mk_attention_kv4");
+    const int D = kv->head_dim;
+    require(n_head % K.KV == 0 && (int64_t)n_head * D < (1ll << 31), "mk_attention_kv4: bad head layout");
+    if (n_head / K.KV > 32) throw mk::Error(MK_ERR_UNSUPPORTED, "mk_attention_kv4: no kernel for this head layout");
+    require(q && out && seq && n_keys, "mk_attention_kv4: null array");
+    require(q_stride >= (int64_t)n_head * D && out_stride >= (int64_t)n_head * D,
+            "mk_attention_kv4: stride shorter than a row");
+    require((int64_t)n * n_head < (1 << 24), "mk_attention_kv4: too many rows");
+    require(max_keys <= (int64_t)kv->max_pages * kv->page, "mk_attention_kv4: max_keys past the sequences' pages");
+    const mk::Kv4Attn A{K, n, n_head, max_keys, max_run, 1.0f / std::sqrt(static_cast<float>(D)), seq, n_keys};
+    require(holds(workspace, workspace_bytes, mk::attention_kv4_need(A, D)),
+            "mk_attention_kv4: workspace smaller than mk_attention_kv4_workspace, or not aligned");
+    require(c != nullptr, "mk_attention_kv4: null context");
+    const DeviceOf on(c);
+    mk::attention_kv4(c->stream, A, D, q, q_stride, out, out_stride, static_cast<mk::BlockQ8*>(xq), workspace);
+  });
+}
+
+size_t mk_kv4_fork_workspace(int n, int max_pages) {
+  return n > 0 && max_pages > 0 ? mk::kv4_fork_workspace(n, max_pages) : 0;
+}
+
+int mk_kv4_fork(mk_ctx* c, const mk_kv4_cache* kv, const int32_t* dst, const int32_t* src, int n, void* workspace,
+                size_t workspace_bytes) {
+  return guard([&] {
+    require(n >= 0, "mk_kv4_fork: bad sizes");
+    if (n == 0) return;
+    const mk::Kv4Pool P = kv4_pool(kv, "mk_kv4_fork");
+    require(src != nullptr, "mk_kv4_fork: null array");
+    require(n <= (1 << 20), "mk_kv4_fork: too many entries");
+    require(holds(workspace, workspace_bytes, mk::kv4_fork_workspace(n, kv->max_pages)),
+            "mk_kv4_fork: workspace smaller than mk_kv4_fork_workspace, or not aligned");
+    require(c != nullptr, "mk_kv4_fork: null context");
+    const DeviceOf on(c);
+    mk::kv4_fork(c->stream, P, dst, src, n, workspace);
+  });
+}
+
+size_t mk_kv4_resize_workspace(int n, int n_page) {
+  return n > 0 && n_page > 0 ? mk::kv4_resize_workspace(n, n_page) : 0;
+}
+
+int mk_kv4_resize(mk_ctx* c, const mk_kv4_cache* kv, const int32_t* seq, const int32_t* new_len, int n, int32_t* status,
+                  void* workspace, size_t workspace_bytes) {
+  return guard([&] {
+    require(n >= 0, "mk_kv4_resize: bad sizes");
+    if (n == 0) return;
+    const mk::Kv4Pool P = kv4_pool(kv, "mk_kv4_resize");
+    require(new_len && status, "mk_kv4_resize: null array");
+    require(n <= 4096, "mk_kv4_resize: more than 4096 entries");
+    require(holds(workspace, workspace_bytes, mk::kv4_resize_workspace(n, kv->n_page)),
+            "mk_kv4_resize: workspace smaller than mk_kv4_resize_workspace, or not aligned");
+    require(c != nullptr, "mk_kv4_resize: null context");
+    const DeviceOf on(c);
+    mk::kv4_resize(c->stream, P, kv->head_dim, seq, new_len, n, status, workspace);
+  });
+}
+
+size_t mk_kv4_compact_workspace(int n_page) { return n_page > 0 ? mk::kv4_compact_workspace(n_page) : 0; }
+
+int mk_kv4_compact(mk_ctx* c, const mk_kv4_cache* kv, int32_t* n_live, void* workspace, size_t workspace_bytes) {
+  return guard([&] {
+    const mk::Kv4Pool P = kv4_pool(kv, "mk_kv4_compact");
+    require(n_live != nullptr, "mk_kv4_compact: null array");
+    require(holds(workspace, workspace_bytes, mk::kv4_compact_workspace(kv->n_page)),
+            "mk_kv4_compact: workspace smaller than mk_kv4_compact_workspace, or not aligned");
+    require(c != nullptr, "mk_kv4_compact: null context");
+    const DeviceOf on(c);
+    mk::kv4_compact(c->stream, P, kv->head_dim, n_live, workspace);
+  });
+}
+
+size_t mk_beam_workspace(int n_group, int beams, int n_vocab, int k) {
+  return n_group > 0 && beams > 0 && beams <= 64 && n_vocab > 0 && k > 0 && k <= 128
+             ? mk::beam_workspace(n_group, beams, n_vocab, k)
+             : 0;
+}
+
+int mk_beam_select(mk_ctx* c, const float* logits, int64_t stride, int n_group, int beams, int n_vocab,
+                   const float* scores, const int32_t* done, int eos, int k, float* out_scores, int32_t* out_seq,
+                   int32_t* out_tokens, void* workspace, size_t workspace_bytes) {
+  return guard([&] {
+    require(n_group >= 0 && n_vocab > 0, "mk_beam_select: bad sizes");
+    require(beams >= 1 && beams <= 64, "mk_beam_select: beams outside 1..64");
+    require(k >= 1 && k <= 128, "mk_beam_select: k outside 1..128");
+    if (n_group == 0) return;
+    require(logits && scores && out_scores && out_seq && out_tokens, "mk_beam_select: null array");
+    require(stride >= n_vocab, "mk_beam_select: stride shorter than a row");
+    require(!done || (eos >= 0 && eos < n_vocab), "mk_beam_select: eos outside the vocabulary");
+    const int64_t rows = (int64_t)n_group * beams;
+    require(n_vocab <= 1 << 21, "mk_beam_select: vocabulary past 2^21");
+    require(rows < (1 << 20) && rows * ((n_vocab + 4095) / 4096) < (1 << 24), "mk_beam_select: too many rows");
+    require(holds(workspace, workspace_bytes, mk::beam_workspace(n_group, beams, n_vocab, k)),
+            "mk_beam_select: workspace smaller than mk_beam_workspace, or not aligned");
+    require(c != nullptr, "mk_beam_select: null context");
+    const DeviceOf on(c);
+    mk::beam_select(c->stream, logits, stride, n_group, beams, n_vocab, scores, done, eos, k, out_scores, out_seq,
+                    out_tokens, workspace);
+  });
+}
+
 size_t mk_lora_workspace(int n, int max_rank, int64_t cols) {
   return n > 0 && max_rank > 0 && cols > 0 ? mk::lora_workspace(n, max_rank, cols) : 0;
 }

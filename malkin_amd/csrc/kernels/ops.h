@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "common.h"
+#include "kv4.h"
 #include "layout.h"
 
 namespace mk {
@@ -160,6 +161,46 @@ size_t attention_prefix_workspace(int n, int H, int KV, int D, int n_prefix, int
 size_t attention_prefix_need(const PrefixAttn& A, int D);
 void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q, int64_t q_stride, float* out,
                       int64_t out_stride, BlockQ8* xq, void* workspace);
+
+// The 4-bit cache in pages (kv4.hip, attn_kv4.hip, pages.hip); include/malkin_hip.h has the layouts and rules.
+void rope_tables(hipStream_t s, const mk_rope& r, const float* divide, int64_t first, int n_pos, float* cos_t, float* sin_t);
+void rope_kv4(hipStream_t s, const Kv4& kv, int D, const float* q, const float* k, const float* v, int64_t stride, int n, int H,
+              const float* q_norm, const float* k_norm, float eps, bool pairs, int rope_dim, const float* cos_t,
+              const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row, float* q_out,
+              int64_t q_out_stride);
+void kv4_rows(hipStream_t s, const Kv4& kv, int D, const int32_t* seq, const int32_t* rows, int n, void* k_out, void* v_out);
+struct Kv4Attn {
+  Kv4 kv;
+  int n, H, max_keys, max_run;
+  float scale;
+  const int32_t* seq;
+  const int32_t* n_keys;
+};
+size_t attention_kv4_workspace(int n, int H, int KV, int D, int max_keys, int max_run);  // never less for a larger batch
+size_t attention_kv4_need(const Kv4Attn& A, int D);  // what this call uses of it
+void attention_kv4(hipStream_t s, const Kv4Attn& A, int D, const float* q, int64_t q_stride, float* out, int64_t out_stride,
+                   BlockQ8* xq, void* workspace);
+// The whole cache, for the calls that move its pages.
+struct Kv4Pool {
+  uint8_t *k, *v;
+  uint16_t *ks, *vs;
+  int32_t *table, *len, *refs;
+  int n_page, n_seq, max_pages, shift;
+  int heads;  // (layer, KV head) pairs of a page
+};
+size_t kv4_fork_workspace(int n, int max_pages);
+void kv4_fork(hipStream_t s, const Kv4Pool& P, const int32_t* dst, const int32_t* src, int n, void* workspace);
+size_t kv4_resize_workspace(int n, int n_page);
+void kv4_resize(hipStream_t s, const Kv4Pool& P, int D, const int32_t* seq, const int32_t* new_len, int n, int32_t* status,
+                void* workspace);
+size_t kv4_compact_workspace(int n_page);
+void kv4_compact(hipStream_t s, const Kv4Pool& P, int D, int32_t* n_live, void* workspace);
+
+// The k best continuations of each group of beams (beam.hip).
+size_t beam_workspace(int n_group, int beams, int n_vocab, int k);
+void beam_select(hipStream_t s, const float* logits, int64_t stride, int n_group, int beams, int n_vocab, const float* scores,
+                 const int32_t* done, int eos, int k, float* out_scores, int32_t* out_seq, int32_t* out_tokens,
+                 void* workspace);
 
 // Scratch the attention of `pairs` (token, head) pairs over max_keys keys uses (0: none).
 size_t attention_scratch_bytes(int D, int max_keys, int pairs);

@@ -1,0 +1,389 @@
+// The pages of the 4-bit cache (include/malkin_hip.h): forking, resizing with copies of shared last pages, compaction.
+//
+// What a sequence holds is a row of page numbers, so that going on from another sequence copies numbers and counts holders;
+// bytes are copied only where a shared page that is not full is to be written, and in compaction. Results do not depend on
+// the order in which threads run: counts change by sums of whole numbers, and free pages are handed out by running sums over
+// the entries and over the pool, lowest number first, in one workgroup. What bounds a call is that workgroup's chain of loads
+// and barriers (a few microseconds) and then the copies' bytes, which a second launch moves with the whole chip.
+#include <algorithm>
+
+#include "ctx.h"
+#include "ops.h"
+
+namespace mk {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPlan = 1024;      // threads of the one workgroup that hands out pages
+constexpr int kMaxEntries = 4096;  // of a resize
+constexpr int kScan = 16;        // pages per thread and step of a walk over the pool
+
+__device__ __forceinline__ int pages_of(int rows, int shift) { return (int)(((int64_t)rows + (1 << shift) - 1) >> shift); }
+
+// Rows that sequence s holds, never more than its entries of the table.
+__device__ __forceinline__ int held(const Kv4Pool& P, int s) {
+  const int64_t room = (int64_t)P.max_pages << P.shift;
+  return (int)min((int64_t)max(P.len[s], 0), room);
+}
+
+// ---- fork ----
+
+// Per entry: its source's pages as they are before the call, to the workspace, and the counts of holders. A count reaches its
+// new value by additions alone, so entries need no order. head[i]: rows, -1 where the entry has no effect.
+__global__ __launch_bounds__(kThreads) void k_fork_take(Kv4Pool P, const int32_t* __restrict__ dst,
+                                                        const int32_t* __restrict__ src, int n, int32_t* __restrict__ head,
+                                                        int32_t* __restrict__ rows) {
+  const int i = blockIdx.x, tid = threadIdx.x;
+  const int d = dst ? dst[i] : i, s = src[i];
+  bool ok = d >= 0 && d < P.n_seq;
+  if (dst && ok) {
+    bool again = false;
+    for (int j = i + 1 + tid; j < n; j += kThreads) again |= dst[j] == d;
+    ok = !__syncthreads_or(again);
+  }
+  const bool from = s >= 0 && s < P.n_seq;
+  if (!ok || s == d) {
+    if (tid == 0) head[i] = -1;
+    return;
+  }
+  const int len = from ? held(P, s) : 0, m = pages_of(len, P.shift), old = pages_of(held(P, d), P.shift);
+  for (int j = tid; j < max(m, old); j += kThreads) {
+    const int a = j < m ? P.table[(int64_t)s * P.max_pages + j] : -1;
+    const int b = j < old ? P.table[(int64_t)d * P.max_pages + j] : -1;
+    rows[(int64_t)i * P.max_pages + j] = a;
+    if (a == b) continue;
+    if (a >= 0 && a < P.n_page) atomicAdd(P.refs + a, 1);
+    if (b >= 0 && b < P.n_page) atomicAdd(P.refs + b, -1);
+  }
+  if (tid == 0) head[i] = len;
+}
+
+__global__ __launch_bounds__(kThreads) void k_fork_put(Kv4Pool P, const int32_t* __restrict__ dst, int n,
+                                                       const int32_t* __restrict__ head, const int32_t* __restrict__ rows) {
+  const int i = blockIdx.x, len = head[i];
+  if (len < 0) return;
+  const int d = dst ? dst[i] : i;
+  const int m = max(pages_of(len, P.shift), pages_of(held(P, d), P.shift));
+  for (int j = threadIdx.x; j < m; j += kThreads) P.table[(int64_t)d * P.max_pages + j] = rows[(int64_t)i * P.max_pages + j];
+  __syncthreads();  // every thread has read the old length
+  if (threadIdx.x == 0) P.len[d] = len;
+}
+
+// ---- copies ----
+
+struct Move {
+  int32_t src, dst, rows;
+};
+
+// Rows 0 .. rows - 1 of page src to page dst, a wave per (move, head of a layer).
+template <int D>
+__device__ __forceinline__ void copy_head(const Kv4Pool& P, const Move& m, int head, int lane) {
+  constexpr int kPieces = D / 32, G = D / 32;  // 16-byte pieces of a row, groups
+  const int64_t from = ((int64_t)m.src * P.heads + head) << P.shift, to = ((int64_t)m.dst * P.heads + head) << P.shift;
+  const uint4 *kf = reinterpret_cast<const uint4*>(P.k) + from * kPieces, *vf = reinterpret_cast<const uint4*>(P.v) + from * kPieces;
+  uint4 *kt = reinterpret_cast<uint4*>(P.k) + to * kPieces, *vt = reinterpret_cast<uint4*>(P.v) + to * kPieces;
+  for (int i = lane; i < m.rows * kPieces; i += 64) {
+    const uint4 a = kf[i], b = vf[i];
+    kt[i] = a, vt[i] = b;
+  }
+  const uint16_t *sf = P.ks + from * G, *wf = P.vs + from * G;
+  uint16_t *st = P.ks + to * G, *wt = P.vs + to * G;
+  for (int i = lane; i < m.rows * G; i += 64) {
+    const int at = (i / m.rows << P.shift) + i % m.rows;
+    const uint16_t a = sf[i], b = wf[at];
+    st[i] = a, wt[at] = b;
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void k_copy_pages(Kv4Pool P, const int32_t* __restrict__ count,
+                                                         const Move* __restrict__ moves) {
+  const int lane = threadIdx.x & 63;
+  const int64_t items = (int64_t)*count * P.heads;
+  for (int64_t it = (int64_t)blockIdx.x * (kThreads / 64) + threadIdx.x / 64; it < items; it += (int64_t)gridDim.x * (kThreads / 64)) {
+    const Move m = moves[it / P.heads];
+    copy_head<D>(P, m, (int)(it % P.heads), lane);
+  }
+}
+
+// ---- in one workgroup ----
+
+// Exclusive running sum over the workgroup's threads, and the total. part: kPlan / 64 + 1 words of LDS, free again after the
+// caller's next barrier.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* part, T& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  T x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const T y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) part[w] = x;
+  __syncthreads();
+  T before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kPlan / 64; ++i) {
+    const T p = part[i];
+    before += i < w ? p : 0;
+    all += p;
+  }
+  total = all;
+  return before + x - v;
+}
+
+__device__ __forceinline__ int refs_now(const int32_t* p) { return (int)ld_coh_u32(reinterpret_cast<const uint32_t*>(p)); }
+
+// Entry i's sequence and end; kind: what becomes of it.
+enum { kSkip = 0, kShrink = 1, kGrow = 2 };
+
+__global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t* __restrict__ seq,
+                                                       const int32_t* __restrict__ new_len, int n, int32_t* __restrict__ status,
+                                                       int32_t* __restrict__ count, Move* __restrict__ moves, int32_t* free_list) {
+  extern __shared__ int32_t lds[];
+  int32_t *seq_s = lds, *last_s = lds + n, *base_s = lds + 2 * n;  // base_s: the entry's first page in free_list, -1 none
+  __shared__ int part[kPlan / 64];
+  __shared__ int64_t part64[kPlan / 64];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int E = (n + kPlan - 1) / kPlan, i0 = tid * E;  // a thread's entries follow each other
+  for (int i = tid; i < n; i += kPlan) seq_s[i] = seq ? seq[i] : i;
+  __syncthreads();
+  const int64_t room = (int64_t)P.max_pages << P.shift;
+  // What does not fit, or comes again; status 2 marks what is to grow.
+  for (int i = tid; i < n; i += kPlan) {
+    const int s = seq_s[i], L = new_len[i];
+    bool ok = s >= 0 && s < P.n_seq && L >= 0 && L <= room;
+    if (seq)
+      for (int j = i + 1; j < n && ok; ++j) ok = seq_s[j] != s;
+    last_s[i] = -1;
+    base_s[i] = !ok ? kSkip : L > held(P, s) ? kGrow : kShrink;
+  }
+  __syncthreads();
+  // Shorter ends, a wave per entry.
+  for (int i = w; i < n; i += kPlan / 64) {
+    if (base_s[i] != kShrink) continue;
+    const int s = seq_s[i], had = pages_of(held(P, s), P.shift), has = pages_of(new_len[i], P.shift);
+    for (int j = has + lane; j < had; j += 64) {
+      int32_t* at = P.table + (int64_t)s * P.max_pages + j;
+      const int p = *at;
+      if (p >= 0 && p < P.n_page) atomicAdd(P.refs + p, -1);
+      *at = -1;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (lane == 0) P.len[s] = new_len[i];
+  }
+  // The last pages of those that grow.
+  for (int i = tid; i < n; i += kPlan) {
+    if (base_s[i] != kGrow) continue;
+    const int s = seq_s[i], len = held(P, s);
+    if (len & ((1 << P.shift) - 1)) {
+      const int p = P.table[(int64_t)s * P.max_pages + (len >> P.shift)];
+      last_s[i] = p >= 0 && p < P.n_page ? p : -1;
+    }
+  }
+  __syncthreads();  // the counts have been taken down too
+  // Copies and pages wanted, and where each entry's pages begin in the list of free ones. More than the pool has counts as one
+  // more than that.
+  int copies[kMaxEntries / kPlan], needs[kMaxEntries / kPlan];
+  int64_t mine = 0;
+#pragma unroll
+  for (int e = 0; e < kMaxEntries / kPlan; ++e) {
+    copies[e] = needs[e] = 0;
+    const int i = i0 + e;
+    if (e >= E || i >= n || base_s[i] != kGrow) continue;
+    if (last_s[i] >= 0) {
+      const int holders = refs_now(P.refs + last_s[i]);
+      int before = 0;
+      if (holders > 1)
+        for (int j = 0; j < i; ++j) before += last_s[j] == last_s[i];
+      copies[e] = before < holders - 1;
+    }
+    needs[e] = min(copies[e] + pages_of(new_len[i], P.shift) - pages_of(held(P, seq_s[i]), P.shift), P.n_page + 1);
+    mine += needs[e];
+  }
+  int64_t wanted = 0;
+  const int64_t at = block_scan(mine, part64, wanted);
+  // The first free pages of the pool, as many as are wanted.
+  int found = 0;
+  for (int p0 = 0; p0 < P.n_page && found < wanted; p0 += kScan * kPlan) {
+    uint32_t free = 0;
+#pragma unroll
+    for (int e = 0; e < kScan; ++e) {
+      const int p = p0 + kScan * tid + e;
+      if (p < P.n_page && refs_now(P.refs + p) <= 0) free |= 1u << e;
+    }
+    int all = 0, to = found + block_scan((int)__popc(free), part, all);
+#pragma unroll
+    for (int e = 0; e < kScan; ++e)
+      if (free >> e & 1) {
+        if (to < wanted) free_list[to] = p0 + kScan * tid + e;
+        ++to;
+      }
+    found += all;
+  }
+  // What does not fit does not happen.
+  int n_copy = 0;
+  int64_t run = at;
+#pragma unroll
+  for (int e = 0; e < kMaxEntries / kPlan; ++e) {
+    if (needs[e] && run + needs[e] > found) copies[e] = 0;
+    n_copy += copies[e];
+    run += needs[e];
+  }
+  int total = 0, slot = block_scan(n_copy, part, total);
+  __syncthreads();  // free_list is written, everyone has read base_s and the counts
+  run = at;
+#pragma unroll
+  for (int e = 0; e < kMaxEntries / kPlan; ++e) {
+    const int i = i0 + e;
+    if (e >= E || i >= n) continue;
+    if (base_s[i] != kGrow) {
+      status[i] = base_s[i] == kSkip ? -1 : 0;
+      base_s[i] = -1;
+      continue;
+    }
+    const bool fits = needs[e] == 0 || run + needs[e] <= found;
+    const int s = seq_s[i], len = held(P, s);
+    if (copies[e]) {
+      const int p = free_list[run];
+      moves[slot++] = Move{last_s[i], p, len & ((1 << P.shift) - 1)};
+      P.table[(int64_t)s * P.max_pages + (len >> P.shift)] = p;
+      atomicAdd(P.refs + last_s[i], -1);
+      atomicAdd(P.refs + p, 1);
+    }
+    status[i] = fits ? 0 : 1;
+    base_s[i] = fits ? (int)run + copies[e] : -1;
+    run += needs[e];
+  }
+  if (tid == 0) *count = total;
+  __syncthreads();
+  // New pages, a wave per entry, and the new lengths.
+  for (int i = w; i < n; i += kPlan / 64) {
+    if (base_s[i] < 0) continue;
+    const int s = seq_s[i], had = pages_of(held(P, s), P.shift), has = pages_of(new_len[i], P.shift);
+    for (int j = lane; j < has - had; j += 64) {
+      const int p = free_list[base_s[i] + j];
+      P.table[(int64_t)s * P.max_pages + had + j] = p;
+      atomicAdd(P.refs + p, 1);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (lane == 0) P.len[s] = new_len[i];
+  }
+}
+
+// ---- compaction ----
+
+// moves: hole j of the first n_live pages gets the j-th page in use beyond them. to[p]: where page p >= n_live went.
+__global__ __launch_bounds__(kPlan) void k_compact_plan(Kv4Pool P, int32_t* __restrict__ n_live, int32_t* __restrict__ count,
+                                                        Move* __restrict__ moves, int32_t* __restrict__ to) {
+  __shared__ int part[kPlan / 64];
+  const int tid = threadIdx.x;
+  int live = 0;
+  for (int p = tid; p < P.n_page; p += kPlan) live += P.refs[p] > 0;
+  int total = 0;
+  block_scan(live, part, total);
+  int holes = 0, movers = 0;  // found so far
+  for (int p0 = 0; p0 < P.n_page; p0 += kScan * kPlan) {
+    int hole = 0, mover = 0;
+    uint32_t used = 0;
+#pragma unroll
+    for (int e = 0; e < kScan; ++e) {
+      const int p = p0 + kScan * tid + e;
+      if (p < P.n_page && P.refs[p] > 0) used |= 1u << e, mover += p >= total;
+      else if (p < total) ++hole;
+      else if (p < P.n_page) to[p] = p;  // nobody's
+    }
+    int all_h = 0, all_m = 0;
+    int h = holes + block_scan(hole, part, all_h);
+    int m = movers + block_scan(mover, part, all_m);
+#pragma unroll
+    for (int e = 0; e < kScan; ++e) {
+      const int p = p0 + kScan * tid + e;
+      if (used >> e & 1) {
+        if (p >= total) moves[m++].src = p;
+      } else if (p < total) {
+        moves[h++].dst = p;
+      }
+    }
+    holes += all_h, movers += all_m;
+  }
+  __syncthreads();
+  for (int j = tid; j < holes; j += kPlan) {
+    const int src = moves[j].src, dst = moves[j].dst;
+    moves[j].rows = 1 << P.shift;
+    to[src] = dst;
+    P.refs[dst] = P.refs[src];
+    P.refs[src] = 0;
+  }
+  if (tid == 0) *count = holes, *n_live = total;
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void k_compact_move(Kv4Pool P, const int32_t* __restrict__ n_live,
+                                                           const int32_t* __restrict__ count, const Move* __restrict__ moves,
+                                                           const int32_t* __restrict__ to) {
+  const int lane = threadIdx.x & 63, live = *n_live;
+  const int64_t entries = (int64_t)P.n_seq * P.max_pages;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < entries; i += (int64_t)gridDim.x * kThreads) {
+    const int p = P.table[i];
+    if (p >= live && p < P.n_page) P.table[i] = to[p];
+  }
+  const int64_t items = (int64_t)*count * P.heads;
+  for (int64_t it = (int64_t)blockIdx.x * (kThreads / 64) + threadIdx.x / 64; it < items; it += (int64_t)gridDim.x * (kThreads / 64))
+    copy_head<D>(P, moves[it / P.heads], (int)(it % P.heads), lane);
+}
+
+constexpr int kHead = 16;  // bytes before a list: its length
+
+unsigned copy_wgs(int64_t moves, int heads) {
+  const int64_t wgs = (moves * heads + kThreads / 64 - 1) / (kThreads / 64);
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(wgs, 8 * device_cus()));
+}
+
+}  // namespace
+
+size_t kv4_fork_workspace(int n, int max_pages) { return (size_t)n * (max_pages + 1ull) * 4; }
+
+void kv4_fork(hipStream_t s, const Kv4Pool& P, const int32_t* dst, const int32_t* src, int n, void* workspace) {
+  int32_t *head = static_cast<int32_t*>(workspace), *rows = head + n;
+  hipLaunchKernelGGL(k_fork_take, dim3((unsigned)n), dim3(kThreads), 0, s, P, dst, src, n, head, rows);
+  check_launch("kv4_fork take");
+  hipLaunchKernelGGL(k_fork_put, dim3((unsigned)n), dim3(kThreads), 0, s, P, dst, n, head, rows);
+  check_launch("kv4_fork put");
+}
+
+size_t kv4_resize_workspace(int n, int n_page) { return kHead + (size_t)n * sizeof(Move) + (size_t)n_page * 4; }
+
+void kv4_resize(hipStream_t s, const Kv4Pool& P, int D, const int32_t* seq, const int32_t* new_len, int n, int32_t* status,
+                void* workspace) {
+  int32_t* count = static_cast<int32_t*>(workspace);
+  Move* moves = reinterpret_cast<Move*>(count + kHead / 4);
+  int32_t* free_list = reinterpret_cast<int32_t*>(moves + n);
+  hipLaunchKernelGGL(k_resize_plan, dim3(1), dim3(kPlan), (size_t)n * 12, s, P, seq, new_len, n, status, count, moves, free_list);
+  check_launch("kv4_resize plan");
+  auto go = [&]<int D_>() {
+    hipLaunchKernelGGL(k_copy_pages<D_>, dim3(copy_wgs(n, P.heads)), dim3(kThreads), 0, s, P, count, moves);
+  };
+  if (D == 128) go.template operator()<128>();
+  else go.template operator()<64>();
+  check_launch("kv4_resize copies");
+}
+
+size_t kv4_compact_workspace(int n_page) { return kHead + (size_t)n_page * (sizeof(Move) + 4); }
+
+void kv4_compact(hipStream_t s, const Kv4Pool& P, int D, int32_t* n_live, void* workspace) {
+  int32_t* count = static_cast<int32_t*>(workspace);
+  Move* moves = reinterpret_cast<Move*>(count + kHead / 4);
+  int32_t* to = reinterpret_cast<int32_t*>(moves + P.n_page);
+  hipLaunchKernelGGL(k_compact_plan, dim3(1), dim3(kPlan), 0, s, P, n_live, count, moves, to);
+  check_launch("kv4_compact plan");
+  auto go = [&]<int D_>() {
+    hipLaunchKernelGGL(k_compact_move<D_>, dim3(copy_wgs(P.n_page, P.heads)), dim3(kThreads), 0, s, P, n_live, count, moves, to);
+  };
+  if (D == 128) go.template operator()<128>();
+  else go.template operator()<64>();
+  check_launch("kv4_compact move");
+}
+
+}  // namespace mk
