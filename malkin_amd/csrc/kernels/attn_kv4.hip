@@ -1,9 +1,12 @@
-// Attention over the 4-bit cache in pages: out = sum_j p_j v_j, p = softmax(scale q.k_j), k = s (n - 8) and v likewise, exact in
-// fp16.
+// Attention over the 4-bit cache in pages: out = sum_j p_j v_j, p = softmax(scale q.k_j), k = s (n - 8) and v likewise, in fp16.
 //
-// Rows and keys. A query row is a (token, query head); the rows of one KV head and of up to 16 / G tokens of one sequence that
-// follow each other (G query heads per KV head) are a block of at most 16 rows that reads the same keys, 64 at a time. A tile's
-// 16-key chunks lie in one page each.
+// Rows and keys. A query row is a (token, query head); the rows of one KV head and of neighbouring tokens of one sequence are a
+// block of at most 16 or 32 rows that reads the same keys, 64 at a time. A tile's 16-key chunks lie in one page each.
+//
+// Split. Where a call has few keys a workgroup takes a block, and that is all. Otherwise as many workgroups as the chip holds
+// share all blocks' tiles evenly, whatever the sequences' lengths: each takes a contiguous run of them, writes the blocks that lie
+// whole in its run, and leaves partial results of the first and the last one, which a second launch adds. A run's place follows
+// from the tokens' lengths alone, by a running sum that every workgroup makes for itself.
 //
 // Arithmetic. v_mfma_f32_16x16x32_f16 with the fp32 side in two fp16 parts, hi = fp16(x) and lo = fp16(x - hi): 2^-23 of x is
 // kept. A row of q is first brought to a largest value of 2^13 .. 2^14 by a power of two; the weights are shifted so that the
@@ -34,8 +37,18 @@ typedef __attribute__((address_space(3))) v2i lds_v2i;
 constexpr float kNone = -3e38f;  // shift of a row that has seen no key
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kTile = 64, kChunk = 16;
-constexpr int kFew = 16;      // query rows of a block
+constexpr int kSet = 16;      // query rows of an MFMA
 constexpr int kIds = 1024;    // pages of chunks held in LDS at a time
+
+// How tokens and heads are taken together: R rows of a block, up to tq tokens with `per` heads each (hs blocks per KV head
+// and token where a KV head has more than R query heads), J blocks per run of tokens.
+struct Shape {
+  int G, tq, hs, J;
+};
+__host__ __device__ inline Shape shape_of(int H, int KV, int R) {
+  const int G = H / KV, hs = (G + R - 1) / R;
+  return Shape{G, G < R ? R / G : 1, hs, KV * hs};
+}
 
 // A block of rows of one KV head, and how many keys its tokens see at most.
 struct Block {
@@ -44,11 +57,23 @@ struct Block {
   __device__ __forceinline__ int rows() const { return m * per; }
   __device__ __forceinline__ int token(int r) const { return t0 + r / per; }
   __device__ __forceinline__ int head(int r) const { return h0 + r % per; }
+  __device__ __forceinline__ int tiles() const { return (keys + kTile - 1) / kTile; }
 };
+template <int R>
+__device__ __forceinline__ void set_heads(Block& b, const Shape& S, int j) {
+  const int sub = j % S.hs;
+  b.g = j / S.hs, b.h0 = b.g * S.G + R * sub, b.per = min(S.G - R * sub, R);
+}
 
 __device__ __forceinline__ int keys_of(const Kv4Attn& A, int t) {
   const int s = A.seq[t];
   return s >= 0 && s < A.kv.n_seq ? max(0, min(A.n_keys[t], A.max_keys)) : 0;
+}
+__device__ __forceinline__ bool starts(const Kv4Attn& A, int t) { return t == 0 || A.seq[t] != A.seq[t - 1]; }
+// The block that token t leads: it and the tokens of its sequence that follow, tq at most.
+__device__ __forceinline__ void set_tokens(Block& b, const Kv4Attn& A, int t, int tq) {
+  b.t0 = t, b.m = 1, b.keys = keys_of(A, t);
+  while (b.m < tq && t + b.m < A.n && !starts(A, t + b.m)) b.keys = max(b.keys, keys_of(A, t + b.m)), ++b.m;
 }
 
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
@@ -86,8 +111,9 @@ __device__ __forceinline__ v8h join8(const v2h (&r)[4]) {
 // Place of the e-th of eight elements (or keys) in that order.
 __device__ __forceinline__ constexpr int place(int e) { return (e & 1) * 4 + (e >> 1); }
 
-template <int D>
+template <int D, int NR, int NW>
 struct Geo {
+  static constexpr int kR = NR * kSet;             // rows of a block
   static constexpr int kSteps = D / 32;            // MFMAs over a row: lane qd of four holds its elements D / 4 qd + ..
   static constexpr int kDt = D / 16;               // 16-element tiles of a row
   static constexpr int kRow = D / 2, kGroups = D / 32;
@@ -95,31 +121,42 @@ struct Geo {
   static constexpr int kScales = kTile * kGroups * 2;
   static constexpr int kCopies = kBytes / 1024 + kScales / 256;
   static constexpr int kWave = 2 * (kBytes + kScales);
-  static constexpr int kStride = D + 4;            // of a row of results
+  static constexpr int kQ = kSteps * NR * 2 * 1024;  // q: [step][set][hi, lo][lane] 16 bytes
+  static constexpr int kStride = 64 + 4;             // of a row of results, 64 elements at a time
+  static constexpr int kOut = NW * kR * kStride * 4;
+  static constexpr int kRing = NW * kWave > kOut ? NW * kWave : kOut;
+  static constexpr int kLds = kQ + kRing;
 };
 
-// What a wave holds of its rows: this lane's is row lane % 16; o[i][j] is its element 16 i + 4 (lane / 16) + j.
-template <int D>
+// What a wave holds of its rows: this lane's of set n is row 16 n + lane % 16; o[i][j] is its element 16 i + 4 (lane / 16) + j.
+template <int D, int NR>
 struct Acc {
-  v4f o[Geo<D>::kDt];
-  float m, l;  // weights are 2^(score - m), l this lane's sum of them
+  v4f o[NR][D / 16];
+  float m[NR], l[NR];  // weights are 2^(score - m), l this lane's sum of them
+};
+
+// Where a tile's chunks lie: their first rows in the pool (chunks without a page: page 0's) and in the scales of V.
+struct Place {
+  int64_t row[4], vs[4];
+  int have;  // chunks that have a page
 };
 
 // One wave's copies and products. Everything here is the wave's own: no barrier.
-template <int D>
+template <int D, int NR, int NW>
 struct Walk {
-  using G_ = Geo<D>;
+  using G_ = Geo<D, NR, NW>;
   const Kv4Attn& A;
   int g, lane, li, qd;
+  const uint8_t* q_s;
   uint8_t *ks_s, *k_s, *v_s, *vs_s;
   uint32_t k_off, v_off;  // this lane's part of a copy
-  v8h hi[G_::kSteps], lo[G_::kSteps];
-  float rf;        // score, in bits, of one unit of a product
-  int lim, least;  // keys that this lane's row sees, and that every row of the block sees
+  float rf[NR];           // score, in bits, of one unit of a product
+  int lim[NR], least;     // keys that this lane's rows see, and that every row of the block sees
 
-  __device__ __forceinline__ Walk(const Kv4Attn& a, uint8_t* lds) : A(a) {
+  __device__ __forceinline__ Walk(const Kv4Attn& a, uint8_t* smem, int w) : A(a) {
     lane = threadIdx.x & 63, li = lane & 15, qd = lane >> 4;
-    k_s = lds, v_s = k_s + G_::kBytes, ks_s = v_s + G_::kBytes, vs_s = ks_s + G_::kScales;
+    q_s = smem;
+    k_s = smem + G_::kQ + w * G_::kWave, v_s = k_s + G_::kBytes, ks_s = v_s + G_::kBytes, vs_s = ks_s + G_::kScales;
     if constexpr (D == 128) {
       k_off = li * 64 + 16 * qd;
       v_off = (lane >> 2) * 64 + 16 * ((lane & 3) ^ (lane >> 4));
@@ -129,109 +166,60 @@ struct Walk {
     }
   }
 
-  // This lane's row of q, scaled, in two parts.
-  __device__ __forceinline__ void load_q(const Block& b, const float* q, int64_t q_stride) {
-    g = b.g;
-    const int r = min(li, b.rows() - 1), t = b.token(r);
-    const float* qr = q + t * q_stride + (int64_t)b.head(r) * D + D / 4 * qd;
-    float x[G_::kSteps][8], top = 0.0f;
+  // ids: the pages of the tile's four chunks; key: its first key.
+  __device__ __forceinline__ Place find(const int* ids, int key) const {
+    const int4 id = *reinterpret_cast<const int4*>(ids);
+    const int p[4] = {__builtin_amdgcn_readfirstlane(id.x), __builtin_amdgcn_readfirstlane(id.y),
+                      __builtin_amdgcn_readfirstlane(id.z), __builtin_amdgcn_readfirstlane(id.w)};
+    Place at;
+    at.have = 0;
 #pragma unroll
-    for (int s = 0; s < G_::kSteps; ++s) {
-      float y[8];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const v4f f = *reinterpret_cast<const v4a*>(qr + 8 * s + 4 * c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[4 * c + e] = f[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[s][e] = y[place(e)], top = fmaxf(top, fabsf(y[e]));
+    for (int c = 0; c < 4; ++c) {
+      const int64_t first = A.kv.first_row(max(p[c], 0), g);
+      const int r = (key + kChunk * c) & ((1 << A.kv.shift) - 1);
+      at.row[c] = first + r, at.vs[c] = first * G_::kGroups + r;
+      at.have |= (p[c] >= 0) << c;
     }
-    lim = keys_of(A, t);
-    least = lim;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) least = min(least, __shfl_xor(least, o));
-    least = __builtin_amdgcn_readfirstlane(least);
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    int ex = 0;
-    if (top > 0.0f && top < INFINITY) ex = min(14 - __builtin_amdgcn_frexp_expf(top), 100);
-    rf = __builtin_ldexpf(A.scale * kLog2e, -ex);
-#pragma unroll
-    for (int s = 0; s < G_::kSteps; ++s) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[s][e] = __builtin_ldexpf(x[s][e], ex);
-      split8(x[s], hi[s], lo[s]);
-    }
+    return at;
   }
-
-  // First row of the tile's chunk c in the pool, less its row in the page, and that row. Chunks without a page: page 0's.
-  struct Place {
-    int64_t first;
-    int r;
-  };
-  __device__ __forceinline__ Place where(const int* ids, int key, int c) const {
-    const int p = max(__builtin_amdgcn_readfirstlane(ids[c]), 0);
-    return Place{A.kv.first_row(p, g), (key + kChunk * c) & ((1 << A.kv.shift) - 1)};
-  }
-  // ids: the tile's four chunks' pages; key: its first key.
-  __device__ __forceinline__ void issue_k(const int* ids, int key) const {
-    Place at[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) at[c] = where(ids, key, c);
+  __device__ __forceinline__ void issue_k(const Place& at) const {
     if constexpr (D == 128) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) lds_copy16(A.kv.k + (at[c].first + at[c].r) * 64, k_off, k_s + 1024 * c);
+      for (int c = 0; c < 4; ++c) lds_copy16(A.kv.k + at.row[c] * 64, k_off, k_s + 1024 * c);
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        const int64_t row = lane < 32 ? at[c].first + at[c].r : at[c + 1].first + at[c + 1].r;
-        lds_copy4(reinterpret_cast<const uint8_t*>(A.kv.ks) + row * 8 + 4 * (lane & 31), ks_s + 128 * c);
-      }
+      for (int c = 0; c < 4; c += 2)
+        lds_copy4(reinterpret_cast<const uint8_t*>(A.kv.ks) + (lane < 32 ? at.row[c] : at.row[c + 1]) * 8 + 4 * (lane & 31),
+                  ks_s + 128 * c);
     } else {
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        const int64_t row = lane < 32 ? at[c].first + at[c].r : at[c + 1].first + at[c + 1].r;
-        lds_copy16(A.kv.k + row * 32 + k_off, k_s + 512 * c);
-      }
-      const int64_t a = lane & 16 ? at[1].first + at[1].r : at[0].first + at[0].r;
-      const int64_t b = lane & 16 ? at[3].first + at[3].r : at[2].first + at[2].r;
+      for (int c = 0; c < 4; c += 2) lds_copy16(A.kv.k + (lane < 32 ? at.row[c] : at.row[c + 1]) * 32 + k_off, k_s + 512 * c);
+      const int64_t a = lane & 16 ? at.row[1] : at.row[0], b = lane & 16 ? at.row[3] : at.row[2];
       lds_copy4(reinterpret_cast<const uint8_t*>(A.kv.ks) + (lane < 32 ? a : b) * 4 + 4 * li, ks_s);
     }
   }
   // The scales of V in LDS: [chunk][group][key].
-  __device__ __forceinline__ void issue_v(const int* ids, int key) const {
-    Place at[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) at[c] = where(ids, key, c);
-    auto scales = [&](int c) { return at[c].first * G_::kGroups + at[c].r; };
-    const int in = ((lane >> 3) & (G_::kGroups - 1)) << A.kv.shift;
+  __device__ __forceinline__ void issue_v(const Place& at) const {
+    const int in = (((lane >> 3) & (G_::kGroups - 1)) << A.kv.shift) + 2 * (lane & 7);
     if constexpr (D == 128) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) lds_copy16(A.kv.v + (at[c].first + at[c].r) * 64, v_off, v_s + 1024 * c);
+      for (int c = 0; c < 4; ++c) lds_copy16(A.kv.v + at.row[c] * 64, v_off, v_s + 1024 * c);
 #pragma unroll
-      for (int c = 0; c < 4; c += 2)
-        lds_copy4(A.kv.vs + (lane < 32 ? scales(c) : scales(c + 1)) + in + 2 * (lane & 7), vs_s + 128 * c);
+      for (int c = 0; c < 4; c += 2) lds_copy4(A.kv.vs + (lane < 32 ? at.vs[c] : at.vs[c + 1]) + in, vs_s + 128 * c);
     } else {
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        const int64_t row = lane < 32 ? at[c].first + at[c].r : at[c + 1].first + at[c + 1].r;
-        lds_copy16(A.kv.v + row * 32 + v_off, v_s + 512 * c);
-      }
-      const int64_t a = lane & 16 ? scales(1) : scales(0), b = lane & 16 ? scales(3) : scales(2);
-      lds_copy4(A.kv.vs + (lane < 32 ? a : b) + in + 2 * (lane & 7), vs_s);
+      for (int c = 0; c < 4; c += 2) lds_copy16(A.kv.v + (lane < 32 ? at.row[c] : at.row[c + 1]) * 32 + v_off, v_s + 512 * c);
+      const int64_t a = lane & 16 ? at.vs[1] : at.vs[0], b = lane & 16 ? at.vs[3] : at.vs[2];
+      lds_copy4(A.kv.vs + (lane < 32 ? a : b) + in, vs_s);
     }
   }
 
-  // One tile: keys key .. key + 63, of which those below `end` count (end <= the block's keys). next: the pages of the wave's
-  // next tile at key `next_key`, or NULL.
-  __device__ __forceinline__ void tile(Acc<D>& acc, bool& fresh, const int* ids, int key, int end, const int* next, int next_key) const {
+  // One tile: keys key .. key + 63, of which those below `end` count (end <= the block's keys) and whose chunk has a page.
+  // more: `next` is the wave's next tile, whose copies are asked for.
+  __device__ __forceinline__ void tile(Acc<D, NR>& acc, bool& fresh, int have, int key, int end, bool more, const Place& next) const {
     wait_vm<G_::kCopies>();  // this tile's K; its V may be under way
     fence();
-    int have = 0;  // chunks that have a page
-#pragma unroll
-    for (int c = 0; c < 4; ++c) have |= (__builtin_amdgcn_readfirstlane(ids[c]) >= 0) << c;
     const bool whole = key + kTile <= min(least, end) && have == 15;
-    v4f s[4];
+    v4f s[NR][4];
     {
       uint32_t w[4][G_::kSteps];
       _Float16 sc[4];
@@ -248,73 +236,89 @@ struct Walk {
         }
       }
       wait_lds();  // K is in registers, and its place free for the next tile's
-      if (next) issue_k(next, next_key);
+      if (more) issue_k(next);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[c] = v4f{};
-        const v2h f = {sc[c], sc[c]};
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int i = 0; i < G_::kSteps; ++i) {
+        for (int c = 0; c < 4; ++c) s[n][c] = v4f{};
+#pragma unroll
+      for (int i = 0; i < G_::kSteps; ++i) {
+        v8h hi[NR], lo[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const v8h* from = reinterpret_cast<const v8h*>(q_s) + (i * NR + n) * 128 + lane;
+          hi[n] = from[0], lo[n] = from[64];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
           v2h r[4];
           less8(w[c][i], r);
+          const v2h f = {sc[c], sc[c]};
 #pragma unroll
           for (int j = 0; j < 4; ++j) r[j] *= f;
           const v8h a = join8(r);
-          s[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[i], s[c], 0, 0, 0);
-          s[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo[i], s[c], 0, 0, 0);
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            s[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[n], s[n][c], 0, 0, 0);
+            s[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo[n], s[n][c], 0, 0, 0);
+          }
         }
       }
     }
     // Register i of chunk c is key 16 c + 4 qd + i.
+    v8h ph[NR][2], pl[NR][2];
+    const bool first = fresh;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      s[c] *= rf;
-      if (!whole)
+    for (int n = 0; n < NR; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = key + kChunk * c + 4 * qd + i;
-          s[c][i] = k < min(lim, end) && (have >> c & 1) ? s[c][i] : -INFINITY;
+      for (int c = 0; c < 4; ++c) {
+        s[n][c] *= rf[n];
+        if (!whole)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = key + kChunk * c + 4 * qd + i;
+            s[n][c][i] = k < min(lim[n], end) && (have >> c & 1) ? s[n][c][i] : -INFINITY;
+          }
+      }
+      float p[16], sum, top;
+      auto weights = [&] __attribute__((always_inline)) {
+        sum = top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(s[n][i / 4][i % 4] - acc.m[n]);
+          sum += p[i];
+          top = fmaxf(top, p[i]);
         }
-    }
-    float p[16], sum, top;
-    auto weights = [&] __attribute__((always_inline)) {
-      sum = top = 0.0f;
+      };
+      if (!first) weights();
+      // The first tile, and one whose weights leave fp16: a new shift, 10 below the largest score (that score itself where 10
+      // is not exact beside it).
+      if (first || __ballot(top > 32768.0f)) {
+        float z = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - acc.m);
-        sum += p[i];
-        top = fmaxf(top, p[i]);
+        for (int i = 0; i < 16; ++i) z = fmaxf(z, s[n][i / 4][i % 4]);
+        z = fmaxf(z, __shfl_xor(z, 16));
+        z = fmaxf(z, __shfl_xor(z, 32));
+        const float m = fmaxf(acc.m[n], fabsf(z) < 0x1p24f ? z - 10.0f : z);
+        const float f = __builtin_amdgcn_exp2f(acc.m[n] - m);
+        acc.m[n] = m, acc.l[n] *= f;
+        if (!first) {
+#pragma unroll
+          for (int i = 0; i < G_::kDt; ++i) acc.o[n][i] *= f;
+        }
+        weights();
       }
-    };
-    if (!fresh) weights();
-    // The first tile, and one whose weights leave fp16: a new shift, 10 below the largest score (that score itself where 10
-    // is not exact beside it).
-    if (fresh || __ballot(top > 32768.0f)) {
-      float z = -INFINITY;
+      acc.l[n] += sum;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) z = fmaxf(z, s[i / 4][i % 4]);
-      z = fmaxf(z, __shfl_xor(z, 16));
-      z = fmaxf(z, __shfl_xor(z, 32));
-      const float m = fmaxf(acc.m, fabsf(z) < 0x1p24f ? z - 10.0f : z);
-      const float f = __builtin_amdgcn_exp2f(acc.m - m);
-      acc.m = m, acc.l *= f;
-      if (!fresh) {
+      for (int u = 0; u < 2; ++u) {
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < G_::kDt; ++i) acc.o[i] *= f;
+        for (int e = 0; e < 8; ++e) y[e] = p[8 * u + e];
+        split8(y, ph[n][u], pl[n][u]);
       }
-      fresh = false;
-      weights();
     }
-    acc.l += sum;
-    v8h ph[2], pl[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = p[8 * u + e];
-      split8(y, ph[u], pl[u]);
-    }
-    if (next) wait_vm<G_::kCopies>();  // this tile's V; the next one's K may be under way
+    fresh = false;
+    if (more) wait_vm<G_::kCopies>();  // this tile's V; the next one's K may be under way
     else wait_vm<0>();
     fence();
     // A lane gives the address of a key's 16 elements and gets an element's 16 keys: number 8 u + x is the key of weight
@@ -333,7 +337,7 @@ struct Walk {
 #pragma unroll
       for (int c = 0; c < 4; ++c) sc[n][c] = *reinterpret_cast<const v4h*>(vs_s + ((c * G_::kGroups + n) * 16 + 4 * qd) * 2);
     wait_lds();
-    if (next) issue_v(next, next_key);
+    if (more) issue_v(next);
     if (!whole) {  // a weight of 0 does not undo what lies in a place that nothing was written to
 #pragma unroll
       for (int n = 0; n < G_::kGroups; ++n)
@@ -352,133 +356,428 @@ struct Walk {
         const v4h a = sc[i / 2][2 * u], b = sc[i / 2][2 * u + 1];
         r[0] *= v2h{a[0], a[1]}, r[1] *= v2h{a[2], a[3]}, r[2] *= v2h{b[0], b[1]}, r[3] *= v2h{b[2], b[3]};
         const v8h x = join8(r);
-        acc.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[u], acc.o[i], 0, 0, 0);
-        acc.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[u], acc.o[i], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          acc.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[n][u], acc.o[n][i], 0, 0, 0);
+          acc.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[n][u], acc.o[n][i], 0, 0, 0);
+        }
       }
   }
 };
 
-// Tiles [ta, tb) of a block by the workgroup's NW waves; then put(row, element, its four values as weighted sums, l, m) by the
-// 16 threads that share a row, 64 / .. elements each.
-template <int D, int NW, class Put>
+template <int NR, int NW>
+struct Shared {  // beside the dynamic part
+  int ids[kIds];
+  v2f ml[NW][NR * kSet];
+};
+
+// Tiles [ta, tb) of a block by the workgroup's NW waves; then put(row, element, its next four as weighted sums, l, m) by the 16
+// threads that share a row, 64 elements at a time. Ends with every thread's own reads of LDS: a barrier comes before it is
+// written again.
+template <int D, int NR, int NW, class Put>
 __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int ta, int tb, const float* q, int64_t q_stride,
-                                          uint8_t* smem, int* ids, v2f (*ml)[kFew], Put put) {
-  using G_ = Geo<D>;
+                                          uint8_t* smem, Shared<NR, NW>& sh, Put put) {
+  using G_ = Geo<D, NR, NW>;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int end = min(b.keys, tb * kTile), seq = A.seq[b.t0];
-  Walk<D> walk(A, smem + w * G_::kWave);
-  walk.load_q(b, q, q_stride);
-  Acc<D> acc;
+  Walk<D, NR, NW> walk(A, smem, w);
+  walk.g = b.g;
+  const int li = walk.li, qd = walk.qd, lane = walk.lane;
+  // q: waves take (step, set) pairs in turn; a row's largest value is the waves' together.
+  constexpr int kPairs = G_::kSteps * NR, kMine = (kPairs + NW - 1) / NW;
+  float x[kMine][8];
 #pragma unroll
-  for (int i = 0; i < G_::kDt; ++i) acc.o[i] = v4f{};
-  acc.m = kNone, acc.l = 0.0f;
+  for (int i = 0; i < kMine; ++i) {
+    const int at = min(w + NW * i, kPairs - 1), s = at / NR, r = min(at % NR * kSet + li, b.rows() - 1);
+    const float* qr = q + b.token(r) * q_stride + (int64_t)b.head(r) * D + D / 4 * qd + 8 * s;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const v4f f = *reinterpret_cast<const v4a*>(qr + 4 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i][4 * c + e] = f[e];
+    }
+  }
+  // Rows beyond the block's are copies of the last one, whose results nobody reads.
+  walk.least = INT32_MAX;
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    walk.lim[n] = keys_of(A, b.token(min(n * kSet + li, b.rows() - 1)));
+    walk.least = min(walk.least, walk.lim[n]);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) walk.least = min(walk.least, __shfl_xor(walk.least, o));
+  walk.least = __builtin_amdgcn_readfirstlane(walk.least);
+  auto load_ids = [&](int t0, int t1) {
+    for (int i = tid; i < 4 * (t1 - t0); i += NW * 64) {
+      const int key = t0 * kTile + kChunk * i;
+      sh.ids[i] = key < end ? A.kv.page_of(seq, key) : -1;
+    }
+  };
+  __syncthreads();  // LDS is free
+  load_ids(ta, min(tb, ta + kIds / 4));
+  float* top_s = reinterpret_cast<float*>(smem + G_::kQ);  // [step][row]
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = w + NW * i;
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (at < kPairs && qd == 0) top_s[at / NR * G_::kR + at % NR * kSet + li] = top;
+  }
+  __syncthreads();
+  int ex[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < G_::kSteps; ++s) top = fmaxf(top, top_s[s * G_::kR + n * kSet + li]);
+    ex[n] = top > 0.0f && top < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(top), 100) : 0;
+    walk.rf[n] = __builtin_ldexpf(A.scale * kLog2e, -ex[n]);
+  }
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = w + NW * i;
+    if (at >= kPairs) continue;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = __builtin_ldexpf(x[i][place(e)], ex[at % NR]);
+    v8h hi, lo;
+    split8(y, hi, lo);
+    v8h* to = reinterpret_cast<v8h*>(smem) + at * 128 + lane;
+    to[0] = hi, to[64] = lo;
+  }
+  __syncthreads();
+  Acc<D, NR> acc;
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+#pragma unroll
+    for (int i = 0; i < G_::kDt; ++i) acc.o[n][i] = v4f{};
+    acc.m[n] = kNone, acc.l[n] = 0.0f;
+  }
   bool fresh = true;
   for (int t0 = ta; t0 < tb; t0 += kIds / 4) {  // pages of as many tiles as LDS holds
     const int t1 = min(tb, t0 + kIds / 4);
-    __syncthreads();
-    for (int i = tid; i < 4 * (t1 - t0); i += NW * 64) {
-      const int key = t0 * kTile + kChunk * i;
-      ids[i] = key < end ? A.kv.page_of(seq, key) : -1;
+    if (t0 > ta) {
+      __syncthreads();
+      load_ids(t0, t1);
+      __syncthreads();
     }
-    __syncthreads();
-    auto pages = [&](int t) { return ids + 4 * (t - t0); };
+    auto find = [&](int t) { return walk.find(sh.ids + 4 * (t - t0), t * kTile); };
     int t = t0 + w;
-    if (t < t1) walk.issue_k(pages(t), t * kTile), walk.issue_v(pages(t), t * kTile);
-    for (; t < t1; t += NW) {
+    if (t >= t1) continue;
+    Place at = find(t);
+    walk.issue_k(at), walk.issue_v(at);
+    for (;;) {
       const bool more = t + NW < t1;
-      walk.tile(acc, fresh, pages(t), t * kTile, end, more ? pages(t + NW) : nullptr, (t + NW) * kTile);
+      const int have = at.have;
+      if (more) at = find(t + NW);
+      walk.tile(acc, fresh, have, t * kTile, end, more, at);
+      if (!more) break;
+      t += NW;
     }
   }
   // The waves' parts of each row, brought to their largest shift and added.
-  float l = acc.l + __shfl_xor(acc.l, 16);
-  l += __shfl_xor(l, 32);
-  __syncthreads();
-  float* ob = reinterpret_cast<float*>(smem);
-  if (walk.qd == 0) ml[w][walk.li] = v2f{acc.m, l};
+  float* ob = reinterpret_cast<float*>(smem + G_::kQ);
 #pragma unroll
-  for (int i = 0; i < G_::kDt; ++i)
-    *reinterpret_cast<v4f*>(ob + (w * kFew + walk.li) * G_::kStride + 16 * i + 4 * walk.qd) = acc.o[i];
-  __syncthreads();
-  for (int r = tid >> 4; r < b.rows(); r += NW * 4) {
-    float f[NW], top = kNone, sum = 0.0f;
+  for (int n = 0; n < NR; ++n) {
+    float l = acc.l[n] + __shfl_xor(acc.l[n], 16);
+    l += __shfl_xor(l, 32);
+    if (qd == 0) sh.ml[w][n * kSet + li] = v2f{acc.m[n], l};
+  }
 #pragma unroll
-    for (int i = 0; i < NW; ++i) top = fmaxf(top, ml[i][r][0]);
+  for (int d0 = 0; d0 < D; d0 += 64) {
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      f[i] = __builtin_amdgcn_exp2f(ml[i][r][0] - top);
-      sum = fma_(f[i], ml[i][r][1], sum);
-    }
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int d0 = 0; d0 < D; d0 += 64) {
-      const int d = d0 + 4 * (tid & 15);
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<v4f*>(ob + (w * G_::kR + n * kSet + li) * G_::kStride + 16 * i + 4 * qd) = acc.o[n][d0 / 16 + i];
+    __syncthreads();
+    for (int r = tid >> 4; r < b.rows(); r += NW * 4) {
+      float f[NW], top = kNone, sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) top = fmaxf(top, sh.ml[i][r][0]);
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        f[i] = __builtin_amdgcn_exp2f(sh.ml[i][r][0] - top);
+        sum = fma_(f[i], sh.ml[i][r][1], sum);
+      }
       v4f a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < NW; ++i) a += f[i] * *reinterpret_cast<const v4f*>(ob + (i * kFew + r) * G_::kStride + d);
-      put(r, d, a, sum, top);
+      for (int i = 0; i < NW; ++i) a += f[i] * *reinterpret_cast<const v4f*>(ob + (i * G_::kR + r) * G_::kStride + 4 * (tid & 15));
+      put(r, d0 + 4 * (tid & 15), a, sum, top);
     }
   }
 }
 
-template <int D, int NW>
-struct FewLds {
-  static constexpr int kRing = NW * Geo<D>::kWave, kOut = NW * kFew * Geo<D>::kStride * 4;
-  static constexpr int kBytes = kRing > kOut ? kRing : kOut;
+// Four values of a row of the output, by the threads of a row together.
+struct Out {
+  float* out;
+  int64_t stride;
+  BlockQ8* xq;
+};
+template <int D>
+__device__ __forceinline__ void put_row(const Kv4Attn& A, const Out& O, int t, int head, int d, v4f a, float l) {
+  const float n = l == 0.0f ? 1.0f : l;  // no key: zeros
+  const float y[4] = {a[0] / n, a[1] / n, a[2] / n, a[3] / n};
+  *reinterpret_cast<v4a*>(O.out + t * O.stride + (int64_t)head * D + d) = v4a{y[0], y[1], y[2], y[3]};
+  if (O.xq) quantize_block_lanes_n<4>(y, (d & 31) / 4, O.xq + (((int64_t)t * A.H + head) * D + d) / 32);
+}
+
+// A workgroup per token and J; the first token of its sequence, or of tq tokens, leads a block and the others' workgroups leave.
+template <int D, int NR, int NW>
+__global__ __launch_bounds__(NW * 64) void k_kv4_whole(Kv4Attn A, const float* __restrict__ q, int64_t q_stride, Out O) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(16) Shared<NR, NW> sh;
+  const Shape S = shape_of(A.H, A.kv.KV, NR * kSet);
+  const int t = blockIdx.x / S.J;
+  int from = t;  // the first token of the run, or of tq of them counted from there
+  while (!starts(A, from)) --from;
+  if ((t - from) % S.tq) return;
+  Block b;
+  set_tokens(b, A, t, S.tq);
+  set_heads<NR * kSet>(b, S, blockIdx.x % S.J);
+  run_block<D, NR, NW>(A, b, 0, b.tiles(), q, q_stride, smem, sh,
+                       [&](int r, int d, v4f a, float l, float m) { put_row<D>(A, O, b.token(r), b.head(r), d, a, l); });
+}
+
+// ---- even shares of all tiles ----
+
+constexpr int kShare = 4;  // waves of a workgroup that takes a share
+
+// Per (token, j): the workgroups whose runs hold its block, first (where it begins) and last (-1: written whole), and the row
+// that the token's first head has in it.
+struct Record {
+  int first, last, row;
+};
+// Partial results of workgroup w: slot 2 w of a block that began before its run, 2 w + 1 of one that begins in it and ends after.
+struct Parts {
+  float* o;    // [slot][row][D]
+  v2f* ml;     // [slot][row] shift and sum
+  Record* rec; // [token][J]
 };
 
-// Four values of a row of the output, by the threads of a row together.
-template <int D>
-__device__ __forceinline__ void put_row(const Kv4Attn& A, float* out, int64_t out_stride, BlockQ8* xq, int t, int head, int d,
-                                        const float (&y)[4]) {
-  *reinterpret_cast<v4a*>(out + t * out_stride + (int64_t)head * D + d) = v4a{y[0], y[1], y[2], y[3]};
-  if (xq) quantize_block_lanes_n<4>(y, (d & 31) / 4, xq + (((int64_t)t * A.H + head) * D + d) / 32);
+// Exclusive running sum (and total) over 256 threads, or the largest before; part: 4 words of LDS.
+template <bool MAX, typename T>
+__device__ __forceinline__ T scan256(T v, T* part, T& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const T none = MAX ? (T)-1 : (T)0;
+  auto op = [](T a, T b) { return MAX ? (a > b ? a : b) : a + b; };
+  T x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const T y = __shfl_up(x, o);
+    if (lane >= o) x = op(x, y);
+  }
+  T before = __shfl_up(x, 1);
+  if (lane == 0) before = none;
+  __syncthreads();
+  if (lane == 63) part[w] = x;
+  __syncthreads();
+  total = none;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < w) before = op(before, part[i]);
+    total = op(total, part[i]);
+  }
+  return before;
 }
 
-// The tokens from t on that a block may have with it, tq at most.
-__device__ __forceinline__ Block block_at(const Kv4Attn& A, int t, int tq, int j) {
-  const int G = A.H / A.kv.KV, hs = (G + kFew - 1) / kFew, sub = j % hs;
-  Block b{t, 1, keys_of(A, t), j / hs, j / hs * G + kFew * sub, min(G - kFew * sub, kFew)};
-  const int s = A.seq[t];
-  while (b.m < tq && t + b.m < A.n && (t + b.m) % tq && A.seq[t + b.m] == s) b.keys = max(b.keys, keys_of(A, t + b.m)), ++b.m;
-  return b;
-}
-
-// A workgroup per token and KV head (per 16 of its query heads); the first token of its sequence, or of tq tokens, leads a
-// block and the others' workgroups leave.
-template <int D, int NW>
-__global__ __launch_bounds__(NW * 64) void k_kv4_whole(Kv4Attn A, const float* __restrict__ q, int64_t q_stride,
-                                                       float* __restrict__ out, int64_t out_stride, BlockQ8* __restrict__ xq) {
+template <int D, int NR>
+__global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4Attn A, const float* __restrict__ q, int64_t q_stride,
+                                                                            Out O, Parts P) {
+  constexpr int R = NR * kSet;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int ids[kIds];
-  __shared__ v2f ml[NW][kFew];
-  const int G = A.H / A.kv.KV, hs = (G + kFew - 1) / kFew, J = A.kv.KV * hs, tq = max(1, kFew / G);
-  const int t = blockIdx.x / J;
-  if (t % tq && A.seq[t - 1] == A.seq[t]) return;
-  const Block b = block_at(A, t, tq, blockIdx.x % J);
-  run_block<D, NW>(A, b, 0, (b.keys + kTile - 1) / kTile, q, q_stride, smem, ids, ml, [&](int r, int d, v4f a, float l, float m) {
-    const float n = l == 0.0f ? 1.0f : l;  // no key: zeros
-    const float y[4] = {a[0] / n, a[1] / n, a[2] / n, a[3] / n};
-    put_row<D>(A, out, out_stride, xq, b.token(r), b.head(r), d, y);
-  });
+  __shared__ __align__(16) Shared<NR, kShare> sh;
+  __shared__ int64_t part[4];
+  __shared__ int64_t start_off;
+  __shared__ int start_t;
+  const int tid = threadIdx.x, w = blockIdx.x;
+  const Shape S = shape_of(A.H, A.kv.KV, R);
+  // This thread's tokens, which follow each other, and the tiles of the blocks that they lead.
+  const int per = (A.n + 255) / 256, ta = min(A.n, tid * per), tb = min(A.n, ta + per);
+  int64_t last = -1, dummy;
+  for (int t = ta; t < tb; ++t)
+    if (starts(A, t)) last = t;
+  const int64_t run0 = scan256<true>(last, part, dummy);
+  auto leaders = [&](auto f) {
+    int from = (int)run0;
+    for (int t = ta; t < tb; ++t) {
+      if (starts(A, t)) from = t;
+      if ((t - from) % S.tq) continue;
+      Block b;
+      set_tokens(b, A, t, S.tq);
+      if (!f(t, b.tiles())) return;
+    }
+  };
+  int64_t mine = 0, total = 0;
+  leaders([&](int, int tiles) { return mine += tiles, true; });
+  const int64_t before = scan256<false>(mine, part, total) * S.J, share = (total * S.J + gridDim.x - 1) / gridDim.x;
+  const int64_t a = w * share, b = min(a + share, total * S.J);
+  if (a >= b) return;
+  // The block that holds tile a is one of exactly one thread's.
+  if (before <= a && a < before + mine * S.J) {
+    int64_t off = before;
+    leaders([&](int t, int tiles) {
+      if (a < off + (int64_t)tiles * S.J) {
+        start_t = t, start_off = off;
+        return false;
+      }
+      off += (int64_t)tiles * S.J;
+      return true;
+    });
+  }
+  __syncthreads();
+  int t = start_t;
+  int64_t off = start_off;  // of token t's blocks
+  Block blk;
+  set_tokens(blk, A, t, S.tq);
+  for (int64_t at = a; at < b;) {
+    const int tiles = blk.tiles();
+    if (at >= off + (int64_t)tiles * S.J) {  // the next tokens'
+      off += (int64_t)tiles * S.J;
+      t += blk.m;
+      set_tokens(blk, A, t, S.tq);
+      continue;
+    }
+    const int j = (int)((at - off) / tiles), k0 = (int)((at - off) % tiles), k1 = (int)min<int64_t>(tiles, k0 + (b - at));
+    set_heads<R>(blk, S, j);
+    const int64_t block_off = at - k0;
+    const int first = (int)(block_off / share), end = (int)((block_off + tiles - 1) / share);
+    if (k0 == 0)
+      for (int i = tid; i < blk.m; i += kShare * 64)
+        P.rec[(int64_t)(t + i) * S.J + j] = Record{first, first == end ? -1 : end, i * blk.per};
+    const int64_t slot = 2 * (int64_t)w + (k0 == 0);
+    run_block<D, NR, kShare>(A, blk, k0, k1, q, q_stride, smem, sh, [&](int r, int d, v4f v, float l, float m) {
+      if (first == end) {
+        put_row<D>(A, O, blk.token(r), blk.head(r), d, v, l);
+      } else {
+        *reinterpret_cast<v4f*>(P.o + (slot * R + r) * D + d) = v;
+        if (d == 0) P.ml[slot * R + r] = v2f{m, l};
+      }
+    });
+    at += k1 - k0;
+  }
+}
+
+// A wave per query row: the parts of rows that several workgroups had, added; zeros for rows without keys.
+template <int D, int R>
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4Attn A, Out O, Parts P) {
+  constexpr int E = D / 64, kAhead = 8;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)A.n * A.H) return;
+  const Shape S = shape_of(A.H, A.kv.KV, R);
+  const int t = (int)(row / A.H), head = (int)(row % A.H), in = head % S.G;
+  float v[E];
+#pragma unroll
+  for (int k = 0; k < E; ++k) v[k] = 0.0f;
+  if (keys_of(A, t) > 0) {
+    const Record rec = P.rec[(int64_t)t * S.J + head / S.G * S.hs + in / R];
+    if (rec.last < 0) return;
+    const int r = rec.row + in % R, parts = rec.last - rec.first + 1;
+    auto slot = [&](int i) { return (2 * ((int64_t)rec.first + i) + (i == 0)) * R + r; };
+    float top = kNone, sum = 0.0f;
+    for (int i = lane; i < parts; i += 64) top = fmaxf(top, P.ml[slot(i)][0]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+      const v2f ml = i0 + lane < parts ? P.ml[slot(i0 + lane)] : v2f{kNone, 0.0f};
+      const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+      sum = fma_(f, ml[1], sum);
+      const int m = min(64, parts - i0);
+      for (int i = 0; i < m; i += kAhead) {
+        float x[kAhead][E];
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e)
+          if (i + e < m)
+#pragma unroll
+            for (int k = 0; k < E; ++k) x[e][k] = P.o[slot(i0 + i + e) * D + E * lane + k];
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e)
+          if (i + e < m) {
+            const float fe = __shfl(f, i + e);
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[k] = fma_(fe, x[e][k], v[k]);
+          }
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    const float n = sum == 0.0f ? 1.0f : sum;
+#pragma unroll
+    for (int k = 0; k < E; ++k) v[k] = v[k] / n;
+  }
+  float* to = O.out + t * O.stride + (int64_t)head * D + E * lane;
+#pragma unroll
+  for (int k = 0; k < E; ++k) to[k] = v[k];
+  if (O.xq) quantize_block_lanes_n<E>(v, lane % (32 / E), O.xq + (row * D + E * lane) / 32);
+}
+
+// How a call is cut.
+struct Cut {
+  int sets;  // 16-row sets of a block
+  int wgs;   // workgroups that share all tiles; 0: one per block
+};
+constexpr int kWholeKeys = 512;
+
+Cut cut_of(int n, int H, int KV, int max_keys, int max_run) {
+  Cut c{std::min<int64_t>(std::max(max_run, 1), n) * (H / KV) > kSet ? 2 : 1, 0};
+  if (max_keys <= kWholeKeys) return c;
+  c.wgs = 256 * (c.sets == 1 ? 3 : 2);  // what the chip holds at once
+  return c;
+}
+
+template <int D>
+size_t parts_bytes(const Cut& c, int n, int H, int KV) {
+  const Shape S = shape_of(H, KV, c.sets * kSet);
+  const size_t rows = 2ull * c.wgs * c.sets * kSet;
+  return rows * (D * sizeof(float) + sizeof(v2f)) + (size_t)n * S.J * sizeof(Record);
 }
 
 }  // namespace
 
-size_t attention_kv4_workspace(int n, int H, int KV, int D, int max_keys, int max_run) { return 0; }
+// Never less for a larger call: the largest number of sets and workgroups there are, and records of the smaller blocks.
+size_t attention_kv4_workspace(int n, int H, int KV, int D, int max_keys, int max_run) {
+  if (max_keys <= kWholeKeys) return 0;
+  const Cut one{1, 256 * 3}, two{2, 256 * 2};
+  return std::max(D == 128 ? parts_bytes<128>(one, n, H, KV) : parts_bytes<64>(one, n, H, KV),
+                  D == 128 ? parts_bytes<128>(two, n, H, KV) : parts_bytes<64>(two, n, H, KV));
+}
 
-size_t attention_kv4_need(const Kv4Attn& A, int D) { return 0; }
+size_t attention_kv4_need(const Kv4Attn& A, int D) {
+  return attention_kv4_workspace(A.n, A.H, A.kv.KV, D, A.max_keys, A.max_run);
+}
 
 void attention_kv4(hipStream_t s, const Kv4Attn& A, int D, const float* q, int64_t q_stride, float* out, int64_t out_stride,
                    BlockQ8* xq, void* workspace) {
-  const int G = A.H / A.kv.KV, J = A.kv.KV * ((G + kFew - 1) / kFew);
-  auto go = [&]<int D_>() {
-    constexpr int NW = 4;
-    allow_lds<k_kv4_whole<D_, NW>>(FewLds<D_, NW>::kBytes);
-    hipLaunchKernelGGL((k_kv4_whole<D_, NW>), dim3((unsigned)((int64_t)A.n * J)), dim3(NW * 64), (FewLds<D_, NW>::kBytes), s, A, q,
-                       q_stride, out, out_stride, xq);
-    check_launch("attention_kv4");
+  const Cut c = cut_of(A.n, A.H, A.kv.KV, A.max_keys, A.max_run);
+  const Out O{out, out_stride, xq};
+  auto go = [&]<int D_, int NR>() {
+    const Shape S = shape_of(A.H, A.kv.KV, NR * kSet);
+    if (c.wgs == 0) {
+      constexpr int NW = 4;
+      constexpr auto lds = Geo<D_, NR, NW>::kLds;
+      allow_lds<k_kv4_whole<D_, NR, NW>>(lds);
+      hipLaunchKernelGGL((k_kv4_whole<D_, NR, NW>), dim3((unsigned)((int64_t)A.n * S.J)), dim3(NW * 64), lds, s, A, q, q_stride, O);
+      check_launch("attention_kv4 whole");
+      return;
+    }
+    constexpr int R = NR * kSet, lds = Geo<D_, NR, kShare>::kLds;
+    Parts P;
+    P.o = static_cast<float*>(workspace);
+    P.ml = reinterpret_cast<v2f*>(P.o + 2ull * c.wgs * R * D_);
+    P.rec = reinterpret_cast<Record*>(P.ml + 2ull * c.wgs * R);
+    allow_lds<k_kv4_share<D_, NR>>(lds);
+    hipLaunchKernelGGL((k_kv4_share<D_, NR>), dim3((unsigned)c.wgs), dim3(kShare * 64), lds, s, A, q, q_stride, O, P);
+    check_launch("attention_kv4 shares");
+    hipLaunchKernelGGL((k_kv4_join<D_, R>), dim3((unsigned)(((int64_t)A.n * A.H + 3) / 4)), dim3(256), 0, s, A, O, P);
+    check_launch("attention_kv4 join");
   };
-  if (D == 128) go.template operator()<128>();
-  else go.template operator()<64>();
+  if (D == 128) c.sets == 1 ? go.template operator()<128, 1>() : go.template operator()<128, 2>();
+  else c.sets == 1 ? go.template operator()<64, 1>() : go.template operator()<64, 2>();
 }
 
 }  // namespace mk
