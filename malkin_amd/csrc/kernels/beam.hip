@@ -49,34 +49,41 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
 // Larger logit first, then the lower token.
 __device__ __forceinline__ bool ahead(float a, int ia, float b, int ib) { return a > b || (a == b && ia < ib); }
 
-// One segment of kThreads * 4 Q logits of a row. PARTS: of which the maxima bound the k-th best: 64 (of 4 threads) or one per
-// thread; k <= PARTS. Only the k parts with the first maxima hold candidates, so at most CAP of them.
-template <int Q, int PARTS>
+// One segment of kThreads * 4 Q logits of a row. The maxima of PARTS parts of it bound the k-th best (k <= MOST <= PARTS): only
+// the k parts with the first maxima hold candidates, so at most CAP of them.
+template <int Q, int PARTS, int MOST>
 __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restrict__ stats, Cand* __restrict__ cands) {
-  constexpr int kSeg = kThreads * 4 * Q, kMost = PARTS == 64 ? 16 : 128, CAP = kMost * (kThreads / PARTS) * 4 * Q;
+  constexpr int kSeg = kThreads * 4 * Q, SHARE = kThreads / PARTS, CAP = MOST * SHARE * 4 * Q;
   __shared__ double table[kTable];
-  __shared__ float part_v[PARTS], wave_max[kThreads / 64], bound_v;
-  __shared__ int part_i[PARTS], bound_i, n_cand;
+  __shared__ __align__(16) float part_v[PARTS];
+  __shared__ __align__(16) int part_i[PARTS];
+  __shared__ float wave_max[kThreads / 64], bound_v;
+  __shared__ int bound_i, n_cand;
   __shared__ double wave_sum[kThreads / 64];
   __shared__ Cand list[CAP];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x / B.segs, seg = blockIdx.x % B.segs;
-  if (!finite(B.scores[row]) || (B.done && B.done[row])) return;  // nobody reads what would be written
-  load_table(table);
   const float* l = B.logits + row * B.stride;
   const int first = seg * kSeg;
+  const float start = B.scores[row];
+  const int over = B.done ? B.done[row] : 0;
+  if (!finite(start) || over) return;  // nobody reads what would be written
   float z[4 * Q];
+  if (first + kSeg <= B.n_vocab) {
 #pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    const int at = first + q * (4 * kThreads) + 4 * tid;
-    if (at + 4 <= B.n_vocab) {
-      const v4f f = *reinterpret_cast<const v4a*>(l + at);
+    for (int q = 0; q < Q; ++q) {
+      const v4f f = *reinterpret_cast<const v4a*>(l + first + q * (4 * kThreads) + 4 * tid);
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[4 * q + e] = f[e];
-    } else {
+    }
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[4 * q + e] = at + e < B.n_vocab ? l[at + e] : -INFINITY;
+    for (int e = 0; e < 4 * Q; ++e) {
+      const int at = first + e / 4 * (4 * kThreads) + 4 * tid + e % 4;
+      z[e] = l[min(at, B.n_vocab - 1)];
+      if (at >= B.n_vocab) z[e] = -INFINITY;
     }
   }
+  load_table(table);
   auto id_of = [&](int e) { return first + e / 4 * (4 * kThreads) + 4 * tid + e % 4; };
   float best = -INFINITY;
   int best_i = INT32_MAX;
@@ -89,29 +96,30 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restric
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   if (lane == 0) wave_max[w] = top;
-  if (PARTS == 64) {
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      const float v = __shfl_xor(best, o);
-      const int i = __shfl_xor(best_i, o);
-      if (ahead(v, i, best, best_i)) best = v, best_i = i;
-    }
-    if (tid % 4 == 0) part_v[tid / 4] = best, part_i[tid / 4] = best_i;
-  } else {
-    part_v[tid] = best, part_i[tid] = best_i;
+  for (int o = 1; o < SHARE; o <<= 1) {
+    const float v = __shfl_xor(best, o);
+    const int i = __shfl_xor(best_i, o);
+    if (ahead(v, i, best, best_i)) best = v, best_i = i;
   }
+  if (tid % SHARE == 0) part_v[tid / SHARE] = best, part_i[tid / SHARE] = best_i;
   if (tid == 0) bound_v = -INFINITY, bound_i = INT32_MAX, n_cand = 0;
   __syncthreads();
   top = wave_max[0];
 #pragma unroll
   for (int i = 1; i < kThreads / 64; ++i) top = fmaxf(top, wave_max[i]);
-  if (tid < PARTS) {
-    const float v = part_v[tid];
-    const int i = part_i[tid];
+  {  // every thread has its part's maximum, and counts a share of those ahead of it
     int before = 0;
-#pragma unroll 8
-    for (int j = 0; j < PARTS; ++j) before += ahead(part_v[j], part_i[j], v, i);
-    if (before == B.k - 1 && v > -INFINITY) bound_v = v, bound_i = i;
+#pragma unroll 4
+    for (int j = PARTS / SHARE * (tid % SHARE); j < PARTS / SHARE * (tid % SHARE + 1); j += 4) {
+      const v4f v = *reinterpret_cast<const v4f*>(part_v + j);
+      const int4 i = *reinterpret_cast<const int4*>(part_i + j);
+      before += ahead(v[0], i.x, best, best_i) + ahead(v[1], i.y, best, best_i) + ahead(v[2], i.z, best, best_i) +
+                ahead(v[3], i.w, best, best_i);
+    }
+#pragma unroll
+    for (int o = 1; o < SHARE; o <<= 1) before += __shfl_xor(before, o);
+    if (before == B.k - 1 && best > -INFINITY && tid % SHARE == 0) bound_v = best, bound_i = best_i;
   }
   double sum = 0.0;
   if (top > -INFINITY) {
@@ -165,9 +173,12 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
                                                               const Cand* __restrict__ cands, Stat* __restrict__ row_stat,
                                                               Cand* __restrict__ row_cand, float* __restrict__ out_scores,
                                                               int32_t* __restrict__ out_seq, int32_t* __restrict__ out_tokens) {
+  constexpr int kAhead = 4;
   __shared__ double lse[64];
-  __shared__ Entry heads[kMaxLists], list[kMergeCap], bound;
-  __shared__ int n_cand;
+  __shared__ Entry list[kMergeCap], bound;
+  __shared__ __align__(16) float heads[kMaxLists];
+  __shared__ int place[kMergeCap], n_cand;
+  __shared__ float least;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, group = blockIdx.x;
   const int beams = ROW ? 1 : B.beams, lists = beams * B.segs, k = B.k;
   const int64_t row0 = (int64_t)group * beams;
@@ -175,16 +186,29 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
   auto ended = [&](int b) { return B.done && B.done[row0 + b]; };
   if (ROW && (!alive(0) || ended(0))) return;
   const Entry none{-INFINITY, -INFINITY, -1, INT32_MAX};
+  // This thread's list, its first elements asked for at once (a list that nothing was written to is not looked at).
+  const int beam = tid / B.segs;
+  const bool in = tid < lists;
+  const Cand* from = cands + (row0 * B.segs + (in ? tid : 0)) * k;
+  Cand c[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) c[j] = from[min(j, k - 1)];
+  const bool mine = in && alive(beam), over = mine && ended(beam);
+  const double start = mine && !ROW ? (double)B.scores[row0 + beam] : 0.0;
   for (int b = w; b < beams; b += kMergeThreads / 64) {
     if (!alive(b) || ended(b)) continue;  // nothing was written for it
     const Stat* s = stats + (row0 + b) * B.segs;
-    float top = -INFINITY;
-    for (int i = lane; i < B.segs; i += 64) top = fmaxf(top, s[i].max);
+    Stat one = lane < B.segs ? s[lane] : Stat{0.0, -INFINITY, 0};  // the lane's segments together
+    for (int i = lane + 64; i < B.segs; i += 64) {
+      const Stat t = s[i];
+      const float m = fmaxf(one.max, t.max);
+      if (m == -INFINITY) continue;
+      one = Stat{one.sum * exp((double)one.max - (double)m) + t.sum * exp((double)t.max - (double)m), m, 0};
+    }
+    float top = one.max;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    double sum = 0.0;
-    for (int i = lane; i < B.segs; i += 64)
-      if (s[i].max > -INFINITY) sum += s[i].sum * exp((double)s[i].max - (double)top);
+    double sum = one.max > -INFINITY ? one.sum * exp((double)one.max - (double)top) : 0.0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (lane == 0) {
@@ -192,77 +216,98 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
       lse[b] = (double)top + log(sum);
     }
   }
-  // This thread's list.
-  const int beam = tid / B.segs;
-  const bool mine = tid < lists && alive(beam);
-  const bool over = mine && ended(beam);
-  const Cand* from = cands + (row0 * B.segs + tid) * k;
-  if (tid == 0) bound = none;
+  if (tid == 0) bound = none, n_cand = 0, least = -INFINITY;
+  for (int i = tid; i < kMergeCap; i += kMergeThreads) place[i] = 0;
   __syncthreads();
-  auto entry = [&](int j) {
+  auto entry = [&](int j, const Cand& v) {
     if (!mine || j >= k) return none;
-    const double start = ROW ? 0.0 : (double)B.scores[row0 + beam];
     if (over) return tid % B.segs == 0 && j == 0 ? Entry{start, 0.0f, B.eos, beam} : none;
-    const Cand c = from[j];
-    return c.id < 0 ? none : Entry{(double)c.z - lse[beam] + start, c.z, c.id, beam};
+    return v.id < 0 ? none : Entry{(double)v.z - lse[beam] + start, v.z, v.id, beam};
   };
-  // A bound by the lists' element p: (p + 1) r >= k, and at least r of them are as good as the r-th best.
-  auto bound_by = [&](int p) {
-    const int r = (k + p) / (p + 1);
-    if (tid < lists) heads[tid] = entry(p);
-    __syncthreads();
-    if (tid < lists && r <= lists) {
-      const Entry e = heads[tid];
-      if (e.beam != INT32_MAX) {
-        int before = 0;
+  auto put = [&](const Entry& e) {
+    const int at = atomicAdd(&n_cand, 1);
+    if (at < kMergeCap) list[at] = e;
+  };
+  // A bound by the lists' element p, rounded: (p + 1) r >= k, and at least r of them are as large as the r-th. Rounding keeps
+  // the order, so nothing among the k best is smaller, rounded, than that.
+  const int p0 = (k + lists - 1) / lists - 1, r0 = (k + p0) / (p0 + 1);
+  const Entry head = entry(p0, p0 == 0 ? c[0] : from[min(p0, k - 1)]);
+  const float mark = (float)head.score;
+  if (in) heads[tid] = mark;
+  for (int i = lists + tid; i < (lists + 3) / 4 * 4; i += kMergeThreads) heads[i] = -INFINITY;
+  __syncthreads();
+  if (in && mark > -INFINITY) {
+    int more = 0, same = 0;
 #pragma unroll 4
-        for (int j = 0; j < lists; ++j) before += ahead(heads[j], e);
+    for (int j = 0; j < lists; j += 4) {
+      const v4f v = *reinterpret_cast<const v4f*>(heads + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) more += v[e] > mark, same += v[e] == mark;
+    }
+    if (more < r0 && r0 <= more + same) least = mark;  // every such thread writes the same
+  }
+  __syncthreads();
+  {
+    bool go = true;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const Entry e = entry(j, c[j]);
+      go = go && e.beam != INT32_MAX && (float)e.score >= least;
+      if (go) put(e);
+    }
+    for (int j = kAhead; go && j < k; ++j) {
+      const Entry e = entry(j, from[j]);
+      go = e.beam != INT32_MAX && (float)e.score >= least;
+      if (go) put(e);
+    }
+  }
+  __syncthreads();
+  if (n_cand > kMergeCap) {
+    // Many that are equal: bounds in the order's own terms, by the elements p = 0, 1, 3, .. of the lists. They leave at most
+    // k (log2 k + 2): of the lists' elements p .. 2 p, fewer than k / (p + 1) + 1 each.
+    Entry* all = list;
+    for (int p = 0;; p = min(2 * p + 1, k - 1)) {
+      const int r = (k + p) / (p + 1);
+      __syncthreads();
+      const Entry e = entry(p, from[min(p, k - 1)]);
+      if (in) all[tid] = e;
+      __syncthreads();
+      if (in && r <= lists && e.beam != INT32_MAX) {
+        int before = 0;
+        for (int j = 0; j < lists; ++j) before += ahead(all[j], e);
         if (before == r - 1 && ahead(e, bound)) bound = e;  // one thread's
       }
+      if (p == k - 1) break;
     }
     if (tid == 0) n_cand = 0;
     __syncthreads();
-  };
-  auto collect = [&] {
-    const Entry least = bound;
+    const Entry last = bound;
     for (int j = 0; j < k; ++j) {
-      const Entry e = entry(j);
-      if (e.beam == INT32_MAX || ahead(least, e)) break;
-      const int at = atomicAdd(&n_cand, 1);
-      if (at < kMergeCap) list[at] = e;
+      const Entry e = entry(j, from[j]);
+      if (e.beam == INT32_MAX || ahead(last, e)) break;
+      put(e);
     }
     __syncthreads();
-  };
-  bound_by((k + lists - 1) / lists - 1);
-  collect();
-  if (n_cand > kMergeCap) {
-    // Bounds of p = 0, 1, 3, .. leave at most k (log2 k + 2) candidates: of the lists' elements p .. 2 p, fewer than
-    // k / (p + 1) + 1 each.
-    for (int p = 0;; p = min(2 * p + 1, k - 1)) {
-      bound_by(p);
-      if (p == k - 1) break;
-    }
-    collect();
   }
-  const int n = min(n_cand, kMergeCap);
-  for (int i = tid; i < n; i += kMergeThreads) {
+  // Each one's place: how many are ahead of it, counted by several threads where there are few.
+  const int n = min(n_cand, kMergeCap), parts = max(1, min(16, kMergeThreads / max(n, 1)));
+  for (int at = tid; at < n * parts; at += kMergeThreads) {
+    const int i = at / parts;
     const Entry e = list[i];
     int before = 0;
-    for (int j = 0; j < n; ++j) before += ahead(list[j], e);
-    if (before >= k) continue;
-    if (ROW) {
-      row_cand[row0 * k + before] = Cand{e.z, e.id};
-    } else {
-      const int64_t at = (int64_t)group * k + before;
-      out_scores[at] = (float)e.score, out_seq[at] = (int32_t)(row0 + e.beam), out_tokens[at] = e.id;
-    }
+    for (int j = at % parts; j < n; j += parts) before += ahead(list[j], e);
+    if (before) atomicAdd(&place[i], before);
   }
-  for (int i = n + tid; i < k; i += kMergeThreads) {
+  __syncthreads();
+  for (int i = tid; i < max(n, k); i += kMergeThreads) {
+    const Entry e = i < n ? list[i] : none;
+    const int to = i < n ? place[i] : i;
+    if (to >= k) continue;
     if (ROW) {
-      row_cand[row0 * k + i] = Cand{-INFINITY, -1};
+      row_cand[row0 * k + to] = Cand{e.z, e.id};
     } else {
-      const int64_t at = (int64_t)group * k + i;
-      out_scores[at] = -INFINITY, out_seq[at] = out_tokens[at] = -1;
+      const int64_t at = (int64_t)group * k + to;
+      out_scores[at] = (float)e.score, out_seq[at] = i < n ? (int32_t)(row0 + e.beam) : -1, out_tokens[at] = e.id;
     }
   }
 }
@@ -291,13 +336,14 @@ void beam_select(hipStream_t s, const float* logits, int64_t stride, int n_group
   Stat* row_stat = stats + (int64_t)rows * segs;
   Cand* cands = reinterpret_cast<Cand*>(row_stat + rows);
   Cand* row_cand = cands + (int64_t)rows * segs * k;
-  auto go = [&]<int Q, int PARTS>() {
-    hipLaunchKernelGGL((k_beam_rows<Q, PARTS>), dim3((unsigned)(rows * segs)), dim3(kThreads), 0, s, B, stats, cands);
+  auto go = [&]<int Q, int PARTS, int MOST>() {
+    hipLaunchKernelGGL((k_beam_rows<Q, PARTS, MOST>), dim3((unsigned)(rows * segs)), dim3(kThreads), 0, s, B, stats, cands);
     check_launch("beam_select rows");
   };
   const bool large = seg_of(rows, n_vocab) == kLargeSeg;
-  if (k <= 16) large ? go.template operator()<8, 64>() : go.template operator()<4, 64>();
-  else large ? go.template operator()<8, 256>() : go.template operator()<4, 256>();
+  if (k <= 16) large ? go.template operator()<8, 64, 16>() : go.template operator()<4, 64, 16>();
+  else if (k <= 48) large ? go.template operator()<8, 128, 48>() : go.template operator()<4, 128, 48>();
+  else large ? go.template operator()<8, 256, 128>() : go.template operator()<4, 256, 128>();
   if ((int64_t)beams * segs > kMaxLists) {  // a list per row first
     hipLaunchKernelGGL(k_beam_merge<true>, dim3((unsigned)rows), dim3(kMergeThreads), 0, s, B, stats, cands, row_stat,
                        row_cand, nullptr, nullptr, nullptr);
