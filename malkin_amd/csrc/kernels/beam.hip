@@ -49,16 +49,23 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
 // Larger logit first, then the lower token.
 __device__ __forceinline__ bool ahead(float a, int ia, float b, int ib) { return a > b || (a == b && ia < ib); }
 
-// One segment of kThreads * 4 Q logits of a row. The maxima of PARTS parts of it bound the k-th best (k <= MOST <= PARTS): only
-// the k parts with the first maxima hold candidates, so at most CAP of them.
+// Order-preserving bits of a float that is not NaN (0 of either sign the same).
+__device__ __forceinline__ uint32_t order_key(float f) {
+  const uint32_t u = __float_as_uint(f + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// One segment of kThreads * 4 Q logits of a row. The k-th largest of the maxima of PARTS parts of it is a bound (k <= MOST <=
+// PARTS): at most (k - 1) parts hold anything larger. Of logits that are equal to it there can be any number; where the list
+// does not hold them, those of the first whole rounds of 4 kThreads logits are taken that have enough.
 template <int Q, int PARTS, int MOST>
 __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restrict__ stats, Cand* __restrict__ cands) {
-  constexpr int kSeg = kThreads * 4 * Q, SHARE = kThreads / PARTS, CAP = MOST * SHARE * 4 * Q;
+  constexpr int kRound = 4 * kThreads, kSeg = Q * kRound, SHARE = kThreads / PARTS, CAP = (MOST - 1) * SHARE * 4 * Q + MOST + kRound;
   __shared__ double table[kTable];
   __shared__ __align__(16) float part_v[PARTS];
-  __shared__ __align__(16) int part_i[PARTS];
-  __shared__ float wave_max[kThreads / 64], bound_v;
-  __shared__ int bound_i, n_cand;
+  __shared__ float wave_max[kThreads / 64];
+  __shared__ uint32_t bound;
+  __shared__ int n_cand;
   __shared__ double wave_sum[kThreads / 64];
   __shared__ Cand list[CAP];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x / B.segs, seg = blockIdx.x % B.segs;
@@ -71,83 +78,105 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restric
   if (first + kSeg <= B.n_vocab) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const v4f f = *reinterpret_cast<const v4a*>(l + first + q * (4 * kThreads) + 4 * tid);
+      const v4f f = *reinterpret_cast<const v4a*>(l + first + q * kRound + 4 * tid);
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[4 * q + e] = f[e];
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 4 * Q; ++e) {
-      const int at = first + e / 4 * (4 * kThreads) + 4 * tid + e % 4;
+      const int at = first + e / 4 * kRound + 4 * tid + e % 4;
       z[e] = l[min(at, B.n_vocab - 1)];
       if (at >= B.n_vocab) z[e] = -INFINITY;
     }
   }
   load_table(table);
-  auto id_of = [&](int e) { return first + e / 4 * (4 * kThreads) + 4 * tid + e % 4; };
+  auto id_of = [&](int e) { return first + e / 4 * kRound + 4 * tid + e % 4; };
   float best = -INFINITY;
-  int best_i = INT32_MAX;
 #pragma unroll
   for (int e = 0; e < 4 * Q; ++e) {
     z[e] = clean(z[e]);
-    if (z[e] > best) best = z[e], best_i = id_of(e);
+    best = fmaxf(best, z[e]);
   }
-  float top = best;
+  float part = best;  // of SHARE neighbouring threads
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  for (int o = 1; o < SHARE; o <<= 1) part = fmaxf(part, __shfl_xor(part, o));
+  float top = part;
+#pragma unroll
+  for (int o = 32; o >= SHARE; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   if (lane == 0) wave_max[w] = top;
-#pragma unroll
-  for (int o = 1; o < SHARE; o <<= 1) {
-    const float v = __shfl_xor(best, o);
-    const int i = __shfl_xor(best_i, o);
-    if (ahead(v, i, best, best_i)) best = v, best_i = i;
-  }
-  if (tid % SHARE == 0) part_v[tid / SHARE] = best, part_i[tid / SHARE] = best_i;
-  if (tid == 0) bound_v = -INFINITY, bound_i = INT32_MAX, n_cand = 0;
+  if (tid % SHARE == 0) part_v[tid / SHARE] = part;
+  if (tid == 0) bound = 0xFFFFFFFFu, n_cand = 0;
   __syncthreads();
   top = wave_max[0];
 #pragma unroll
   for (int i = 1; i < kThreads / 64; ++i) top = fmaxf(top, wave_max[i]);
-  {  // every thread has its part's maximum, and counts a share of those ahead of it
-    int before = 0;
+  {  // every thread counts a share of the parts' maxima that are larger than its own part's
+    int more = 0;
 #pragma unroll 4
     for (int j = PARTS / SHARE * (tid % SHARE); j < PARTS / SHARE * (tid % SHARE + 1); j += 4) {
       const v4f v = *reinterpret_cast<const v4f*>(part_v + j);
-      const int4 i = *reinterpret_cast<const int4*>(part_i + j);
-      before += ahead(v[0], i.x, best, best_i) + ahead(v[1], i.y, best, best_i) + ahead(v[2], i.z, best, best_i) +
-                ahead(v[3], i.w, best, best_i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) more += v[e] > part;
     }
 #pragma unroll
-    for (int o = 1; o < SHARE; o <<= 1) before += __shfl_xor(before, o);
-    if (before == B.k - 1 && best > -INFINITY && tid % SHARE == 0) bound_v = best, bound_i = best_i;
+    for (int o = 1; o < SHARE; o <<= 1) more += __shfl_xor(more, o);
+    if (more < B.k && tid % SHARE == 0) atomicMin(&bound, order_key(part));
   }
   double sum = 0.0;
   if (top > -INFINITY) {
+    constexpr double c = kTable * 1.4426950408889634074, least = -63000.0 / c;  // below 2^-984 there is nothing
 #pragma unroll
     for (int e = 0; e < 4 * Q; ++e) {
-      const double d = ((double)z[e] - (double)top) * (kTable * 1.4426950408889634074);
-      const bool in = d > -63000.0;  // below 2^-984 there is nothing
-      const Power p = pow2(in ? d : 0.0, table);
-      sum += in ? p.factor * p.rest : 0.0;
+      const Power p = pow2_of(fmax((double)z[e] - (double)top, least), c, table);
+      sum = __builtin_fma(p.factor, p.rest, sum);
     }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane == 0) wave_sum[w] = sum;
   __syncthreads();
-  const float bv = bound_v;
-  const int bi = bound_i;
+  const uint32_t key = bound;  // fewer than k parts: of -inf
+  const float limit = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+  auto put = [&](int e) {
+    const int at = atomicAdd(&n_cand, 1);
+    if (at < CAP) list[at] = Cand{z[e], id_of(e)};
+  };
+  if (best >= limit && best > -INFINITY)
 #pragma unroll
-  for (int e = 0; e < 4 * Q; ++e)
-    if (z[e] > -INFINITY && !ahead(bv, bi, z[e], id_of(e))) list[atomicAdd(&n_cand, 1)] = Cand{z[e], id_of(e)};
+    for (int e = 0; e < 4 * Q; ++e)
+      if (z[e] >= limit && z[e] > -INFINITY) put(e);
   __syncthreads();
+  if (n_cand > CAP) {
+    __syncthreads();
+    if (tid == 0) n_cand = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4 * Q; ++e)
+      if (z[e] > limit) put(e);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      __syncthreads();
+      const bool want = n_cand < B.k;
+      __syncthreads();
+      if (want)
+#pragma unroll
+        for (int e = 4 * q; e < 4 * q + 4; ++e)
+          if (z[e] == limit) put(e);
+    }
+    __syncthreads();
+  }
   const int n = n_cand;
   Cand* out = cands + ((int64_t)row * B.segs + seg) * B.k;
-  for (int i = tid; i < n; i += kThreads) {
+  // Each one's place: how many are ahead of it, counted by four threads.
+  for (int i = tid >> 2; i < n; i += kThreads / 4) {
     const Cand c = list[i];
     int before = 0;
-    for (int j = 0; j < n; ++j) before += ahead(list[j].z, list[j].id, c.z, c.id);
-    if (before < B.k) out[before] = c;
+#pragma unroll 4
+    for (int j = tid & 3; j < n; j += 4) before += ahead(list[j].z, list[j].id, c.z, c.id);
+    before += __shfl_xor(before, 1);
+    before += __shfl_xor(before, 2);
+    if (before < B.k && (tid & 3) == 0) out[before] = c;
   }
   for (int i = n + tid; i < B.k; i += kThreads) out[i] = Cand{-INFINITY, -1};
   if (tid == 0) {
@@ -195,23 +224,25 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
   for (int j = 0; j < kAhead; ++j) c[j] = from[min(j, k - 1)];
   const bool mine = in && alive(beam), over = mine && ended(beam);
   const double start = mine && !ROW ? (double)B.scores[row0 + beam] : 0.0;
-  for (int b = w; b < beams; b += kMergeThreads / 64) {
-    if (!alive(b) || ended(b)) continue;  // nothing was written for it
-    const Stat* s = stats + (row0 + b) * B.segs;
-    Stat one = lane < B.segs ? s[lane] : Stat{0.0, -INFINITY, 0};  // the lane's segments together
-    for (int i = lane + 64; i < B.segs; i += 64) {
+  // Sums of the rows, a group of lanes for each: as many lanes as it has segments, at most a wave.
+  int width = 1;
+  while (width < B.segs && width < 64) width <<= 1;
+  for (int b0 = w * (64 / width); b0 < beams; b0 += kMergeThreads / width) {
+    const int b = b0 + lane / width, at = lane % width;
+    const bool live = b < beams && alive(b) && !ended(b);  // nothing was written for the others
+    const Stat* s = stats + (row0 + (live ? b : 0)) * B.segs;
+    Stat one{0.0, -INFINITY, 0};
+    for (int i = at; i < B.segs && live; i += width) {
       const Stat t = s[i];
       const float m = fmaxf(one.max, t.max);
       if (m == -INFINITY) continue;
-      one = Stat{one.sum * exp((double)one.max - (double)m) + t.sum * exp((double)t.max - (double)m), m, 0};
+      one = one.max == -INFINITY ? t : Stat{one.sum * exp((double)one.max - (double)m) + t.sum * exp((double)t.max - (double)m), m, 0};
     }
     float top = one.max;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    for (int o = width / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     double sum = one.max > -INFINITY ? one.sum * exp((double)one.max - (double)top) : 0.0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if (lane == 0) {
+    for (int o = width / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (live && at == 0) {
       if (ROW) row_stat[row0] = Stat{sum, top, 0};
       lse[b] = (double)top + log(sum);
     }
@@ -314,11 +345,10 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
 
 constexpr int kSmallSeg = kThreads * 4 * 4, kLargeSeg = kThreads * 4 * 8;
 
-// Longer segments where there are many rows.
-int seg_of(int rows, int n_vocab) {
-  return (int64_t)rows * n_vocab > (int64_t)kLargeSeg * 1024 ? kLargeSeg : kSmallSeg;
+// Longer segments where there are many rows and few candidates of each.
+int seg_of(int rows, int n_vocab, int k) {
+  return k <= 16 && (int64_t)rows * n_vocab > (int64_t)kLargeSeg * 1024 ? kLargeSeg : kSmallSeg;
 }
-int segs_of(int rows, int n_vocab) { return (n_vocab + seg_of(rows, n_vocab) - 1) / seg_of(rows, n_vocab); }
 
 }  // namespace
 
@@ -330,7 +360,7 @@ size_t beam_workspace(int n_group, int beams, int n_vocab, int k) {
 void beam_select(hipStream_t s, const float* logits, int64_t stride, int n_group, int beams, int n_vocab, const float* scores,
                  const int32_t* done, int eos, int k, float* out_scores, int32_t* out_seq, int32_t* out_tokens,
                  void* workspace) {
-  const int rows = n_group * beams, segs = segs_of(rows, n_vocab);
+  const int rows = n_group * beams, seg = seg_of(rows, n_vocab, k), segs = (n_vocab + seg - 1) / seg;
   Beams B{logits, stride, scores, done, n_vocab, segs, k, beams, eos};
   Stat* stats = static_cast<Stat*>(workspace);
   Stat* row_stat = stats + (int64_t)rows * segs;
@@ -340,10 +370,10 @@ void beam_select(hipStream_t s, const float* logits, int64_t stride, int n_group
     hipLaunchKernelGGL((k_beam_rows<Q, PARTS, MOST>), dim3((unsigned)(rows * segs)), dim3(kThreads), 0, s, B, stats, cands);
     check_launch("beam_select rows");
   };
-  const bool large = seg_of(rows, n_vocab) == kLargeSeg;
+  const bool large = seg == kLargeSeg;
   if (k <= 16) large ? go.template operator()<8, 64, 16>() : go.template operator()<4, 64, 16>();
-  else if (k <= 48) large ? go.template operator()<8, 128, 48>() : go.template operator()<4, 128, 48>();
-  else large ? go.template operator()<8, 256, 128>() : go.template operator()<4, 256, 128>();
+  else if (k <= 64) go.template operator()<4, 128, 64>();
+  else go.template operator()<4, 256, 128>();
   if ((int64_t)beams * segs > kMaxLists) {  // a list per row first
     hipLaunchKernelGGL(k_beam_merge<true>, dim3((unsigned)rows), dim3(kMergeThreads), 0, s, B, stats, cands, row_stat,
                        row_cand, nullptr, nullptr, nullptr);

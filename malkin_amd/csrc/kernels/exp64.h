@@ -61,6 +61,18 @@ __device__ __forceinline__ Power pow2(double d, const double* table) {
   p = fma_s(p, g, k1);
   return Power{__builtin_bit_cast(double, t), __builtin_fma(p, g, 1.0)};
 }
+// 2^(x c / 64) of it, x c as above, in one rounding less.
+__device__ __forceinline__ Power pow2_of(double x, double c, const double* table) {
+  constexpr double kRound = 0x1.8p52, k1 = 6.931471805599453094e-1 / 64;
+  const double r = __builtin_fma(x, c, kRound), g = __builtin_fma(x, c, -(r - kRound));
+  const uint32_t word = (uint32_t)__builtin_bit_cast(uint64_t, r);
+  v2u t = __builtin_bit_cast(v2u, table[word & (kTable - 1)]);
+  t[1] += word << 14;
+  double p = fma_s(g, k1 * k1 * k1 * k1 / 24, k1 * k1 * k1 / 6);
+  p = fma_s(p, g, k1 * k1 / 2);
+  p = fma_s(p, g, k1);
+  return Power{__builtin_bit_cast(double, t), __builtin_fma(p, g, 1.0)};
+}
 // The table to LDS, where lanes read entries of their own; a barrier follows before its first use.
 __device__ __forceinline__ void load_table(double* table) {
   if (threadIdx.x < kTable) table[threadIdx.x] = __builtin_bit_cast(double, kPowers[threadIdx.x]);
