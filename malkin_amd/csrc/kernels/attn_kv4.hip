@@ -83,28 +83,45 @@ __device__ __forceinline__ void wait_lds() {
   fence();
 }
 
-// x as hi + lo.
+// x as hi + lo, two at a time: the difference is taken from the halves as they lie.
+__device__ __forceinline__ void split2(float a, float b, v2h& hi, v2h& lo) {
+  hi = __builtin_convertvector((v2f{a, b}), v2h);
+  uint32_t r;
+  asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\t"
+      "v_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+      : "=&v"(r)
+      : "v"(__builtin_bit_cast(uint32_t, hi)), "v"(a), "v"(b));
+  lo = __builtin_bit_cast(v2h, r);
+}
 __device__ __forceinline__ void split8(const float (&x)[8], v8h& hi, v8h& lo) {
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const v2f f = {x[i], x[i + 1]};
-    const v2h h = __builtin_convertvector(f, v2h);
-    const v2f g = {x[i] - (float)h[0], x[i + 1] - (float)h[1]};
-    const v2h l = __builtin_convertvector(g, v2h);
+    v2h h, l;
+    split2(x[i], x[i + 1], h, l);
     hi[i] = h[0], hi[i + 1] = h[1], lo[i] = l[0], lo[i + 1] = l[1];
   }
 }
 
 // Eight numbers of a word as n - 8, exactly, in the order 0, 4, 1, 5, 2, 6, 3, 7: a number under the exponent of 1024 reads
-// 1024 + n in the lowest four bits of the fraction, under that of 64 reads 64 + n four bits further up.
-__device__ __forceinline__ void less8(uint32_t w, v2h (&r)[4]) {
-  const v2h a = {(_Float16)1032.0f, (_Float16)1032.0f}, b = {(_Float16)72.0f, (_Float16)72.0f};
-  r[0] = __builtin_bit_cast(v2h, (w & 0x000F000Fu) | 0x64006400u) - a;
-  r[1] = __builtin_bit_cast(v2h, (w & 0x00F000F0u) | 0x54005400u) - b;
-  w >>= 8;
-  r[2] = __builtin_bit_cast(v2h, (w & 0x000F000Fu) | 0x64006400u) - a;
-  r[3] = __builtin_bit_cast(v2h, (w & 0x00F000F0u) | 0x54005400u) - b;
-}
+// 1024 + n in the lowest four bits of the fraction, under that of 64 reads 64 + n four bits further up. Masks and exponents are
+// kept in registers, one scalar and one vector, which an and-or takes together (as literals each would be an instruction).
+struct Unpack {
+  uint32_t mask_a, mask_b, exp_a, exp_b;
+  __device__ __forceinline__ Unpack() {
+    asm("s_mov_b32 %0, 0x000F000F" : "=s"(mask_a));
+    asm("s_mov_b32 %0, 0x00F000F0" : "=s"(mask_b));
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(exp_a));
+    asm("v_mov_b32 %0, 0x54005400" : "=v"(exp_b));
+  }
+  __device__ __forceinline__ void less8(uint32_t w, v2h (&r)[4]) const {
+    const v2h a = {(_Float16)1032.0f, (_Float16)1032.0f}, b = {(_Float16)72.0f, (_Float16)72.0f};
+    r[0] = __builtin_bit_cast(v2h, (w & mask_a) | exp_a) - a;
+    r[1] = __builtin_bit_cast(v2h, (w & mask_b) | exp_b) - b;
+    w >>= 8;
+    r[2] = __builtin_bit_cast(v2h, (w & mask_a) | exp_a) - a;
+    r[3] = __builtin_bit_cast(v2h, (w & mask_b) | exp_b) - b;
+  }
+};
 __device__ __forceinline__ v8h join8(const v2h (&r)[4]) {
   return v8h{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
 }
@@ -135,27 +152,34 @@ struct Acc {
   float m[NR], l[NR];  // weights are 2^(score - m), l this lane's sum of them
 };
 
-// Where a tile's chunks lie: their first rows in the pool (chunks without a page: page 0's) and in the scales of V.
+// Where a tile's four chunks lie: numbers of 16 rows among all rows of the pool (those without a page: 0).
 struct Place {
-  int64_t row[4], vs[4];
+  uint32_t at[4];
   int have;  // chunks that have a page
 };
+constexpr uint32_t kNoChunk = 0xFFFFFFFFu;
 
 // One wave's copies and products. Everything here is the wave's own: no barrier.
 template <int D, int NR, int NW>
 struct Walk {
   using G_ = Geo<D, NR, NW>;
   const Kv4Attn& A;
-  int g, lane, li, qd;
+  int lane, li, qd;
   const uint8_t* q_s;
   uint8_t *ks_s, *k_s, *v_s, *vs_s;
-  uint32_t k_off, v_off;  // this lane's part of a copy
+  uint32_t k_off, v_off, vs_off;  // this lane's part of a copy
+  Unpack un;
   float rf[NR];           // score, in bits, of one unit of a product
+  // Scores past 2^16 bits (a bit of `wide` per set): the shift's own rounding would count beside them. They are rounded to fp32
+  // first (by rg; rf is 1 then).
+  float rg[NR];
+  int wide;
   int lim[NR], least;     // keys that this lane's rows see, and that every row of the block sees
 
   __device__ __forceinline__ Walk(const Kv4Attn& a, uint8_t* smem, int w) : A(a) {
-    lane = threadIdx.x & 63, li = lane & 15, qd = lane >> 4;
+    lane = threadIdx.x & 63, li = lane & 15, qd = lane >> 4, wide = 0;
     q_s = smem;
+    vs_off = (((lane >> 3) & (G_::kGroups - 1)) << A.kv.shift) + 2 * (lane & 7);
     k_s = smem + G_::kQ + w * G_::kWave, v_s = k_s + G_::kBytes, ks_s = v_s + G_::kBytes, vs_s = ks_s + G_::kScales;
     if constexpr (D == 128) {
       k_off = li * 64 + 16 * qd;
@@ -166,56 +190,59 @@ struct Walk {
     }
   }
 
-  // ids: the pages of the tile's four chunks; key: its first key.
-  __device__ __forceinline__ Place find(const int* ids, int key) const {
-    const int4 id = *reinterpret_cast<const int4*>(ids);
-    const int p[4] = {__builtin_amdgcn_readfirstlane(id.x), __builtin_amdgcn_readfirstlane(id.y),
-                      __builtin_amdgcn_readfirstlane(id.z), __builtin_amdgcn_readfirstlane(id.w)};
-    Place at;
-    at.have = 0;
+  __device__ __forceinline__ Place find(const uint32_t* ids) const {
+    const uint4 id = *reinterpret_cast<const uint4*>(ids);
+    Place p;
+    p.at[0] = __builtin_amdgcn_readfirstlane(id.x), p.at[1] = __builtin_amdgcn_readfirstlane(id.y);
+    p.at[2] = __builtin_amdgcn_readfirstlane(id.z), p.at[3] = __builtin_amdgcn_readfirstlane(id.w);
+    p.have = 0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int64_t first = A.kv.first_row(max(p[c], 0), g);
-      const int r = (key + kChunk * c) & ((1 << A.kv.shift) - 1);
-      at.row[c] = first + r, at.vs[c] = first * G_::kGroups + r;
-      at.have |= (p[c] >= 0) << c;
+      const bool in = p.at[c] != kNoChunk;
+      p.have |= in << c, p.at[c] = in ? p.at[c] : 0u;
     }
-    return at;
+    return p;
   }
-  __device__ __forceinline__ void issue_k(const Place& at) const {
+  // This lane's of two or of four chunks, for copies whose lanes have them side by side.
+  __device__ __forceinline__ uint32_t of2(const Place& p, int c) const { return lane < 32 ? p.at[c] : p.at[c + 1]; }
+  __device__ __forceinline__ uint32_t of4(const Place& p) const {
+    const uint32_t a = lane & 16 ? p.at[1] : p.at[0], b = lane & 16 ? p.at[3] : p.at[2];
+    return lane < 32 ? a : b;
+  }
+  __device__ __forceinline__ void issue_k(const Place& p) const {
+    const uint8_t* ks = reinterpret_cast<const uint8_t*>(A.kv.ks);
     if constexpr (D == 128) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) lds_copy16(A.kv.k + at.row[c] * 64, k_off, k_s + 1024 * c);
+      for (int c = 0; c < 4; ++c) lds_copy16(A.kv.k + (uint64_t)p.at[c] * 1024, k_off, k_s + 1024 * c);
 #pragma unroll
-      for (int c = 0; c < 4; c += 2)
-        lds_copy4(reinterpret_cast<const uint8_t*>(A.kv.ks) + (lane < 32 ? at.row[c] : at.row[c + 1]) * 8 + 4 * (lane & 31),
-                  ks_s + 128 * c);
+      for (int c = 0; c < 4; c += 2) lds_copy4(ks + (uint64_t)of2(p, c) * 128 + 4 * (lane & 31), ks_s + 128 * c);
     } else {
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) lds_copy16(A.kv.k + (lane < 32 ? at.row[c] : at.row[c + 1]) * 32 + k_off, k_s + 512 * c);
-      const int64_t a = lane & 16 ? at.row[1] : at.row[0], b = lane & 16 ? at.row[3] : at.row[2];
-      lds_copy4(reinterpret_cast<const uint8_t*>(A.kv.ks) + (lane < 32 ? a : b) * 4 + 4 * li, ks_s);
+      for (int c = 0; c < 4; c += 2) lds_copy16(A.kv.k + (uint64_t)of2(p, c) * 512 + k_off, k_s + 512 * c);
+      lds_copy4(ks + (uint64_t)of4(p) * 64 + 4 * li, ks_s);
     }
   }
-  // The scales of V in LDS: [chunk][group][key].
-  __device__ __forceinline__ void issue_v(const Place& at) const {
-    const int in = (((lane >> 3) & (G_::kGroups - 1)) << A.kv.shift) + 2 * (lane & 7);
+  // The scales of V in LDS: [chunk][group][key]. A page's are its groups' one after the other.
+  __device__ __forceinline__ const uint16_t* scales_at(uint32_t chunk) const {
+    const uint32_t in = chunk & ((1u << (A.kv.shift - 4)) - 1);
+    return A.kv.vs + (uint64_t)(chunk - in) * (kChunk * G_::kGroups) + kChunk * in + vs_off;
+  }
+  __device__ __forceinline__ void issue_v(const Place& p) const {
     if constexpr (D == 128) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) lds_copy16(A.kv.v + at.row[c] * 64, v_off, v_s + 1024 * c);
+      for (int c = 0; c < 4; ++c) lds_copy16(A.kv.v + (uint64_t)p.at[c] * 1024, v_off, v_s + 1024 * c);
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) lds_copy4(A.kv.vs + (lane < 32 ? at.vs[c] : at.vs[c + 1]) + in, vs_s + 128 * c);
+      for (int c = 0; c < 4; c += 2) lds_copy4(scales_at(of2(p, c)), vs_s + 128 * c);
     } else {
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) lds_copy16(A.kv.v + (lane < 32 ? at.row[c] : at.row[c + 1]) * 32 + v_off, v_s + 512 * c);
-      const int64_t a = lane & 16 ? at.vs[1] : at.vs[0], b = lane & 16 ? at.vs[3] : at.vs[2];
-      lds_copy4(A.kv.vs + (lane < 32 ? a : b) + in, vs_s);
+      for (int c = 0; c < 4; c += 2) lds_copy16(A.kv.v + (uint64_t)of2(p, c) * 512 + v_off, v_s + 512 * c);
+      lds_copy4(scales_at(of4(p)), vs_s);
     }
   }
 
   // One tile: keys key .. key + 63, of which those below `end` count (end <= the block's keys) and whose chunk has a page.
   // more: `next` is the wave's next tile, whose copies are asked for.
-  __device__ __forceinline__ void tile(Acc<D, NR>& acc, bool& fresh, int have, int key, int end, bool more, const Place& next) const {
+  __device__ __forceinline__ void tile(Acc<D, NR>& acc, bool& fresh, int have, int key, int end, bool more, const Place& next) {
     wait_vm<G_::kCopies>();  // this tile's K; its V may be under way
     fence();
     const bool whole = key + kTile <= min(least, end) && have == 15;
@@ -252,16 +279,15 @@ struct Walk {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           v2h r[4];
-          less8(w[c][i], r);
+          un.less8(w[c][i], r);
           const v2h f = {sc[c], sc[c]};
 #pragma unroll
           for (int j = 0; j < 4; ++j) r[j] *= f;
           const v8h a = join8(r);
 #pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            s[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[n], s[n][c], 0, 0, 0);
-            s[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo[n], s[n][c], 0, 0, 0);
-          }
+          for (int n = 0; n < NR; ++n) s[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[n], s[n][c], 0, 0, 0);
+#pragma unroll
+          for (int n = 0; n < NR; ++n) s[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo[n], s[n][c], 0, 0, 0);
         }
       }
     }
@@ -270,35 +296,44 @@ struct Walk {
     const bool first = fresh;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
+      if (wide >> n & 1)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[n][c] *= rf[n];
-        if (!whole)
+        for (int c = 0; c < 4; ++c) s[n][c] *= rg[n];
+      if (!whole)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int k = key + kChunk * c + 4 * qd + i;
             s[n][c][i] = k < min(lim[n], end) && (have >> c & 1) ? s[n][c][i] : -INFINITY;
           }
-      }
-      float p[16], sum, top;
+      float p[16], sum;
       auto weights = [&] __attribute__((always_inline)) {
-        sum = top = 0.0f;
+        sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(s[n][i / 4][i % 4] - acc.m[n]);
+          p[i] = __builtin_amdgcn_exp2f(fma_(s[n][i / 4][i % 4], rf[n], -acc.m[n]));
           sum += p[i];
-          top = fmaxf(top, p[i]);
         }
       };
       if (!first) weights();
-      // The first tile, and one whose weights leave fp16: a new shift, 10 below the largest score (that score itself where 10
-      // is not exact beside it).
-      if (first || __ballot(top > 32768.0f)) {
-        float z = -INFINITY;
+      // The first tile, and one whose weights may leave fp16: a new shift, 10 below the largest score (that score itself where
+      // 10 is not exact beside it).
+      if (first || __ballot(sum > 32768.0f)) {
+        auto largest = [&] __attribute__((always_inline)) {
+          float z = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) z = fmaxf(z, s[n][i / 4][i % 4]);
-        z = fmaxf(z, __shfl_xor(z, 16));
-        z = fmaxf(z, __shfl_xor(z, 32));
+          for (int i = 0; i < 16; ++i) z = fmaxf(z, s[n][i / 4][i % 4] * rf[n]);
+          z = fmaxf(z, __shfl_xor(z, 16));
+          return fmaxf(z, __shfl_xor(z, 32));
+        };
+        float z = largest();
+        if (!(wide >> n & 1) && __ballot(fabsf(z) > 65536.0f && z > -INFINITY)) {
+          wide |= 1 << n, rg[n] = rf[n], rf[n] = 1.0f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[n][c] *= rg[n];
+          z = largest();
+        }
         const float m = fmaxf(acc.m[n], fabsf(z) < 0x1p24f ? z - 10.0f : z);
         const float f = __builtin_amdgcn_exp2f(acc.m[n] - m);
         acc.m[n] = m, acc.l[n] *= f;
@@ -352,22 +387,21 @@ struct Walk {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         v2h r[4];
-        less8((uint32_t)vv[i][u], r);
+        un.less8((uint32_t)vv[i][u], r);
         const v4h a = sc[i / 2][2 * u], b = sc[i / 2][2 * u + 1];
         r[0] *= v2h{a[0], a[1]}, r[1] *= v2h{a[2], a[3]}, r[2] *= v2h{b[0], b[1]}, r[3] *= v2h{b[2], b[3]};
         const v8h x = join8(r);
 #pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          acc.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[n][u], acc.o[n][i], 0, 0, 0);
-          acc.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[n][u], acc.o[n][i], 0, 0, 0);
-        }
+        for (int n = 0; n < NR; ++n) acc.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[n][u], acc.o[n][i], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) acc.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[n][u], acc.o[n][i], 0, 0, 0);
       }
   }
 };
 
 template <int NR, int NW>
 struct Shared {  // beside the dynamic part
-  int ids[kIds];
+  uint32_t ids[kIds];  // chunks' places
   v2f ml[NW][NR * kSet];
 };
 
@@ -381,7 +415,6 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int end = min(b.keys, tb * kTile), seq = A.seq[b.t0];
   Walk<D, NR, NW> walk(A, smem, w);
-  walk.g = b.g;
   const int li = walk.li, qd = walk.qd, lane = walk.lane;
   // q: waves take (step, set) pairs in turn; a row's largest value is the waves' together.
   constexpr int kPairs = G_::kSteps * NR, kMine = (kPairs + NW - 1) / NW;
@@ -410,7 +443,8 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
   auto load_ids = [&](int t0, int t1) {
     for (int i = tid; i < 4 * (t1 - t0); i += NW * 64) {
       const int key = t0 * kTile + kChunk * i;
-      sh.ids[i] = key < end ? A.kv.page_of(seq, key) : -1;
+      const int p = key < end ? A.kv.page_of(seq, key) : -1;
+      sh.ids[i] = p < 0 ? kNoChunk : (uint32_t)((A.kv.first_row(p, b.g) + (key & ((1 << A.kv.shift) - 1))) >> 4);
     }
   };
   __syncthreads();  // LDS is free
@@ -464,7 +498,7 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
       load_ids(t0, t1);
       __syncthreads();
     }
-    auto find = [&](int t) { return walk.find(sh.ids + 4 * (t - t0), t * kTile); };
+    auto find = [&](int t) { return walk.find(sh.ids + 4 * (t - t0)); };
     int t = t0 + w;
     if (t >= t1) continue;
     Place at = find(t);
