@@ -45,9 +45,9 @@ constexpr int kIds = 1024;    // pages of chunks held in LDS at a time
 struct Shape {
   int G, tq, hs, J;
 };
-__host__ __device__ inline Shape shape_of(int H, int KV, int R) {
-  const int G = H / KV, hs = (G + R - 1) / R;
-  return Shape{G, G < R ? R / G : 1, hs, KV * hs};
+__host__ __device__ inline Shape shape_of(int H, int KV, int R, int max_run) {
+  const int G = H / KV, hs = (G + R - 1) / R, tq = G < R ? R / G : 1;
+  return Shape{G, max_run < 1 ? 1 : max_run < tq ? max_run : tq, hs, KV * hs};
 }
 
 // A block of rows of one KV head, and how many keys its tokens see at most.
@@ -70,10 +70,24 @@ __device__ __forceinline__ int keys_of(const Kv4Attn& A, int t) {
   return s >= 0 && s < A.kv.n_seq ? max(0, min(A.n_keys[t], A.max_keys)) : 0;
 }
 __device__ __forceinline__ bool starts(const Kv4Attn& A, int t) { return t == 0 || A.seq[t] != A.seq[t - 1]; }
-// The block that token t leads: it and the tokens of its sequence that follow, tq at most.
+// The first token of the run of its sequence's that t is in, found by a wave.
+__device__ __forceinline__ int run_start(const Kv4Attn& A, int t) {
+  const int lane = threadIdx.x & 63;
+  for (;; t -= 64) {
+    const uint64_t at = __ballot(t - lane >= 0 && starts(A, t - lane));
+    if (at) return t - __builtin_ctzll(at);
+  }
+}
+// The block that token t leads: it and the tokens of its sequence that follow, tq at most, found by a wave.
 __device__ __forceinline__ void set_tokens(Block& b, const Kv4Attn& A, int t, int tq) {
-  b.t0 = t, b.m = 1, b.keys = keys_of(A, t);
-  while (b.m < tq && t + b.m < A.n && !starts(A, t + b.m)) b.keys = max(b.keys, keys_of(A, t + b.m)), ++b.m;
+  const int lane = threadIdx.x & 63, i = min(t + lane, A.n - 1);
+  const int s = A.seq[i];
+  const uint64_t same = __ballot(lane < tq && t + lane < A.n && s == __builtin_amdgcn_readfirstlane(s));
+  b.t0 = t, b.m = __builtin_ctzll(~same);
+  int keys = lane < b.m ? keys_of(A, i) : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) keys = max(keys, __shfl_xor(keys, o));
+  b.keys = __builtin_amdgcn_readfirstlane(keys);
 }
 
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
@@ -402,7 +416,7 @@ struct Walk {
 template <int NR, int NW>
 struct Shared {  // beside the dynamic part
   uint32_t ids[kIds];  // chunks' places
-  v2f ml[NW][NR * kSet];
+  v2f ml[NW][NR * kSet];  // and, before, the largest values of q's rows: NW >= 4 / NR, 4 steps at most
 };
 
 // Tiles [ta, tb) of a block by the workgroup's NW waves; then put(row, element, its next four as weighted sums, l, m) by the 16
@@ -449,7 +463,7 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
   };
   __syncthreads();  // LDS is free
   load_ids(ta, min(tb, ta + kIds / 4));
-  float* top_s = reinterpret_cast<float*>(smem + G_::kQ);  // [step][row]
+  float* top_s = reinterpret_cast<float*>(sh.ml);  // [step][row]
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     const int at = w + NW * i;
@@ -461,6 +475,13 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
     if (at < kPairs && qd == 0) top_s[at / NR * G_::kR + at % NR * kSet + li] = top;
   }
   __syncthreads();
+  // The first tile's copies go while q is made ready.
+  auto find = [&](int t, int t0) { return walk.find(sh.ids + 4 * (t - t0)); };
+  Place at{};
+  if (ta + w < tb) {
+    at = find(ta + w, ta);
+    walk.issue_k(at), walk.issue_v(at);
+  }
   int ex[NR];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
@@ -498,15 +519,16 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
       load_ids(t0, t1);
       __syncthreads();
     }
-    auto find = [&](int t) { return walk.find(sh.ids + 4 * (t - t0)); };
     int t = t0 + w;
     if (t >= t1) continue;
-    Place at = find(t);
-    walk.issue_k(at), walk.issue_v(at);
+    if (t0 > ta) {
+      at = find(t, t0);
+      walk.issue_k(at), walk.issue_v(at);
+    }
     for (;;) {
       const bool more = t + NW < t1;
       const int have = at.have;
-      if (more) at = find(t + NW);
+      if (more) at = find(t + NW, t0);
       walk.tile(acc, fresh, have, t * kTile, end, more, at);
       if (!more) break;
       t += NW;
@@ -565,11 +587,9 @@ template <int D, int NR, int NW>
 __global__ __launch_bounds__(NW * 64) void k_kv4_whole(Kv4Attn A, const float* __restrict__ q, int64_t q_stride, Out O) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) Shared<NR, NW> sh;
-  const Shape S = shape_of(A.H, A.kv.KV, NR * kSet);
+  const Shape S = shape_of(A.H, A.kv.KV, NR * kSet, A.max_run);
   const int t = blockIdx.x / S.J;
-  int from = t;  // the first token of the run, or of tq of them counted from there
-  while (!starts(A, from)) --from;
-  if ((t - from) % S.tq) return;
+  if (S.tq > 1 && (t - run_start(A, t)) % S.tq) return;
   Block b;
   set_tokens(b, A, t, S.tq);
   set_heads<NR * kSet>(b, S, blockIdx.x % S.J);
@@ -580,6 +600,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv4_whole(Kv4Attn A, const float* _
 // ---- even shares of all tiles ----
 
 constexpr int kShare = 4;  // waves of a workgroup that takes a share
+constexpr int kLeast = 4;  // tiles of a share
 
 // Per (token, j): the workgroups whose runs hold its block, first (where it begins) and last (-1: written whole), and the row
 // that the token's first head has in it.
@@ -625,43 +646,46 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
   constexpr int R = NR * kSet;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) Shared<NR, kShare> sh;
-  __shared__ int64_t part[4];
+  __shared__ int tok_seq[256 + R], tok_keys[256 + R], part[4], start_t;
   __shared__ int64_t start_off;
-  __shared__ int start_t;
   const int tid = threadIdx.x, w = blockIdx.x;
-  const Shape S = shape_of(A.H, A.kv.KV, R);
-  // This thread's tokens, which follow each other, and the tiles of the blocks that they lead.
-  const int per = (A.n + 255) / 256, ta = min(A.n, tid * per), tb = min(A.n, ta + per);
-  int64_t last = -1, dummy;
-  for (int t = ta; t < tb; ++t)
-    if (starts(A, t)) last = t;
-  const int64_t run0 = scan256<true>(last, part, dummy);
-  auto leaders = [&](auto f) {
-    int from = (int)run0;
-    for (int t = ta; t < tb; ++t) {
-      if (starts(A, t)) from = t;
-      if ((t - from) % S.tq) continue;
-      Block b;
-      set_tokens(b, A, t, S.tq);
-      if (!f(t, b.tiles())) return;
+  const Shape S = shape_of(A.H, A.kv.KV, R, A.max_run);
+  // Tokens 256 at a time, a thread each: the tiles of the block that it leads, if any, and the running sum of them.
+  int run = 0, tiles = 0, before = 0, all = 0;
+  auto look = [&](int c0) {
+    __syncthreads();
+    for (int i = tid; i < 256 + R; i += 256) {
+      const int t = c0 + i;
+      tok_seq[i] = t < A.n ? A.seq[t] : 0;
+      tok_keys[i] = t < A.n ? keys_of(A, t) : 0;
     }
+    const bool first = tid == 0 ? starts(A, min(c0, A.n - 1)) : false;
+    __syncthreads();
+    const int t = c0 + tid;
+    int from = t < A.n && (tid ? tok_seq[tid] != tok_seq[tid - 1] : first) ? t : -1, last;
+    from = max(from, scan256<true>(from, part, last));  // the run's first token; of an earlier 256: none
+    if (from < 0) from = run;
+    tiles = 0;
+    if (t < A.n && (t - from) % S.tq == 0) {
+      int keys = tok_keys[tid];
+      for (int m = 1; m < S.tq && t + m < A.n && tok_seq[tid + m] == tok_seq[tid]; ++m) keys = max(keys, tok_keys[tid + m]);
+      tiles = (keys + kTile - 1) / kTile;
+    }
+    before = scan256<false>(tiles, part, all);
+    if (last >= 0) run = last;
   };
-  int64_t mine = 0, total = 0;
-  leaders([&](int, int tiles) { return mine += tiles, true; });
-  const int64_t before = scan256<false>(mine, part, total) * S.J, share = (total * S.J + gridDim.x - 1) / gridDim.x;
-  const int64_t a = w * share, b = min(a + share, total * S.J);
+  int64_t total = 0;
+  for (int c0 = 0; c0 < A.n; c0 += 256) look(c0), total += all;
+  const int64_t share = max<int64_t>((total * S.J + gridDim.x - 1) / gridDim.x, kLeast), a = w * share, b = min(a + share, total * S.J);
   if (a >= b) return;
   // The block that holds tile a is one of exactly one thread's.
-  if (before <= a && a < before + mine * S.J) {
-    int64_t off = before;
-    leaders([&](int t, int tiles) {
-      if (a < off + (int64_t)tiles * S.J) {
-        start_t = t, start_off = off;
-        return false;
-      }
-      off += (int64_t)tiles * S.J;
-      return true;
-    });
+  run = 0, total = 0;
+  for (int c0 = 0;; c0 += 256) {
+    if (A.n > 256) look(c0);
+    const int64_t off = (total + before) * S.J;
+    if (off <= a && a < off + (int64_t)tiles * S.J) start_t = c0 + tid, start_off = off;
+    total += all;
+    if (a < total * S.J) break;
   }
   __syncthreads();
   int t = start_t;
@@ -703,7 +727,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attn A, Out O, Parts P) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)A.n * A.H) return;
-  const Shape S = shape_of(A.H, A.kv.KV, R);
+  const Shape S = shape_of(A.H, A.kv.KV, R, A.max_run);
   const int t = (int)(row / A.H), head = (int)(row % A.H), in = head % S.G;
   float v[E];
 #pragma unroll
@@ -752,37 +776,42 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attn A, Out O, Parts P) {
 
 // How a call is cut.
 struct Cut {
-  int sets;  // 16-row sets of a block
-  int wgs;   // workgroups that share all tiles; 0: one per block
+  int sets;   // 16-row sets of a block
+  int wgs;    // workgroups that share all tiles; 0: one per block
+  int waves;  // of a workgroup that has a block to itself
 };
-constexpr int kWholeKeys = 512;
+constexpr int kWholeKeys = 1024, kWholeKeysMany = 2048, kMany = 512;
 
 Cut cut_of(int n, int H, int KV, int max_keys, int max_run) {
-  Cut c{std::min<int64_t>(std::max(max_run, 1), n) * (H / KV) > kSet ? 2 : 1, 0};
-  if (max_keys <= kWholeKeys) return c;
+  const int64_t rows = std::min<int64_t>(std::max(max_run, 1), n) * (H / KV);
+  Cut c{rows > kSet ? 2 : 1, 0, 8};
+  const int64_t blocks = (int64_t)n * shape_of(H, KV, c.sets * kSet, max_run).J;
+  if (blocks >= kMany) c.waves = 4;
+  if (rows <= 2 * kSet && max_keys <= (blocks >= kMany ? kWholeKeysMany : kWholeKeys)) return c;
   c.wgs = 256 * (c.sets == 1 ? 3 : 2);  // what the chip holds at once
   return c;
 }
 
 template <int D>
 size_t parts_bytes(const Cut& c, int n, int H, int KV) {
-  const Shape S = shape_of(H, KV, c.sets * kSet);
+  const Shape S = shape_of(H, KV, c.sets * kSet, 1);
   const size_t rows = 2ull * c.wgs * c.sets * kSet;
   return rows * (D * sizeof(float) + sizeof(v2f)) + (size_t)n * S.J * sizeof(Record);
 }
 
 }  // namespace
 
-// Never less for a larger call: the largest number of sets and workgroups there are, and records of the smaller blocks.
+// Never less for a larger call: the larger of both kinds of blocks, the records those of the smaller ones, also where this call
+// has no parts and a larger one may.
 size_t attention_kv4_workspace(int n, int H, int KV, int D, int max_keys, int max_run) {
-  if (max_keys <= kWholeKeys) return 0;
-  const Cut one{1, 256 * 3}, two{2, 256 * 2};
+  const Cut one{1, 256 * 3, 0}, two{2, 256 * 2, 0};
   return std::max(D == 128 ? parts_bytes<128>(one, n, H, KV) : parts_bytes<64>(one, n, H, KV),
                   D == 128 ? parts_bytes<128>(two, n, H, KV) : parts_bytes<64>(two, n, H, KV));
 }
 
 size_t attention_kv4_need(const Kv4Attn& A, int D) {
-  return attention_kv4_workspace(A.n, A.H, A.kv.KV, D, A.max_keys, A.max_run);
+  const Cut c = cut_of(A.n, A.H, A.kv.KV, A.max_keys, A.max_run);
+  return c.wgs == 0 ? 0 : D == 128 ? parts_bytes<128>(c, A.n, A.H, A.kv.KV) : parts_bytes<64>(c, A.n, A.H, A.kv.KV);
 }
 
 void attention_kv4(hipStream_t s, const Kv4Attn& A, int D, const float* q, int64_t q_stride, float* out, int64_t out_stride,
@@ -790,15 +819,14 @@ void attention_kv4(hipStream_t s, const Kv4Attn& A, int D, const float* q, int64
   const Cut c = cut_of(A.n, A.H, A.kv.KV, A.max_keys, A.max_run);
   const Out O{out, out_stride, xq};
   auto go = [&]<int D_, int NR>() {
-    const Shape S = shape_of(A.H, A.kv.KV, NR * kSet);
-    if (c.wgs == 0) {
-      constexpr int NW = 4;
+    const Shape S = shape_of(A.H, A.kv.KV, NR * kSet, A.max_run);
+    auto whole = [&]<int NW>() {
       constexpr auto lds = Geo<D_, NR, NW>::kLds;
       allow_lds<k_kv4_whole<D_, NR, NW>>(lds);
       hipLaunchKernelGGL((k_kv4_whole<D_, NR, NW>), dim3((unsigned)((int64_t)A.n * S.J)), dim3(NW * 64), lds, s, A, q, q_stride, O);
       check_launch("attention_kv4 whole");
-      return;
-    }
+    };
+    if (c.wgs == 0) return c.waves == 8 ? whole.template operator()<8>() : whole.template operator()<4>();
     constexpr int R = NR * kSet, lds = Geo<D_, NR, kShare>::kLds;
     Parts P;
     P.o = static_cast<float*>(workspace);
