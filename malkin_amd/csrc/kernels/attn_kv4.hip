@@ -720,43 +720,50 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
   }
 }
 
-// A wave per query row: the parts of rows that several workgroups had, added; zeros for rows without keys.
-template <int D, int R>
+// W waves per query row: the parts of rows that several workgroups had, added; zeros for rows without keys. Wave w of a row takes
+// every W-th part, and asks for kAhead of them before their weights are known.
+template <int D, int R, int W>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attn A, Out O, Parts P) {
   constexpr int E = D / 64, kAhead = 8;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % W;
+  const int64_t row = (int64_t)blockIdx.x * (4 / W) + wave / W;
   if (row >= (int64_t)A.n * A.H) return;
   const Shape S = shape_of(A.H, A.kv.KV, R, A.max_run);
   const int t = (int)(row / A.H), head = (int)(row % A.H), in = head % S.G;
-  float v[E];
+  const Record rec = P.rec[(int64_t)t * S.J + head / S.G * S.hs + in / R];  // what it says counts where there are keys
+  const bool any = keys_of(A, t) > 0;
+  if (any && rec.last < 0) return;
+  float v[E], sum = 0.0f;
 #pragma unroll
   for (int k = 0; k < E; ++k) v[k] = 0.0f;
-  if (keys_of(A, t) > 0) {
-    const Record rec = P.rec[(int64_t)t * S.J + head / S.G * S.hs + in / R];
-    if (rec.last < 0) return;
+  if (any) {
     const int r = rec.row + in % R, parts = rec.last - rec.first + 1;
     auto slot = [&](int i) { return (2 * ((int64_t)rec.first + i) + (i == 0)) * R + r; };
-    float top = kNone, sum = 0.0f;
-    for (int i = lane; i < parts; i += 64) top = fmaxf(top, P.ml[slot(i)][0]);
+    auto read = [&](int i0, float (&x)[kAhead][E]) {
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e)
+        if (i0 + W * e < parts)
+#pragma unroll
+          for (int k = 0; k < E; ++k) x[e][k] = P.o[slot(i0 + W * e) * D + E * lane + k];
+    };
+    float x[kAhead][E];
+    read(w, x);
+    v2f ml = lane < parts ? P.ml[slot(lane)] : v2f{kNone, 0.0f};
+    float top = ml[0];
+    for (int i = 64 + lane; i < parts; i += 64) top = fmaxf(top, P.ml[slot(i)][0]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     for (int i0 = 0; i0 < parts; i0 += 64) {
-      const v2f ml = i0 + lane < parts ? P.ml[slot(i0 + lane)] : v2f{kNone, 0.0f};
+      if (i0) ml = i0 + lane < parts ? P.ml[slot(i0 + lane)] : v2f{kNone, 0.0f};
       const float f = __builtin_amdgcn_exp2f(ml[0] - top);
       sum = fma_(f, ml[1], sum);
       const int m = min(64, parts - i0);
-      for (int i = 0; i < m; i += kAhead) {
-        float x[kAhead][E];
+      for (int i = w; i < m; i += W * kAhead) {
+        if (i0 + i != w) read(i0 + i, x);
 #pragma unroll
         for (int e = 0; e < kAhead; ++e)
-          if (i + e < m)
-#pragma unroll
-            for (int k = 0; k < E; ++k) x[e][k] = P.o[slot(i0 + i + e) * D + E * lane + k];
-#pragma unroll
-        for (int e = 0; e < kAhead; ++e)
-          if (i + e < m) {
-            const float fe = __shfl(f, i + e);
+          if (i + W * e < m) {
+            const float fe = __shfl(f, i + W * e);
 #pragma unroll
             for (int k = 0; k < E; ++k) v[k] = fma_(fe, x[e][k], v[k]);
           }
@@ -764,10 +771,23 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attn A, Out O, Parts P) {
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    const float n = sum == 0.0f ? 1.0f : sum;
-#pragma unroll
-    for (int k = 0; k < E; ++k) v[k] = v[k] / n;
   }
+  if constexpr (W > 1) {
+    __shared__ float part[W - 1][D];
+    static_assert(W == 4, "one row per workgroup");
+    if (w)
+#pragma unroll
+      for (int k = 0; k < E; ++k) part[w - 1][E * lane + k] = v[k];
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i)
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] += part[i][E * lane + k];
+  }
+  const float n = sum == 0.0f ? 1.0f : sum;
+#pragma unroll
+  for (int k = 0; k < E; ++k) v[k] = v[k] / n;
   float* to = O.out + t * O.stride + (int64_t)head * D + E * lane;
 #pragma unroll
   for (int k = 0; k < E; ++k) to[k] = v[k];
@@ -781,6 +801,7 @@ struct Cut {
   int waves;  // of a workgroup that has a block to itself
 };
 constexpr int kWholeKeys = 1024, kWholeKeysMany = 2048, kMany = 512;
+constexpr int kJoinRows = 2048;  // up to so many rows are joined by four waves each
 
 Cut cut_of(int n, int H, int KV, int max_keys, int max_run) {
   const int64_t rows = std::min<int64_t>(std::max(max_run, 1), n) * (H / KV);
@@ -835,7 +856,9 @@ void attention_kv4(hipStream_t s, const Kv4Attn& A, int D, const float* q, int64
     allow_lds<k_kv4_share<D_, NR>>(lds);
     hipLaunchKernelGGL((k_kv4_share<D_, NR>), dim3((unsigned)c.wgs), dim3(kShare * 64), lds, s, A, q, q_stride, O, P);
     check_launch("attention_kv4 shares");
-    hipLaunchKernelGGL((k_kv4_join<D_, R>), dim3((unsigned)(((int64_t)A.n * A.H + 3) / 4)), dim3(256), 0, s, A, O, P);
+    const int64_t rows = (int64_t)A.n * A.H;
+    if (rows <= kJoinRows) hipLaunchKernelGGL((k_kv4_join<D_, R, 4>), dim3((unsigned)rows), dim3(256), 0, s, A, O, P);
+    else hipLaunchKernelGGL((k_kv4_join<D_, R, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, A, O, P);
     check_launch("attention_kv4 join");
   };
   if (D == 128) c.sets == 1 ? go.template operator()<128, 1>() : go.template operator()<128, 2>();
