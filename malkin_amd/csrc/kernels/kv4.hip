@@ -94,7 +94,7 @@ struct Rope {
 };
 
 // One (token, head) per D / 8 lanes: lane l holds elements 8 l .. 8 l + 7. FAST: a lane's elements rotate
-// with eight neighbours.
+// with eight neighbours, or with each other, all of them or none.
 template <int D, bool FAST>
 __global__ __launch_bounds__(kThreads) void k_rope_kv4(Rope R, Kv4 kv, const float* q, const float* __restrict__ k,
                                                        const float* __restrict__ v, int64_t stride, float* q_out,
@@ -131,14 +131,22 @@ __global__ __launch_bounds__(kThreads) void k_rope_kv4(Rope R, Kv4 kv, const flo
     }
     const float *ct = R.cos_t + (int64_t)pos * R.half, *st = R.sin_t + (int64_t)pos * R.half;
     if (R.pairs) {
+      const int i0 = kPer / 2 * l;
+      auto turn = [&](int e, float c, float s) {
+        const float a = x[2 * e], b = x[2 * e + 1];
+        x[2 * e] = fma_(a, c, -(b * s));
+        x[2 * e + 1] = fma_(a, s, b * c);
+      };
+      if constexpr (FAST) {
+        if (i0 < R.half) {
+          const v4f c = *reinterpret_cast<const v4a*>(ct + i0), s = *reinterpret_cast<const v4a*>(st + i0);
 #pragma unroll
-      for (int e = 0; e < kPer; e += 2) {
-        const int i = (kPer * l + e) / 2;
-        if (i < R.half) {
-          const float c = ct[i], s = st[i], a = x[e], b = x[e + 1];
-          x[e] = fma_(a, c, -(b * s));
-          x[e + 1] = fma_(a, s, b * c);
+          for (int e = 0; e < kPer / 2; ++e) turn(e, c[e], s[e]);
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e)
+          if (i0 + e < R.half) turn(e, ct[i0 + e], st[i0 + e]);
       }
     } else {
       float* mine = sh[threadIdx.x / L];
@@ -271,7 +279,7 @@ void rope_kv4(hipStream_t s, const Kv4& kv, int D, const float* q, const float* 
               int64_t q_out_stride) {
   const Rope R{cos_t, sin_t, q_norm, k_norm, rpos, seq, kv_row, eps, rope_dim / 2, n_pos, pairs, n, H};
   const int64_t items = (int64_t)n * (H + 2 * kv.KV), per = kThreads / (D / kPer), wgs = (items + per - 1) / per;
-  const bool fast = !pairs && R.half % kPer == 0;
+  const bool fast = R.half % (pairs ? kPer / 2 : kPer) == 0;
   auto go = [&]<int D_, bool F>() {
     hipLaunchKernelGGL((k_rope_kv4<D_, F>), dim3((unsigned)wgs), dim3(kThreads), 0, s, R, kv, q, k, v, stride, q_out,
                        q_out_stride);

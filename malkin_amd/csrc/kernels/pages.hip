@@ -69,6 +69,46 @@ __global__ __launch_bounds__(kThreads) void k_fork_put(Kv4Pool P, const int32_t*
   if (threadIdx.x == 0) P.len[d] = len;
 }
 
+// The same by one workgroup, the sources' pages in LDS between: a launch less where there is little to move.
+constexpr int kFewEntries = 1024, kFewNumbers = 16384;
+__global__ __launch_bounds__(kPlan) void k_fork_few(Kv4Pool P, const int32_t* __restrict__ dst, const int32_t* __restrict__ src,
+                                                    int n) {
+  extern __shared__ int32_t lds[];
+  int32_t *d_s = lds, *s_s = d_s + n, *new_s = s_s + n, *old_s = new_s + n, *rows = old_s + n;
+  const int tid = threadIdx.x;
+  for (int i = tid; i < n; i += kPlan) {
+    d_s[i] = dst ? dst[i] : i;
+    s_s[i] = src[i];
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kPlan) {
+    const int d = d_s[i], s = s_s[i];
+    bool ok = d >= 0 && d < P.n_seq && s != d;
+    if (dst && d >= 0 && d < P.n_seq)
+      for (int j = i + 1; j < n && ok; ++j) ok = d_s[j] != d;
+    new_s[i] = ok ? (s >= 0 && s < P.n_seq ? held(P, s) : 0) : -1;
+    old_s[i] = ok ? held(P, d) : 0;
+  }
+  __syncthreads();
+  for (int at = tid; at < n * P.max_pages; at += kPlan) {
+    const int i = at / P.max_pages, j = at - i * P.max_pages;
+    if (new_s[i] < 0) continue;
+    const int a = j < pages_of(new_s[i], P.shift) ? P.table[(int64_t)s_s[i] * P.max_pages + j] : -1;
+    const int b = j < pages_of(old_s[i], P.shift) ? P.table[(int64_t)d_s[i] * P.max_pages + j] : -1;
+    rows[at] = a;
+    if (a == b) continue;
+    if (a >= 0 && a < P.n_page) atomicAdd(P.refs + a, 1);
+    if (b >= 0 && b < P.n_page) atomicAdd(P.refs + b, -1);
+  }
+  __syncthreads();
+  for (int at = tid; at < n * P.max_pages; at += kPlan) {
+    const int i = at / P.max_pages, j = at - i * P.max_pages;
+    if (new_s[i] >= 0 && j < pages_of(max(new_s[i], old_s[i]), P.shift)) P.table[(int64_t)d_s[i] * P.max_pages + j] = rows[at];
+  }
+  for (int i = tid; i < n; i += kPlan)
+    if (new_s[i] >= 0) P.len[d_s[i]] = new_s[i];
+}
+
 // ---- copies ----
 
 struct Move {
@@ -135,63 +175,74 @@ __device__ __forceinline__ T block_scan(T v, T* part, T& total) {
 
 __device__ __forceinline__ int refs_now(const int32_t* p) { return (int)ld_coh_u32(reinterpret_cast<const uint32_t*>(p)); }
 
-// Entry i's sequence and end; kind: what becomes of it.
+// What becomes of an entry.
 enum { kSkip = 0, kShrink = 1, kGrow = 2 };
+constexpr int kFreeInLds = 1024;  // free pages that are kept at hand
 
 __global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t* __restrict__ seq,
                                                        const int32_t* __restrict__ new_len, int n, int32_t* __restrict__ status,
                                                        int32_t* __restrict__ count, Move* __restrict__ moves, int32_t* free_list) {
   extern __shared__ int32_t lds[];
-  int32_t *seq_s = lds, *last_s = lds + n, *base_s = lds + 2 * n;  // base_s: the entry's first page in free_list, -1 none
-  __shared__ int part[kPlan / 64];
+  int32_t *seq_s = lds, *len_s = seq_s + n, *new_s = len_s + n, *last_s = new_s + n;
+  __shared__ int part[kPlan / 64], free_s[kFreeInLds];
   __shared__ int64_t part64[kPlan / 64];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  __shared__ uint8_t kind_s[kMaxEntries];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, in_page = (1 << P.shift) - 1;
   const int E = (n + kPlan - 1) / kPlan, i0 = tid * E;  // a thread's entries follow each other
-  for (int i = tid; i < n; i += kPlan) seq_s[i] = seq ? seq[i] : i;
-  __syncthreads();
   const int64_t room = (int64_t)P.max_pages << P.shift;
-  // What does not fit, or comes again; status 2 marks what is to grow.
+  for (int i = tid; i < n; i += kPlan) seq_s[i] = seq ? seq[i] : i, new_s[i] = new_len[i];
+  if (seq) __syncthreads();  // else each thread looks at its own
+  bool shrinks = false;
   for (int i = tid; i < n; i += kPlan) {
-    const int s = seq_s[i], L = new_len[i];
+    const int s = seq_s[i], L = new_s[i];
     bool ok = s >= 0 && s < P.n_seq && L >= 0 && L <= room;
     if (seq)
       for (int j = i + 1; j < n && ok; ++j) ok = seq_s[j] != s;
-    last_s[i] = -1;
-    base_s[i] = !ok ? kSkip : L > held(P, s) ? kGrow : kShrink;
-  }
-  __syncthreads();
-  // Shorter ends, a wave per entry.
-  for (int i = w; i < n; i += kPlan / 64) {
-    if (base_s[i] != kShrink) continue;
-    const int s = seq_s[i], had = pages_of(held(P, s), P.shift), has = pages_of(new_len[i], P.shift);
-    for (int j = has + lane; j < had; j += 64) {
-      int32_t* at = P.table + (int64_t)s * P.max_pages + j;
-      const int p = *at;
-      if (p >= 0 && p < P.n_page) atomicAdd(P.refs + p, -1);
-      *at = -1;
+    const int len = ok ? held(P, s) : 0;
+    const int kind = !ok ? kSkip : L > len ? kGrow : kShrink;
+    int last = -1;
+    if (kind == kGrow && len & in_page) {
+      last = P.table[(int64_t)s * P.max_pages + (len >> P.shift)];
+      if (last >= P.n_page) last = -1;
     }
-    __builtin_amdgcn_wave_barrier();
-    if (lane == 0) P.len[s] = new_len[i];
+    len_s[i] = len, last_s[i] = max(last, -1), kind_s[i] = (uint8_t)kind;
+    shrinks |= kind == kShrink && L < len;
   }
-  // The last pages of those that grow.
-  for (int i = tid; i < n; i += kPlan) {
-    if (base_s[i] != kGrow) continue;
-    const int s = seq_s[i], len = held(P, s);
-    if (len & ((1 << P.shift) - 1)) {
-      const int p = P.table[(int64_t)s * P.max_pages + (len >> P.shift)];
-      last_s[i] = p >= 0 && p < P.n_page ? p : -1;
+  if (__syncthreads_or(shrinks)) {  // shorter ends, a wave per entry
+    for (int i = w; i < n; i += kPlan / 64) {
+      if (kind_s[i] != kShrink) continue;
+      const int s = seq_s[i], had = pages_of(len_s[i], P.shift), has = pages_of(new_s[i], P.shift);
+      for (int j = has + lane; j < had; j += 64) {
+        int32_t* at = P.table + (int64_t)s * P.max_pages + j;
+        const int p = *at;
+        if (p >= 0 && p < P.n_page) atomicAdd(P.refs + p, -1);
+        *at = -1;
+      }
+      if (lane == 0) P.len[s] = new_s[i];
     }
+    __syncthreads();  // the counts have been taken down
   }
-  __syncthreads();  // the counts have been taken down too
-  // Copies and pages wanted, and where each entry's pages begin in the list of free ones. More than the pool has counts as one
-  // more than that.
+  // The first pages of the pool, asked for beside the counts of the last pages.
+  auto free_of = [&](int p0) {
+    uint32_t free = 0;
+#pragma unroll
+    for (int e = 0; e < kScan; ++e) {
+      const int p = p0 + kScan * tid + e;
+      const int r = refs_now(P.refs + min(p, P.n_page - 1));
+      free |= (uint32_t)(p < P.n_page && r <= 0) << e;
+    }
+    return free;
+  };
+  uint32_t free = kScan * (tid & ~63) < P.n_page ? free_of(0) : 0;
+  // Copies and pages wanted, and where each entry's begin in the list of free pages and in that of the copies. More than the
+  // pool has counts as one more than that.
   int copies[kMaxEntries / kPlan], needs[kMaxEntries / kPlan];
   int64_t mine = 0;
 #pragma unroll
   for (int e = 0; e < kMaxEntries / kPlan; ++e) {
     copies[e] = needs[e] = 0;
     const int i = i0 + e;
-    if (e >= E || i >= n || base_s[i] != kGrow) continue;
+    if (e >= E || i >= n || kind_s[i] != kGrow) continue;
     if (last_s[i] >= 0) {
       const int holders = refs_now(P.refs + last_s[i]);
       int before = 0;
@@ -199,76 +250,65 @@ __global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t*
         for (int j = 0; j < i; ++j) before += last_s[j] == last_s[i];
       copies[e] = before < holders - 1;
     }
-    needs[e] = min(copies[e] + pages_of(new_len[i], P.shift) - pages_of(held(P, seq_s[i]), P.shift), P.n_page + 1);
-    mine += needs[e];
+    needs[e] = min(copies[e] + pages_of(new_s[i], P.shift) - pages_of(len_s[i], P.shift), P.n_page + 1);
+    mine += ((int64_t)needs[e] << 16) + copies[e];
   }
-  int64_t wanted = 0;
-  const int64_t at = block_scan(mine, part64, wanted);
+  int64_t all = 0;
+  const int64_t before = block_scan(mine, part64, all);
+  const int64_t wanted = all >> 16;
   // The first free pages of the pool, as many as are wanted.
   int found = 0;
   for (int p0 = 0; p0 < P.n_page && found < wanted; p0 += kScan * kPlan) {
-    uint32_t free = 0;
-#pragma unroll
-    for (int e = 0; e < kScan; ++e) {
-      const int p = p0 + kScan * tid + e;
-      if (p < P.n_page && refs_now(P.refs + p) <= 0) free |= 1u << e;
-    }
-    int all = 0, to = found + block_scan((int)__popc(free), part, all);
+    if (p0) free = free_of(p0);
+    int here = 0, to = found + block_scan((int)__popc(free), part, here);
 #pragma unroll
     for (int e = 0; e < kScan; ++e)
       if (free >> e & 1) {
-        if (to < wanted) free_list[to] = p0 + kScan * tid + e;
+        if (to < wanted) {
+          if (to < kFreeInLds) free_s[to] = p0 + kScan * tid + e;
+          else free_list[to] = p0 + kScan * tid + e;
+        }
         ++to;
       }
-    found += all;
+    found += here;
   }
-  // What does not fit does not happen.
-  int n_copy = 0;
-  int64_t run = at;
-#pragma unroll
-  for (int e = 0; e < kMaxEntries / kPlan; ++e) {
-    if (needs[e] && run + needs[e] > found) copies[e] = 0;
-    n_copy += copies[e];
-    run += needs[e];
-  }
-  int total = 0, slot = block_scan(n_copy, part, total);
-  __syncthreads();  // free_list is written, everyone has read base_s and the counts
-  run = at;
+  __syncthreads();  // the list is written
+  auto page_at = [&](int64_t i) { return i < kFreeInLds ? free_s[i] : free_list[i]; };
+  int64_t run = before >> 16;
+  int slot = (int)(before & 0xFFFF);
 #pragma unroll
   for (int e = 0; e < kMaxEntries / kPlan; ++e) {
     const int i = i0 + e;
     if (e >= E || i >= n) continue;
-    if (base_s[i] != kGrow) {
-      status[i] = base_s[i] == kSkip ? -1 : 0;
-      base_s[i] = -1;
-      continue;
+    const int kind = kind_s[i];
+    const bool fits = kind == kGrow && (needs[e] == 0 || run + needs[e] <= found);
+    if (copies[e]) {  // one that does not fit stays in the list, with no rows
+      Move m{0, 0, 0};
+      if (fits) {
+        const int p = page_at(run), s = seq_s[i], len = len_s[i];
+        m = Move{last_s[i], p, len & in_page};
+        P.table[(int64_t)s * P.max_pages + (len >> P.shift)] = p;
+        atomicAdd(P.refs + m.src, -1);
+        atomicAdd(P.refs + p, 1);
+      }
+      moves[slot++] = m;
     }
-    const bool fits = needs[e] == 0 || run + needs[e] <= found;
-    const int s = seq_s[i], len = held(P, s);
-    if (copies[e]) {
-      const int p = free_list[run];
-      moves[slot++] = Move{last_s[i], p, len & ((1 << P.shift) - 1)};
-      P.table[(int64_t)s * P.max_pages + (len >> P.shift)] = p;
-      atomicAdd(P.refs + last_s[i], -1);
-      atomicAdd(P.refs + p, 1);
-    }
-    status[i] = fits ? 0 : 1;
-    base_s[i] = fits ? (int)run + copies[e] : -1;
+    status[i] = kind == kSkip ? -1 : kind == kGrow && !fits;
+    if (fits) P.len[seq_s[i]] = new_s[i];
+    last_s[i] = fits ? (int)run + copies[e] : -1;  // its first new page in the list
     run += needs[e];
   }
-  if (tid == 0) *count = total;
-  __syncthreads();
-  // New pages, a wave per entry, and the new lengths.
+  if (tid == 0) *count = (int)(all & 0xFFFF);
+  // Does any entry have new pages? Then a wave per entry puts them down.
+  if (!__syncthreads_or(wanted > (all & 0xFFFF))) return;
   for (int i = w; i < n; i += kPlan / 64) {
-    if (base_s[i] < 0) continue;
-    const int s = seq_s[i], had = pages_of(held(P, s), P.shift), has = pages_of(new_len[i], P.shift);
+    if (last_s[i] < 0) continue;
+    const int s = seq_s[i], had = pages_of(len_s[i], P.shift), has = pages_of(new_s[i], P.shift);
     for (int j = lane; j < has - had; j += 64) {
-      const int p = free_list[base_s[i] + j];
+      const int p = page_at(last_s[i] + j);
       P.table[(int64_t)s * P.max_pages + had + j] = p;
       atomicAdd(P.refs + p, 1);
     }
-    __builtin_amdgcn_wave_barrier();
-    if (lane == 0) P.len[s] = new_len[i];
   }
 }
 
@@ -346,6 +386,12 @@ unsigned copy_wgs(int64_t moves, int heads) {
 size_t kv4_fork_workspace(int n, int max_pages) { return (size_t)n * (max_pages + 1ull) * 4; }
 
 void kv4_fork(hipStream_t s, const Kv4Pool& P, const int32_t* dst, const int32_t* src, int n, void* workspace) {
+  if (n <= kFewEntries && (int64_t)n * P.max_pages <= kFewNumbers) {
+    allow_lds<k_fork_few>(4 * (4 * kFewEntries + kFewNumbers));
+    hipLaunchKernelGGL(k_fork_few, dim3(1), dim3(kPlan), (size_t)n * (4 + P.max_pages) * 4, s, P, dst, src, n);
+    check_launch("kv4_fork few");
+    return;
+  }
   int32_t *head = static_cast<int32_t*>(workspace), *rows = head + n;
   hipLaunchKernelGGL(k_fork_take, dim3((unsigned)n), dim3(kThreads), 0, s, P, dst, src, n, head, rows);
   check_launch("kv4_fork take");
@@ -360,7 +406,8 @@ void kv4_resize(hipStream_t s, const Kv4Pool& P, int D, const int32_t* seq, cons
   int32_t* count = static_cast<int32_t*>(workspace);
   Move* moves = reinterpret_cast<Move*>(count + kHead / 4);
   int32_t* free_list = reinterpret_cast<int32_t*>(moves + n);
-  hipLaunchKernelGGL(k_resize_plan, dim3(1), dim3(kPlan), (size_t)n * 12, s, P, seq, new_len, n, status, count, moves, free_list);
+  allow_lds<k_resize_plan>(16 * kMaxEntries);
+  hipLaunchKernelGGL(k_resize_plan, dim3(1), dim3(kPlan), (size_t)n * 16, s, P, seq, new_len, n, status, count, moves, free_list);
   check_launch("kv4_resize plan");
   auto go = [&]<int D_>() {
     hipLaunchKernelGGL(k_copy_pages<D_>, dim3(copy_wgs(n, P.heads)), dim3(kThreads), 0, s, P, count, moves);
