@@ -73,11 +73,13 @@ WRITES = [  # heads, KV heads, head_dim, page, rope_dim, layout, norm, pad, in p
     (5, 5, 128, 1024, 26, mk_.ROPE_PAIRS, True, 0, True),
     (2, 2, 128, 16, 0, mk_.ROPE_HALVES, False, 0, False),
     (40, 8, 128, 64, 80, mk_.ROPE_HALVES, False, 0, False),
+    (40, 8, 128, 64, 128, mk_.ROPE_PAIRS, True, 0, False),
+    (25, 8, 64, 256, 64, mk_.ROPE_HALVES, True, 3, True),
 ]
 
 
 @pytest.mark.parametrize("case", WRITES, ids=str)
-@pytest.mark.parametrize("n", [1, 37])
+@pytest.mark.parametrize("n", [1, 37, 1300])
 def test_write(mk, case, n):
     H, KV, d, page, rope_dim, layout, norm, pad, in_place = case
     rng = np.random.default_rng(H + d + n)
@@ -87,6 +89,7 @@ def test_write(mk, case, n):
     c.put(mk)
     at = [(s, r) for s in range(n_seq) for r in range(c.a["len"][s])]
     at = [at[i] for i in rng.permutation(len(at))[:n]]
+    n = len(at)
     seq, row = [list(v) for v in zip(*at)]
     n_pos = 50
     rpos = list(rng.integers(0, n_pos, n))
