@@ -264,12 +264,13 @@ int mk_move_kv(mk_ctx* ctx, const mk_kv_cache* kv, int seq, int from, int to);
 
 /* ---- KV cache in 4 bits and in pages (no reference counterpart: its cache is int8, a slot's rows in one piece) ----
  * A row of head_dim elements is held in groups of 32, each with an fp16 scale s: element n of 0..15 stands for s (n - 8) in
- * fp16. mk_rope_kv4 writes scales of at most 8 significant bits, of which that is exact. Byte b of a row has element 2 b in its low and 2 b + 1 in its high
- * half. Rows lie in pages of `page` positions (a power of two, 16..1024) of all layers and KV heads, taken from one pool;
- * position j of sequence q is row j % page of page table[q * max_pages + j / page]. head_dim 64 or 128
- * (MK_ERR_UNSUPPORTED otherwise). Device arrays; k and v 16-byte aligned, k_scale 8, v_scale 16. Beams and chats that go
- * on from one text share its pages: refs counts the entries of the table that name a page. table, len and refs are the
- * caller's to fill at first (-1, 0 and 0: nothing held); mk_kv4_fork, mk_kv4_resize and mk_kv4_compact keep them. */
+ * fp16. mk_rope_kv4 writes scales of at most 8 significant bits, of which that is exact. Byte b of a row has element 2 b in
+ * its low and 2 b + 1 in its high half. Rows lie in pages of `page` positions (a power of two, 16..1024) of all layers and KV
+ * heads, taken from one pool of fewer than 2^34 rows; position j of sequence q is row j % page of page
+ * table[q * max_pages + j / page]. head_dim 64 or 128 (MK_ERR_UNSUPPORTED otherwise). Device arrays; k and v 16-byte aligned,
+ * k_scale 8, v_scale 16. Beams and chats that go on from one text share its pages: refs counts the entries of the table that
+ * name a page. table, len and refs are the caller's to fill at first (-1, 0 and 0: nothing held); mk_kv4_fork, mk_kv4_resize
+ * and mk_kv4_compact keep them. */
 typedef struct {
   uint8_t* k;        /* [n_page][n_layer][n_head_kv][page][head_dim / 2] */
   uint8_t* v;
@@ -318,8 +319,8 @@ int mk_rope_kv4(mk_ctx* ctx, const float* q, const float* k, const float* v, int
 int mk_kv4_rows(mk_ctx* ctx, const mk_kv4_cache* kv, int layer, const int32_t* seq, const int32_t* row, int n, void* k_out,
                 void* v_out);
 /* mk_attention for plain tokens over the 4-bit cache: token t attends with its n_head query heads to positions
-   0..n_keys[t]-1 of sequence seq[t]; fp32 sums. max_keys bounds n_keys[t]: keys past it are not read. max_run is the number
-   of tokens of one sequence that follow each other at most (1: decoding), a hint that changes no result beyond rounding. A
+   0..n_keys[t]-1 of sequence seq[t]; fp32 sums. max_keys (at most 2^28) bounds n_keys[t]: keys past it are not read. max_run
+   is the number of tokens of one sequence that follow each other at most (1: decoding), a hint that changes no result beyond rounding. A
    token with n_keys[t] <= 0 or seq[t] outside the cache gets zeros, and keys whose page is not in the pool have no weight.
    Tokens may come in any order; those of one sequence that follow each other read its rows together. xq: the BlockQ8 rows of
    out, as mk_attention_q8 (NULL: not written). workspace: at least mk_attention_kv4_workspace bytes for the same sizes or
@@ -331,17 +332,17 @@ int mk_attention_kv4(mk_ctx* ctx, const float* q, int64_t q_stride, float* out, 
                      int max_run, void* xq, void* workspace, size_t workspace_bytes);
 /* Sequence dst[i] (dst NULL: i) holds what sequence src[i] held before the call, for all i at once: its pages are shared, no
    row is copied; what dst[i] held is let go. src[i] outside the cache: dst[i] holds nothing then. An entry whose dst[i] lies
-   outside, or comes again further on, has no effect. Beam search: src from mk_beam_select. workspace: 16-byte aligned, one per
-   call at a time (mk_kv4_resize and mk_kv4_compact too). */
+   outside, or comes again further on, has no effect. n at most 2^20. Beam search: src from mk_beam_select. workspace: 16-byte
+   aligned, one per call at a time (mk_kv4_resize and mk_kv4_compact too). */
 size_t mk_kv4_fork_workspace(int n, int max_pages);
 int mk_kv4_fork(mk_ctx* ctx, const mk_kv4_cache* kv, const int32_t* dst, const int32_t* src, int n, void* workspace,
                 size_t workspace_bytes);
 /* Sequence seq[i] (seq NULL: i) is to hold new_len[i] rows: pages past a shorter end are let go; a longer one gets pages, and
    where its last page is shared and not full, a copy of the rows it holds there (all layers), so that it can be written.
    Shorter ends come first, then the longer ones in order, each taking the free pages of the lowest numbers; of those that
-   share a page and nobody else, the last keeps it. status[i]: 0, or 1 where new_len[i] needs a page and the pool has too few for it and
-   all entries before it, or -1 where seq[i] or new_len[i] (0..max_pages * page) lies outside or seq[i] comes again further
-   on; such entries change nothing. */
+   share a page and nobody else, the last keeps it. status[i]: 0, or 1 where new_len[i] needs a page and the pool has too few
+   for it and all entries before it, or -1 where seq[i] or new_len[i] (0..max_pages * page) lies outside or seq[i] comes again
+   further on; such entries change nothing. n at most 4096. */
 size_t mk_kv4_resize_workspace(int n, int n_page);
 int mk_kv4_resize(mk_ctx* ctx, const mk_kv4_cache* kv, const int32_t* seq, const int32_t* new_len, int n, int32_t* status,
                   void* workspace, size_t workspace_bytes);
@@ -507,8 +508,8 @@ int mk_verify_topk(mk_ctx* ctx, const float* p_values, const int32_t* p_ids, int
  * beam with done[row] != 0 (done NULL: none) has only itself, token eos, its score as it is. Equal scores: the lower beam, then
  * the lower token. Logits: NaN counts as -inf (no candidate), +inf as the largest float; a beam whose score is not finite has
  * no part. out_scores (rounded), out_seq (the row it goes on from: mk_kv4_fork's src) and out_tokens are [n_group][k]; places
- * without a candidate: -inf, -1, -1. beams 1..64, k 1..128. workspace: at least mk_beam_workspace bytes, 16-byte aligned; two
- * calls that may run at the same time need one each. */
+ * without a candidate: -inf, -1, -1. beams 1..64, k 1..128, n_vocab at most 2^21. workspace: at least mk_beam_workspace bytes,
+ * 16-byte aligned; two calls that may run at the same time need one each. */
 size_t mk_beam_workspace(int n_group, int beams, int n_vocab, int k);
 int mk_beam_select(mk_ctx* ctx, const float* logits, int64_t stride, int n_group, int beams, int n_vocab,
                    const float* scores, const int32_t* done, int eos, int k, float* out_scores, int32_t* out_seq,

@@ -547,8 +547,8 @@ int mk_attention_prefix(mk_ctx* c, const float* q, int64_t q_stride, float* out,
 
 namespace {
 
-// The cache's own sizes; 2^31 bounds what the kernels count in 32 bits: the rows of one page of all layers and heads, a
-// sequence's positions, the table's entries.
+// The cache's own sizes. 2^31 bounds what the kernels count in 32 bits: the rows of one page of all layers and heads, a
+// sequence's positions, the table's entries. The pool's rows, 2^34 (a TiB at the least), bound its pages and its 16-row chunks.
 void kv4_sizes(const mk_kv4_cache* kv, const char* call) {
   auto need = [&](bool ok, const char* what) {
     if (!ok) throw mk::Error(MK_ERR_INVALID, std::string(call) + what);
@@ -560,7 +560,8 @@ void kv4_sizes(const mk_kv4_cache* kv, const char* call) {
     throw mk::Error(MK_ERR_UNSUPPORTED, std::string(call) + ": no kernel for this head_dim");
   const int64_t most = 1ll << 31;
   need((int64_t)kv->n_layer * kv->n_head_kv < (1 << 20) && (int64_t)kv->n_seq * kv->max_pages < most &&
-           (int64_t)kv->max_pages * kv->page < most,
+           (int64_t)kv->max_pages * kv->page < most &&
+           (int64_t)kv->n_page * kv->page < (1ll << 34) / ((int64_t)kv->n_layer * kv->n_head_kv),
        ": cache too large");
   need(kv->k && kv->v && kv->k_scale && kv->v_scale && kv->table, ": null cache array");
   need((((uintptr_t)kv->k | (uintptr_t)kv->v | (uintptr_t)kv->v_scale) & 15) == 0 && ((uintptr_t)kv->k_scale & 7) == 0,
@@ -672,6 +673,7 @@ int mk_attention_kv4(mk_ctx* c, const float* q, int64_t q_stride, float* out, in
     require(q_stride >= (int64_t)n_head * D && out_stride >= (int64_t)n_head * D,
             "mk_attention_kv4: stride shorter than a row");
     require((int64_t)n * n_head < (1 << 24), "mk_attention_kv4: too many rows");
+    require(max_keys <= 1 << 28, "mk_attention_kv4: max_keys past 2^28");  // 256 tokens' tiles are added up in 32 bits
     require(max_keys <= (int64_t)kv->max_pages * kv->page, "mk_attention_kv4: max_keys past the sequences' pages");
     const mk::Kv4Attn A{K, n, n_head, max_keys, max_run, 1.0f / std::sqrt(static_cast<float>(D)), seq, n_keys};
     require(holds(workspace, workspace_bytes, mk::attention_kv4_need(A, D)),

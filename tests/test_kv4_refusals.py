@@ -91,6 +91,7 @@ BAD_CACHES = [
     (dict(kv=cache(k=X + 8)), "not aligned"), (dict(kv=cache(v=X + 4)), "not aligned"), (dict(kv=cache(k_scale=X + 4)), "not aligned"),
     (dict(kv=cache(v_scale=X + 8)), "not aligned"), (dict(kv=cache(max_pages=1 << 26)), "too large"),
     (dict(kv=cache(n_seq=1 << 28)), "too large"), (dict(kv=cache(n_layer=1 << 19)), "too large"),
+    (dict(kv=cache(n_page=1 << 30)), "too large"), (dict(kv=cache(n_page=1 << 27)), "too large"),
 ]
 
 
@@ -241,3 +242,10 @@ def test_plain_forms_agree():
     cases.fork_model(a, 16, None, [1, 0, -1])
     assert a["table"].tolist() == [[0, 1], [0, 3], [-1, -1]] and a["refs"].tolist() == [2, 1, 0, 1, 0]
     assert cases.compact_model(a) == (3, [(3, 2, None)]) and a["table"].tolist() == [[0, 1], [0, 2], [-1, -1]]
+
+
+def test_keys_that_are_counted_in_32_bits():
+    big = cache(max_pages=1 << 25)
+    refused(attention(kv=big, most=(1 << 28) + 1), mk_.MK_ERR_INVALID, "max_keys past 2^28")
+    refused(attention(kv=big, most=1 << 28), mk_.MK_ERR_INVALID, "null context")
+    refused(attention(kv=cache(n_page=(1 << 27) - 1)), mk_.MK_ERR_INVALID, "null context")
