@@ -54,6 +54,9 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   const uint32_t u = __float_as_uint(f + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
+// A candidate as one number: of two, the larger one is ahead.
+__device__ __forceinline__ uint64_t rank_key(float z, int id) { return (uint64_t)order_key(z) << 32 | (uint32_t)~id; }
 
 // One segment of kThreads * 4 Q logits of a row. The k-th largest of the maxima of PARTS parts of it is a bound (k <= MOST <=
 // PARTS): at most (k - 1) parts hold anything larger. Of logits that are equal to it there can be any number; where the list
@@ -67,7 +70,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restric
   __shared__ uint32_t bound;
   __shared__ int n_cand;
   __shared__ double wave_sum[kThreads / 64];
-  __shared__ Cand list[CAP];
+  __shared__ uint64_t list[CAP];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x / B.segs, seg = blockIdx.x % B.segs;
   const float* l = B.logits + row * B.stride;
   const int first = seg * kSeg;
@@ -137,10 +140,10 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restric
   if (lane == 0) wave_sum[w] = sum;
   __syncthreads();
   const uint32_t key = bound;  // fewer than k parts: of -inf
-  const float limit = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+  const float limit = of_key(key);
   auto put = [&](int e) {
     const int at = atomicAdd(&n_cand, 1);
-    if (at < CAP) list[at] = Cand{z[e], id_of(e)};
+    if (at < CAP) list[at] = rank_key(z[e], id_of(e));
   };
   if (best >= limit && best > -INFINITY)
 #pragma unroll
@@ -170,13 +173,13 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restric
   Cand* out = cands + ((int64_t)row * B.segs + seg) * B.k;
   // Each one's place: how many are ahead of it, counted by four threads.
   for (int i = tid >> 2; i < n; i += kThreads / 4) {
-    const Cand c = list[i];
+    const uint64_t c = list[i];
     int before = 0;
 #pragma unroll 4
-    for (int j = tid & 3; j < n; j += 4) before += ahead(list[j].z, list[j].id, c.z, c.id);
+    for (int j = tid & 3; j < n; j += 4) before += list[j] > c;
     before += __shfl_xor(before, 1);
     before += __shfl_xor(before, 2);
-    if (before < B.k && (tid & 3) == 0) out[before] = c;
+    if (before < B.k && (tid & 3) == 0) out[before] = Cand{of_key((uint32_t)(c >> 32)), (int32_t)~(uint32_t)c};
   }
   for (int i = n + tid; i < B.k; i += kThreads) out[i] = Cand{-INFINITY, -1};
   if (tid == 0) {
@@ -211,29 +214,32 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, group = blockIdx.x;
   const int beams = ROW ? 1 : B.beams, lists = beams * B.segs, k = B.k;
   const int64_t row0 = (int64_t)group * beams;
-  auto alive = [&](int b) { return finite(B.scores[row0 + b]); };
-  auto ended = [&](int b) { return B.done && B.done[row0 + b]; };
-  if (ROW && (!alive(0) || ended(0))) return;
   const Entry none{-INFINITY, -INFINITY, -1, INT32_MAX};
-  // This thread's list, its first elements asked for at once (a list that nothing was written to is not looked at).
+  // This thread's list, its first elements asked for at once, beside everything else that the addresses are known of (what lies
+  // where nothing was written is not looked at).
   const int beam = tid / B.segs;
   const bool in = tid < lists;
   const Cand* from = cands + (row0 * B.segs + (in ? tid : 0)) * k;
   Cand c[kAhead];
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) c[j] = from[min(j, k - 1)];
-  const bool mine = in && alive(beam), over = mine && ended(beam);
-  const double start = mine && !ROW ? (double)B.scores[row0 + beam] : 0.0;
+  const int64_t row = row0 + (in ? beam : 0);
+  const float score = B.scores[row];
+  const int done = B.done ? B.done[row] : 0;
   // Sums of the rows, a group of lanes for each: as many lanes as it has segments, at most a wave.
   int width = 1;
   while (width < B.segs && width < 64) width <<= 1;
   for (int b0 = w * (64 / width); b0 < beams; b0 += kMergeThreads / width) {
     const int b = b0 + lane / width, at = lane % width;
-    const bool live = b < beams && alive(b) && !ended(b);  // nothing was written for the others
-    const Stat* s = stats + (row0 + (live ? b : 0)) * B.segs;
+    const int64_t r = row0 + min(b, beams - 1);
+    const Stat* s = stats + r * B.segs;
+    const Stat first = s[min(at, B.segs - 1)];
+    const float its = B.scores[r];
+    const int end = B.done ? B.done[r] : 0;
+    const bool live = b < beams && finite(its) && !end;  // nothing was written for the others
     Stat one{0.0, -INFINITY, 0};
     for (int i = at; i < B.segs && live; i += width) {
-      const Stat t = s[i];
+      const Stat t = i == at ? first : s[i];
       const float m = fmaxf(one.max, t.max);
       if (m == -INFINITY) continue;
       one = one.max == -INFINITY ? t : Stat{one.sum * exp((double)one.max - (double)m) + t.sum * exp((double)t.max - (double)m), m, 0};
@@ -247,6 +253,9 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
       lse[b] = (double)top + log(sum);
     }
   }
+  const bool mine = in && finite(score), over = mine && done;
+  if (ROW && (!finite(score) || done)) return;
+  const double start = ROW ? 0.0 : (double)score;
   if (tid == 0) bound = none, n_cand = 0, least = -INFINITY;
   for (int i = tid; i < kMergeCap; i += kMergeThreads) place[i] = 0;
   __syncthreads();
@@ -326,7 +335,18 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
     const int i = at / parts;
     const Entry e = list[i];
     int before = 0;
-    for (int j = at % parts; j < n; j += parts) before += ahead(list[j], e);
+    auto count = [&](int j, double s) {  // of one beam's, the scores have the logits' order
+      if (s > e.score || (s == e.score && ahead(list[j], e))) ++before;
+    };
+    int j = at % parts;
+    for (; j + 3 * parts < n; j += 4 * parts) {
+      double s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] = list[j + u * parts].score;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) count(j + u * parts, s[u]);
+    }
+    for (; j < n; j += parts) count(j, list[j].score);
     if (before) atomicAdd(&place[i], before);
   }
   __syncthreads();
