@@ -53,6 +53,7 @@ __host__ __device__ inline Shape shape_of(int H, int KV, int R, int max_run) {
 // A block of rows of one KV head, and how many keys its tokens see at most.
 struct Block {
   int t0, m, keys;  // tokens t0 .. t0 + m - 1
+  int seq, mine;    // their sequence; keys of token t0 + lane, lane < m
   int g, h0, per;   // KV head, first query head, heads per token
   __device__ __forceinline__ int rows() const { return m * per; }
   __device__ __forceinline__ int token(int r) const { return t0 + r / per; }
@@ -65,9 +66,13 @@ __device__ __forceinline__ void set_heads(Block& b, const Shape& S, int j) {
   b.g = j / S.hs, b.h0 = b.g * S.G + R * sub, b.per = min(S.G - R * sub, R);
 }
 
+// Both loads go at once.
+__device__ __forceinline__ int keys_of(const Kv4Attn& A, int s, int k) {
+  return s >= 0 && s < A.kv.n_seq ? max(0, min(k, A.max_keys)) : 0;
+}
 __device__ __forceinline__ int keys_of(const Kv4Attn& A, int t) {
-  const int s = A.seq[t];
-  return s >= 0 && s < A.kv.n_seq ? max(0, min(A.n_keys[t], A.max_keys)) : 0;
+  const int s = A.seq[t], k = A.n_keys[t];
+  return keys_of(A, s, k);
 }
 __device__ __forceinline__ bool starts(const Kv4Attn& A, int t) { return t == 0 || A.seq[t] != A.seq[t - 1]; }
 // The first token of the run of its sequence's that t is in, found by a wave.
@@ -81,10 +86,11 @@ __device__ __forceinline__ int run_start(const Kv4Attn& A, int t) {
 // The block that token t leads: it and the tokens of its sequence that follow, tq at most, found by a wave.
 __device__ __forceinline__ void set_tokens(Block& b, const Kv4Attn& A, int t, int tq) {
   const int lane = threadIdx.x & 63, i = min(t + lane, A.n - 1);
-  const int s = A.seq[i];
-  const uint64_t same = __ballot(lane < tq && t + lane < A.n && s == __builtin_amdgcn_readfirstlane(s));
+  const int s = A.seq[i], k = A.n_keys[i];
+  b.seq = __builtin_amdgcn_readfirstlane(s);
+  const uint64_t same = __ballot(lane < tq && t + lane < A.n && s == b.seq);
   b.t0 = t, b.m = __builtin_ctzll(~same);
-  int keys = lane < b.m ? keys_of(A, i) : 0;
+  int keys = b.mine = lane < b.m ? keys_of(A, s, k) : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) keys = max(keys, __shfl_xor(keys, o));
   b.keys = __builtin_amdgcn_readfirstlane(keys);
@@ -427,7 +433,7 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
                                           uint8_t* smem, Shared<NR, NW>& sh, Put put) {
   using G_ = Geo<D, NR, NW>;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int end = min(b.keys, tb * kTile), seq = A.seq[b.t0];
+  const int end = min(b.keys, tb * kTile), seq = b.seq;
   Walk<D, NR, NW> walk(A, smem, w);
   const int li = walk.li, qd = walk.qd, lane = walk.lane;
   // q: waves take (step, set) pairs in turn; a row's largest value is the waves' together.
@@ -448,7 +454,7 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
   walk.least = INT32_MAX;
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    walk.lim[n] = keys_of(A, b.token(min(n * kSet + li, b.rows() - 1)));
+    walk.lim[n] = __shfl(b.mine, min(n * kSet + li, b.rows() - 1) / b.per);
     walk.least = min(walk.least, walk.lim[n]);
   }
 #pragma unroll
@@ -655,9 +661,8 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
   auto look = [&](int c0) {
     __syncthreads();
     for (int i = tid; i < 256 + R; i += 256) {
-      const int t = c0 + i;
-      tok_seq[i] = t < A.n ? A.seq[t] : 0;
-      tok_keys[i] = t < A.n ? keys_of(A, t) : 0;
+      const int t = c0 + i, s = A.seq[min(t, A.n - 1)], k = A.n_keys[min(t, A.n - 1)];
+      tok_seq[i] = s, tok_keys[i] = t < A.n ? keys_of(A, s, k) : 0;
     }
     const bool first = tid == 0 ? starts(A, min(c0, A.n - 1)) : false;
     __syncthreads();
@@ -688,28 +693,29 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
     if (a < total * S.J) break;
   }
   __syncthreads();
+  // Blocks follow each other by (token, j); tile a is tile k0 of block j of those that token t leads.
   int t = start_t;
-  int64_t off = start_off;  // of token t's blocks
   Block blk;
   set_tokens(blk, A, t, S.tq);
+  int j = (int)((a - start_off) / blk.tiles()), k0 = (int)((a - start_off) % blk.tiles());
   for (int64_t at = a; at < b;) {
     const int tiles = blk.tiles();
-    if (at >= off + (int64_t)tiles * S.J) {  // the next tokens'
-      off += (int64_t)tiles * S.J;
-      t += blk.m;
+    if (j == S.J || tiles == 0) {  // the next tokens'
+      t += blk.m, j = 0;
       set_tokens(blk, A, t, S.tq);
       continue;
     }
-    const int j = (int)((at - off) / tiles), k0 = (int)((at - off) % tiles), k1 = (int)min<int64_t>(tiles, k0 + (b - at));
+    const int k1 = (int)min<int64_t>(tiles, k0 + (b - at));
     set_heads<R>(blk, S, j);
-    const int64_t block_off = at - k0;
-    const int first = (int)(block_off / share), end = (int)((block_off + tiles - 1) / share);
-    if (k0 == 0)
-      for (int i = tid; i < blk.m; i += kShare * 64)
-        P.rec[(int64_t)(t + i) * S.J + j] = Record{first, first == end ? -1 : end, i * blk.per};
-    const int64_t slot = 2 * (int64_t)w + (k0 == 0);
+    // A block that begins here and ends before the next workgroup's run is written whole.
+    const bool begins = k0 == 0, whole = begins && at + tiles <= a + share;
+    if (begins) {
+      const int end = whole ? -1 : (int)((at + tiles - 1) / share);
+      for (int i = tid; i < blk.m; i += kShare * 64) P.rec[(int64_t)(t + i) * S.J + j] = Record{w, end, i * blk.per};
+    }
+    const int64_t slot = 2 * (int64_t)w + begins;
     run_block<D, NR, kShare>(A, blk, k0, k1, q, q_stride, smem, sh, [&](int r, int d, v4f v, float l, float m) {
-      if (first == end) {
+      if (whole) {
         put_row<D>(A, O, blk.token(r), blk.head(r), d, v, l);
       } else {
         *reinterpret_cast<v4f*>(P.o + (slot * R + r) * D + d) = v;
@@ -717,6 +723,7 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
       }
     });
     at += k1 - k0;
+    ++j, k0 = 0;
   }
 }
 
