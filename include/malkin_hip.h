@@ -319,7 +319,7 @@ int mk_rope_kv4(mk_ctx* ctx, const float* q, const float* k, const float* v, int
 int mk_kv4_rows(mk_ctx* ctx, const mk_kv4_cache* kv, int layer, const int32_t* seq, const int32_t* row, int n, void* k_out,
                 void* v_out);
 /* mk_attention for plain tokens over the 4-bit cache: token t attends with its n_head query heads to positions
-   0..n_keys[t]-1 of sequence seq[t]; fp32 sums. max_keys (at most 2^28) bounds n_keys[t]: keys past it are not read. max_run
+   0..n_keys[t]-1 of sequence seq[t]; fp32 sums. max_keys (at most 2^26) bounds n_keys[t]: keys past it are not read. max_run
    is the number of tokens of one sequence that follow each other at most (1: decoding), a hint that changes no result beyond rounding. A
    token with n_keys[t] <= 0 or seq[t] outside the cache gets zeros, and keys whose page is not in the pool have no weight.
    Tokens may come in any order; those of one sequence that follow each other read its rows together. xq: the BlockQ8 rows of

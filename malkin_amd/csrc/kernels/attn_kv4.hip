@@ -55,15 +55,18 @@ struct Block {
   int t0, m, keys;  // tokens t0 .. t0 + m - 1
   int seq, mine;    // their sequence; keys of token t0 + lane, lane < m
   int g, h0, per;   // KV head, first query head, heads per token
+  int inv;          // 2^16 / per, rounded up
   __device__ __forceinline__ int rows() const { return m * per; }
-  __device__ __forceinline__ int token(int r) const { return t0 + r / per; }
-  __device__ __forceinline__ int head(int r) const { return h0 + r % per; }
+  __device__ __forceinline__ int turn(int r) const { return r * inv >> 16; }  // r / per, for r < 2^8
+  __device__ __forceinline__ int token(int r) const { return t0 + turn(r); }
+  __device__ __forceinline__ int head(int r) const { return h0 + r - turn(r) * per; }
   __device__ __forceinline__ int tiles() const { return (keys + kTile - 1) / kTile; }
 };
 template <int R>
 __device__ __forceinline__ void set_heads(Block& b, const Shape& S, int j) {
   const int sub = j % S.hs;
   b.g = j / S.hs, b.h0 = b.g * S.G + R * sub, b.per = min(S.G - R * sub, R);
+  b.inv = (65535 + b.per) / b.per;
 }
 
 // Both loads go at once.
@@ -454,7 +457,7 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
   walk.least = INT32_MAX;
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    walk.lim[n] = __shfl(b.mine, min(n * kSet + li, b.rows() - 1) / b.per);
+    walk.lim[n] = __shfl(b.mine, b.turn(min(n * kSet + li, b.rows() - 1)));
     walk.least = min(walk.least, walk.lim[n]);
   }
 #pragma unroll
@@ -557,6 +560,7 @@ __device__ __forceinline__ void run_block(const Kv4Attn& A, const Block& b, int 
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<v4f*>(ob + (w * G_::kR + n * kSet + li) * G_::kStride + 16 * i + 4 * qd) = acc.o[n][d0 / 16 + i];
     __syncthreads();
+#pragma unroll 1
     for (int r = tid >> 4; r < b.rows(); r += NW * 4) {
       float f[NW], top = kNone, sum = 0.0f;
 #pragma unroll
@@ -582,8 +586,8 @@ struct Out {
 };
 template <int D>
 __device__ __forceinline__ void put_row(const Kv4Attn& A, const Out& O, int t, int head, int d, v4f a, float l) {
-  const float n = l == 0.0f ? 1.0f : l;  // no key: zeros
-  const float y[4] = {a[0] / n, a[1] / n, a[2] / n, a[3] / n};
+  const float n = l == 0.0f ? 1.0f : 1.0f / l;  // no key: zeros
+  const float y[4] = {a[0] * n, a[1] * n, a[2] * n, a[3] * n};
   *reinterpret_cast<v4a*>(O.out + t * O.stride + (int64_t)head * D + d) = v4a{y[0], y[1], y[2], y[3]};
   if (O.xq) quantize_block_lanes_n<4>(y, (d & 31) / 4, O.xq + (((int64_t)t * A.H + head) * D + d) / 32);
 }
@@ -646,49 +650,70 @@ __device__ __forceinline__ T scan256(T v, T* part, T& total) {
   return before;
 }
 
+// Tokens that a thread looks at together: prompts have many.
+template <int NR>
+constexpr int kTokens = NR == 1 ? 1 : 4;
+
 template <int D, int NR>
 __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4Attn A, const float* __restrict__ q, int64_t q_stride,
                                                                             Out O, Parts P) {
-  constexpr int R = NR * kSet;
+  constexpr int R = NR * kSet, kTok = kTokens<NR>, kOnce = 256 * kTok;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) Shared<NR, kShare> sh;
-  __shared__ int tok_seq[256 + R], tok_keys[256 + R], part[4], start_t;
+  __shared__ int part[4], start_t;
   __shared__ int64_t start_off;
   const int tid = threadIdx.x, w = blockIdx.x;
   const Shape S = shape_of(A.H, A.kv.KV, R, A.max_run);
-  // Tokens 256 at a time, a thread each: the tiles of the block that it leads, if any, and the running sum of them.
-  int run = 0, tiles = 0, before = 0, all = 0;
+  // kOnce tokens at a time, kTok to a thread: the tiles of the blocks that they lead, and the running sum of those.
+  static_assert(2 * 4 * (kOnce + R) <= Geo<D, NR, kShare>::kLds);
+  int *tok_seq = reinterpret_cast<int*>(smem), *tok_keys = tok_seq + kOnce + R;
+  int run = 0, tiles[kTok], before = 0, all = 0;
   auto look = [&](int c0) {
+    const int prior = A.seq[max(c0 - 1, 0)];
     __syncthreads();
-    for (int i = tid; i < 256 + R; i += 256) {
+#pragma unroll
+    for (int i = tid; i < kOnce + R; i += 256) {
       const int t = c0 + i, s = A.seq[min(t, A.n - 1)], k = A.n_keys[min(t, A.n - 1)];
       tok_seq[i] = s, tok_keys[i] = t < A.n ? keys_of(A, s, k) : 0;
     }
-    const bool first = tid == 0 ? starts(A, min(c0, A.n - 1)) : false;
     __syncthreads();
-    const int t = c0 + tid;
-    int from = t < A.n && (tid ? tok_seq[tid] != tok_seq[tid - 1] : first) ? t : -1, last;
-    from = max(from, scan256<true>(from, part, last));  // the run's first token; of an earlier 256: none
+    auto begins = [&](int i) { return c0 + i == 0 || (c0 + i < A.n && tok_seq[i] != (i ? tok_seq[i - 1] : prior)); };
+    int from = -1, last;
+#pragma unroll
+    for (int e = 0; e < kTok; ++e)
+      if (begins(kTok * tid + e)) from = c0 + kTok * tid + e;
+    from = scan256<true>(from, part, last);  // the last run's first token before this thread's; of an earlier kOnce: none
     if (from < 0) from = run;
-    tiles = 0;
-    if (t < A.n && (t - from) % S.tq == 0) {
-      int keys = tok_keys[tid];
-      for (int m = 1; m < S.tq && t + m < A.n && tok_seq[tid + m] == tok_seq[tid]; ++m) keys = max(keys, tok_keys[tid + m]);
-      tiles = (keys + kTile - 1) / kTile;
+    int sum = 0;
+#pragma unroll
+    for (int e = 0; e < kTok; ++e) {
+      const int i = kTok * tid + e, t = c0 + i;
+      if (begins(i)) from = t;
+      tiles[e] = 0;
+      if (t < A.n && (t - from) % S.tq == 0) {
+        int keys = tok_keys[i];
+        for (int m = 1; m < S.tq && t + m < A.n && tok_seq[i + m] == tok_seq[i]; ++m) keys = max(keys, tok_keys[i + m]);
+        tiles[e] = (keys + kTile - 1) / kTile;
+      }
+      sum += tiles[e];
     }
-    before = scan256<false>(tiles, part, all);
+    before = scan256<false>(sum, part, all);
     if (last >= 0) run = last;
   };
   int64_t total = 0;
-  for (int c0 = 0; c0 < A.n; c0 += 256) look(c0), total += all;
+  for (int c0 = 0; c0 < A.n; c0 += kOnce) look(c0), total += all;
   const int64_t share = max<int64_t>((total * S.J + gridDim.x - 1) / gridDim.x, kLeast), a = w * share, b = min(a + share, total * S.J);
   if (a >= b) return;
   // The block that holds tile a is one of exactly one thread's.
   run = 0, total = 0;
-  for (int c0 = 0;; c0 += 256) {
-    if (A.n > 256) look(c0);
-    const int64_t off = (total + before) * S.J;
-    if (off <= a && a < off + (int64_t)tiles * S.J) start_t = c0 + tid, start_off = off;
+  for (int c0 = 0;; c0 += kOnce) {
+    if (A.n > kOnce) look(c0);
+    int64_t off = (total + before) * S.J;
+#pragma unroll
+    for (int e = 0; e < kTok; ++e) {
+      if (off <= a && a < off + (int64_t)tiles[e] * S.J) start_t = c0 + kTok * tid + e, start_off = off;
+      off += (int64_t)tiles[e] * S.J;
+    }
     total += all;
     if (a < total * S.J) break;
   }

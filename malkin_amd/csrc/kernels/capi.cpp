@@ -673,7 +673,7 @@ int mk_attention_kv4(mk_ctx* c, const float* q, int64_t q_stride, float* out, in
     require(q_stride >= (int64_t)n_head * D && out_stride >= (int64_t)n_head * D,
             "mk_attention_kv4: stride shorter than a row");
     require((int64_t)n * n_head < (1 << 24), "mk_attention_kv4: too many rows");
-    require(max_keys <= 1 << 28, "mk_attention_kv4: max_keys past 2^28");  // 256 tokens' tiles are added up in 32 bits
+    require(max_keys <= 1 << 26, "mk_attention_kv4: max_keys past 2^26");  // 1024 tokens' tiles are added up in 32 bits
     require(max_keys <= (int64_t)kv->max_pages * kv->page, "mk_attention_kv4: max_keys past the sequences' pages");
     const mk::Kv4Attn A{K, n, n_head, max_keys, max_run, 1.0f / std::sqrt(static_cast<float>(D)), seq, n_keys};
     require(holds(workspace, workspace_bytes, mk::attention_kv4_need(A, D)),

@@ -246,6 +246,6 @@ def test_plain_forms_agree():
 
 def test_keys_that_are_counted_in_32_bits():
     big = cache(max_pages=1 << 25)
-    refused(attention(kv=big, most=(1 << 28) + 1), mk_.MK_ERR_INVALID, "max_keys past 2^28")
-    refused(attention(kv=big, most=1 << 28), mk_.MK_ERR_INVALID, "null context")
+    refused(attention(kv=big, most=(1 << 26) + 1), mk_.MK_ERR_INVALID, "max_keys past 2^26")
+    refused(attention(kv=big, most=1 << 26), mk_.MK_ERR_INVALID, "null context")
     refused(attention(kv=cache(n_page=(1 << 27) - 1)), mk_.MK_ERR_INVALID, "null context")
