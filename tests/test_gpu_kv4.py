@@ -278,6 +278,8 @@ CASES = [
     (8, 8, 64, 32, [770], [1500]),
     (8, 2, 128, 64, [5] * 10, [300 + 131 * i for i in range(10)]),
     (16, 8, 128, 256, [1], [20000]),
+    (2, 2, 64, 16, [1] * 300, [1 + i % 37 for i in range(299)] + [2100]),
+    (4, 2, 64, 32, [600, 500, 100], [610, 500, 1100]),
 ]
 
 
