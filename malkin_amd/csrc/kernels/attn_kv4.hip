@@ -664,15 +664,16 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
   __shared__ int64_t start_off;
   const int tid = threadIdx.x, w = blockIdx.x;
   const Shape S = shape_of(A.H, A.kv.KV, R, A.max_run);
-  // kOnce tokens at a time, kTok to a thread: the tiles of the blocks that they lead, and the running sum of those.
+  // kOnce tokens at a time, kTok to a thread (one, where there are few): the tiles of the blocks that they lead, and the running
+  // sum of those.
   static_assert(2 * 4 * (kOnce + R) <= Geo<D, NR, kShare>::kLds);
   int *tok_seq = reinterpret_cast<int*>(smem), *tok_keys = tok_seq + kOnce + R;
+  const int per = A.n > 256 ? kTok : 1;
   int run = 0, tiles[kTok], before = 0, all = 0;
   auto look = [&](int c0) {
     const int prior = A.seq[max(c0 - 1, 0)];
     __syncthreads();
-#pragma unroll
-    for (int i = tid; i < kOnce + R; i += 256) {
+    for (int i = tid; i < 256 * per + R; i += 256) {
       const int t = c0 + i, s = A.seq[min(t, A.n - 1)], k = A.n_keys[min(t, A.n - 1)];
       tok_seq[i] = s, tok_keys[i] = t < A.n ? keys_of(A, s, k) : 0;
     }
@@ -681,15 +682,16 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
     int from = -1, last;
 #pragma unroll
     for (int e = 0; e < kTok; ++e)
-      if (begins(kTok * tid + e)) from = c0 + kTok * tid + e;
+      if (e < per && begins(per * tid + e)) from = c0 + per * tid + e;
     from = scan256<true>(from, part, last);  // the last run's first token before this thread's; of an earlier kOnce: none
     if (from < 0) from = run;
     int sum = 0;
 #pragma unroll
     for (int e = 0; e < kTok; ++e) {
-      const int i = kTok * tid + e, t = c0 + i;
-      if (begins(i)) from = t;
+      const int i = per * tid + e, t = c0 + i;
       tiles[e] = 0;
+      if (e >= per) continue;
+      if (begins(i)) from = t;
       if (t < A.n && (t - from) % S.tq == 0) {
         int keys = tok_keys[i];
         for (int m = 1; m < S.tq && t + m < A.n && tok_seq[i + m] == tok_seq[i]; ++m) keys = max(keys, tok_keys[i + m]);
@@ -702,7 +704,9 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
   };
   int64_t total = 0;
   for (int c0 = 0; c0 < A.n; c0 += kOnce) look(c0), total += all;
-  const int64_t share = max<int64_t>((total * S.J + gridDim.x - 1) / gridDim.x, kLeast), a = w * share, b = min(a + share, total * S.J);
+  // No share is smaller than kLeast tiles, or than a block where those are small on average.
+  const int least = (int)max<int64_t>(1, min<int64_t>(total * S.tq / A.n, kLeast));
+  const int64_t share = max<int64_t>((total * S.J + gridDim.x - 1) / gridDim.x, least), a = w * share, b = min(a + share, total * S.J);
   if (a >= b) return;
   // The block that holds tile a is one of exactly one thread's.
   run = 0, total = 0;
@@ -711,7 +715,7 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
     int64_t off = (total + before) * S.J;
 #pragma unroll
     for (int e = 0; e < kTok; ++e) {
-      if (off <= a && a < off + (int64_t)tiles[e] * S.J) start_t = c0 + kTok * tid + e, start_off = off;
+      if (off <= a && a < off + (int64_t)tiles[e] * S.J) start_t = c0 + per * tid + e, start_off = off;
       off += (int64_t)tiles[e] * S.J;
     }
     total += all;
