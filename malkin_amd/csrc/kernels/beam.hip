@@ -3,12 +3,13 @@
 // A row's order does not need its sum: k_beam_rows reads the logits once, in segments, and leaves each segment's k best,
 // sorted, with its maximum and the sum of exp(z - max) in 64 bits (candidates of two beams are often nearer to each other
 // than a 32-bit sum is exact). k_beam_merge adds a row's sums and merges the sorted lists of a group. Neither sorts: a lower
-// bound of the k-th best thins the candidates out, first in a segment (the k-th best of the maxima of 64 or 256 parts of it),
+// bound of the k-th best thins the candidates out, first in a segment (the k-th best of the maxima of 64 to 256 parts of it),
 // then over the lists (the r-th best of their p-th elements, where (p + 1) r >= k), and what is left finds its place by
 // counting what is better.
 //
-// What bounds it: the logits' bytes, beside about 25 vector instructions a logit (12 of them 64-bit); for one request the
-// latency of two launches and of the merge's chain.
+// What bounds it: for one request of four beams (13 us) the latency of two launches (5.8 and 7.1 us) and of their chains of loads,
+// barriers and 64-bit exponentials; for 24 of them (58 MB of logits, 22 us) the reading of the logits (16.3 us, 3.6 TB/s), with
+// about 20 vector instructions for each, half of them for its exponential.
 #include <algorithm>
 #include <cfloat>
 
@@ -42,7 +43,7 @@ struct Beams {
   int64_t stride;
   const float* scores;
   const int32_t* done;
-  int n_vocab, segs, k, beams, eos;
+  int n_vocab, segs, len, k, beams, eos;  // len: logits of a segment
 };
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
@@ -58,12 +59,12 @@ __device__ __forceinline__ float of_key(uint32_t key) { return __uint_as_float(k
 // A candidate as one number: of two, the larger one is ahead.
 __device__ __forceinline__ uint64_t rank_key(float z, int id) { return (uint64_t)order_key(z) << 32 | (uint32_t)~id; }
 
-// One segment of kThreads * 4 Q logits of a row. The k-th largest of the maxima of PARTS parts of it is a bound (k <= MOST <=
+// One segment of a row, at most kThreads * 4 Q logits. The k-th largest of the maxima of PARTS parts of it is a bound (k <= MOST <=
 // PARTS): at most (k - 1) parts hold anything larger. Of logits that are equal to it there can be any number; where the list
 // does not hold them, those of the first whole rounds of 4 kThreads logits are taken that have enough.
 template <int Q, int PARTS, int MOST>
 __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restrict__ stats, Cand* __restrict__ cands) {
-  constexpr int kRound = 4 * kThreads, kSeg = Q * kRound, SHARE = kThreads / PARTS, CAP = (MOST - 1) * SHARE * 4 * Q + MOST + kRound;
+  constexpr int kRound = 4 * kThreads, SHARE = kThreads / PARTS, CAP = (MOST - 1) * SHARE * 4 * Q + MOST + kRound;
   __shared__ double table[kTable];
   __shared__ __align__(16) float part_v[PARTS];
   __shared__ float wave_max[kThreads / 64];
@@ -73,25 +74,22 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restric
   __shared__ uint64_t list[CAP];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x / B.segs, seg = blockIdx.x % B.segs;
   const float* l = B.logits + row * B.stride;
-  const int first = seg * kSeg;
+  const int first = seg * B.len, end = min(first + B.len, B.n_vocab);
   const float start = B.scores[row];
   const int over = B.done ? B.done[row] : 0;
   if (!finite(start) || over) return;  // nobody reads what would be written
   float z[4 * Q];
-  if (first + kSeg <= B.n_vocab) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const v4f f = *reinterpret_cast<const v4a*>(l + first + q * kRound + 4 * tid);
+  for (int q = 0; q < Q; ++q) {
+    const int at = first + q * kRound + 4 * tid;
+    v4f f = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (at + 4 <= end) f = *reinterpret_cast<const v4a*>(l + at);
+    else
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[4 * q + e] = f[e];
-    }
-  } else {
+      for (int e = 0; e < 3; ++e)
+        if (at + e < end) f[e] = l[at + e];
 #pragma unroll
-    for (int e = 0; e < 4 * Q; ++e) {
-      const int at = first + e / 4 * kRound + 4 * tid + e % 4;
-      z[e] = l[min(at, B.n_vocab - 1)];
-      if (at >= B.n_vocab) z[e] = -INFINITY;
-    }
+    for (int e = 0; e < 4; ++e) z[4 * q + e] = f[e];
   }
   load_table(table);
   auto id_of = [&](int e) { return first + e / 4 * kRound + 4 * tid + e % 4; };
@@ -175,7 +173,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_rows(Beams B, Stat* __restric
   for (int i = tid >> 2; i < n; i += kThreads / 4) {
     const uint64_t c = list[i];
     int before = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int j = tid & 3; j < n; j += 4) before += list[j] > c;
     before += __shfl_xor(before, 1);
     before += __shfl_xor(before, 2);
@@ -205,7 +203,7 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
                                                               const Cand* __restrict__ cands, Stat* __restrict__ row_stat,
                                                               Cand* __restrict__ row_cand, float* __restrict__ out_scores,
                                                               int32_t* __restrict__ out_seq, int32_t* __restrict__ out_tokens) {
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 4, kNext = 8;
   __shared__ double lse[64];
   __shared__ Entry list[kMergeCap], bound;
   __shared__ __align__(16) float heads[kMaxLists];
@@ -295,10 +293,16 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
       go = go && e.beam != INT32_MAX && (float)e.score >= least;
       if (go) put(e);
     }
-    for (int j = kAhead; go && j < k; ++j) {
-      const Entry e = entry(j, from[j]);
-      go = e.beam != INT32_MAX && (float)e.score >= least;
-      if (go) put(e);
+    for (int j0 = kAhead; go && j0 < k; j0 += kNext) {  // a good beam's list has many: asked for together
+      Cand more[kNext];
+#pragma unroll
+      for (int j = 0; j < kNext; ++j) more[j] = from[min(j0 + j, k - 1)];
+#pragma unroll
+      for (int j = 0; j < kNext; ++j) {
+        const Entry e = entry(j0 + j, more[j]);
+        go = go && e.beam != INT32_MAX && (float)e.score >= least;
+        if (go) put(e);
+      }
     }
   }
   __syncthreads();
@@ -365,7 +369,8 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
 
 constexpr int kSmallSeg = kThreads * 4 * 4, kLargeSeg = kThreads * 4 * 8;
 
-// Longer segments where there are many rows and few candidates of each.
+// Longer segments where there are many rows and few candidates of each: 96 rows of 151936 logits, k 4, 23.5 us with long ones
+// and 24.5 with short ones, k 16 25.1 and 26.5; 4 rows 13.7 and 13.1, 56 rows 20.8 and 20.3.
 int seg_of(int rows, int n_vocab, int k) {
   return k <= 16 && (int64_t)rows * n_vocab > (int64_t)kLargeSeg * 1024 ? kLargeSeg : kSmallSeg;
 }
@@ -381,7 +386,10 @@ void beam_select(hipStream_t s, const float* logits, int64_t stride, int n_group
                  const int32_t* done, int eos, int k, float* out_scores, int32_t* out_seq, int32_t* out_tokens,
                  void* workspace) {
   const int rows = n_group * beams, seg = seg_of(rows, n_vocab, k), segs = (n_vocab + seg - 1) / seg;
-  Beams B{logits, stride, scores, done, n_vocab, segs, k, beams, eos};
+  // Segments of one length: a short one at the end would have fewer parts than k, and rank all that it has (32 rows of 151936
+  // logits, k 64: 25 us instead of 16).
+  const int len = (n_vocab + segs - 1) / segs, whole = (len + 3) / 4 * 4;
+  Beams B{logits, stride, scores, done, n_vocab, segs, whole, k, beams, eos};
   Stat* stats = static_cast<Stat*>(workspace);
   Stat* row_stat = stats + (int64_t)rows * segs;
   Cand* cands = reinterpret_cast<Cand*>(row_stat + rows);
@@ -391,6 +399,8 @@ void beam_select(hipStream_t s, const float* logits, int64_t stride, int n_group
     check_launch("beam_select rows");
   };
   const bool large = seg == kLargeSeg;
+  // As many parts as k needs: a thread compares its own with all others. 160 rows of 32003 logits, k 64: 26 us with 128, 29.6
+  // with 256; 32 rows of 151936, k 16: 18.2 with 64, 19.1 with 128.
   if (k <= 16) large ? go.template operator()<8, 64, 16>() : go.template operator()<4, 64, 16>();
   else if (k <= 64) go.template operator()<4, 128, 64>();
   else go.template operator()<4, 256, 128>();
