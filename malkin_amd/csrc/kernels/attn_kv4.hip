@@ -17,6 +17,14 @@
 // in the order that its numbers come out of a word, are the order in which q's elements are multiplied; the same goes for the
 // keys of V. Each wave takes every NW-th tile through a K and a V buffer of its own, which direct copies fill: a buffer's next
 // tile is asked for as soon as this one is in registers, and the waves meet only to add their results.
+//
+// What bounds it: the vector instructions that turn 4 bits into fp16 factors, 13 for eight values and as many for K as for V,
+// which is 416 of a tile's 560 to 700 (16 or 32 rows); two or three waves a SIMD cover them with matrix instructions in part.
+// Long documents of four users (4 x 5 drafted tokens) take 125 us, 3.0 TB/s of the cache's bytes, where the copies alone take
+// 63; 24 users of up to 6000 keys 40 us, of which 12 are spent before the first and after the last tile and 4 on joining; 512
+// tokens of three prompts 78 us, 21 of them for setting up and ending each workgroup's two or three blocks and 10 on joining.
+// Blocks of 128 rows, whose four waves take a tile's numbers out of 4 bits once for all of them, took 78 us there, but 69 for a
+// prompt of 300 tokens by itself, which takes 31 here, so that form is not kept.
 #include <algorithm>
 
 #include "ctx.h"
@@ -610,7 +618,8 @@ __global__ __launch_bounds__(NW * 64) void k_kv4_whole(Kv4Attn A, const float* _
 // ---- even shares of all tiles ----
 
 constexpr int kShare = 4;  // waves of a workgroup that takes a share
-constexpr int kLeast = 4;  // tiles of a share
+// Tiles of a share. One user, 8000 keys: 18.5 us, with 2 23, with 8 20.2; 4 x 5 drafts, 3000 keys: 26.7, 29.4 and 28.7.
+constexpr int kLeast = 4;
 
 // Per (token, j): the workgroups whose runs hold its block, first (where it begins) and last (-1: written whole), and the row
 // that the token's first head has in it.
@@ -650,7 +659,8 @@ __device__ __forceinline__ T scan256(T v, T* part, T& total) {
   return before;
 }
 
-// Tokens that a thread looks at together: prompts have many.
+// Tokens that a thread looks at together where there are more than 256 (a 512-token prompt, 2600 keys: 72 us, one at a time 76;
+// 120 drafted tokens: 46, four at a time 49).
 template <int NR>
 constexpr int kTokens = NR == 1 ? 1 : 4;
 
@@ -704,7 +714,8 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
   };
   int64_t total = 0;
   for (int c0 = 0; c0 < A.n; c0 += kOnce) look(c0), total += all;
-  // No share is smaller than kLeast tiles, or than a block where those are small on average.
+  // No share is smaller than kLeast tiles, or than a block where those are small on average (a prompt of 300 tokens: 31 us, with
+  // kLeast 44: two blocks a workgroup instead of one).
   const int least = (int)max<int64_t>(1, min<int64_t>(total * S.tq / A.n, kLeast));
   const int64_t share = max<int64_t>((total * S.J + gridDim.x - 1) / gridDim.x, least), a = w * share, b = min(a + share, total * S.J);
   if (a >= b) return;
@@ -836,8 +847,14 @@ struct Cut {
   int wgs;    // workgroups that share all tiles; 0: one per block
   int waves;  // of a workgroup that has a block to itself
 };
+// A workgroup of eight waves per block up to kWholeKeys keys, with kMany blocks one of four waves up to kWholeKeysMany. 8 heads
+// for K and V, 32 for q: 8 users, 1000 keys 12.5 us, in shares 19.1 (four waves 14.6); one user, 2000 keys 18.9, in shares 13.7; 64
+// users, 1000 keys 22.2, in shares 34 (eight waves 25.8), 2000 keys 34 and 42, 3000 keys 46 and 51, but there one long sequence
+// among short ones would be one workgroup's alone.
 constexpr int kWholeKeys = 1024, kWholeKeysMany = 2048, kMany = 512;
-constexpr int kJoinRows = 2048;  // up to so many rows are joined by four waves each
+// Up to so many rows are joined by four waves each: 4 x 5 drafts over 120000 keys 6 us, by one 13; 16384 rows of a prompt 10,
+// by four 24.
+constexpr int kJoinRows = 2048;
 
 Cut cut_of(int n, int H, int KV, int max_keys, int max_run) {
   const int64_t rows = std::min<int64_t>(std::max(max_run, 1), n) * (H / KV);

@@ -8,8 +8,8 @@
 // counting what is better.
 //
 // What bounds it: for one request of four beams (13 us) the latency of two launches (5.8 and 7.1 us) and of their chains of loads,
-// barriers and 64-bit exponentials; for 24 of them (58 MB of logits, 22 us) the reading of the logits (16.3 us, 3.6 TB/s), with
-// about 20 vector instructions for each, half of them for its exponential.
+// barriers and 64-bit exponentials; for 24 of them (22 us; about 42 MB of logits, those of ended beams are not read) the first
+// launch, 16.3 us or 2.6 TB/s, with about 20 vector instructions a logit, half of them for its exponential.
 #include <algorithm>
 #include <cfloat>
 
