@@ -190,15 +190,21 @@ __global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t*
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, in_page = (1 << P.shift) - 1;
   const int E = (n + kPlan - 1) / kPlan, i0 = tid * E;  // a thread's entries follow each other
   const int64_t room = (int64_t)P.max_pages << P.shift;
-  for (int i = tid; i < n; i += kPlan) seq_s[i] = seq ? seq[i] : i, new_s[i] = new_len[i];
-  if (seq) __syncthreads();  // else each thread looks at its own
+  if (seq) {
+    for (int i = tid; i < n; i += kPlan) seq_s[i] = seq[i];
+    __syncthreads();
+  }
   bool shrinks = false;
   for (int i = tid; i < n; i += kPlan) {
-    const int s = seq_s[i], L = new_s[i];
+    const int s = seq ? seq_s[i] : i, now = held(P, min(max(s, 0), P.n_seq - 1)), L = new_len[i];  // both loads at once
     bool ok = s >= 0 && s < P.n_seq && L >= 0 && L <= room;
-    if (seq)
+    if (seq) {
       for (int j = i + 1; j < n && ok; ++j) ok = seq_s[j] != s;
-    const int len = ok ? held(P, s) : 0;
+    } else {
+      seq_s[i] = i;
+    }
+    new_s[i] = L;
+    const int len = ok ? now : 0;
     const int kind = !ok ? kSkip : L > len ? kGrow : kShrink;
     int last = -1;
     if (kind == kGrow && len & in_page) {
