@@ -77,13 +77,16 @@ __global__ __launch_bounds__(kThreads) void k_rope_tables(Turns T, int half, con
 // ---- norm, rotation, 4-bit rows ----
 
 // The scale of a group whose extremes are hi and lo (include/malkin_hip.h): m / -8 to 8 significant bits, then to fp16.
-__device__ __forceinline__ _Float16 scale_of(float hi, float lo) {
-  const float m = hi >= -lo ? hi : lo;
-  const float s = fminf(fmaxf(m * -0.125f, -4096.0f), 4096.0f);
-  uint32_t u = __builtin_bit_cast(uint32_t, s);
-  u = (u + 0x7FFFu + (u >> 16 & 1)) & 0xFFFF0000u;  // to nearest, ties to even
-  return (_Float16)__builtin_bit_cast(float, u);
+__device__ __forceinline__ _Float16 scale_of(double hi, double lo) {
+  const double m = hi >= -lo ? hi : lo;
+  const double s = fmin(fmax(m * -0.125, -4096.0), 4096.0);
+  uint64_t u = __builtin_bit_cast(uint64_t, s);
+  u = (u + ((1ull << 44) - 1) + (u >> 45 & 1)) & ~((1ull << 45) - 1);  // to nearest, ties to even
+  return (_Float16)(float)__builtin_bit_cast(double, u);
 }
+
+__device__ __forceinline__ double fma_(double a, double b, double c) { return __builtin_fma(a, b, c); }
+typedef double v4d __attribute__((ext_vector_type(4)));
 
 struct Rope {
   const float *cos_t, *sin_t;
@@ -93,14 +96,84 @@ struct Rope {
   int half, n_pos, pairs, n, H;  // half: pairs of elements that rotate
 };
 
-// One (token, head) per D / 8 lanes: lane l holds elements 8 l .. 8 l + 7. FAST: a lane's elements rotate
-// with eight neighbours, or with each other, all of them or none.
+// Norm and rotation of a lane's eight elements. FAST: they rotate with eight neighbours, or with each other, all of them or none.
+// mine: the head's row in LDS.
+template <int D, bool FAST, class T>
+__device__ __forceinline__ void turn_row(const Rope& R, T (&x)[kPer], const float* w, int pos, int l, T* mine) {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  constexpr int L = D / kPer;
+  if (w) {
+    T acc = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc = fma_(x[e], x[e], acc);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) acc += __shfl_xor(acc, o, L);
+    const T s = (T)1 / sqrt(acc / (T)D + (T)R.eps);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = x[e] * s * (T)w[kPer * l + e];
+  }
+  const float *ct = R.cos_t + (int64_t)pos * R.half, *st = R.sin_t + (int64_t)pos * R.half;
+  if (R.pairs) {
+    const int i0 = kPer / 2 * l;
+    auto turn = [&](int e, T c, T s) {
+      const T a = x[2 * e], b = x[2 * e + 1];
+      x[2 * e] = fma_(a, c, -(b * s));
+      x[2 * e + 1] = fma_(a, s, b * c);
+    };
+    if constexpr (FAST) {
+      if (i0 < R.half) {
+        const v4f c = *reinterpret_cast<const v4a*>(ct + i0), s = *reinterpret_cast<const v4a*>(st + i0);
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e) turn(e, (T)c[e], (T)s[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer / 2; ++e)
+        if (i0 + e < R.half) turn(e, (T)ct[i0 + e], (T)st[i0 + e]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    *reinterpret_cast<v4*>(mine + kPer * l + 4 * c) = v4{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if constexpr (FAST) {  // a lane's elements are all of one half, or none rotates
+    const int i0 = kPer * l;
+    if (i0 >= 2 * R.half) return;
+    const bool up = i0 >= R.half;
+    const int i = up ? i0 - R.half : i0, other = up ? i0 - R.half : i0 + R.half;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const v4f cv = *reinterpret_cast<const v4a*>(ct + i + 4 * c), sv = *reinterpret_cast<const v4a*>(st + i + 4 * c);
+      const v4 y = *reinterpret_cast<const v4*>(mine + other + 4 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const T s = (T)(up ? sv[e] : -sv[e]);
+        x[4 * c + e] = fma_(x[4 * c + e], (T)cv[e], y[e] * s);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int i0 = kPer * l + e;
+      if (i0 < 2 * R.half) {
+        const bool up = i0 >= R.half;
+        const int i = up ? i0 - R.half : i0;
+        const T s = (T)(up ? st[i] : -st[i]);
+        x[e] = fma_(x[e], (T)ct[i], mine[up ? i : i0 + R.half] * s);
+      }
+    }
+  }
+}
+
+// One (token, head) per D / 8 lanes: lane l holds elements 8 l .. 8 l + 7. Keys are turned, and keys and values brought to their
+// steps, in 64 bits: a number next to the border between two of them would else go with the rounding (one in a million does).
 template <int D, bool FAST>
 __global__ __launch_bounds__(kThreads) void k_rope_kv4(Rope R, Kv4 kv, const float* q, const float* __restrict__ k,
                                                        const float* __restrict__ v, int64_t stride, float* q_out,
                                                        int64_t q_out_stride) {
   constexpr int L = D / kPer;  // lanes per head
-  __shared__ __align__(16) float sh[kThreads / L][D];
+  __shared__ __align__(32) double sh[kThreads / L][D];
   const int l = threadIdx.x % L, nh = R.H + 2 * kv.KV;
   const int64_t it = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
   if (it >= (int64_t)R.n * nh) return;  // all lanes of a head
@@ -108,104 +181,43 @@ __global__ __launch_bounds__(kThreads) void k_rope_kv4(Rope R, Kv4 kv, const flo
   const bool is_q = hh < R.H, is_v = hh >= R.H + kv.KV;
   const int head = is_q ? hh : is_v ? hh - R.H - kv.KV : hh - R.H;
   const float* src = (is_q ? q : is_v ? v : k) + t * stride + (int64_t)head * D + kPer * l;
-  float x[kPer];
+  float f[kPer];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const v4f f = *reinterpret_cast<const v4a*>(src + 4 * c);
+    const v4f y = *reinterpret_cast<const v4a*>(src + 4 * c);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[4 * c + e] = f[e];
+    for (int e = 0; e < 4; ++e) f[4 * c + e] = y[e];
   }
   const int pos = R.rpos[t], row = R.kv_row[t], p = kv.page_of(R.seq[t], row);
   if (p < 0 || pos < 0 || pos >= R.n_pos) return;
-  if (!is_v) {
-    const float* w = is_q ? R.q_norm : R.k_norm;
-    if (w) {
-      float acc = 0.0f;
+  if (is_q) {
+    turn_row<D, FAST, float>(R, f, R.q_norm, pos, l, reinterpret_cast<float*>(sh[threadIdx.x / L]));
+    float* to = q_out + t * q_out_stride + (int64_t)head * D + kPer * l;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) acc = fma_(x[e], x[e], acc);
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) acc += __shfl_xor(acc, o, L);
-      const float s = 1.0f / sqrtf(acc / (float)D + R.eps);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) x[e] = x[e] * s * w[kPer * l + e];
-    }
-    const float *ct = R.cos_t + (int64_t)pos * R.half, *st = R.sin_t + (int64_t)pos * R.half;
-    if (R.pairs) {
-      const int i0 = kPer / 2 * l;
-      auto turn = [&](int e, float c, float s) {
-        const float a = x[2 * e], b = x[2 * e + 1];
-        x[2 * e] = fma_(a, c, -(b * s));
-        x[2 * e + 1] = fma_(a, s, b * c);
-      };
-      if constexpr (FAST) {
-        if (i0 < R.half) {
-          const v4f c = *reinterpret_cast<const v4a*>(ct + i0), s = *reinterpret_cast<const v4a*>(st + i0);
-#pragma unroll
-          for (int e = 0; e < kPer / 2; ++e) turn(e, c[e], s[e]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kPer / 2; ++e)
-          if (i0 + e < R.half) turn(e, ct[i0 + e], st[i0 + e]);
-      }
-    } else {
-      float* mine = sh[threadIdx.x / L];
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<v4f*>(mine + kPer * l + 4 * c) = v4f{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if constexpr (FAST) {  // a lane's elements are all of one half, or none rotates
-        const int i0 = kPer * l;
-        if (i0 < 2 * R.half) {
-          const bool up = i0 >= R.half;
-          const int i = up ? i0 - R.half : i0, other = up ? i0 - R.half : i0 + R.half;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const v4f cv = *reinterpret_cast<const v4a*>(ct + i + 4 * c), sv = *reinterpret_cast<const v4a*>(st + i + 4 * c);
-            const v4f y = *reinterpret_cast<const v4f*>(mine + other + 4 * c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float s = up ? sv[e] : -sv[e];
-              x[4 * c + e] = fma_(x[4 * c + e], cv[e], y[e] * s);
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const int i0 = kPer * l + e;
-          if (i0 < 2 * R.half) {
-            const bool up = i0 >= R.half;
-            const int i = up ? i0 - R.half : i0;
-            const float s = up ? st[i] : -st[i];
-            x[e] = fma_(x[e], ct[i], mine[up ? i : i0 + R.half] * s);
-          }
-        }
-      }
-    }
-    if (is_q) {
-      float* to = q_out + t * q_out_stride + (int64_t)head * D + kPer * l;
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<v4a*>(to + 4 * c) = v4a{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
-      return;
-    }
+    for (int c = 0; c < 2; ++c) *reinterpret_cast<v4a*>(to + 4 * c) = v4a{f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]};
+    return;
   }
-  float hi = -INFINITY, lo = INFINITY;
+  double x[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) x[e] = (double)f[e];
+  if (!is_v) turn_row<D, FAST, double>(R, x, R.k_norm, pos, l, sh[threadIdx.x / L]);
+  double hi = -INFINITY, lo = INFINITY;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
-    if (x[e] != x[e]) x[e] = 0.0f;
-    hi = fmaxf(hi, x[e]), lo = fminf(lo, x[e]);
+    if (x[e] != x[e]) x[e] = 0.0;
+    hi = fmax(hi, x[e]), lo = fmin(lo, x[e]);
   }
 #pragma unroll
-  for (int o = 1; o < kKv4Group / kPer; o <<= 1) hi = fmaxf(hi, __shfl_xor(hi, o)), lo = fminf(lo, __shfl_xor(lo, o));
+  for (int o = 1; o < kKv4Group / kPer; o <<= 1) hi = fmax(hi, __shfl_xor(hi, o)), lo = fmin(lo, __shfl_xor(lo, o));
   const _Float16 s = scale_of(hi, lo);
-  const float inv = s != (_Float16)0.0f ? 1.0f / (float)s : 0.0f;
+  const double inv = s != (_Float16)0.0f ? 1.0 / (double)s : 0.0;
   uint32_t w = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
-    const float y = fminf(fmaxf(__builtin_rintf(x[e] * inv), -8.0f), 7.0f);
-    w |= (uint32_t)((int)y + 8) << (4 * e);
+    const double y = x[e] * inv;
+    double n = __builtin_rint(y);
+    if (fabs(fabs(y - n) - 0.5) < 0x1p-40) n = __builtin_rint(x[e] / (double)s);  // in the middle, as far as inv says
+    w |= (uint32_t)((int)fmin(fmax(n, -8.0), 7.0) + 8) << (4 * e);
   }
   const int64_t first = kv.first_row(p, head);
   const int r = row & ((1 << kv.shift) - 1), grp = l / (kKv4Group / kPer);

@@ -13,22 +13,21 @@ GROUP = 32
 # ---- numbers in 4 bits ----
 
 def scale_of(x):
-    """fp16 scales of groups x [..., 32] of floats, as the header has them: exact in every step."""
+    """fp16 scales of groups x [..., 32], as the header has them: exact in every step before the last two roundings."""
     hi, lo = x.max(-1), x.min(-1)
-    m = np.where(hi >= -lo, hi, lo).astype(np.float32)
-    s = np.clip(m * np.float32(-0.125), -4096, 4096).astype(np.float32)
-    u = s.view(np.uint32).astype(np.uint64)
-    u = (u + 0x7FFF + (u >> 16 & 1)) & 0xFFFF0000
-    return u.astype(np.uint32).view(np.float32).astype(np.float16)
+    s = np.clip(np.where(hi >= -lo, hi, lo).astype(np.float64) * -0.125, -4096, 4096)
+    u = s.view(np.uint64)
+    half = np.uint64(2 ** 44 - 1)  # 8 significant bits, ties to even
+    u = (u + half + (u >> np.uint64(45) & np.uint64(1))) & ~np.uint64(2 ** 45 - 1)
+    return u.view(np.float64).astype(np.float32).astype(np.float16)
 
 
 def in4(x):
-    """Rows of floats [..., d] as numbers 0..15 and scales, every step rounded as the header says (fp32)."""
-    g = np.where(np.isnan(x), np.float32(0), x.astype(np.float32)).reshape(*x.shape[:-1], -1, GROUP)
+    """Rows [..., d] as numbers 0..15 and scales: quotients in 64 bits, which are exact beside their borders."""
+    g = np.where(np.isnan(x), 0, x).astype(np.float64).reshape(*x.shape[:-1], -1, GROUP)
     s = scale_of(g)
     with np.errstate(divide="ignore", invalid="ignore"):
-        inv = np.where(s == 0, np.float32(0), np.float32(1) / s.astype(np.float32)).astype(np.float32)
-        y = np.rint(np.where(np.isinf(g) & (inv == 0)[..., None], 0, g * inv[..., None]))
+        y = np.where((s == 0)[..., None], 0, np.rint(g / s.astype(np.float64)[..., None]))
     n = (np.clip(y, -8, 7) + 8).astype(np.uint8)
     return n.reshape(x.shape), s
 
