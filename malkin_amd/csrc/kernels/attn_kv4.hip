@@ -742,6 +742,7 @@ __global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4A
     const int tiles = blk.tiles();
     if (j == S.J || tiles == 0) {  // the next tokens'
       t += blk.m, j = 0;
+      if (t >= A.n) return;  // lengths that change while they are read: no reason to wait for ever
       set_tokens(blk, A, t, S.tq);
       continue;
     }

@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
   __shared__ Entry list[kMergeCap], bound;
   __shared__ __align__(16) float heads[kMaxLists];
   __shared__ int place[kMergeCap], n_cand;
-  __shared__ float least;
+  __shared__ uint32_t least_key;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, group = blockIdx.x;
   const int beams = ROW ? 1 : B.beams, lists = beams * B.segs, k = B.k;
   const int64_t row0 = (int64_t)group * beams;
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
   const bool mine = in && finite(score), over = mine && done;
   if (ROW && (!finite(score) || done)) return;
   const double start = ROW ? 0.0 : (double)score;
-  if (tid == 0) bound = none, n_cand = 0, least = -INFINITY;
+  if (tid == 0) bound = none, n_cand = 0, least_key = 0xFFFFFFFFu;
   for (int i = tid; i < kMergeCap; i += kMergeThreads) place[i] = 0;
   __syncthreads();
   auto entry = [&](int j, const Cand& v) {
@@ -274,17 +274,18 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(Beams B, const Sta
   if (in) heads[tid] = mark;
   for (int i = lists + tid; i < (lists + 3) / 4 * 4; i += kMergeThreads) heads[i] = -INFINITY;
   __syncthreads();
-  if (in && mark > -INFINITY) {
-    int more = 0, same = 0;
-#pragma unroll 4
+  if (in) {
+    int more = 0;
+#pragma unroll 8
     for (int j = 0; j < lists; j += 4) {
       const v4f v = *reinterpret_cast<const v4f*>(heads + j);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) more += v[e] > mark, same += v[e] == mark;
+      for (int e = 0; e < 4; ++e) more += v[e] > mark;
     }
-    if (more < r0 && r0 <= more + same) least = mark;  // every such thread writes the same
+    if (more < r0) atomicMin(&least_key, order_key(mark));  // the r-th is the least of those
   }
   __syncthreads();
+  const float least = of_key(least_key);
   {
     bool go = true;
 #pragma unroll
