@@ -7,8 +7,8 @@
 // then over the lists (the r-th best of their p-th elements, where (p + 1) r >= k), and what is left finds its place by
 // counting what is better.
 //
-// What bounds it: for one request of four beams (13 us) the latency of two launches (5.8 and 7.1 us) and of their chains of loads,
-// barriers and 64-bit exponentials; for 24 of them (22 us; about 42 MB of logits, those of ended beams are not read) the first
+// What bounds it: for one request of four beams (12.4 us) the latency of two launches (5.6 and 6.7 us) and of their chains of
+// loads, barriers and 64-bit exponentials; for 24 of them (22 us; about 42 MB of logits, those of ended beams are not read) the first
 // launch, 16.3 us or 2.6 TB/s, with about 20 vector instructions a logit, half of them for its exponential.
 #include <algorithm>
 #include <cfloat>
