@@ -307,9 +307,10 @@ enum { MK_ROPE_HALVES = 0, MK_ROPE_PAIRS = 1 };
    heads, rotation of each one's first rope_dim elements at position rpos[t] of the tables [n_pos][rope_dim / 2], the query
    heads to q_out (q itself: in place, of the same stride), keys and values in 4 bits into row kv_row[t] of sequence seq[t] of
    `layer`: s is the group's element furthest from 0 over -8 (the positive one of two), rounded to 8 significant bits, within
-   +-4096 and to fp16; n = rint(x / s) + 8 within 0..15. NaN counts as 0 there. q, k and v share the token stride. A token whose seq, rpos or kv_row lies outside, or whose row has no page, is left
-   out: its row of q_out and the cache stay as they were. Rows of one call are different ones, and no two sequences share a page
-   that is written (mk_kv4_resize sees to that). */
+   +-4096 and to fp16; n = rint(x / s) + 8 within 0..15; both of x in 64 bits (norm and rotation of keys too). NaN counts as 0
+   there. q, k and v share the token stride. A token whose seq, rpos or kv_row lies outside, or whose row has no page, is left
+   out: its row of q_out and the cache stay as they were. Rows of one call are different ones, and no two sequences share a
+   page that is written (mk_kv4_resize sees to that). */
 int mk_rope_kv4(mk_ctx* ctx, const float* q, const float* k, const float* v, int64_t stride, int n, int n_head,
                 const float* q_norm, const float* k_norm, float eps, int layout, int rope_dim, const float* cos_t,
                 const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row,

@@ -155,6 +155,31 @@ def test_write(mk, case, n):
         assert np.array_equal(v.view(np.uint8), want[name].view(np.uint8)), name
 
 
+@pytest.mark.parametrize("layout,norm,d", [(mk_.ROPE_HALVES, True, 128), (mk_.ROPE_PAIRS, False, 64)])
+def test_numbers_beside_borders(mk, layout, norm, d):
+    """A million numbers of K, each the one that 64 bits give: a rounding of 2^-52 turns one in 10^12, one of 2^-23 some of these."""
+    rng = np.random.default_rng(d)
+    H, KV, page, n, n_pos = 1, 8 * 128 // d, 64, 1024, 64
+    c = Cache(rng, 1, n // page, page, KV, d, 1, n // page)
+    c.hold(0, list(rng.permutation(n // page)), n)
+    c.put(mk)
+    x = rng.standard_normal((n, (H + 2 * KV) * d)).astype(np.float32)
+    turn = rng.random((n_pos, d // 2)) * 2 * np.pi
+    cos, sin = np.cos(turn).astype(np.float32), np.sin(turn).astype(np.float32)
+    w = [(1 + 0.2 * rng.standard_normal(d)).astype(np.float32) for _ in range(2)] if norm else None
+    rpos = rng.integers(0, n_pos, n)
+    print("kv4 write, borders", layout, norm, d, flush=True)
+    write_call(mk, c, x, H, w, layout, d, cos, sin, list(rpos), [0] * n, list(range(n)), 0)
+    k = x.reshape(n, -1, d)[:, H:H + KV].astype(np.float64)
+    if norm:
+        k *= w[1] / np.sqrt((k ** 2).mean(-1, keepdims=True) + np.float64(np.float32(1e-6)))
+    num, s = in4(rotated64(k, cos[rpos, None].astype(np.float64), sin[rpos, None].astype(np.float64), layout == mk_.ROPE_PAIRS))
+    kd, sd = c.get("k", "k_scale")
+    p, r = c.a["table"][0, np.arange(n) // page], np.arange(n) % page
+    assert np.array_equal(sd[p, 0, :, r].view(np.uint16), s.reshape(n, KV, -1).view(np.uint16))
+    assert np.array_equal(unpacked(kd[p, 0, :, r]), num)
+
+
 def test_values_at_the_edges(mk):
     """Zeros, the smallest and the largest values, infinities and NaN, extremes of both signs, ties of a half."""
     rng = np.random.default_rng(1)
