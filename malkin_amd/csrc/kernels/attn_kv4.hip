@@ -19,9 +19,9 @@
 // tile is asked for as soon as this one is in registers, and the waves meet only to add their results.
 //
 // What bounds it: the vector instructions that turn 4 bits into fp16 factors, 13 for eight values and as many for K as for V,
-// which is 416 of a tile's 560 to 700 (16 or 32 rows); two or three waves a SIMD cover them with matrix instructions in part.
+// which is 416 of a tile's 560 to 700 (16 or 32 rows); two waves a SIMD cover them with matrix instructions in part.
 // Long documents of four users (4 x 5 drafted tokens) take 125 us, 3.0 TB/s of the cache's bytes, where the copies alone take
-// 63; 24 users of up to 6000 keys 40 us, of which 12 are spent before the first and after the last tile and 4 on joining; 512
+// 63; 24 users of up to 6000 keys 38.5 us, of which 12 are spent before the first and after the last tile and 4 on joining; 512
 // tokens of three prompts 78 us, 21 of them for setting up and ending each workgroup's two or three blocks and 10 on joining.
 // Blocks of 128 rows, whose four waves take a tile's numbers out of 4 bits once for all of them, took 78 us there, but 69 for a
 // prompt of 300 tokens by itself, which takes 31 here, so that form is not kept.
@@ -665,7 +665,7 @@ template <int NR>
 constexpr int kTokens = NR == 1 ? 1 : 4;
 
 template <int D, int NR>
-__global__ __launch_bounds__(kShare * 64, NR == 1 ? 3 : 2) void k_kv4_share(Kv4Attn A, const float* __restrict__ q, int64_t q_stride,
+__global__ __launch_bounds__(kShare * 64, 2) void k_kv4_share(Kv4Attn A, const float* __restrict__ q, int64_t q_stride,
                                                                             Out O, Parts P) {
   constexpr int R = NR * kSet, kTok = kTokens<NR>, kOnce = 256 * kTok;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -853,6 +853,9 @@ struct Cut {
 // users, 1000 keys 22.2, in shares 34 (eight waves 25.8), 2000 keys 34 and 42, 3000 keys 46 and 51, but there one long sequence
 // among short ones would be one workgroup's alone.
 constexpr int kWholeKeys = 1024, kWholeKeysMany = 2048, kMany = 512;
+// Workgroups that share all tiles: two a CU, which leaves a wave 256 registers. Three of 168 took 41.6 us where two take 39.5 (24
+// users of up to 6000 keys), 49 where 42.6 (one user of 100000), and as long for 64 users of 4000.
+constexpr int kShares = 2 * 256;
 // Up to so many rows are joined by four waves each: 4 x 5 drafts over 120000 keys 6 us, by one 13; 16384 rows of a prompt 10,
 // by four 24.
 constexpr int kJoinRows = 2048;
@@ -863,7 +866,7 @@ Cut cut_of(int n, int H, int KV, int max_keys, int max_run) {
   const int64_t blocks = (int64_t)n * shape_of(H, KV, c.sets * kSet, max_run).J;
   if (blocks >= kMany) c.waves = 4;
   if (rows <= 2 * kSet && max_keys <= (blocks >= kMany ? kWholeKeysMany : kWholeKeys)) return c;
-  c.wgs = 256 * (c.sets == 1 ? 3 : 2);  // what the chip holds at once
+  c.wgs = kShares;
   return c;
 }
 
@@ -879,7 +882,7 @@ size_t parts_bytes(const Cut& c, int n, int H, int KV) {
 // Never less for a larger call: the larger of both kinds of blocks, the records those of the smaller ones, also where this call
 // has no parts and a larger one may.
 size_t attention_kv4_workspace(int n, int H, int KV, int D, int max_keys, int max_run) {
-  const Cut one{1, 256 * 3, 0}, two{2, 256 * 2, 0};
+  const Cut one{1, kShares, 0}, two{2, kShares, 0};
   return std::max(D == 128 ? parts_bytes<128>(one, n, H, KV) : parts_bytes<64>(one, n, H, KV),
                   D == 128 ? parts_bytes<128>(two, n, H, KV) : parts_bytes<64>(two, n, H, KV));
 }
