@@ -848,11 +848,11 @@ struct Cut {
   int wgs;    // workgroups that share all tiles; 0: one per block
   int waves;  // of a workgroup that has a block to itself
 };
-// A workgroup of eight waves per block up to kWholeKeys keys, with kMany blocks one of four waves up to kWholeKeysMany. 8 heads
-// for K and V, 32 for q: 8 users, 1000 keys 12.5 us, in shares 19.1 (four waves 14.6); one user, 2000 keys 18.9, in shares 13.7; 64
-// users, 1000 keys 22.2, in shares 34 (eight waves 25.8), 2000 keys 34 and 42, 3000 keys 46 and 51, but there one long sequence
-// among short ones would be one workgroup's alone.
-constexpr int kWholeKeys = 1024, kWholeKeysMany = 2048, kMany = 512;
+// A workgroup of eight waves per block up to kWholeKeys keys, with kMany blocks one of four waves up to kWholeKeysMany. 32 query
+// heads on 8: 8 users, 1000 keys 12.5 us, in shares 18.8 (four waves 14.6); one user, 2000 keys 18.9, in shares 13.7; 64 users,
+// 1000 keys 22, in shares 33 (eight waves 25.8), 2000 keys 33 and 47, 3000 keys 46.5 and 53.4, 4000 keys 60 and 61, where one
+// long sequence among short ones begins to be felt.
+constexpr int kWholeKeys = 1024, kWholeKeysMany = 3200, kMany = 512;
 // Workgroups that share all tiles: two a CU, which leaves a wave 256 registers. Three of 168 took 41.6 us where two take 39.5 (24
 // users of up to 6000 keys), 49 where 42.6 (one user of 100000), and as long for 64 users of 4000.
 constexpr int kShares = 2 * 256;

@@ -305,6 +305,7 @@ CASES = [
     (16, 8, 128, 256, [1], [20000]),
     (2, 2, 64, 16, [1] * 300, [1 + i % 37 for i in range(299)] + [2100]),
     (4, 2, 64, 32, [600, 500, 100], [610, 500, 1100]),
+    (2, 2, 64, 16, [1] * 300, [1 + i % 41 for i in range(299)] + [3300]),
 ]
 
 
