@@ -341,8 +341,8 @@ int mk_kv4_fork(mk_ctx* ctx, const mk_kv4_cache* kv, const int32_t* dst, const i
 /* Sequence seq[i] (seq NULL: i) is to hold new_len[i] rows: pages past a shorter end are let go; a longer one gets pages, and
    where its last page is shared and not full, a copy of the rows it holds there (all layers), so that it can be written.
    Shorter ends come first, then the longer ones in order, each taking the free pages of the lowest numbers; of those that
-   share a page and nobody else, the last keeps it. status[i]: 0, or 1 where new_len[i] needs a page and the pool has too few
-   for it and all entries before it, or -1 where seq[i] or new_len[i] (0..max_pages * page) lies outside or seq[i] comes again
+   share a page and nobody else, the last keeps it if all others left. status[i]: 0, or 1 where new_len[i] needs a page (one
+   for the copy too) and the pool has too few for it and all entries before it, or -1 where seq[i] or new_len[i] (0..max_pages * page) lies outside or seq[i] comes again
    further on; such entries change nothing. n at most 4096. */
 size_t mk_kv4_resize_workspace(int n, int n_page);
 int mk_kv4_resize(mk_ctx* ctx, const mk_kv4_cache* kv, const int32_t* seq, const int32_t* new_len, int n, int32_t* status,

@@ -190,6 +190,7 @@ __global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t*
   __shared__ int part[kPlan / 64], free_s[kFreeInLds];
   __shared__ int64_t part64[kPlan / 64];
   __shared__ uint8_t kind_s[kMaxEntries];
+  __shared__ int cut;  // the first entry that wants pages and finds too few
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, in_page = (1 << P.shift) - 1;
   const int E = (n + kPlan - 1) / kPlan, i0 = tid * E;  // a thread's entries follow each other
   const int64_t room = (int64_t)P.max_pages << P.shift;
@@ -197,6 +198,7 @@ __global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t*
     for (int i = tid; i < n; i += kPlan) seq_s[i] = seq[i];
     __syncthreads();
   }
+  if (tid == 0) cut = INT32_MAX;
   bool shrinks = false;
   for (int i = tid; i < n; i += kPlan) {
     const int s = seq ? seq_s[i] : i, now = held(P, min(max(s, 0), P.n_seq - 1)), L = new_len[i];  // both loads at once
@@ -244,19 +246,21 @@ __global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t*
   };
   uint32_t free = kScan * (tid & ~63) < P.n_page ? free_of(0) : 0;
   // Copies and pages wanted, and where each entry's begin in the list of free pages and in that of the copies. More than the
-  // pool has counts as one more than that.
-  int copies[kMaxEntries / kPlan], needs[kMaxEntries / kPlan];
+  // pool has counts as one more than that. prior: the entry before this one that is the last to leave the page which this one
+  // keeps, with what it needs (-1: none).
+  int copies[kMaxEntries / kPlan], needs[kMaxEntries / kPlan], prior[kMaxEntries / kPlan];
   int64_t mine = 0;
 #pragma unroll
   for (int e = 0; e < kMaxEntries / kPlan; ++e) {
-    copies[e] = needs[e] = 0;
+    copies[e] = needs[e] = 0, prior[e] = -1;
     const int i = i0 + e;
     if (e >= E || i >= n || kind_s[i] != kGrow) continue;
     if (last_s[i] >= 0) {
       const int holders = refs_now(P.refs + last_s[i]);
       int before = 0;
       if (holders > 1)
-        for (int j = 0; j < i; ++j) before += last_s[j] == last_s[i];
+        for (int j = 0; j < i; ++j)
+          if (last_s[j] == last_s[i]) ++before, prior[e] = j;
       copies[e] = before < holders - 1;
     }
     needs[e] = min(copies[e] + pages_of(new_s[i], P.shift) - pages_of(len_s[i], P.shift), P.n_page + 1);
@@ -281,6 +285,16 @@ __global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t*
       }
     found += here;
   }
+  // An entry that wants pages has them if those up to it all do, so one number says which do. One that keeps a page because
+  // all who share it leave, keeps it only if the last of them does.
+  if (found < wanted) {
+    int64_t end = before >> 16;
+#pragma unroll
+    for (int e = 0; e < kMaxEntries / kPlan; ++e) {
+      end += needs[e];
+      if (needs[e] && end > found) atomicMin(&cut, i0 + e);
+    }
+  }
   __syncthreads();  // the list is written
   auto page_at = [&](int64_t i) { return i < kFreeInLds ? free_s[i] : free_list[i]; };
   int64_t run = before >> 16;
@@ -290,7 +304,7 @@ __global__ __launch_bounds__(kPlan) void k_resize_plan(Kv4Pool P, const int32_t*
     const int i = i0 + e;
     if (e >= E || i >= n) continue;
     const int kind = kind_s[i];
-    const bool fits = kind == kGrow && (needs[e] == 0 || run + needs[e] <= found);
+    const bool fits = kind == kGrow && (needs[e] ? i : prior[e]) < cut;
     if (copies[e]) {  // one that does not fit stays in the list, with no rows
       Move m{0, 0, 0};
       if (fits) {
