@@ -277,7 +277,7 @@ typedef struct {
   uint16_t* k_scale; /* [n_page][n_layer][n_head_kv][page][head_dim / 32] */
   uint16_t* v_scale; /* [n_page][n_layer][n_head_kv][head_dim / 32][page] */
   int32_t* table;    /* [n_seq][max_pages]; -1 past a sequence's pages */
-  int32_t* len;      /* [n_seq] rows that a sequence holds; NULL where no call below that reads it is made */
+  int32_t* len;      /* [n_seq] rows that a sequence holds; NULL where no call that moves pages is made */
   int32_t* refs;     /* [n_page]; 0: the page is free; NULL as len */
   int32_t n_layer, n_page, page, n_head_kv, head_dim, n_seq, max_pages;
 } mk_kv4_cache;
@@ -308,9 +308,10 @@ enum { MK_ROPE_HALVES = 0, MK_ROPE_PAIRS = 1 };
    heads to q_out (q itself: in place, of the same stride), keys and values in 4 bits into row kv_row[t] of sequence seq[t] of
    `layer`: s is the group's element furthest from 0 over -8 (the positive one of two), rounded to 8 significant bits, within
    +-4096 and to fp16; n = rint(x / s) + 8 within 0..15; both of x in 64 bits (norm and rotation of keys too). NaN counts as 0
-   there. q, k and v share the token stride. A token whose seq, rpos or kv_row lies outside, or whose row has no page, is left
-   out: its row of q_out and the cache stay as they were. Rows of one call are different ones, and no two sequences share a
-   page that is written (mk_kv4_resize sees to that). */
+   there. q, k and v share the token stride. A token whose seq, rpos or kv_row lies outside, whose row has no page, or whose row
+   its sequence does not hold (where the cache has a len: mk_kv4_resize found no room for it, say), is left out: its row of
+   q_out and the cache stay as they were. Rows of one call are different ones, and no two sequences share a page that is
+   written (mk_kv4_resize sees to that). */
 int mk_rope_kv4(mk_ctx* ctx, const float* q, const float* k, const float* v, int64_t stride, int n, int n_head,
                 const float* q_norm, const float* k_norm, float eps, int layout, int rope_dim, const float* cos_t,
                 const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row,

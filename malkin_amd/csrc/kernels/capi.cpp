@@ -632,7 +632,7 @@ int mk_rope_kv4(mk_ctx* c, const float* q, const float* k, const float* v, int64
     require(c != nullptr, "mk_rope_kv4: null context");
     const DeviceOf on(c);
     mk::rope_kv4(c->stream, K, D, q, k, v, stride, n, n_head, q_norm, k_norm, eps, layout == MK_ROPE_PAIRS, rope_dim, cos_t,
-                 sin_t, n_pos, rpos, seq, kv_row, q_out, q_out_stride);
+                 sin_t, n_pos, rpos, seq, kv_row, kv->len, q_out, q_out_stride);
   });
 }
 

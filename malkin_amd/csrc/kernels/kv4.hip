@@ -93,6 +93,7 @@ struct Rope {
   const float *cos_t, *sin_t;
   const float *q_norm, *k_norm;
   const int32_t *rpos, *seq, *kv_row;
+  const int32_t* len;  // rows that sequences hold, or null
   float eps;
   int half, n_pos, pairs, n, H;  // half: pairs of elements that rotate
 };
@@ -189,8 +190,10 @@ __global__ __launch_bounds__(kThreads) void k_rope_kv4(Rope R, Kv4 kv, const flo
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[4 * c + e] = y[e];
   }
-  const int pos = R.rpos[t], row = R.kv_row[t], p = kv.page_of(R.seq[t], row);
-  if (p < 0 || pos < 0 || pos >= R.n_pos) return;
+  const int pos = R.rpos[t], row = R.kv_row[t], sq = R.seq[t], p = kv.page_of(sq, row);
+  // A row past its sequence's may be one of somebody who holds the page too. The length comes with the page's number.
+  const int len = R.len ? R.len[min(max(sq, 0), kv.n_seq - 1)] : INT32_MAX;
+  if (p < 0 || row >= len || pos < 0 || pos >= R.n_pos) return;
   if (is_q) {
     turn_row<D, FAST, float>(R, f, R.q_norm, pos, l, reinterpret_cast<float*>(sh[threadIdx.x / L]));
     float* to = q_out + t * q_out_stride + (int64_t)head * D + kPer * l;
@@ -288,9 +291,9 @@ void rope_tables(hipStream_t s, const mk_rope& r, const float* divide, int64_t f
 
 void rope_kv4(hipStream_t s, const Kv4& kv, int D, const float* q, const float* k, const float* v, int64_t stride, int n, int H,
               const float* q_norm, const float* k_norm, float eps, bool pairs, int rope_dim, const float* cos_t,
-              const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row, float* q_out,
-              int64_t q_out_stride) {
-  const Rope R{cos_t, sin_t, q_norm, k_norm, rpos, seq, kv_row, eps, rope_dim / 2, n_pos, pairs, n, H};
+              const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row, const int32_t* len,
+              float* q_out, int64_t q_out_stride) {
+  const Rope R{cos_t, sin_t, q_norm, k_norm, rpos, seq, kv_row, len, eps, rope_dim / 2, n_pos, pairs, n, H};
   const int64_t items = (int64_t)n * (H + 2 * kv.KV), per = kThreads / (D / kPer), wgs = (items + per - 1) / per;
   const bool fast = R.half % (pairs ? kPer / 2 : kPer) == 0;
   auto go = [&]<int D_, bool F>() {

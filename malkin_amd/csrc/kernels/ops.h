@@ -166,8 +166,8 @@ void attention_prefix(hipStream_t s, const PrefixAttn& A, int D, const float* q,
 void rope_tables(hipStream_t s, const mk_rope& r, const float* divide, int64_t first, int n_pos, float* cos_t, float* sin_t);
 void rope_kv4(hipStream_t s, const Kv4& kv, int D, const float* q, const float* k, const float* v, int64_t stride, int n, int H,
               const float* q_norm, const float* k_norm, float eps, bool pairs, int rope_dim, const float* cos_t,
-              const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row, float* q_out,
-              int64_t q_out_stride);
+              const float* sin_t, int n_pos, const int32_t* rpos, const int32_t* seq, const int32_t* kv_row, const int32_t* len,
+              float* q_out, int64_t q_out_stride);
 void kv4_rows(hipStream_t s, const Kv4& kv, int D, const int32_t* seq, const int32_t* rows, int n, void* k_out, void* v_out);
 struct Kv4Attn {
   Kv4 kv;

@@ -4,8 +4,9 @@ import pytest
 
 import malkin_amd as mk_
 import test_gpu_pages
-from kv4_cases import copied
+from kv4_cases import copied, in4, packed
 from kv4_full_pool import resize_in_order, written_pages
+from test_gpu_kv4 import write_call
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +84,42 @@ def test_lives_on_a_small_pool(mk, n_seq, n_page, page):
         new = [int(x) for x in np.clip(p.a["len"][seq] + rng.integers(-page // 2, page, n_seq), 0, 4 * page)]
         failed += p.resize(seq, new).count(1)
     assert failed
+
+
+@pytest.mark.parametrize("d,layout,rope_dim,in_place", [(128, mk_.ROPE_HALVES, 128, True), (64, mk_.ROPE_PAIRS, 22, False)])
+def test_writes_of_who_found_no_room(mk, d, layout, rope_dim, in_place):
+    """Rows past a sequence's end, in a page that it shares and in one of its own: nothing is written, q stays as it was. The others
+    of the batch are written, and without lengths all are."""
+    rng = np.random.default_rng(d)
+    H, KV, page, n_pos = 4, 2, 16, 40
+    p = Pool(mk, rng, 2, 5, page, KV, d, 4, 3)
+    p.resize([0, 2], [20, 35])
+    p.fork([1], [0])
+    p.resize([1], [18])
+    assert p.resize([1, 0, 2], [19, 20, 36]) == [1, 0, 0]
+    seq, row = [1, 2, 0, 1, 2], [18, 35, 19, 21, 36]
+    cos, sin = (rng.standard_normal((n_pos, rope_dim // 2)).astype(np.float32) for _ in range(2))
+    for lengths in (True, False):
+        x = rng.standard_normal((len(seq), (H + 2 * KV) * d)).astype(np.float32)
+        before = {k: p.c.get(k) for k in test_gpu_pages.DATA}
+        length = p.c.c.len
+        p.c.c.len = length if lengths else None
+        print("full pool, writes", d, lengths, flush=True)
+        q = write_call(mk, p.c, x, H, None, layout, rope_dim, cos, sin, [3, 1, 4, 1, 5], seq, row, 1, in_place)
+        p.c.c.len = length
+        live = [1, 2] if lengths else range(5)
+        after = {k: p.c.get(k) for k in test_gpu_pages.DATA}
+        for t in range(5):
+            same = np.array_equal(q[t, :H * d], x[t, :H * d] if in_place else np.full(H * d, 3.0, np.float32))
+            assert same == (t not in live)
+        for t in live:
+            pg, r = p.a["table"][seq[t], row[t] // page], row[t] % page
+            num, s = in4(x[t, (H + KV) * d:].reshape(KV, d))
+            assert np.array_equal(after["v"][pg, 1, :, r], packed(num))
+            assert np.array_equal(after["v_scale"][pg, 1, :, :, r], s)
+            assert not np.array_equal(after["k"][pg, 1, :, r], before["k"][pg, 1, :, r])
+            for k in test_gpu_pages.DATA:
+                at = (pg, 1, slice(None), slice(None), r) if k == "v_scale" else (pg, 1, slice(None), r)
+                before[k][at] = after[k][at]
+        for k in test_gpu_pages.DATA:
+            assert np.array_equal(after[k].view(np.uint8), before[k].view(np.uint8)), k
