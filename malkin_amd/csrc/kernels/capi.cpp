@@ -602,7 +602,7 @@ int mk_rope_tables(mk_ctx* c, const mk_rope* rope, const float* divide, int64_t 
       require(rope->n_orig > 0 && rope->base != 1.0 && rope->beta_fast > 0.0 && rope->beta_slow > 0.0 &&
                   std::isfinite(rope->beta_fast) && std::isfinite(rope->beta_slow) && std::isfinite(rope->attn_factor),
               "mk_rope_tables: bad YaRN parameters");
-    require(n_pos >= 0 && first >= 0 && first + n_pos <= (1ll << 31), "mk_rope_tables: bad positions");
+    require(n_pos >= 0 && first >= 0 && first <= (1ll << 31) - n_pos, "mk_rope_tables: bad positions");
     if (n_pos == 0) return;
     require(cos_t && sin_t, "mk_rope_tables: null array");
     require(c != nullptr, "mk_rope_tables: null context");
