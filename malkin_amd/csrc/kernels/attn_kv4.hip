@@ -848,10 +848,14 @@ struct Cut {
   int wgs;    // workgroups that share all tiles; 0: one per block
   int waves;  // of a workgroup that has a block to itself
 };
-// A workgroup of eight waves per block up to kWholeKeys keys, with kMany blocks one of four waves up to kWholeKeysMany. 32 query
-// heads on 8: 8 users, 1000 keys 12.5 us, in shares 18.8 (four waves 14.6); one user, 2000 keys 18.9, in shares 13.7; 64 users,
-// 1000 keys 22, in shares 33 (eight waves 25.8), 2000 keys 33 and 47, 3000 keys 46.5 and 53.4, 4000 keys 60 and 61, where one
-// long sequence among short ones begins to be felt.
+// A workgroup of eight waves per block up to kWholeKeys keys, with kMany workgroups one of four waves: tokens that lead no block
+// have workgroups too, which leave at once but need their place on a CU before (16 x 4 drafts over 200 keys 10 us, with eight
+// waves 15.7; over 900 keys, 24 x 5, 21 and 18.7). 32 query heads on 8: 8 users, 1000 keys 12.5 us, in shares 18.8 (four waves
+// 14.6); one user, 2000 keys 18.9, in shares 13.7; 64 users, 1000 keys 22, in shares 33 (eight waves 25.8).
+// Up to kWholeKeysMany keys where kMany blocks have work. 64 users of 600 to 3000 keys 47 us, in shares 54; all of 3000 57 and
+// 58.5; one of 3000 among such of 375 32 and 26.5, but up to 2000 keys as long (23.8), and with 128 users 33 and 36; of 800 to
+// 4000 keys 60 and 61.5, one of 4000 among short ones 40.5 and 28.5. Fewer blocks: 16 x 4 drafts over 3000 keys 45.7 and 28.5,
+// 8 x 8 41.2 and 30.4, over 1500 keys 25.1 and 26.7.
 constexpr int kWholeKeys = 1024, kWholeKeysMany = 3200, kMany = 512;
 // Workgroups that share all tiles: two a CU, which leaves a wave 256 registers. Three of 168 took 41.6 us where two take 39.5 (24
 // users of up to 6000 keys), 49 where 42.6 (one user of 100000), and as long for 64 users of 4000.
@@ -863,8 +867,9 @@ constexpr int kJoinRows = 2048;
 Cut cut_of(int n, int H, int KV, int max_keys, int max_run) {
   const int64_t rows = std::min<int64_t>(std::max(max_run, 1), n) * (H / KV);
   Cut c{rows > kSet ? 2 : 1, 0, 8};
-  const int64_t blocks = (int64_t)n * shape_of(H, KV, c.sets * kSet, max_run).J;
-  if (blocks >= kMany) c.waves = 4;
+  const Shape S = shape_of(H, KV, c.sets * kSet, max_run);
+  const int64_t wgs = (int64_t)n * S.J, blocks = (int64_t)((n + S.tq - 1) / S.tq) * S.J;  // launched, and with work
+  if (wgs >= kMany) c.waves = 4;
   if (rows <= 2 * kSet && max_keys <= (blocks >= kMany ? kWholeKeysMany : kWholeKeys)) return c;
   c.wgs = kShares;
   return c;
