@@ -507,11 +507,12 @@ int mk_verify_topk(mk_ctx* ctx, const float* p_values, const int32_t* p_ids, int
 /* ---- beam search (no reference counterpart: its engine samples) ----
  * Per group of `beams` rows of logits (row g * beams + b: beam b of group g, `stride` floats apart), the k best ways to go on,
  * best first: beam b with token v has the score scores[row] + logits[row][v] - log(sum_u exp(logits[row][u])), in 64 bits; a
- * beam with done[row] != 0 (done NULL: none) has only itself, token eos, its score as it is. Equal scores: the lower beam, then
- * the lower token. Logits: NaN counts as -inf (no candidate), +inf as the largest float; a beam whose score is not finite has
- * no part. out_scores (rounded), out_seq (the row it goes on from: mk_kv4_fork's src) and out_tokens are [n_group][k]; places
- * without a candidate: -inf, -1, -1. beams 1..64, k 1..128, n_vocab at most 2^21. workspace: at least mk_beam_workspace bytes,
- * 16-byte aligned; two calls that may run at the same time need one each. Outputs and inputs are different arrays. */
+ * beam with done[row] != 0 (done NULL: none) has only itself, token eos, its score as it is. Equal scores: the lower beam, of
+ * one beam the larger logit (two may have one score in 64 bits), then the lower token. Logits: NaN counts as -inf (no
+ * candidate), +inf as the largest float; a beam whose score is not finite has no part. out_scores (rounded), out_seq (the row it
+ * goes on from: mk_kv4_fork's src) and out_tokens are [n_group][k]; places without a candidate: -inf, -1, -1. beams 1..64, k
+ * 1..128, n_vocab at most 2^21. workspace: at least mk_beam_workspace bytes, 16-byte aligned; two calls that may run at the same
+ * time need one each. Outputs and inputs are different arrays. */
 size_t mk_beam_workspace(int n_group, int beams, int n_vocab, int k);
 int mk_beam_select(mk_ctx* ctx, const float* logits, int64_t stride, int n_group, int beams, int n_vocab,
                    const float* scores, const int32_t* done, int eos, int k, float* out_scores, int32_t* out_seq,
