@@ -48,14 +48,14 @@ constexpr int kTile = 64, kChunk = 16;
 constexpr int kSet = 16;      // query rows of an MFMA
 constexpr int kIds = 1024;    // pages of chunks held in LDS at a time
 
-// How tokens and heads are taken together: R rows of a block, up to tq tokens with `per` heads each (hs blocks per KV head
-// and token where a KV head has more than R query heads), J blocks per run of tokens.
+// How tokens and heads are taken together: R rows of a block, which are all G query heads of a KV head (G <= R) for up to tq
+// tokens; J blocks per run of tokens.
 struct Shape {
-  int G, tq, hs, J;
+  int G, tq, J;
 };
 __host__ __device__ inline Shape shape_of(int H, int KV, int R, int max_run) {
-  const int G = H / KV, hs = (G + R - 1) / R, tq = G < R ? R / G : 1;
-  return Shape{G, max_run < 1 ? 1 : max_run < tq ? max_run : tq, hs, KV * hs};
+  const int G = H / KV, tq = R / G;
+  return Shape{G, max_run < 1 ? 1 : max_run < tq ? max_run : tq, KV};
 }
 
 // A block of rows of one KV head, and how many keys its tokens see at most.
@@ -70,10 +70,8 @@ struct Block {
   __device__ __forceinline__ int head(int r) const { return h0 + r - turn(r) * per; }
   __device__ __forceinline__ int tiles() const { return (keys + kTile - 1) / kTile; }
 };
-template <int R>
 __device__ __forceinline__ void set_heads(Block& b, const Shape& S, int j) {
-  const int sub = j % S.hs;
-  b.g = j / S.hs, b.h0 = b.g * S.G + R * sub, b.per = min(S.G - R * sub, R);
+  b.g = j, b.h0 = j * S.G, b.per = S.G;
   b.inv = (65535 + b.per) / b.per;
 }
 
@@ -610,7 +608,7 @@ __global__ __launch_bounds__(NW * 64) void k_kv4_whole(Kv4Attn A, const float* _
   if (S.tq > 1 && (t - run_start(A, t)) % S.tq) return;
   Block b;
   set_tokens(b, A, t, S.tq);
-  set_heads<NR * kSet>(b, S, blockIdx.x % S.J);
+  set_heads(b, S, blockIdx.x % S.J);
   run_block<D, NR, NW>(A, b, 0, b.tiles(), q, q_stride, smem, sh,
                        [&](int r, int d, v4f a, float l, float m) { put_row<D>(A, O, b.token(r), b.head(r), d, a, l); });
 }
@@ -747,7 +745,7 @@ __global__ __launch_bounds__(kShare * 64, 2) void k_kv4_share(Kv4Attn A, const f
       continue;
     }
     const int k1 = (int)min<int64_t>(tiles, k0 + (b - at));
-    set_heads<R>(blk, S, j);
+    set_heads(blk, S, j);
     // A block that begins here and ends before the next workgroup's run is written whole.
     const bool begins = k0 == 0, whole = begins && at + tiles <= a + share;
     if (begins) {
@@ -777,15 +775,15 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attn A, Out O, Parts P) {
   const int64_t row = (int64_t)blockIdx.x * (4 / W) + wave / W;
   if (row >= (int64_t)A.n * A.H) return;
   const Shape S = shape_of(A.H, A.kv.KV, R, A.max_run);
-  const int t = (int)(row / A.H), head = (int)(row % A.H), in = head % S.G;
-  const Record rec = P.rec[(int64_t)t * S.J + head / S.G * S.hs + in / R];  // what it says counts where there are keys
+  const int t = (int)(row / A.H), head = (int)(row % A.H);
+  const Record rec = P.rec[(int64_t)t * S.J + head / S.G];  // what it says counts where there are keys
   const bool any = keys_of(A, t) > 0;
   if (any && rec.last < 0) return;
   float v[E], sum = 0.0f;
 #pragma unroll
   for (int k = 0; k < E; ++k) v[k] = 0.0f;
   if (any) {
-    const int r = rec.row + in % R, parts = rec.last - rec.first + 1;
+    const int r = rec.row + head % S.G, parts = rec.last - rec.first + 1;
     auto slot = [&](int i) { return (2 * ((int64_t)rec.first + i) + (i == 0)) * R + r; };
     auto read = [&](int i0, float (&x)[kAhead][E]) {
 #pragma unroll
@@ -877,9 +875,8 @@ Cut cut_of(int n, int H, int KV, int max_keys, int max_run) {
 
 template <int D>
 size_t parts_bytes(const Cut& c, int n, int H, int KV) {
-  const Shape S = shape_of(H, KV, c.sets * kSet, 1);
   const size_t rows = 2ull * c.wgs * c.sets * kSet;
-  return rows * (D * sizeof(float) + sizeof(v2f)) + (size_t)n * S.J * sizeof(Record);
+  return rows * (D * sizeof(float) + sizeof(v2f)) + (size_t)n * KV * sizeof(Record);
 }
 
 }  // namespace
