@@ -326,8 +326,8 @@ int mk_kv4_rows(mk_ctx* ctx, const mk_kv4_cache* kv, int layer, const int32_t* s
    token with n_keys[t] <= 0 or seq[t] outside the cache gets zeros, and keys whose page is not in the pool have no weight.
    Tokens may come in any order; those of one sequence that follow each other read its rows together. xq: the BlockQ8 rows of
    out, as mk_attention_q8 (NULL: not written). workspace: at least mk_attention_kv4_workspace bytes for the same sizes or
-   larger ones, 16-byte aligned; two calls that may run at the same time need one each. out and q must not overlap.
-   MK_ERR_UNSUPPORTED for more than 32 query heads per KV head. */
+   larger ones, 16-byte aligned; two calls that may run at the same time need one each. out and q must not overlap; seq, n_keys
+   and the table stay as they are until the call has run. MK_ERR_UNSUPPORTED for more than 32 query heads per KV head. */
 size_t mk_attention_kv4_workspace(int n, int n_head, int n_head_kv, int head_dim, int max_keys, int max_run);
 int mk_attention_kv4(mk_ctx* ctx, const float* q, int64_t q_stride, float* out, int64_t out_stride, int n, int n_head,
                      const mk_kv4_cache* kv, int layer, const int32_t* seq, const int32_t* n_keys, int max_keys,

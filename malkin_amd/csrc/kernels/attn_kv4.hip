@@ -719,7 +719,8 @@ __global__ __launch_bounds__(kShare * 64, 2) void k_kv4_share(Kv4Attn A, const f
   if (a >= b) return;
   // The block that holds tile a is one of exactly one thread's.
   run = 0, total = 0;
-  for (int c0 = 0;; c0 += kOnce) {
+  bool found = false;
+  for (int c0 = 0; c0 < A.n && !found; c0 += kOnce) {
     if (A.n > kOnce) look(c0);
     int64_t off = (total + before) * S.J;
 #pragma unroll
@@ -728,8 +729,9 @@ __global__ __launch_bounds__(kShare * 64, 2) void k_kv4_share(Kv4Attn A, const f
       off += (int64_t)tiles[e] * S.J;
     }
     total += all;
-    if (a < total * S.J) break;
+    found = a < total * S.J;
   }
+  if (!found) return;  // lengths that changed in between, which no caller may do: every loop ends all the same
   __syncthreads();
   // Blocks follow each other by (token, j); tile a is tile k0 of block j of those that token t leads.
   int t = start_t;
@@ -740,7 +742,7 @@ __global__ __launch_bounds__(kShare * 64, 2) void k_kv4_share(Kv4Attn A, const f
     const int tiles = blk.tiles();
     if (j == S.J || tiles == 0) {  // the next tokens'
       t += blk.m, j = 0;
-      if (t >= A.n) return;  // lengths that change while they are read: no reason to wait for ever
+      if (t >= A.n) return;  // as above
       set_tokens(blk, A, t, S.tq);
       continue;
     }
