@@ -18,11 +18,13 @@
 // keys of V. Each wave takes every NW-th tile through a K and a V buffer of its own, which direct copies fill: a buffer's next
 // tile is asked for as soon as this one is in registers, and the waves meet only to add their results.
 //
-// What bounds it: the vector instructions that turn 4 bits into fp16 factors, 13 for eight values and as many for K as for V,
-// which is 416 of a tile's 560 to 700 (16 or 32 rows); two waves a SIMD cover them with matrix instructions in part.
-// Long documents of four users (4 x 5 drafted tokens) take 125 us, 3.0 TB/s of the cache's bytes, where the copies alone take
-// 63; 24 users of up to 6000 keys 38.5 us, of which 12 are spent before the first and after the last tile and 4 on joining; 512
-// tokens of three prompts 78 us, 21 of them for setting up and ending each workgroup's two or three blocks and 10 on joining.
+// What bounds it: long documents the vector instructions that turn 4 bits into fp16 factors, 13 for eight values and as many for K
+// as for V, which is 416 of a tile's 560 to 700 (16 or 32 rows); two waves a SIMD cover them with matrix instructions in part.
+// Four users with 5 drafted tokens each take 125 us, 3.0 TB/s of the cache's bytes, where the copies alone take 63; vector
+// instructions are issued in 53 % of the cycles, the matrix units work in 31. Other calls reach no unit's limit, but wait:
+// 24 users of up to 6000 keys 38 us (33 % and 11, 2.6 TB/s), of which 12 are spent before the first and after the last tile and
+// 5 on joining; 512 tokens of three prompts 77 us (36 % and 17), 21 of them for setting up and ending each workgroup's two or
+// three blocks and 10 on joining.
 // Blocks of 128 rows, whose four waves take a tile's numbers out of 4 bits once for all of them, took 78 us there, but 69 for a
 // prompt of 300 tokens by itself, which takes 31 here, so that form is not kept.
 #include <algorithm>

@@ -5,10 +5,12 @@
 // fp16 holds, and attention multiplies by it without a rounding. An error of s is no error of a value: n is chosen for the s
 // that is stored.
 //
-// What bounds them: the bytes, and for a few tokens the launch. 8 tokens take 4.2 us, 1500 tokens of 16 + 2 x 8 heads 13 us (47 MB,
-// 3.6 TB/s; four heads a group of lanes took as long), 131072 positions of tables 14.7 us (4.6 TB/s, near a copy). A head's row
-// is 16 lanes of 8 elements (8 for head_dim 64); a group's extremes are exchanged in registers, the halves of a rotation through
-// LDS, which only a head's own lanes share (no barrier).
+// What bounds them: tables the memory (131072 positions 14.7 us, 4.6 TB/s, near a copy); the write of a few tokens the launch (8 of
+// them 4.4 us); that of a prompt the loads that a head waits for one after the other: its elements beside position, row and
+// sequence, then page, length and tables. 1500 tokens of 16 + 2 x 8 heads take 13.5 us for 39 MB, 2.9 of a copy's 5.5 TB/s, with
+// vector instructions in 27 % of the cycles (four heads a group of lanes took as long); their rows read back 4.4 us. A head's
+// row is 16 lanes of 8 elements (8 for head_dim 64); a group's extremes are exchanged in registers, the halves of a rotation
+// through LDS, which only a head's own lanes share (no barrier).
 #include <algorithm>
 #include <cmath>
 

@@ -4,7 +4,7 @@
 // bytes are copied only where a shared page that is not full is to be written, and in compaction. Results do not depend on
 // the order in which threads run: counts change by sums of whole numbers, and free pages are handed out by running sums over
 // the entries and over the pool, lowest number first, in one workgroup. What bounds a call is that workgroup's chain of four
-// or five loads that wait for each other and as many barriers (8.3 us for 64 entries; with 512 threads the same, with 256
+// or five loads that wait for each other and as many barriers (8.5 us for 64 entries; with 512 threads the same, with 256
 // 9.4) and then the copies' bytes, which a second launch moves with the whole chip: 4.7 us for 64 last pages of 28 layers,
 // 92 us for the 436 MB read and written of a compaction (4.7 TB/s).
 #include <algorithm>
